@@ -21,6 +21,7 @@ HEADER = os.path.join(os.path.dirname(PKG), "include", "qlinear_b200.h")
 
 # GGML type codes (reference src/tensor/TensorCommon.h:15-33)
 F32, F16, Q4_0, Q5_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 6, 8, 12, 14
+BF16 = 30  # activations of the kv8_* calls
 BLOCK = {Q4_0: (32, 18), Q5_0: (32, 22), Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210)}
 QL_OK, QL_EINVAL, QL_ECUDA, QL_EDEVICE = 0, 1, 2, 3
 PATH_AUTO, PATH_GEMV, PATH_TENSOR = 0, 1, 2
@@ -62,6 +63,11 @@ SIGNATURES = {
     "ql_quantize_q8_1_mmq": (I, [P, P, I, I, I]),
     "ql_quant_matmul_q8_1_mmq": (I, [I32, P, SZ, P, P, I, I, I]),
     "ql_full_attention_attend_batch": (I, [P, P, P, P, I, P, I, I, I, I, I, I]),
+    "ql_kv8_append": (I, [P, I32, P, I64, P, I64, P, I64, P, I64, I, P, P, F, P, I, I, P, P, I, I]),
+    "ql_kv8_attend_workspace": (SZ, [I, I, I, I, I, I, I]),
+    "ql_kv8_attend": (I, [P, I32, P, I64, P, I64, P, I64, I, F, P, P, I, I, I, P, SZ]),
+    "ql_kv8_gather": (I, [P, I32, P, P, P, I, P]),
+    "ql_logits_apply": (I, [P, I64, P, I64, I, I, P, P, P, SZ]),
     "ql_moe_swiglu_grouped": (I, [I32, P, P, SZ, SZ, SZ, SZ, P, I64, P, I, I, P, I, I, I, I]),
     "ql_moe_down_grouped_accum_ordered": (I, [I32, P, SZ, SZ, P, P, I, I, P, P, I64, I, I, I, I]),
     "ql_quant_embedding": (I, [I32, P, P, P, SZ, I, I]),
@@ -353,6 +359,65 @@ def full_attention_attend_batch(q, gate, kc, vc, kv_bf16, attn, tokens, n_heads,
                                 start_pos):
     _call("ql_full_attention_attend_batch", q, gate, kc, vc, int(kv_bf16), attn, tokens, n_heads, kv_heads, head_dim,
           max_seq_len, start_pos)
+
+
+KV8_BLOCK = 32
+
+
+class KV8Cache(C.Structure):
+    """ql_kv8_cache (include/qlinear_b200.h): the caller's buffers of a paged 8-bit KV cache."""
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_open", C.c_void_p), ("v_open", C.c_void_p), ("page_table", C.c_void_p), ("slots", C.c_void_p),
+                ("n_pages", C.c_int32), ("n_slots", C.c_int32), ("n_seqs", C.c_int32), ("max_pages", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+def kv8_cache(k_codes, v_codes, k_scale, v_scale, k_open, v_open, page_table, slots, n_pages, n_slots, n_seqs,
+              max_pages, kv_heads, head_dim):
+    return KV8Cache(k_codes, v_codes, k_scale, v_scale, k_open, v_open, page_table, slots, n_pages, n_slots, n_seqs,
+                    max_pages, kv_heads, head_dim)
+
+
+def kv8_append(cache, t, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, n_heads, q_gamma, k_gamma, eps,
+               rope, rotary_dim, max_positions, kv_len, q_start, rows, max_q_len):
+    """Norm and rotation of q and k per head, k and v stored into the cache (see include/qlinear_b200.h)."""
+    _call("ql_kv8_append", C.byref(cache), t, q, q_stride, k, k_stride, v, v_stride, q_out, q_out_stride, n_heads,
+          q_gamma, k_gamma, eps, rope, rotary_dim, max_positions, kv_len, q_start, rows, max_q_len)
+
+
+def kv8_attend_workspace(n_heads, kv_heads, head_dim, n_seqs, rows, max_q_len, max_kv_len) -> int:
+    return int(lib().ql_kv8_attend_workspace(n_heads, kv_heads, head_dim, n_seqs, rows, max_q_len, max_kv_len))
+
+
+def kv8_attend(cache, t, q, q_stride, gate, gate_stride, out, out_stride, n_heads, scale, kv_len, q_start, rows,
+               max_q_len, max_kv_len, workspace, workspace_bytes):
+    _call("ql_kv8_attend", C.byref(cache), t, q, q_stride, gate, gate_stride, out, out_stride, n_heads, scale, kv_len,
+          q_start, rows, max_q_len, max_kv_len, workspace, workspace_bytes)
+
+
+def kv8_gather(cache, t, k_out, v_out, start, count, kv_len):
+    _call("ql_kv8_gather", C.byref(cache), t, k_out, v_out, start, count, kv_len)
+
+
+class LogitsRules(C.Structure):
+    """ql_logits_rules (include/qlinear_b200.h)."""
+    _fields_ = [("history", C.c_void_p), ("history_stride", C.c_int64), ("history_len", C.c_void_p),
+                ("prompt_len", C.c_void_p), ("repetition", C.c_void_p), ("frequency", C.c_void_p),
+                ("presence", C.c_void_p), ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p),
+                ("bias_start", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+                ("mask_rows", C.c_int32), ("mask_row", C.c_void_p)]
+
+
+def logits_rules(history=None, history_stride=0, history_len=None, prompt_len=None, repetition=None, frequency=None,
+                 presence=None, bias_ids=None, bias_values=None, bias_start=None, mask=None, mask_stride=0, mask_rows=0,
+                 mask_row=None):
+    return LogitsRules(history, history_stride, history_len, prompt_len, repetition, frequency, presence, bias_ids,
+                       bias_values, bias_start, mask, mask_stride, mask_rows, mask_row)
+
+
+def logits_apply(logits, logits_stride, out, out_stride, rows, vocab, rules, token, workspace, workspace_bytes):
+    _call("ql_logits_apply", logits, logits_stride, out, out_stride, rows, vocab, C.byref(rules), token, workspace,
+          workspace_bytes)
 
 
 def moe_swiglu_grouped(t, gw, uw, geb, ueb, grb, urb, x, x_stride, ids, expert_begin, n_experts, act, tokens, k,

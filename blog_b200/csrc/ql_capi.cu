@@ -21,6 +21,8 @@
 #include "ql_gemv.cuh"
 #include "ql_moe.cuh"
 #include "ql_attn.cuh"
+#include "ql_kv8.cuh"
+#include "ql_logits.cuh"
 #include "ql_q81.cuh"
 
 namespace ql {
@@ -582,6 +584,16 @@ int chain_workspace(float **part, unsigned **counters, int **err, int *sms) {
     return QL_OK;
 }
 
+// Runs an entry's body; no exception (e.g. a message that finds no memory) leaves the C boundary.
+template <typename F>
+int guarded(F &&f) noexcept {
+    try {
+        return f();
+    } catch (...) {
+        return QL_ECUDA;
+    }
+}
+
 // The current device's error word (initialising the workspace if needed), or null.
 int *device_error_word() {
     int st;
@@ -618,6 +630,13 @@ int ql_check_device(void) {
         cudaMemset(ws->amax, 0, kMaxArgmaxRows * sizeof(unsigned long long));
         cudaMemset(ws->amax_done, 0, sizeof(unsigned));
         cudaDeviceSynchronize();
+        if (h >= kErrKvPage)
+            return fail(QL_EDEVICE, std::string(h == kErrKvPage       ? "a page outside the KV cache"
+                                                : h == kErrKvSlot     ? "a slot outside the KV cache's open rows"
+                                                : h == kErrKvLength   ? "more rows than the sequence has tokens"
+                                                : h == kErrKvPosition ? "a position past the rotation table"
+                                                                      : "a mask row outside the masks") +
+                                        " (device error code " + std::to_string(h) + ")");
         return fail(QL_EDEVICE, "a kernel gave up a bounded wait (device error code " + std::to_string(h) + ")");
     }
     return QL_OK;
@@ -1172,6 +1191,236 @@ int ql_full_attention_attend_batch(const float *q, const float *gate, const void
         return fail(QL_EINVAL, "ql_full_attention_attend_batch: start_pos + tokens > max_seq_len");
     return attention(q, gate, key_cache, value_cache, kv_bf16, attn, tokens, n_heads, kv_heads, head_dim, max_seq_len,
                      nullptr, start_pos, "ql_full_attention_attend_batch");
+}
+
+// ---- 8-bit KV cache, rules on logits -------------------------------------------------
+namespace {
+int kv8_view(const ql_kv8_cache *c, int32_t type, Kv8View &v, const std::string &what) {
+    if (type != QL_F32 && type != QL_BF16) return fail(QL_EINVAL, what + ": type must be QL_F32 or QL_BF16");
+    if (!c) return fail(QL_EINVAL, what + ": null cache");
+    if (c->head_dim <= 0 || c->head_dim > kKvMaxHeadDim || c->head_dim % 32)
+        return fail(QL_EINVAL, what + ": head_dim must be a multiple of 32 up to 256");
+    if (c->kv_heads <= 0 || c->kv_heads > 1024 || c->n_seqs < 0 || c->n_pages < 0 || c->n_slots < 0 || c->max_pages < 0 ||
+        c->max_pages > INT32_MAX / kKvBlock)
+        return fail(QL_EINVAL, what + ": need kv_heads in 1..1024 and n_seqs, n_pages, n_slots, max_pages >= 0");
+    if (c->n_seqs > 65535) return fail(QL_EINVAL, what + ": at most 65535 sequences per call");
+    if (c->n_seqs > 0) {
+        const void *need[] = {c->k_codes, c->v_codes, c->k_scale, c->v_scale, c->k_open, c->v_open, c->page_table};
+        for (const void *p : need)
+            if (!p) return fail(QL_EINVAL, what + ": null cache buffer");
+        for (const void *p : {need[0], need[1], need[4], need[5]})
+            if (reinterpret_cast<uintptr_t>(p) % 16) return fail(QL_EINVAL, what + ": cache buffers must be 16-byte aligned");
+        for (const void *p : {need[2], need[3], need[6], static_cast<const void *>(c->slots)})
+            if (reinterpret_cast<uintptr_t>(p) % 4) return fail(QL_EINVAL, what + ": misaligned cache buffer");
+    }
+    v = Kv8View{c->k_codes, c->v_codes, c->k_scale, c->v_scale, c->k_open,    c->v_open,   c->page_table,
+                c->slots,   c->n_pages, c->n_slots, c->n_seqs,  c->max_pages, c->kv_heads, c->head_dim, nullptr};
+    return QL_OK;
+}
+int kv8_rows(const Kv8View &c, const int32_t *kv_len, const int32_t *q_start, int rows, int max_q_len, Kv8Rows &r,
+             const std::string &what) {
+    if (rows < 0 || max_q_len < 0) return fail(QL_EINVAL, what + ": rows and max_q_len must not be negative");
+    if (!q_start && rows != c.n_seqs)
+        return fail(QL_EINVAL, what + ": without q_start there is one row per sequence (rows == n_seqs)");
+    if (rows > 0 && c.n_seqs == 0) return fail(QL_EINVAL, what + ": rows without sequences");
+    if (rows > 0 && !kv_len) return fail(QL_EINVAL, what + ": null kv_len");
+    if (rows > 0 && max_q_len < (q_start ? (rows + c.n_seqs - 1) / c.n_seqs : 1))
+        return fail(QL_EINVAL, what + ": max_q_len is less than the rows need");
+    r = Kv8Rows{kv_len, q_start, rows};
+    return QL_OK;
+}
+// Rows of heads x head_dim elements, a stride that holds them, aligned to the element.
+int kv8_operand(const void *p, int64_t stride, int64_t width, int32_t type, const char *name, const std::string &what) {
+    if (!p) return fail(QL_EINVAL, what + ": null " + name);
+    if (stride < width) return fail(QL_EINVAL, what + ": " + name + "'s stride is less than its row");
+    if (reinterpret_cast<uintptr_t>(p) % (type == QL_F32 ? 4 : 2)) return fail(QL_EINVAL, what + ": misaligned " + name);
+    return QL_OK;
+}
+
+// Launch shape of the attention over split keys, from the caller's bounds alone (so the workspace can be
+// sized before the call and a captured launch fits every length).
+struct Kv8AttnShape {
+    int row_groups, splits;
+    size_t bytes;
+};
+Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs, int max_q_len, int max_kv_len, int sms) {
+    Kv8AttnShape s{};
+    s.row_groups = (int)(((int64_t)max_q_len * (n_heads / kv_heads) + kKvAttnRows - 1) / kKvAttnRows);
+    const int64_t groups = (int64_t)n_seqs * kv_heads * s.row_groups;
+    const int64_t slots = (int64_t)sms * kv8_attn_ctas_per_sm(head_dim);
+    const int64_t blocks = (max_kv_len + kKvBlock - 1) / kKvBlock;
+    int64_t n = groups > 0 ? (slots + groups - 1) / groups : 1;
+    n = std::min<int64_t>(n, (blocks + kKvAttnWarps - 1) / kKvAttnWarps);
+    n = std::min<int64_t>(n, kKvAttnMaxSplits);
+    if (groups > kKvAttnCounters) n = 1;
+    s.splits = (int)std::max<int64_t>(n, 1);
+    s.bytes = sizeof(unsigned) * kKvAttnCounters;
+    if (s.splits > 1) s.bytes += sizeof(float) * (size_t)groups * s.splits * kKvAttnRows * (head_dim + 2);
+    return s;
+}
+}  // namespace
+
+int ql_kv8_append(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                  const void *v, int64_t v_stride, void *q_out, int64_t q_out_stride, int n_heads, const float *q_gamma,
+                  const float *k_gamma, float eps, const float *rope, int rotary_dim, int max_positions,
+                  const int32_t *kv_len, const int32_t *q_start, int rows, int max_q_len) {
+    return guarded([&] {
+        const std::string what = "ql_kv8_append";
+        t_launches = 0;
+        Kv8AppendArgs a{};
+        int st;
+        if ((st = kv8_view(cache, type, a.c, what)) || (st = kv8_rows(a.c, kv_len, q_start, rows, max_q_len, a.r, what)))
+            return st;
+        const int hd = a.c.head_dim;
+        if (n_heads < 0 || (q == nullptr) != (n_heads == 0))
+            return fail(QL_EINVAL, what + ": n_heads > 0 with q, 0 without");
+        if (rotary_dim < 0 || rotary_dim > hd || rotary_dim % (hd / 16))
+            return fail(QL_EINVAL, what + ": rotary_dim must be a multiple of head_dim / 16, at most head_dim");
+        if (!(eps >= 0.f)) return fail(QL_EINVAL, what + ": eps must not be negative");
+        if (rows == 0) return (int)QL_OK;
+        if (rotary_dim > 0 && (!rope || max_positions <= 0 || reinterpret_cast<uintptr_t>(rope) % 4))
+            return fail(QL_EINVAL, what + ": rotation needs a table of max_positions > 0 rows");
+        if (n_heads > 0 && ((st = kv8_operand(q, q_stride, (int64_t)n_heads * hd, type, "q", what)) ||
+                            (st = kv8_operand(q_out, q_out_stride, (int64_t)n_heads * hd, type, "q_out", what))))
+            return st;
+        if ((st = kv8_operand(k, k_stride, (int64_t)a.c.kv_heads * hd, type, "k", what)) ||
+            (st = kv8_operand(v, v_stride, (int64_t)a.c.kv_heads * hd, type, "v", what)))
+            return st;
+        const int64_t ctas = ((int64_t)rows * n_heads + 7) / 8 + ((int64_t)rows + 2 * (int64_t)a.c.n_seqs) * a.c.kv_heads * 2;
+        if (ctas > INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
+        Workspace *ws = workspace(&st);
+        if (!ws) return st;
+        a.c.err = ws->err;
+        a.q = q, a.k = k, a.v = v, a.q_out = q_out;
+        a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.q_out_stride = q_out_stride;
+        a.n_heads = n_heads;
+        a.q_gamma = q_gamma, a.k_gamma = k_gamma, a.eps = eps;
+        a.rope = rope, a.rotary_dim = rotary_dim, a.max_positions = max_positions;
+        const cudaError_t e = kv8_append_launch(a, type == QL_BF16, g_stream);
+        ++t_launches;
+        return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
+    });
+}
+
+size_t ql_kv8_attend_workspace(int n_heads, int kv_heads, int head_dim, int n_seqs, int rows, int max_q_len, int max_kv_len) {
+    if (n_heads <= 0 || kv_heads <= 0 || n_heads % kv_heads || head_dim <= 0 || head_dim > kKvMaxHeadDim || head_dim % 32 ||
+        n_seqs < 0 || rows < 0 || max_q_len < 0 || max_kv_len < 0)
+        return 0;
+    int st;
+    Workspace *ws = workspace(&st);
+    if (!ws) return 0;
+    return kv8_attn_shape(n_heads, kv_heads, head_dim, n_seqs, max_q_len, max_kv_len, ws->sms).bytes;
+}
+
+int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *gate,
+                  int64_t gate_stride, void *out, int64_t out_stride, int n_heads, float scale, const int32_t *kv_len,
+                  const int32_t *q_start, int rows, int max_q_len, int max_kv_len, void *workspace_, size_t workspace_bytes) {
+    return guarded([&] {
+        const std::string what = "ql_kv8_attend";
+        t_launches = 0;
+        Kv8AttnArgs a{};
+        int st;
+        if ((st = kv8_view(cache, type, a.c, what)) || (st = kv8_rows(a.c, kv_len, q_start, rows, max_q_len, a.r, what)))
+            return st;
+        const int hd = a.c.head_dim;
+        if (n_heads <= 0 || n_heads % a.c.kv_heads) return fail(QL_EINVAL, what + ": n_heads must be a multiple of kv_heads");
+        if (max_kv_len < 0) return fail(QL_EINVAL, what + ": max_kv_len must not be negative");
+        if (rows == 0) return (int)QL_OK;
+        const int64_t width = (int64_t)n_heads * hd;
+        if ((st = kv8_operand(q, q_stride, width, type, "q", what)) || (st = kv8_operand(out, out_stride, width, type, "out", what)))
+            return st;
+        if (gate && (st = kv8_operand(gate, gate_stride, width, type, "gate", what))) return st;
+        Workspace *ws = workspace(&st);
+        if (!ws) return st;
+        const int mq = q_start ? max_q_len : 1;
+        const Kv8AttnShape sh = kv8_attn_shape(n_heads, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len, ws->sms);
+        if ((int64_t)sh.row_groups * a.c.kv_heads > 65535)
+            return fail(QL_EINVAL, what + ": max_q_len x n_heads too large for one call");
+        if (!workspace_ || workspace_bytes < sh.bytes || reinterpret_cast<uintptr_t>(workspace_) % 16)
+            return fail(QL_EINVAL, what + ": the workspace must be 16-byte aligned and hold " + std::to_string(sh.bytes) +
+                                       " bytes (ql_kv8_attend_workspace)");
+        a.c.err = ws->err;
+        a.q = q, a.gate = gate, a.out = out;
+        a.q_stride = q_stride, a.gate_stride = gate_stride, a.out_stride = out_stride;
+        a.n_heads = n_heads;
+        a.scale_log2 = scale * 1.4426950408889634f;
+        a.splits = sh.splits;
+        a.row_groups = sh.row_groups;
+        a.arrivals = static_cast<unsigned *>(workspace_);
+        a.part = reinterpret_cast<float *>(a.arrivals + kKvAttnCounters);
+        const cudaError_t e = kv8_attn_launch(a, type == QL_BF16, g_stream);
+        ++t_launches;
+        return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
+    });
+}
+
+int ql_kv8_gather(const ql_kv8_cache *cache, int32_t type, void *k_out, void *v_out, const int32_t *start, int count,
+                  const int32_t *kv_len) {
+    return guarded([&] {
+        const std::string what = "ql_kv8_gather";
+        t_launches = 0;
+        Kv8View c{};
+        int st;
+        if ((st = kv8_view(cache, type, c, what))) return st;
+        if (count < 0) return fail(QL_EINVAL, what + ": count must not be negative");
+        if (count == 0 || c.n_seqs == 0 || (!k_out && !v_out)) return (int)QL_OK;
+        if (!kv_len) return fail(QL_EINVAL, what + ": null kv_len");
+        if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16)
+            return fail(QL_EINVAL, what + ": outputs must be 16-byte aligned");
+        if ((int64_t)c.n_seqs * count * c.kv_heads * 2 / 8 >= INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
+        Workspace *ws = workspace(&st);
+        if (!ws) return st;
+        c.err = ws->err;
+        const cudaError_t e = kv8_gather_launch(c, kv_len, start, count, k_out, v_out, type == QL_BF16, g_stream);
+        ++t_launches;
+        return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
+    });
+}
+
+int ql_logits_apply(const float *logits, int64_t logits_stride, float *out, int64_t out_stride, int rows, int vocab,
+                    const ql_logits_rules *rules, int32_t *token, void *workspace_, size_t workspace_bytes) {
+    return guarded([&] {
+        const std::string what = "ql_logits_apply";
+        t_launches = 0;
+        if (rows < 0 || rows > 65535 || vocab < 0 || vocab > (1 << 30))
+            return fail(QL_EINVAL, what + ": need 0 <= rows <= 65535 and 0 <= vocab <= 2^30");
+        if (!rules) return fail(QL_EINVAL, what + ": null rules");
+        if (rows == 0) return (int)QL_OK;
+        if (vocab == 0) return fail(QL_EINVAL, what + ": rows of no logits");
+        if (!logits || logits_stride < vocab) return fail(QL_EINVAL, what + ": null logits, or a stride below vocab");
+        if (out && out_stride < vocab) return fail(QL_EINVAL, what + ": out's stride is below vocab");
+        if (out == logits && out_stride != logits_stride) return fail(QL_EINVAL, what + ": in place the strides are the same");
+        if (reinterpret_cast<uintptr_t>(logits) % 4 || reinterpret_cast<uintptr_t>(out) % 4)
+            return fail(QL_EINVAL, what + ": misaligned logits or out");
+        if (rules->history && (!rules->history_len || rules->history_stride < 0 || rules->history_stride > INT32_MAX))
+            return fail(QL_EINVAL, what + ": a history needs history_len and a stride");
+        if (rules->bias_ids && (!rules->bias_values || !rules->bias_start))
+            return fail(QL_EINVAL, what + ": biases need bias_values and bias_start");
+        if (rules->mask && (rules->mask_rows < 0 || rules->mask_stride < ((int64_t)vocab + 31) / 32 ||
+                            (!rules->mask_row && rules->mask_rows < rows)))
+            return fail(QL_EINVAL, what + ": masks need vocab / 32 words a row, and a row for each row of logits or mask_row");
+        if (token && (!workspace_ || workspace_bytes < 16 * (size_t)rows || reinterpret_cast<uintptr_t>(workspace_) % 16))
+            return fail(QL_EINVAL, what + ": the token needs a 16-byte aligned workspace of 16 bytes per row");
+        int st;
+        Workspace *ws = workspace(&st);
+        if (!ws) return st;
+        LogitsArgs a{};
+        a.logits = logits, a.out = out;
+        a.logits_stride = logits_stride, a.out_stride = out_stride;
+        a.rows = rows, a.vocab = vocab;
+        a.history = rules->history, a.history_len = rules->history_len, a.prompt_len = rules->prompt_len;
+        a.history_stride = rules->history_stride;
+        a.repetition = rules->repetition, a.frequency = rules->frequency, a.presence = rules->presence;
+        a.bias_ids = rules->bias_ids, a.bias_start = rules->bias_start, a.bias_values = rules->bias_values;
+        a.mask = rules->mask, a.mask_stride = rules->mask_stride, a.mask_rows = rules->mask_rows, a.mask_row = rules->mask_row;
+        a.token = token;
+        a.keys = static_cast<unsigned long long *>(workspace_);
+        a.done = reinterpret_cast<unsigned *>(a.keys + rows);
+        a.err = ws->err;
+        const cudaError_t e = logits_launch(a, ws->sms, g_stream);
+        ++t_launches;
+        return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
+    });
 }
 
 // ---- opt-in Q8_1 activation path ----------------------------------------------------

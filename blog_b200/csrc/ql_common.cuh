@@ -54,7 +54,17 @@ constexpr int kRowGroup = 32;
 constexpr int kMaxParts = 64;  // most CTAs that may share one row group
 
 // Error codes written to the device error word (read back by the host).
-enum DevErr : int { kErrNone = 0, kErrWaitFull = 1, kErrWaitEmpty = 2, kErrBadExpert = 3 };
+enum DevErr : int {
+    kErrNone = 0,
+    kErrWaitFull = 1,
+    kErrWaitEmpty = 2,
+    kErrBadExpert = 3,
+    kErrKvPage = 16,      // a page table entry outside the cache, or a block past the table
+    kErrKvSlot = 17,      // a slot outside the open rows
+    kErrKvLength = 18,    // more rows in a call than the sequence holds tokens
+    kErrKvPosition = 19,  // a position past the rotation table
+    kErrMaskRow = 20    // a mask row outside the masks
+};
 
 // ---------------------------------------------------------------------------
 // PTX helpers (sm_100a).

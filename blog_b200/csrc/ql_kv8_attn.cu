@@ -1,0 +1,578 @@
+// Attention over the 8-bit KV cache, split over the keys: the form for single tokens and few queries.
+//
+//   out_h = softmax_j(scale q_h . k_j) . v_j  (* sigmoid(gate_h)),   j = 0 .. the query's position,
+//   k_j = (ck_j - 128) sk_b,  v_j = (cv_j - 128) sv_b,  b = j / 32 the token's block,
+// and the exact f32 rows for the tokens of the block that is not full.
+//
+// Mathematics.  A code is an integer of 8 bits and so exact in f16: with q = 2^-e (qh + ql) in two f16 limbs
+// (22 bits) the products q . c are exact and summed in fp32, and one multiplication by sk_b scale 2^-e gives
+// the score.  Weights p = 2^(s - m) are multiplied by sv_b / vref (vref: the largest scale met, like the
+// running maximum m) and split into two f16 limbs in the same way, so the result is as exact as fp32 sums
+// make it.  The two limbs cost nothing: mma.m16n8k16 has 16 rows, the 8 rows' upper limbs and their lower
+// ones, and the two halves of an accumulator fragment are added.
+//
+// Layout.  A CTA has 4 warps and 8 rows (query token, head of one KV head's group); each warp walks over
+// key blocks of its own (32 tokens x head_dim codes of K and of V, two contiguous pieces of a page) through
+// a ring in shared memory filled by cp.async, with its own m, l and accumulators, so the loop has no barrier.
+// The order of the head dimension within a product and of the tokens within a block is free as long as both
+// operands agree, so the fragments are 16-byte pieces of the rows as they lie in the page: 16 codes of K
+// serve four k-steps, and V pairs of tokens are gathered from two rows by one byte permute.
+// Warps are merged in shared memory, CTAs of one (sequence, KV head, row group) by the last to arrive, in
+// split order: the result does not depend on which CTA that is.
+//
+// Bound: HBM for the codes (2 head_dim bytes per token and KV head).
+#include <cuda_fp16.h>
+
+#include "ql_kv8.cuh"
+
+namespace ql {
+namespace {
+
+constexpr int kThreads = 32 * kKvAttnWarps;
+constexpr float kPScale = 16384.0f;    // weights are scaled to use f16's range
+constexpr float kVHeadroom = 3.9f;     // a block's scale may pass vref by this before the sums are rescaled
+
+__device__ __forceinline__ void cp16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two codes (bytes sel of w) as f16: 0x6400 | u is 1024 + u, minus 1152 is exact.
+__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t sel) {
+    uint32_t r = __byte_perm(w, 0x64646464u, sel);
+    const uint32_t bias = 0x64806480u;  // 1152, 1152
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(bias));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+// x = hi + lo in two f16 limbs, two values packed.
+__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t &hi, uint32_t &lo) {
+    hi = pack_f16(x0, x1);
+    const float2 h = unpack_f16(hi);
+    lo = pack_f16(x0 - h.x, x1 - h.y);
+}
+// 2^k with amax * 2^k in [2^10, 2^11) (within the normal range), and 2^-k.
+__device__ __forceinline__ float limb_scale(float amax, float &inv) {
+    const int e = (int)(__float_as_uint(amax) >> 23) & 0xFF;
+    const int f = min(max(264 - e, 1), 253);
+    inv = __uint_as_float((uint32_t)(254 - f) << 23);
+    return __uint_as_float((uint32_t)f << 23);
+}
+template <typename T>
+__device__ __forceinline__ float load_f32(const T *p);
+template <>
+__device__ __forceinline__ float load_f32<float>(const float *p) { return *p; }
+template <>
+__device__ __forceinline__ float load_f32<__nv_bfloat16>(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void store_f32(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store_f32(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Ring stages per warp, and CTAs per SM, by head_dim: 64 head_dim bytes per stage, 4 warps, 227 KB per SM.
+constexpr int stages(int hd) { return hd <= 64 ? 4 : 3; }
+constexpr int ctas_per_sm(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
+
+// 16-byte chunk of a row at which chunk c of row t lies.  K: a load phase (8 lanes) reads 64 bytes of two
+// rows, which share their banks where a row is a multiple of 128 bytes: the odd row's halves are swapped.
+// V: a phase reads two chunks of four rows (the lanes' token pairs); the XOR spreads them over all banks.
+template <int HD>
+__device__ __forceinline__ int k_chunk(int c, int t) {
+    return HD % 128 == 0 ? c ^ ((t & 1) << 2) : c;
+}
+template <int HD>
+__device__ __forceinline__ int v_chunk(int c, int t) {
+    const int p = (t >> 1) & 3;
+    if (HD == 128) return c ^ (p << 1);
+    if (HD == 256) return c ^ ((p & 1) | ((p & 2) << 1));
+    if (HD == 64) return c ^ ((p & 1) << 1);
+    return c;
+}
+
+// Factor of a partial (maximum pm, total pt) in the sum with maximum m: 0 where it saw no key, NaN where
+// its total is one (its maximum then says nothing).
+__device__ __forceinline__ float part_factor(float pm, float pt, float m) {
+    return pt != pt ? pt : pm == -INFINITY ? 0.f : ex2(pm - m);
+}
+
+// Running state of one warp: row g8 = lane / 4 in the first two floats of a fragment (upper limbs) and the
+// last two (lower limbs).
+template <int HD>
+struct Acc {
+    float o[HD / 8][4];
+    float m, l, vref;
+
+    // Block's scores s[n][2] (base-2 logarithms) of row g8, columns 2 q4, 2 q4 + 1 of n-tile n, to weights:
+    // returns the two limbs' A fragments.  vs: the scale of the block's values.
+    template <int NT>
+    __device__ __forceinline__ void weights(const float (&s)[NT][2], float vs, uint32_t (&hi)[NT], uint32_t (&lo)[NT]) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[n][0], s[n][1]));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        const float m_new = fmaxf(m, t);
+        float r = m_new > m ? ex2(m - m_new) : 1.0f;  // m = -inf: 0
+        m = m_new;
+        l *= r;
+        if (vs > kVHeadroom * vref) {  // warp-uniform; vref = 0 before the first block
+            r *= vref / vs;
+            vref = vs;
+        }
+        if (__any_sync(0xffffffffu, r != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[n][i] *= r;
+        }
+        const float f = vref > 0.f ? vs / vref * kPScale : vs * 0.f;  // (a NaN scale stays one)
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float p0 = ex2(s[n][0] - base), p1 = ex2(s[n][1] - base);
+            l += p0 + p1;
+            // (a NaN scale must not reach the weights of masked keys)
+            split_f16(s[n][0] == -INFINITY ? 0.f : p0 * f, s[n][1] == -INFINITY ? 0.f : p1 * f, hi[n], lo[n]);
+        }
+    }
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    extern __shared__ __align__(128) uint8_t sm[];
+    constexpr int ST = stages(HD), BLK = kKvBlock * HD;  // codes of one operand's block
+    constexpr int G64 = HD / 64, REM = HD % 64 / 32;     // K row: groups of 64 codes, and one of 32
+    constexpr int KS = HD / 16;                          // k-steps of q . k
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
+    const int G = a.n_heads / a.c.kv_heads;
+    const int split = blockIdx.x, kh = blockIdx.y % a.c.kv_heads, rg = blockIdx.y / a.c.kv_heads, seq = blockIdx.z;
+    uint8_t *ring = sm + warp * (ST * 2 * BLK);
+    uint4 *qf = reinterpret_cast<uint4 *>(sm + kKvAttnWarps * ST * 2 * BLK);  // [KS][32] A fragments of q
+    __shared__ float s_m[kKvAttnWarps][kKvAttnRows], s_l[kKvAttnWarps][kKvAttnRows];
+    __shared__ unsigned s_last;
+
+    int row0, q_len;
+    kv8_rows_of(a.r, seq, row0, q_len);
+    int kv_len = a.r.kv_len[seq];
+    if (rg * kKvAttnRows >= q_len * G) return;  // (uniform: every split of the group leaves here)
+    if ((kv_len + kKvBlock - 1) / kKvBlock > a.c.max_pages) {
+        if (threadIdx.x == 0) atomicExch(a.c.err, kErrKvPage);
+        kv_len = 0;
+    }
+    // this lane's row: token t of the call, head h
+    const int grow = rg * kKvAttnRows + g8;
+    const bool live = grow < q_len * G;
+    const int tok = live ? grow / G : 0, head = kh * G + (live ? grow % G : 0);
+    const int pos = live ? kv_len - q_len + tok : -1;  // the last key that the row sees (-1: none)
+    // keys that any row of this CTA sees, and keys that all of them see
+    const int tok_hi = min(rg * kKvAttnRows + kKvAttnRows - 1, q_len * G - 1) / G, tok_lo = rg * kKvAttnRows / G;
+    const int keys = max(0, min(kv_len, kv_len - q_len + tok_hi + 1)), keys_all = kv_len - q_len + tok_lo + 1;
+    const int full_blocks = min((keys + kKvBlock - 1) / kKvBlock, kv_len / kKvBlock);
+    const int open0 = kv_len / kKvBlock * kKvBlock;  // the first open token
+    const int open_units = keys > open0 ? (keys - open0 + 7) / 8 : 0;
+
+    // blocks of this warp: w, w + W, ...; page numbers and scales of 32 of them at a time, one per lane
+    const int W = a.splits * kKvAttnWarps, w = split * kKvAttnWarps + warp;
+    const int n_blocks = full_blocks > w ? (full_blocks - w + W - 1) / W : 0;
+    int page = -1;
+    float ks = 0.f, vs = 0.f;
+    auto fetch_pages = [&](int i0) {  // blocks i0 .. i0 + 31 of the warp's list
+        page = -1;
+        if (i0 + lane < n_blocks) page = kv8_page(a.c, seq, w + (i0 + lane) * W);
+        if (page >= 0) {
+            ks = a.c.k_scale[(int64_t)page * a.c.kv_heads + kh];
+            vs = a.c.v_scale[(int64_t)page * a.c.kv_heads + kh];
+        }
+    };
+    auto issue = [&](int i, int pg) {  // block i of the list into its stage (one group, empty past the end)
+        if (i < n_blocks && pg >= 0) {
+            uint8_t *dst = ring + i % ST * 2 * BLK;
+            const int64_t at = kv8_codes_at(a.c, pg, kh);
+            constexpr int RC = HD / 16;
+#pragma unroll
+            for (int u = 0; u < BLK / 16 / 32; ++u) {
+                const int x = u * 32 + lane, t = x / RC, c = x % RC;
+                cp16(dst + t * HD + k_chunk<HD>(c, t) * 16, a.c.k_codes + at + x * 16);
+            }
+#pragma unroll
+            for (int u = 0; u < BLK / 16 / 32; ++u) {
+                const int x = u * 32 + lane, t = x / RC, c = x % RC;
+                cp16(dst + BLK + t * HD + v_chunk<HD>(c, t) * 16, a.c.v_codes + at + x * 16);
+            }
+        }
+        cp_commit();
+    };
+    fetch_pages(0);
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) issue(i, __shfl_sync(0xffffffffu, page, i));
+
+    // q: two limbs per row, scaled by a power of two, as A fragments (warp 0 writes, all read)
+    float row_scale = 0.f;
+    {
+        float x[KS][4], amax = 0.f;
+        const T *q = static_cast<const T *>(a.q) + (int64_t)(row0 + tok) * a.q_stride + (int64_t)head * HD;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int d = k < 4 * G64 ? k / 4 * 64 + 16 * q4 + k % 4 * 4 : 64 * G64 + 8 * q4 + (k - 4 * G64) * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[k][i] = live ? load_f32<T>(q + d + i) : 0.f;
+                amax = fmaxf(amax, fabsf(x[k][i]));
+            }
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        float inv;
+        const float f = limb_scale(amax, inv);
+        row_scale = a.scale_log2 * inv;
+        if (warp == 0) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                uint4 u;
+                split_f16(x[k][0] * f, x[k][1] * f, u.x, u.y);  // rows g8 (upper limb), g8 + 8 (lower)
+                split_f16(x[k][2] * f, x[k][3] * f, u.z, u.w);
+                qf[k * 32 + lane] = u;
+            }
+        }
+    }
+    __syncthreads();
+
+    Acc<HD> acc;
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc.o[n][i] = 0.f;
+    acc.m = -INFINITY;
+    acc.l = 0.f;
+    acc.vref = 0.f;
+
+    for (int i = 0; i < n_blocks; ++i) {
+        const int pg = __shfl_sync(0xffffffffu, page, i & 31);
+        const float bk = __shfl_sync(0xffffffffu, ks, i & 31), bv = __shfl_sync(0xffffffffu, vs, i & 31);
+        {   // the block ST - 1 ahead; its page may be in the next batch, which is fetched when this one ends
+            const int nx = i + ST - 1;
+            int npg;
+            if ((nx & ~31) == (i & ~31))
+                npg = __shfl_sync(0xffffffffu, page, nx & 31);
+            else
+                npg = nx < n_blocks ? kv8_page(a.c, seq, w + nx * W) : -1;
+            cp_wait<ST - 2>();
+            __syncwarp();
+            issue(nx, npg);
+        }
+        if ((i & 31) == 31) fetch_pages(i + 1);
+        if (pg < 0) continue;
+        const uint8_t *kt = ring + i % ST * 2 * BLK, *vt = kt + BLK;
+
+        // scores of 32 tokens: n-tile n holds tokens 8 n .. 8 n + 7, this lane's column g8 of K
+        float c[4][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[n][j] = 0.f;
+#pragma unroll
+        for (int g = 0; g < G64; ++g) {
+            uint4 kw[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int t = 8 * n + g8;
+                kw[n] = *reinterpret_cast<const uint4 *>(kt + t * HD + k_chunk<HD>(4 * g + q4, t) * 16);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint4 qa = qf[(4 * g + j) * 32 + lane];
+                const uint32_t af[4] = {qa.x, qa.y, qa.z, qa.w};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t u = reinterpret_cast<const uint32_t *>(&kw[n])[j];
+                    mma16816(c[n], af, codes2(u, 0x4140), codes2(u, 0x4342));
+                }
+            }
+        }
+        if constexpr (REM != 0) {
+            uint2 kw[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                kw[n] = *reinterpret_cast<const uint2 *>(kt + (8 * n + g8) * HD + 64 * G64 + q4 * 8);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint4 qa = qf[(4 * G64 + j) * 32 + lane];
+                const uint32_t af[4] = {qa.x, qa.y, qa.z, qa.w};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t u = j ? kw[n].y : kw[n].x;
+                    mma16816(c[n], af, codes2(u, 0x4140), codes2(u, 0x4342));
+                }
+            }
+        }
+        const int key0 = (w + i * W) * kKvBlock;
+        const float f = bk * row_scale;
+        float s[4][2];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[n][e] = (c[n][e] + c[n][e + 2]) * f;
+        if (key0 + kKvBlock > keys_all) {  // some row does not see the whole block
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (key0 + 8 * n + 2 * q4 + e > pos) s[n][e] = -INFINITY;
+        }
+        uint32_t hi[4], lo[4];
+        acc.weights(s, bv, hi, lo);
+
+        // values: n-tile n's column g8 is dimension g8 * HD / 8 + n; the k-step's tokens are those of two
+        // score n-tiles, so the weights are already the A fragment
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const uint32_t af[4] = {hi[2 * kk], lo[2 * kk], hi[2 * kk + 1], lo[2 * kk + 1]};
+            const int t0 = 16 * kk + 2 * q4;
+            constexpr int WD = HD / 32;  // 4-byte words per lane and row
+            constexpr int WC = WD % 4 == 0 ? 4 : WD % 2 == 0 ? 2 : 1;
+#pragma unroll
+            for (int x = 0; x < WD; x += WC) {
+                uint32_t r[4][WC];  // rows t0, t0 + 1, t0 + 8, t0 + 9
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int t = t0 + (y & 1) + (y >> 1) * 8, byte = g8 * (HD / 8) + 4 * x;
+                    const uint8_t *p = vt + t * HD + v_chunk<HD>(byte / 16, t) * 16 + byte % 16;
+                    if constexpr (WC == 4) {
+                        const uint4 z = *reinterpret_cast<const uint4 *>(p);
+                        r[y][0] = z.x, r[y][1] = z.y, r[y][2] = z.z, r[y][3] = z.w;
+                    } else if constexpr (WC == 2) {
+                        const uint2 z = *reinterpret_cast<const uint2 *>(p);
+                        r[y][0] = z.x, r[y][1] = z.y;
+                    } else {
+                        r[y][0] = *reinterpret_cast<const uint32_t *>(p);
+                    }
+                }
+#pragma unroll
+                for (int z = 0; z < WC; ++z) {
+                    const uint32_t a01 = __byte_perm(r[0][z], r[1][z], 0x5140), a23 = __byte_perm(r[0][z], r[1][z], 0x7362);
+                    const uint32_t b01 = __byte_perm(r[2][z], r[3][z], 0x5140), b23 = __byte_perm(r[2][z], r[3][z], 0x7362);
+                    const int n = 4 * (x + z);
+                    mma16816(acc.o[n], af, codes2(a01, 0x4140), codes2(b01, 0x4140));
+                    mma16816(acc.o[n + 1], af, codes2(a01, 0x4342), codes2(b01, 0x4342));
+                    mma16816(acc.o[n + 2], af, codes2(a23, 0x4140), codes2(b23, 0x4140));
+                    mma16816(acc.o[n + 3], af, codes2(a23, 0x4342), codes2(b23, 0x4342));
+                }
+            }
+        }
+    }
+    cp_wait<0>();
+
+    // Open rows: units of 8 tokens, given to the warps with the fewest blocks; K and V split into two limbs
+    // like q.  A token with a NaN or infinity gives NaN to the rows that see it and nothing to the others.
+    for (int u = W - 1 - w; u < open_units; u += W) {
+        const int slot = kv8_slot(a.c, seq);
+        if (slot < 0) break;
+        const int64_t at = kv8_open_at(a.c, slot, open0 / kKvBlock, kh) + (int64_t)u * 8 * HD;
+        const int key0 = open0 + 8 * u, there = min(8, kv_len - key0);
+        unsigned bad = 0;
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        float kinv;
+        {
+            float x[KS][4], amax = 0.f;
+            const float *k = a.c.k_open + at + g8 * HD;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = s < 4 * G64 ? s / 4 * 64 + 16 * q4 + s % 4 * 4 : 64 * G64 + 8 * q4 + (s - 4 * G64) * 4;
+                const float4 z = g8 < there ? *reinterpret_cast<const float4 *>(k + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                x[s][0] = z.x, x[s][1] = z.y, x[s][2] = z.z, x[s][3] = z.w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!(fabsf(x[s][i]) < INFINITY)) {
+                        bad |= 1u << g8;
+                        x[s][i] = 0.f;
+                    }
+                    amax = fmaxf(amax, fabsf(x[s][i]));
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const float f = limb_scale(amax, kinv);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const uint4 qa = qf[s * 32 + lane];
+                const uint32_t af[4] = {qa.x, qa.y, qa.z, qa.w};
+                uint32_t h0, l0, h1, l1;
+                split_f16(x[s][0] * f, x[s][1] * f, h0, l0);
+                split_f16(x[s][2] * f, x[s][3] * f, h1, l1);
+                mma16816(c, af, h0, h1);
+                mma16816(c, af, l0, l1);
+            }
+        }
+        float v[2][HD / 8], vmax = 0.f, vinv;
+        const float *vp = a.c.v_open + at + g8 * (HD / 8);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const int t = 2 * q4 + y;
+#pragma unroll
+            for (int n = 0; n < HD / 8; n += 4) {
+                const float4 z =
+                    t < there ? *reinterpret_cast<const float4 *>(vp + t * HD + n) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[y][n] = z.x, v[y][n + 1] = z.y, v[y][n + 2] = z.z, v[y][n + 3] = z.w;
+            }
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) {
+                if (!(fabsf(v[y][n]) < INFINITY)) {
+                    bad |= 1u << t;
+                    v[y][n] = 0.f;
+                }
+                vmax = fmaxf(vmax, fabsf(v[y][n]));
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+        const float vf = limb_scale(vmax, vinv);
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        float s[1][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int t = 2 * q4 + e;
+            // (q times 2^10 .. 2^11 and k too: the product of the two inverse scales may leave the range)
+            s[0][e] = (c[e] + c[e + 2]) * kinv * row_scale;
+            if (bad >> t & 1) s[0][e] = __int_as_float(0x7FC00000);
+            if (key0 + t > pos) s[0][e] = -INFINITY;
+        }
+        uint32_t hi[1], lo[1];
+        acc.weights(s, vinv, hi, lo);
+        const uint32_t af[4] = {hi[0], lo[0], 0u, 0u};
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+            uint32_t h, l;
+            split_f16(v[0][n] * vf, v[1][n] * vf, h, l);
+            mma16816(acc.o[n], af, h, 0u);
+            mma16816(acc.o[n], af, l, 0u);
+        }
+    }
+
+    // warps: [warp][row][HD] in the ring's memory
+    float l = acc.l + __shfl_xor_sync(0xffffffffu, acc.l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    __syncthreads();
+    float *so = reinterpret_cast<float *>(sm);
+    {
+        const float f = acc.vref * (1.0f / kPScale);
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                so[(warp * kKvAttnRows + g8) * HD + (2 * q4 + e) * (HD / 8) + n] = (acc.o[n][e] + acc.o[n][e + 2]) * f;
+        if (q4 == 0) {
+            s_m[warp][g8] = acc.m;
+            s_l[warp][g8] = l;
+        }
+    }
+    __syncthreads();
+    const int64_t group = ((int64_t)seq * a.row_groups + rg) * a.c.kv_heads + kh;
+    constexpr int PR = HD + 2;  // a partial's row: sums, maximum, total
+    auto finish = [&](int r, int d, float o, float total) {
+        const int gr = rg * kKvAttnRows + r;
+        if (gr >= q_len * G) return;
+        const int64_t row = row0 + gr / G;
+        const int h = kh * G + gr % G;
+        float v = total == 0.f ? 0.f : o / total;  // a row that sees no key: zeros (a NaN total: NaN)
+        if (a.gate != nullptr) {
+            const float g = load_f32<T>(static_cast<const T *>(a.gate) + row * a.gate_stride + (int64_t)h * HD + d);
+            v *= 1.0f / (1.0f + expf(-g));
+        }
+        store_f32(static_cast<T *>(a.out) + row * a.out_stride + (int64_t)h * HD + d, v);
+    };
+    for (int x = threadIdx.x; x < kKvAttnRows * HD; x += kThreads) {
+        const int r = x / HD, d = x % HD;
+        float m = -INFINITY, o = 0.f, t = 0.f;
+#pragma unroll
+        for (int y = 0; y < kKvAttnWarps; ++y) m = fmaxf(m, s_m[y][r]);
+#pragma unroll
+        for (int y = 0; y < kKvAttnWarps; ++y) {
+            const float f = part_factor(s_m[y][r], s_l[y][r], m);
+            o += f == 0.f ? 0.f : so[(y * kKvAttnRows + r) * HD + d] * f;
+            t += f == 0.f ? 0.f : s_l[y][r] * f;
+        }
+        if (a.splits == 1) {
+            finish(r, d, o, t);
+        } else {
+            float *p = a.part + ((group * a.splits + split) * kKvAttnRows + r) * PR;
+            p[d] = o;
+            if (d == 0) {
+                p[HD] = m;
+                p[HD + 1] = t;
+            }
+        }
+    }
+    if (a.splits == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) s_last = atomicAdd(a.arrivals + group, 1u) == (unsigned)a.splits - 1;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    for (int x = threadIdx.x; x < kKvAttnRows * HD; x += kThreads) {
+        const int r = x / HD, d = x % HD;
+        const float *p = a.part + (group * a.splits * kKvAttnRows + r) * PR;
+        float m = -INFINITY, o = 0.f, t = 0.f;
+        for (int y = 0; y < a.splits; ++y) m = fmaxf(m, __ldcg(p + (int64_t)y * kKvAttnRows * PR + HD));
+        for (int y = 0; y < a.splits; ++y) {
+            const float *z = p + (int64_t)y * kKvAttnRows * PR;
+            const float pm = __ldcg(z + HD), pt = __ldcg(z + HD + 1);
+            const float f = part_factor(pm, pt, m);
+            o += f == 0.f ? 0.f : __ldcg(z + d) * f;
+            t += f == 0.f ? 0.f : pt * f;
+        }
+        finish(r, d, o, t);
+    }
+    if (threadIdx.x == 0) a.arrivals[group] = 0;
+}
+
+template <typename T, int HD>
+cudaError_t launch_hd(const Kv8AttnArgs &a, cudaStream_t s) {
+    const int smem = kKvAttnWarps * stages(HD) * 2 * kKvBlock * HD + HD / 16 * 32 * 16;
+    cudaError_t e = cudaFuncSetAttribute(attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    attn_kernel<T, HD><<<dim3(a.splits, a.c.kv_heads * a.row_groups, a.c.n_seqs), kThreads, smem, s>>>(a);
+    return cudaGetLastError();
+}
+template <typename T>
+cudaError_t launch_t(const Kv8AttnArgs &a, cudaStream_t s) {
+    switch (a.c.head_dim) {
+        case 32: return launch_hd<T, 32>(a, s);
+        case 64: return launch_hd<T, 64>(a, s);
+        case 96: return launch_hd<T, 96>(a, s);
+        case 128: return launch_hd<T, 128>(a, s);
+        case 160: return launch_hd<T, 160>(a, s);
+        case 192: return launch_hd<T, 192>(a, s);
+        case 224: return launch_hd<T, 224>(a, s);
+        default: return launch_hd<T, 256>(a, s);
+    }
+}
+}  // namespace
+
+int kv8_attn_ctas_per_sm(int head_dim) { return ctas_per_sm(head_dim); }
+
+cudaError_t kv8_attn_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s) {
+    return bf16 ? launch_t<__nv_bfloat16>(a, s) : launch_t<float>(a, s);
+}
+
+}  // namespace ql

@@ -40,6 +40,7 @@ extern "C" {
 #define QL_Q8_0 8
 #define QL_Q4_K 12
 #define QL_Q6_K 14
+#define QL_BF16 30 /* activations of the ql_kv8_* calls only */
 
 /* Status codes. */
 #define QL_OK 0
@@ -278,6 +279,95 @@ QL_API int ql_full_attention_attend(const float *q, const float *gate, const voi
 QL_API int ql_full_attention_attend_batch(const float *q, const float *gate, const void *key_cache,
                                           const void *value_cache, int kv_bf16, float *attn, int tokens, int n_heads,
                                           int kv_heads, int head_dim, int max_seq_len, int start_pos);
+
+/* ---- 8-bit KV cache (no reference twin; the reference's cache is f32 or bf16, read by
+ *      ql_full_attention_attend) --------------------------------------------------------
+ * What a serving step does between the q/k/v projection and the attention's output, over a paged
+ * cache of one byte per value.  A page holds QL_KV8_BLOCK tokens of every KV head; a full page has one
+ * f32 scale per KV head for K and one for V:
+ *   scale = max|x| / 127 over the page's tokens and the head's dimensions, byte = rint(x / scale) + 128
+ * (scale 0: bytes 128; a page that holds NaN or infinity has a NaN scale).  The tokens of a sequence's
+ * last, unfinished page are exact: their rows stand in f32 in the "open" rows, from which the page is
+ * quantised once, when it is full.  So the bytes do not depend on how a sequence was cut into calls, and
+ * since the open rows hold the last two pages, kv_len may go back by up to QL_KV8_BLOCK tokens (rejected
+ * speculative tokens) between calls.
+ * All buffers are the caller's device memory; every base is 16-byte aligned.  head_dim: a multiple of 32
+ * up to 256; activations f32 (QL_F32) or bf16 (QL_BF16).  kv_len, q_start, page_table and slots are read
+ * on the device, so a captured CUDA graph follows them.  A page, slot, length or position outside the
+ * given extents is not accessed, and is reported by the next ql_check_device (QL_EDEVICE). */
+#define QL_KV8_BLOCK 32
+typedef struct ql_kv8_cache {
+    uint8_t *k_codes, *v_codes;  /* [n_pages][kv_heads][QL_KV8_BLOCK][head_dim] */
+    float *k_scale, *v_scale;    /* [n_pages][kv_heads] */
+    float *k_open, *v_open;      /* [n_slots][2][kv_heads][QL_KV8_BLOCK][head_dim]; page b of a sequence in [b % 2] */
+    const int32_t *page_table;   /* [n_seqs][max_pages] */
+    const int32_t *slots;        /* [n_seqs] open rows of each sequence; NULL: sequence s has slot s */
+    int32_t n_pages, n_slots, n_seqs, max_pages, kv_heads, head_dim;
+} ql_kv8_cache;
+/* Rows of a call.  q_start == NULL: row s is the one new token of sequence s (rows == n_seqs).  Otherwise
+ * sequence s has rows q_start[s] .. q_start[s + 1] - 1 (q_start[0] = 0, q_start[n_seqs] = rows; none is
+ * allowed), at most max_q_len.  kv_len[s] counts the sequence's tokens with this call's among them: its
+ * last row has position kv_len[s] - 1.  kv_len[s] == 0: an idle sequence, its row is skipped.
+ *
+ * ql_kv8_append: per head, q and k are normalised and rotated, k and v stored into the cache.
+ *   norm (gamma != NULL): x / sqrt(mean(x^2) + eps) * gamma, gamma [head_dim] f32;
+ *   rotation of the first rotary_dim elements (0: none; a multiple of head_dim / 16), pairs (i, i +
+ *   rotary_dim / 2) as elsewhere here, by rope [max_positions][rotary_dim] f32 on the device: the cosines
+ *   of the position's rotary_dim / 2 angles, then their sines.
+ * Row r of q: n_heads heads of head_dim elements from q + r * q_stride (elements), k and v kv_heads heads
+ * in the same way, so the stacked output of one projection serves all three; q_out likewise, of the same
+ * type, and may be q.  q == NULL (n_heads 0): k and v only.  One launch. */
+QL_API int ql_kv8_append(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *k,
+                         int64_t k_stride, const void *v, int64_t v_stride, void *q_out, int64_t q_out_stride,
+                         int n_heads, const float *q_gamma, const float *k_gamma, float eps, const float *rope,
+                         int rotary_dim, int max_positions, const int32_t *kv_len, const int32_t *q_start, int rows,
+                         int max_q_len);
+/* Causal attention of the call's rows over the cache (after ql_kv8_append):
+ *   out_h = softmax_j(scale q_h . k_j) . v_j [* sigmoid(gate_h)],  j = 0 .. the row's position,
+ * query head h reads KV head h / (n_heads / kv_heads).  gate == NULL: none.  A row that sees no key gets
+ * zeros; one that sees a NaN or infinity gets NaN.  f32: fp32 results (1e-6); bf16: operands and weights of
+ * 16 bits, sums of 32.  max_q_len and max_kv_len bound the lengths on the device (a longer sequence is
+ * read whole all the same; they size the launch).  The workspace, ql_kv8_attend_workspace bytes, 16-byte
+ * aligned, is zeroed by the caller before its first use and left usable by every call; calls that may
+ * overlap on the GPU need one each. */
+QL_API size_t ql_kv8_attend_workspace(int n_heads, int kv_heads, int head_dim, int n_seqs, int rows, int max_q_len,
+                                      int max_kv_len);
+QL_API int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *gate,
+                         int64_t gate_stride, void *out, int64_t out_stride, int n_heads, float scale,
+                         const int32_t *kv_len, const int32_t *q_start, int rows, int max_q_len, int max_kv_len,
+                         void *workspace, size_t workspace_bytes);
+/* The cache's values back: k_out and v_out [n_seqs][count][kv_heads][head_dim] of `type` (either may be
+ * NULL), positions start[s] .. start[s] + count - 1 of sequence s (start == NULL: from 0), zeros where the
+ * sequence has none.  E.g. to move a sequence to the bf16 cache of ql_full_attention_attend. */
+QL_API int ql_kv8_gather(const ql_kv8_cache *cache, int32_t type, void *k_out, void *v_out, const int32_t *start,
+                         int count, const int32_t *kv_len);
+
+/* ---- rules on logits (no reference twin; the reference samples from raw logits, Sampler.cpp:24-50) ---
+ * Any pointer but history_len and bias_start (which go with history and bias_ids) may be NULL: that rule
+ * is off.  All are device pointers. */
+typedef struct ql_logits_rules {
+    const int32_t *history;      /* [rows][history_stride] token ids: the prompt, then what was generated; */
+    int64_t history_stride;      /*   ids outside [0, vocab) are ignored */
+    const int32_t *history_len;  /* [rows] */
+    const int32_t *prompt_len;   /* [rows] leading ids that are the prompt; NULL: none */
+    const float *repetition;     /* [rows] > 0: x / r where x > 0, else x * r, for ids anywhere in the history */
+    const float *frequency;      /* [rows]: minus frequency times the number of generated occurrences */
+    const float *presence;       /* [rows]: minus presence for generated ids */
+    const int32_t *bias_ids;     /* added to ids bias_ids[bias_start[r] .. bias_start[r + 1]); an id listed */
+    const float *bias_values;    /*   twice gets both, in list order */
+    const int32_t *bias_start;   /* [rows + 1] */
+    const uint32_t *mask;        /* [mask_rows][mask_stride] words: bit t % 32 of word t / 32 allows token t, */
+    int64_t mask_stride;         /*   0 sets it to -inf */
+    int32_t mask_rows;
+    const int32_t *mask_row;     /* [rows] mask of each row, < 0: none; NULL: mask r for row r */
+} ql_logits_rules;
+/* out = the rules applied to logits in the order above, each step rounded once to f32; rows logits_stride
+ * and out_stride floats apart; out may be logits (same stride) or NULL.  token (nullable): [rows] the
+ * greedy token, lowest id among equals, NaN never; -1 where nothing is above -inf.  With token != NULL the
+ * workspace has 16 bytes per row, zeroed by the caller before its first use and left zero by every call. */
+QL_API int ql_logits_apply(const float *logits, int64_t logits_stride, float *out, int64_t out_stride, int rows,
+                           int vocab, const ql_logits_rules *rules, int32_t *token, void *workspace,
+                           size_t workspace_bytes);
 
 /* ---- opt-in int8 activation path, Q8_1 (reference kernel.cuh:47-52) -------------------
  * Changes numerics (activations rounded to int8 per 32), as in the reference, which keeps it off
