@@ -1392,8 +1392,9 @@ int ql_logits_apply(const float *logits, int64_t logits_stride, float *out, int6
         if (out == logits && out_stride != logits_stride) return fail(QL_EINVAL, what + ": in place the strides are the same");
         if (reinterpret_cast<uintptr_t>(logits) % 4 || reinterpret_cast<uintptr_t>(out) % 4)
             return fail(QL_EINVAL, what + ": misaligned logits or out");
-        if (rules->history && (!rules->history_len || rules->history_stride < 0 || rules->history_stride > INT32_MAX))
-            return fail(QL_EINVAL, what + ": a history needs history_len and a stride");
+        if (rules->history && (!rules->history_len || rules->history_stride < 0 ||
+                               rules->history_stride > (int64_t)kLogitsMaxHistory))
+            return fail(QL_EINVAL, what + ": a history needs history_len and a stride of at most 1048575 ids");
         if (rules->bias_ids && (!rules->bias_values || !rules->bias_start))
             return fail(QL_EINVAL, what + ": biases need bias_values and bias_start");
         if (rules->mask && (rules->mask_rows < 0 || rules->mask_stride < ((int64_t)vocab + 31) / 32 ||

@@ -4,6 +4,8 @@
 
 namespace ql {
 
+constexpr uint32_t kLogitsMaxHistory = (1u << 20) - 1;  // ids per row
+
 struct LogitsArgs {
     const float *logits;
     float *out;  // null: the token only

@@ -347,7 +347,7 @@ QL_API int ql_kv8_gather(const ql_kv8_cache *cache, int32_t type, void *k_out, v
  * is off.  All are device pointers. */
 typedef struct ql_logits_rules {
     const int32_t *history;      /* [rows][history_stride] token ids: the prompt, then what was generated; */
-    int64_t history_stride;      /*   ids outside [0, vocab) are ignored */
+    int64_t history_stride;      /*   ids outside [0, vocab) are ignored; at most 1048575 ids a row */
     const int32_t *history_len;  /* [rows] */
     const int32_t *prompt_len;   /* [rows] leading ids that are the prompt; NULL: none */
     const float *repetition;     /* [rows] > 0: x / r where x > 0, else x * r, for ids anywhere in the history */
