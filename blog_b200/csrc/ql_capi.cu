@@ -1286,7 +1286,7 @@ int ql_kv8_append(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         if ((st = kv8_operand(k, k_stride, (int64_t)a.c.kv_heads * hd, type, "k", what)) ||
             (st = kv8_operand(v, v_stride, (int64_t)a.c.kv_heads * hd, type, "v", what)))
             return st;
-        const int64_t ctas = ((int64_t)rows * n_heads + 7) / 8 + ((int64_t)rows + 2 * (int64_t)a.c.n_seqs) * a.c.kv_heads * 2;
+        const int64_t ctas = (int64_t)rows * ((n_heads + 7) / 8) + ((int64_t)rows + 2 * (int64_t)a.c.n_seqs) * a.c.kv_heads * 2;
         if (ctas > INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
         Workspace *ws = workspace(&st);
         if (!ws) return st;
@@ -1367,7 +1367,7 @@ int ql_kv8_gather(const ql_kv8_cache *cache, int32_t type, void *k_out, void *v_
         if (!kv_len) return fail(QL_EINVAL, what + ": null kv_len");
         if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16)
             return fail(QL_EINVAL, what + ": outputs must be 16-byte aligned");
-        if ((int64_t)c.n_seqs * count * c.kv_heads * 2 / 8 >= INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
+        if ((int64_t)c.n_seqs * count * c.kv_heads * (c.head_dim / 16) / 256 >= INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
         Workspace *ws = workspace(&st);
         if (!ws) return st;
         c.err = ws->err;

@@ -77,9 +77,15 @@ __device__ __forceinline__ void store_row(T *p, const float *x) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             P w;
-            T *e = reinterpret_cast<T *>(&w);
+            if constexpr (sizeof(T) == 2 && PE % 2 == 0) {
+                __nv_bfloat162 *e = reinterpret_cast<__nv_bfloat162 *>(&w);
 #pragma unroll
-            for (int j = 0; j < PE; ++j) e[j] = from_f32<T>(x[i * PE + j]);
+                for (int j = 0; j < PE / 2; ++j) e[j] = __floats2bfloat162_rn(x[i * PE + 2 * j], x[i * PE + 2 * j + 1]);
+            } else {
+                T *e = reinterpret_cast<T *>(&w);
+#pragma unroll
+                for (int j = 0; j < PE; ++j) e[j] = from_f32<T>(x[i * PE + j]);
+            }
             reinterpret_cast<P *>(p)[i] = w;
         }
     } else {
@@ -88,36 +94,47 @@ __device__ __forceinline__ void store_row(T *p, const float *x) {
     }
 }
 
-// Norm (gamma non-null) and rotation of one row spread over a warp, V consecutive elements per lane.
-// cs: the position's cosines and sines, or null.  rotary_dim / 2 is a multiple of V, so an element and
-// its partner have the same index in two lanes.
+// What a lane needs of a position's rotation: the cosines and sines of its V elements, the lane that holds
+// their partners (the same index there: rotary_dim / 2 is a multiple of V) and the sign of the partner's term.
 template <int V>
-__device__ __forceinline__ void norm_rope(float *x, const float *gamma, float eps, const float *cs, int rotary_dim,
-                                          int lane) {
-    if (gamma != nullptr) {
-        float g[V];
-        load_row<V, false>(g, gamma + lane * V);
+struct Rotation {
+    float c[V], s[V];
+    int partner;
+    bool in;
+    __device__ __forceinline__ void load(const float *cs, int rotary_dim, int lane) {
+        const int hl = rotary_dim / (2 * V);  // lanes [0, hl): first halves; [hl, 2 hl): second
+        const bool first = lane < hl;
+        in = cs != nullptr && lane < 2 * hl;
+        partner = in ? (first ? lane + hl : lane - hl) : lane;
+        const int at = (first ? lane : lane - hl) * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            c[i] = in ? cs[at + i] : 1.f;
+            const float z = in ? cs[rotary_dim / 2 + at + i] : 0.f;
+            s[i] = first ? -z : z;
+        }
+    }
+};
+
+// Norm (gamma non-null: the lane's g) and rotation of one row spread over a warp, V consecutive elements per
+// lane.
+template <int V>
+__device__ __forceinline__ void norm_rope(float *x, bool norm, const float *g, float eps, bool rotate, const Rotation<V> &r) {
+    if (norm) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < V; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float r = 1.0f / sqrtf(ss * (1.0f / (32 * V)) + eps);
+        const float f = rsqrtf(fmaf(ss, 1.0f / (32 * V), eps));
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = x[i] * r * g[i];
+        for (int i = 0; i < V; ++i) x[i] = x[i] * f * g[i];
     }
-    if (cs != nullptr) {
-        const int half = rotary_dim / 2, hl = half / V;  // lanes [0, hl): first halves; [hl, 2 hl): second
-        const bool first = lane < hl, in = lane < 2 * hl;
-        const int partner = in ? (first ? lane + hl : lane - hl) : lane;
-        const int at = (first ? lane : lane - hl) * V;
+    if (rotate) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float o = __shfl_sync(0xffffffffu, x[i], partner);
-            if (in) {
-                const float c = cs[at + i], s = cs[half + at + i];
-                x[i] = first ? x[i] * c - o * s : x[i] * c + o * s;
-            }
+            const float o = __shfl_sync(0xffffffffu, x[i], r.partner);
+            if (r.in) x[i] = fmaf(o, r.s[i], x[i] * r.c[i]);
         }
     }
 }
@@ -144,7 +161,9 @@ __device__ void append_block(const Kv8AppendArgs &a, bool is_v, int seq, int slo
     const T *src = static_cast<const T *>(is_v ? a.v : a.k) + (int64_t)kh * HD + lane * V;
     const int64_t stride = is_v ? a.v_stride : a.k_stride;
     float *open = (is_v ? a.c.v_open : a.c.k_open) + kv8_open_at(a.c, slot, block, kh) + lane * V;
-    float x[kRowsPerWarp][V];
+    float x[kRowsPerWarp][V], g[V];
+    const bool norm = !is_v && a.k_gamma != nullptr, rotate = !is_v && a.rotary_dim > 0;
+    if (norm) load_row<V, false>(g, a.k_gamma + lane * V);
 #pragma unroll
     for (int u = 0; u < kRowsPerWarp; ++u) {
         const int t = warp + u * kWarps, pos = base + t;
@@ -161,7 +180,9 @@ __device__ void append_block(const Kv8AppendArgs &a, bool is_v, int seq, int slo
     for (int u = 0; u < kRowsPerWarp; ++u) {
         const int t = warp + u * kWarps, pos = base + t;
         if (pos < pos0 || pos >= kv_len) continue;
-        if (!is_v) norm_rope<V>(x[u], a.k_gamma, a.eps, rope_row(a, pos), a.rotary_dim, lane);
+        Rotation<V> rot;
+        if (rotate) rot.load(rope_row(a, pos), a.rotary_dim, lane);
+        norm_rope<V>(x[u], norm, g, a.eps, rotate, rot);
         if (keep) store_row<V, true>(open + t * HD, x[u]);
     }
     if (!full) return;
@@ -185,43 +206,64 @@ __device__ void append_block(const Kv8AppendArgs &a, bool is_v, int seq, int slo
     const int page = kv8_page(a.c, seq, block);
     if (page < 0) return;
     uint8_t *codes = (is_v ? a.c.v_codes : a.c.k_codes) + kv8_codes_at(a.c, page, kh) + lane * V;
+    // rint(x / scale): the quotient from the block's one reciprocal and a residual step, which rounds it
+    // correctly (P. Markstein, 1990; ties of bf16 values are common and go by the last bit), then 1.5 x 2^23
+    // added, which rounds to an integer, half to even, with the code in the low byte.  Scales near the ends of
+    // the range are divided by.
+    const float inv = 1.0f / scale;
+    const bool divide = !(scale > 1e-30f && scale < 1e30f);
 #pragma unroll
     for (int u = 0; u < kRowsPerWarp; ++u) {
         const int t = warp + u * kWarps;
         constexpr int PB = piece_bytes(V);
         using P = typename Piece<PB>::type;
-        uint8_t c[V];
+        uint32_t c[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const float r = scale > 0.f ? fminf(fmaxf(rintf(x[u][i] / scale), -127.f), 127.f) : 0.f;
-            c[i] = (uint8_t)((int)r + 128);
+            float r = x[u][i] * inv;
+            r = divide ? (scale > 0.f ? x[u][i] / scale : 0.f) : fmaf(fmaf(-r, scale, x[u][i]), inv, r);
+            c[i] = __float_as_uint(r + 12582912.0f) ^ 0x80u;
         }
 #pragma unroll
         for (int i = 0; i < V / PB; ++i) {
             P w;
-            uint8_t *e = reinterpret_cast<uint8_t *>(&w);
+            if constexpr (PB >= 4) {
+                uint32_t *e = reinterpret_cast<uint32_t *>(&w);
 #pragma unroll
-            for (int j = 0; j < PB; ++j) e[j] = c[i * PB + j];
+                for (int j = 0; j < PB / 4; ++j) {
+                    const uint32_t *z = c + i * PB + 4 * j;
+                    e[j] = __byte_perm(__byte_perm(z[0], z[1], 0x0040), __byte_perm(z[2], z[3], 0x0040), 0x5410);
+                }
+            } else {
+                uint8_t *e = reinterpret_cast<uint8_t *>(&w);
+#pragma unroll
+                for (int j = 0; j < PB; ++j) e[j] = (uint8_t)c[i * PB + j];
+            }
             reinterpret_cast<P *>(codes + (int64_t)t * HD)[i] = w;
         }
     }
     if (threadIdx.x == 0) (is_v ? a.c.v_scale : a.c.k_scale)[(int64_t)page * a.c.kv_heads + kh] = scale;
 }
 
-// Grid: [0, q_ctas): query heads, a warp per (row, head); then a CTA per (tile, KV head, K or V).  With
-// q_start, tile t belongs to the sequence s with start(s) <= t < start(s + 1), start(s) = q_start[s] / 32 +
+// Grid: [0, q_ctas): query heads, a warp per row and HPW heads of it; then a CTA per (tile, KV head, K or V).
+// With q_start, tile t belongs to the sequence s with start(s) <= t < start(s + 1), start(s) = q_start[s] / 32 +
 // 2 s: a sequence of n rows touches at most floor(n / 32) + 2 blocks, and start(s + 1) - start(s) is at
 // least that, so every block has a tile.
-template <typename T, int V, bool VEC>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ Kv8AppendArgs a, int q_ctas) {
+template <typename T, int V, bool VEC, int HPW>
+__global__ void __launch_bounds__(kThreads, V <= 4 ? 5 : 3) append_kernel(const __grid_constant__ Kv8AppendArgs a, int q_ctas) {
     constexpr int HD = 32 * V;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if ((int)blockIdx.x < q_ctas) {
-        const int64_t task = (int64_t)blockIdx.x * kWarps + warp;
-        const int row = (int)(task / a.n_heads), h = (int)(task - (int64_t)row * a.n_heads);
-        if (row >= a.r.rows) return;
-        float x[V];
-        load_row<V, VEC>(x, static_cast<const T *>(a.q) + (int64_t)row * a.q_stride + (int64_t)h * HD + lane * V);
+        const int per_row = (a.n_heads + HPW * kWarps - 1) / (HPW * kWarps);  // CTAs
+        const int row = blockIdx.x / per_row, h0 = ((blockIdx.x - row * per_row) * kWarps + warp) * HPW;
+        if (h0 >= a.n_heads) return;
+        float x[HPW][V], g[V];
+        const T *q = static_cast<const T *>(a.q) + (int64_t)row * a.q_stride + (int64_t)h0 * HD + lane * V;
+#pragma unroll
+        for (int u = 0; u < HPW; ++u)
+            if (h0 + u < a.n_heads) load_row<V, VEC>(x[u], q + u * HD);
+        const bool norm = a.q_gamma != nullptr;
+        if (norm) load_row<V, false>(g, a.q_gamma + lane * V);
         int seq = row, left = 1;  // rows of the sequence from this one on
         if (a.r.q_start != nullptr) {
             seq = kv8_seq_of_row(a.r.q_start, a.c.n_seqs, row, lane);
@@ -229,8 +271,15 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
         }
         const int pos = a.r.kv_len[seq] - left;
         if (pos < 0) return;  // an empty sequence (a length below its rows is recorded by the cache's CTAs)
-        norm_rope<V>(x, a.q_gamma, a.eps, rope_row(a, pos), a.rotary_dim, lane);
-        store_row<V, VEC>(static_cast<T *>(a.q_out) + (int64_t)row * a.q_out_stride + (int64_t)h * HD + lane * V, x);
+        Rotation<V> rot;
+        if (a.rotary_dim > 0) rot.load(rope_row(a, pos), a.rotary_dim, lane);
+        T *o = static_cast<T *>(a.q_out) + (int64_t)row * a.q_out_stride + (int64_t)h0 * HD + lane * V;
+#pragma unroll
+        for (int u = 0; u < HPW; ++u)
+            if (h0 + u < a.n_heads) {
+                norm_rope<V>(x[u], norm, g, a.eps, a.rotary_dim > 0, rot);
+                store_row<V, VEC>(o + u * HD, x[u]);
+            }
         return;
     }
     __shared__ float red[kWarps];
@@ -285,68 +334,68 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 }
 
 // Rows start .. start + count - 1 of every sequence, [n_seqs][count][kv_heads][head_dim]; positions outside
-// the sequence give zeros.  A warp per (position, KV head, K or V).
-template <typename T, int V>
+// the sequence give zeros.  A thread per 16 values of K or of V.
+template <typename T>
 __global__ void __launch_bounds__(kThreads) gather_kernel(const __grid_constant__ Kv8View c, const int *kv_len,
-                                                          const int *start, int count, T *k_out, T *v_out) {
-    constexpr int HD = 32 * V;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t tasks = (int64_t)c.n_seqs * count * c.kv_heads * 2;
-    const int64_t task = (int64_t)blockIdx.x * kWarps + warp;
-    if (task >= tasks) return;
-    const bool is_v = task >= tasks / 2;
-    const int64_t row = is_v ? task - tasks / 2 : task;  // (seq, i, kh)
+                                                          const int *start, int count, T *k_out, T *v_out, int64_t pieces) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const bool is_v = blockIdx.y != 0;
     T *out = is_v ? v_out : k_out;
-    if (out == nullptr) return;
-    const int kh = (int)(row % c.kv_heads);
+    if (i >= pieces || out == nullptr) return;
+    const int per = c.head_dim / 16;
+    const int64_t row = i / per;  // (seq, token, kh)
+    const int at = (int)(i - row * per) * 16, kh = (int)(row % c.kv_heads);
     const int64_t si = row / c.kv_heads;
     const int seq = (int)(si / count);
-    const int64_t pos64 = (int64_t)(start != nullptr ? start[seq] : 0) + si % count;
+    const int64_t pos64 = (int64_t)(start != nullptr ? start[seq] : 0) + (si - (int64_t)seq * count);
     const int len = kv_len[seq];
-    float x[V];
+    float x[16];
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = 0.f;
+    for (int j = 0; j < 16; ++j) x[j] = 0.f;
     if (pos64 >= 0 && pos64 < len) {
         const int pos = (int)pos64, block = pos / kKvBlock, t = pos % kKvBlock;
         if ((block + 1) * kKvBlock > len) {
             const int slot = kv8_slot(c, seq);
             if (slot >= 0)
-                load_row<V, true>(x, (is_v ? c.v_open : c.k_open) + kv8_open_at(c, slot, block, kh) + t * HD + lane * V);
+                load_row<16, true>(x, (is_v ? c.v_open : c.k_open) + kv8_open_at(c, slot, block, kh) + t * c.head_dim + at);
         } else {
             const int page = kv8_page(c, seq, block);
             if (page >= 0) {
-                const uint8_t *p = (is_v ? c.v_codes : c.k_codes) + kv8_codes_at(c, page, kh) + t * HD + lane * V;
+                const uint4 w = *reinterpret_cast<const uint4 *>((is_v ? c.v_codes : c.k_codes) + kv8_codes_at(c, page, kh) +
+                                                                 t * c.head_dim + at);
                 const float s = (is_v ? c.v_scale : c.k_scale)[(int64_t)page * c.kv_heads + kh];
-                constexpr int PB = piece_bytes(V);
-                using P = typename Piece<PB>::type;
+                const uint8_t *e = reinterpret_cast<const uint8_t *>(&w);
 #pragma unroll
-                for (int i = 0; i < V / PB; ++i) {
-                    const P w = reinterpret_cast<const P *>(p)[i];
-                    const uint8_t *e = reinterpret_cast<const uint8_t *>(&w);
-#pragma unroll
-                    for (int j = 0; j < PB; ++j) x[i * PB + j] = (float)((int)e[j] - 128) * s;
-                }
+                for (int j = 0; j < 16; ++j) x[j] = (float)((int)e[j] - 128) * s;
             }
         }
     }
-    store_row<V, true>(out + row * HD + lane * V, x);
+    store_row<16, true>(out + i * 16, x);
 }
 
+template <typename T, int V, bool VEC>
+cudaError_t append_hpw(const Kv8AppendArgs &a, cudaStream_t s) {
+    const int64_t tiles = a.r.q_start != nullptr ? a.r.rows / kKvBlock + 2 * (int64_t)a.c.n_seqs : a.r.rows;
+    const int64_t kv_ctas = tiles * a.c.kv_heads * 2;
+    // Heads per warp: 1 for single tokens, where the launch is as long as one warp's chain of loads; for
+    // prompts 4, whose loads are in flight together and share the row's cosines and sines.
+    const bool many = (int64_t)a.r.rows * a.n_heads >= 8192;
+    const int hpw = many ? 4 : 1;
+    const int64_t q_ctas = a.q != nullptr ? (int64_t)a.r.rows * ((a.n_heads + hpw * kWarps - 1) / (hpw * kWarps)) : 0;
+    if (many)
+        append_kernel<T, V, VEC, 4><<<(unsigned)(q_ctas + kv_ctas), kThreads, 0, s>>>(a, (int)q_ctas);
+    else
+        append_kernel<T, V, VEC, 1><<<(unsigned)(q_ctas + kv_ctas), kThreads, 0, s>>>(a, (int)q_ctas);
+    return cudaGetLastError();
+}
 template <typename T, int V>
 cudaError_t append_v(const Kv8AppendArgs &a, cudaStream_t s) {
-    const int64_t q_ctas = a.q != nullptr ? ((int64_t)a.r.rows * a.n_heads + kWarps - 1) / kWarps : 0;
-    const int64_t tiles = a.r.q_start != nullptr ? a.r.rows / kKvBlock + 2 * (int64_t)a.c.n_seqs : a.r.rows;
-    const int64_t grid = q_ctas + tiles * a.c.kv_heads * 2;
-    const size_t el = sizeof(T);
-    auto ok = [&](const void *p, int64_t stride) {
-        return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride * el) % 16 == 0);
+    auto ok = [](const void *p, int64_t stride) {
+        return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0);
     };
-    const bool vec = ok(a.q, a.q_stride) && ok(a.k, a.k_stride) && ok(a.v, a.v_stride) && ok(a.q_out, a.q_out_stride);
-    if (vec)
-        append_kernel<T, V, true><<<(unsigned)grid, kThreads, 0, s>>>(a, (int)q_ctas);
-    else
-        append_kernel<T, V, false><<<(unsigned)grid, kThreads, 0, s>>>(a, (int)q_ctas);
-    return cudaGetLastError();
+    return ok(a.q, a.q_stride) && ok(a.k, a.k_stride) && ok(a.v, a.v_stride) && ok(a.q_out, a.q_out_stride)
+               ? append_hpw<T, V, true>(a, s)
+               : append_hpw<T, V, false>(a, s);
 }
 template <typename T>
 cudaError_t append_t(const Kv8AppendArgs &a, cudaStream_t s) {
@@ -361,25 +410,12 @@ cudaError_t append_t(const Kv8AppendArgs &a, cudaStream_t s) {
         default: return append_v<T, 8>(a, s);
     }
 }
-template <typename T, int V>
-cudaError_t gather_v(const Kv8View &c, const int *kv_len, const int *start, int count, void *k, void *v, cudaStream_t s) {
-    const int64_t tasks = (int64_t)c.n_seqs * count * c.kv_heads * 2;
-    gather_kernel<T, V><<<(unsigned)((tasks + kWarps - 1) / kWarps), kThreads, 0, s>>>(
-        c, kv_len, start, count, static_cast<T *>(k), static_cast<T *>(v));
-    return cudaGetLastError();
-}
 template <typename T>
 cudaError_t gather_t(const Kv8View &c, const int *kv_len, const int *start, int count, void *k, void *v, cudaStream_t s) {
-    switch (c.head_dim / 32) {
-        case 1: return gather_v<T, 1>(c, kv_len, start, count, k, v, s);
-        case 2: return gather_v<T, 2>(c, kv_len, start, count, k, v, s);
-        case 3: return gather_v<T, 3>(c, kv_len, start, count, k, v, s);
-        case 4: return gather_v<T, 4>(c, kv_len, start, count, k, v, s);
-        case 5: return gather_v<T, 5>(c, kv_len, start, count, k, v, s);
-        case 6: return gather_v<T, 6>(c, kv_len, start, count, k, v, s);
-        case 7: return gather_v<T, 7>(c, kv_len, start, count, k, v, s);
-        default: return gather_v<T, 8>(c, kv_len, start, count, k, v, s);
-    }
+    const int64_t pieces = (int64_t)c.n_seqs * count * c.kv_heads * (c.head_dim / 16);
+    gather_kernel<T><<<dim3((unsigned)((pieces + kThreads - 1) / kThreads), 2), kThreads, 0, s>>>(
+        c, kv_len, start, count, static_cast<T *>(k), static_cast<T *>(v), pieces);
+    return cudaGetLastError();
 }
 }  // namespace
 

@@ -260,6 +260,28 @@ def test_append_odd_strides_and_alignment(t):
     _check_cache(c, [k], [x[:, nh + kvh:].astype(np.float64)], [37])
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1.0, 1e-20, 1e-34, 1e32])
+def test_codes_are_the_rounded_quotients(size, t):
+    """V is stored as it comes: its bytes are rint(x / scale) + 128 of the f32 quotient, bit for bit, ties of bf16
+    values and of halves of the largest among them."""
+    kvh, hd, n = 2, 128, 640
+    rng = np.random.default_rng(17)
+    x = rng.standard_normal((n, 2, kvh, hd)) * size
+    x[:, :, :, ::7] = rng.integers(-254, 255, x[:, :, :, ::7].shape) * (size / 254)
+    xd, x = _dev(x, t)
+    c = Cache(1, n, kvh, hd, seed=6)
+    _append(c, t, xd.reshape(n, -1), 0, None, _i32([n]), _i32([0, n]), n)
+    vc, vs = host(c.vc), host(c.vs)
+    for b in range(n // 32):
+        for h in range(kvh):
+            z = x[32 * b:32 * b + 32, 1, h]
+            scale = np.abs(z).max() / np.float32(127)
+            assert vs[c.table[0, b], h] == scale
+            assert np.array_equal(vc[c.table[0, b], h], np.rint(z / scale) + 128)
+    Q.check_device()
+
+
 def test_gather():
     """Positions before, in and past a sequence, closed pages and open rows, an empty sequence."""
     kvh, hd = 3, 96
