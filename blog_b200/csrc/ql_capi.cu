@@ -1240,7 +1240,7 @@ int kv8_operand(const void *p, int64_t stride, int64_t width, int32_t type, cons
 // Launch shape of the attention over split keys, from the caller's bounds alone (so the workspace can be
 // sized before the call and a captured launch fits every length).
 struct Kv8AttnShape {
-    int row_groups, splits;
+    int row_groups, splits, cluster;
     size_t bytes;
 };
 Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs, int max_q_len, int max_kv_len, int sms) {
@@ -1251,11 +1251,12 @@ Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs,
     const int64_t blocks = (max_kv_len + kKvBlock - 1) / kKvBlock;
     int64_t n = groups > 0 ? (slots + groups - 1) / groups : 1;
     n = std::min<int64_t>(n, (blocks + kKvAttnWarps - 1) / kKvAttnWarps);
-    n = std::min<int64_t>(n, kKvAttnMaxSplits);
-    if (groups > kKvAttnCounters) n = 1;
-    s.splits = (int)std::max<int64_t>(n, 1);
+    s.cluster = n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
+    int64_t clusters = std::min<int64_t>(n / s.cluster, kKvAttnMaxClusters);
+    if (groups * kKvAttnRows > kKvAttnCounters) clusters = 1;
+    s.splits = s.cluster * (int)std::max<int64_t>(clusters, 1);
     s.bytes = sizeof(unsigned) * kKvAttnCounters;
-    if (s.splits > 1) s.bytes += sizeof(float) * (size_t)groups * s.splits * kKvAttnRows * (head_dim + 2);
+    if (clusters > 1) s.bytes += sizeof(float) * (size_t)groups * clusters * kKvAttnRows * (head_dim + 4);
     return s;
 }
 }  // namespace
@@ -1344,7 +1345,12 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         a.q_stride = q_stride, a.gate_stride = gate_stride, a.out_stride = out_stride;
         a.n_heads = n_heads;
         a.scale_log2 = scale * 1.4426950408889634f;
+        auto on16 = [&](const void *p, int64_t stride) {
+            return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * (type == QL_F32 ? 4 : 2) % 16 == 0;
+        };
+        a.vec = on16(q, q_stride) && on16(out, out_stride);
         a.splits = sh.splits;
+        a.cluster = sh.cluster;
         a.row_groups = sh.row_groups;
         a.arrivals = static_cast<unsigned *>(workspace_);
         a.part = reinterpret_cast<float *>(a.arrivals + kKvAttnCounters);

@@ -49,10 +49,12 @@ struct Kv8AttnArgs {
     int64_t q_stride, gate_stride, out_stride;
     int n_heads;
     float scale_log2;  // softmax scale x log2(e)
-    int splits;        // CTAs over the keys of one (sequence, KV head, row group)
+    bool vec;          // q and out: every row starts on 16 bytes
+    int splits;        // CTAs over the keys of one (sequence, KV head, row group): clusters of `cluster`
+    int cluster;       // 1, 2, 4 or 8
     int row_groups;    // groups of 8 (query token, head of the KV head's group) rows per sequence
-    unsigned *arrivals;  // [n_seqs x kv_heads x row_groups] zero between calls (splits > 1)
-    float *part;         // [...][splits][8][head_dim + 2]
+    unsigned *arrivals;  // [n_seqs x kv_heads x row_groups][8] zero between calls (several clusters)
+    float *part;         // [...][clusters][8][head_dim + 4]
 };
 
 // Slot of a sequence's open rows, or -1 (recorded in the error word).
@@ -114,7 +116,7 @@ cudaError_t kv8_attn_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s);
 int kv8_attn_ctas_per_sm(int head_dim);
 constexpr int kKvAttnWarps = 4;           // warps per CTA, each with key blocks of its own
 constexpr int kKvAttnRows = 8;            // rows per CTA: query tokens x heads of one KV head's group
-constexpr int kKvAttnMaxSplits = 128;
+constexpr int kKvAttnMaxClusters = 16;
 constexpr int kKvAttnCounters = 16384;    // arrival counters at the head of the workspace
 
 }  // namespace ql

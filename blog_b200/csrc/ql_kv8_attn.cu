@@ -17,20 +17,26 @@
 // The order of the head dimension within a product and of the tokens within a block is free as long as both
 // operands agree, so the fragments are 16-byte pieces of the rows as they lie in the page: 16 codes of K
 // serve four k-steps, and V pairs of tokens are gathered from two rows by one byte permute.
-// Warps are merged in shared memory, CTAs of one (sequence, KV head, row group) by the last to arrive, in
-// split order: the result does not depend on which CTA that is.
+// The CTAs of one (sequence, KV head, row group) form clusters of up to 8; warps are merged in shared memory,
+// a cluster's CTAs through distributed shared memory (each finishes its share of the rows), and clusters by
+// the last to arrive, always in split order: the result does not depend on which that is.
 //
 // Bound: HBM for the codes (2 head_dim bytes per token and KV head).
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "ql_kv8.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace ql {
 namespace {
 
 constexpr int kThreads = 32 * kKvAttnWarps;
-constexpr float kPScale = 16384.0f;    // weights are scaled to use f16's range
-constexpr float kVHeadroom = 3.9f;     // a block's scale may pass vref by this before the sums are rescaled
+// Weights are 2^(s - m) sv_b / vref, m and vref being kept until a score passes m by kMHeadroom or a scale
+// vref by kVHeadroom (so the sums are seldom rescaled), times kPScale: at most 2^7 x 3.9 x 64 = 31949 in f16,
+// and limbs down to 2^-24 / 64 of a weight of one.
+constexpr float kPScale = 64.0f, kMHeadroom = 7.0f, kVHeadroom = 3.9f;
 
 __device__ __forceinline__ void cp16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -86,12 +92,24 @@ template <>
 __device__ __forceinline__ float load_f32<float>(const float *p) { return *p; }
 template <>
 __device__ __forceinline__ float load_f32<__nv_bfloat16>(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+// Four elements whose address is a multiple of theirs together.
+template <typename T>
+__device__ __forceinline__ void load4(float *x, const T *p) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 z = *reinterpret_cast<const float4 *>(p);
+        x[0] = z.x, x[1] = z.y, x[2] = z.z, x[3] = z.w;
+    } else {
+        const uint2 z = *reinterpret_cast<const uint2 *>(p);  // bf16: the upper half of an f32
+        x[0] = __uint_as_float(z.x << 16), x[1] = __uint_as_float(z.x & 0xFFFF0000u);
+        x[2] = __uint_as_float(z.y << 16), x[3] = __uint_as_float(z.y & 0xFFFF0000u);
+    }
+}
 __device__ __forceinline__ void store_f32(float *p, float v) { *p = v; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 
 // Ring stages per warp, and CTAs per SM, by head_dim: 64 head_dim bytes per stage, 4 warps, 227 KB per SM.
-constexpr int stages(int hd) { return hd <= 64 ? 4 : 3; }
-constexpr int ctas_per_sm(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 1; }
+constexpr int stages(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 3; }
+constexpr int ctas_per_sm(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 1; }
 
 // 16-byte chunk of a row at which chunk c of row t lies.  K: a load phase (8 lanes) reads 64 bytes of two
 // rows, which share their banks where a row is a multiple of 128 bytes: the odd row's halves are swapped.
@@ -120,7 +138,7 @@ __device__ __forceinline__ float part_factor(float pm, float pt, float m) {
 template <int HD>
 struct Acc {
     float o[HD / 8][4];
-    float m, l, vref;
+    float m, l, vref, inv;  // inv: kPScale / vref (0 while vref is)
 
     // Block's scores s[n][2] (base-2 logarithms) of row g8, columns 2 q4, 2 q4 + 1 of n-tile n, to weights:
     // returns the two limbs' A fragments.  vs: the scale of the block's values.
@@ -129,23 +147,29 @@ struct Acc {
         float t = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[n][0], s[n][1]));
-        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-        const float m_new = fmaxf(m, t);
-        float r = m_new > m ? ex2(m - m_new) : 1.0f;  // m = -inf: 0
-        m = m_new;
-        l *= r;
-        if (vs > kVHeadroom * vref) {  // warp-uniform; vref = 0 before the first block
-            r *= vref / vs;
-            vref = vs;
-        }
-        if (__any_sync(0xffffffffu, r != 1.0f)) {
+        const bool grown = vs > kVHeadroom * vref;  // warp-uniform; vref = 0 before the first block
+        // (m = -inf: any score passes it; the four lanes of a row agree after the shuffles)
+        if (__any_sync(0xffffffffu, t > m + kMHeadroom) || grown) {
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+            float r = 1.0f;
+            if (t > m) {
+                r = ex2(m - t);  // m = -inf: 0
+                m = t;
+            }
+            l *= r;
+            if (grown) {
+                const float v = fmaxf(vs, 1e-36f);  // (its reciprocal stays finite)
+                r *= vref / v;
+                vref = v;
+                inv = kPScale / v;
+            }
 #pragma unroll
             for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[n][i] *= r;
         }
-        const float f = vref > 0.f ? vs / vref * kPScale : vs * 0.f;  // (a NaN scale stays one)
+        const float f = vs * inv;
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -168,7 +192,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     const int split = blockIdx.x, kh = blockIdx.y % a.c.kv_heads, rg = blockIdx.y / a.c.kv_heads, seq = blockIdx.z;
     uint8_t *ring = sm + warp * (ST * 2 * BLK);
     uint4 *qf = reinterpret_cast<uint4 *>(sm + kKvAttnWarps * ST * 2 * BLK);  // [KS][32] A fragments of q
-    __shared__ float s_m[kKvAttnWarps][kKvAttnRows], s_l[kKvAttnWarps][kKvAttnRows];
+    __shared__ float s_m[kKvAttnWarps][kKvAttnRows], s_l[kKvAttnWarps][kKvAttnRows], s_q[kKvAttnRows];
+    __shared__ float c_m[kKvAttnRows], c_l[kKvAttnRows];  // this CTA's maximum and total, read by its cluster
     __shared__ unsigned s_last;
 
     int row0, q_len;
@@ -204,21 +229,25 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
             vs = a.c.v_scale[(int64_t)page * a.c.kv_heads + kh];
         }
     };
+    // a lane's 16-byte pieces of a block: u * 512 + lane * 16; their places repeat every P pieces (8 rows)
+    constexpr int NU = BLK / 512, P = NU < 4 ? NU : HD == 128 ? 2 : 4;
+    static_assert(HD * 8 == P * 512 || P == NU || (HD != 64 && HD != 128 && HD != 256), "8 rows per P pieces");
+    int k_off[P], v_off[P];
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+        const int x = u * 32 + lane, t = x / (HD / 16), c = x % (HD / 16);
+        k_off[u] = t * HD + k_chunk<HD>(c, t) * 16;
+        v_off[u] = t * HD + v_chunk<HD>(c, t) * 16;
+    }
     auto issue = [&](int i, int pg) {  // block i of the list into its stage (one group, empty past the end)
         if (i < n_blocks && pg >= 0) {
             uint8_t *dst = ring + i % ST * 2 * BLK;
-            const int64_t at = kv8_codes_at(a.c, pg, kh);
-            constexpr int RC = HD / 16;
+            const int64_t at = kv8_codes_at(a.c, pg, kh) + lane * 16;
+            const uint8_t *kp = a.c.k_codes + at, *vp = a.c.v_codes + at;
 #pragma unroll
-            for (int u = 0; u < BLK / 16 / 32; ++u) {
-                const int x = u * 32 + lane, t = x / RC, c = x % RC;
-                cp16(dst + t * HD + k_chunk<HD>(c, t) * 16, a.c.k_codes + at + x * 16);
-            }
+            for (int u = 0; u < NU; ++u) cp16(dst + u / P * (P * 512) + k_off[u % P], kp + u * 512);
 #pragma unroll
-            for (int u = 0; u < BLK / 16 / 32; ++u) {
-                const int x = u * 32 + lane, t = x / RC, c = x % RC;
-                cp16(dst + BLK + t * HD + v_chunk<HD>(c, t) * 16, a.c.v_codes + at + x * 16);
-            }
+            for (int u = 0; u < NU; ++u) cp16(dst + BLK + u / P * (P * 512) + v_off[u % P], vp + u * 512);
         }
         cp_commit();
     };
@@ -227,35 +256,36 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     for (int i = 0; i < ST - 1; ++i) issue(i, __shfl_sync(0xffffffffu, page, i));
 
     // q: two limbs per row, scaled by a power of two, as A fragments (warp 0 writes, all read)
-    float row_scale = 0.f;
-    {
+    if (warp == 0) {
         float x[KS][4], amax = 0.f;
         const T *q = static_cast<const T *>(a.q) + (int64_t)(row0 + tok) * a.q_stride + (int64_t)head * HD;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             const int d = k < 4 * G64 ? k / 4 * 64 + 16 * q4 + k % 4 * 4 : 64 * G64 + 8 * q4 + (k - 4 * G64) * 4;
+            if (live && a.vec) {
+                load4<T>(x[k], q + d);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[k][i] = live ? load_f32<T>(q + d + i) : 0.f;
-                amax = fmaxf(amax, fabsf(x[k][i]));
+                for (int i = 0; i < 4; ++i) x[k][i] = live ? load_f32<T>(q + d + i) : 0.f;
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[k][i]));
         }
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float inv;
         const float f = limb_scale(amax, inv);
-        row_scale = a.scale_log2 * inv;
-        if (warp == 0) {
+        if (q4 == 0) s_q[g8] = a.scale_log2 * inv;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                uint4 u;
-                split_f16(x[k][0] * f, x[k][1] * f, u.x, u.y);  // rows g8 (upper limb), g8 + 8 (lower)
-                split_f16(x[k][2] * f, x[k][3] * f, u.z, u.w);
-                qf[k * 32 + lane] = u;
-            }
+        for (int k = 0; k < KS; ++k) {
+            uint4 u;
+            split_f16(x[k][0] * f, x[k][1] * f, u.x, u.y);  // rows g8 (upper limb), g8 + 8 (lower)
+            split_f16(x[k][2] * f, x[k][3] * f, u.z, u.w);
+            qf[k * 32 + lane] = u;
         }
     }
     __syncthreads();
+    const float row_scale = s_q[g8];
 
     Acc<HD> acc;
 #pragma unroll
@@ -265,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     acc.m = -INFINITY;
     acc.l = 0.f;
     acc.vref = 0.f;
+    acc.inv = 0.f;
 
     for (int i = 0; i < n_blocks; ++i) {
         const int pg = __shfl_sync(0xffffffffu, page, i & 31);
@@ -468,82 +499,171 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
         }
     }
 
-    // warps: [warp][row][HD] in the ring's memory
+    // Warps: [warp][row][HD] in the ring's memory, in chunks of 4 dimensions; the lanes of a store phase (two
+    // rows, four q4) have the same chunk modulo 8 and are spread by an XOR.
     float l = acc.l + __shfl_xor_sync(0xffffffffu, acc.l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     __syncthreads();
     float *so = reinterpret_cast<float *>(sm);
+    auto so_at = [&](int y, int r, int chunk) {
+        // (the key must not change within 8 chunks: head_dim 64, 128, 256)
+        constexpr bool pow2 = HD == 64 || HD == 128 || HD == 256;
+        return so + (y * kKvAttnRows + r) * HD + (pow2 ? chunk ^ ((chunk / (HD / 16) * 2 + (r & 1)) & 7) : chunk) * 4;
+    };
     {
         const float f = acc.vref * (1.0f / kPScale);
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n)
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                so[(warp * kKvAttnRows + g8) * HD + (2 * q4 + e) * (HD / 8) + n] = (acc.o[n][e] + acc.o[n][e + 2]) * f;
+            for (int n = 0; n < HD / 8; n += 4) {
+                float4 z;
+                z.x = (acc.o[n][e] + acc.o[n][e + 2]) * f;
+                z.y = (acc.o[n + 1][e] + acc.o[n + 1][e + 2]) * f;
+                z.z = (acc.o[n + 2][e] + acc.o[n + 2][e + 2]) * f;
+                z.w = (acc.o[n + 3][e] + acc.o[n + 3][e + 2]) * f;
+                *reinterpret_cast<float4 *>(so_at(warp, g8, (2 * q4 + e) * (HD / 32) + n / 4)) = z;
+            }
         if (q4 == 0) {
             s_m[warp][g8] = acc.m;
             s_l[warp][g8] = l;
         }
     }
     __syncthreads();
-    const int64_t group = ((int64_t)seq * a.row_groups + rg) * a.c.kv_heads + kh;
-    constexpr int PR = HD + 2;  // a partial's row: sums, maximum, total
-    auto finish = [&](int r, int d, float o, float total) {
-        const int gr = rg * kKvAttnRows + r;
-        if (gr >= q_len * G) return;
-        const int64_t row = row0 + gr / G;
-        const int h = kh * G + gr % G;
-        float v = total == 0.f ? 0.f : o / total;  // a row that sees no key: zeros (a NaN total: NaN)
-        if (a.gate != nullptr) {
-            const float g = load_f32<T>(static_cast<const T *>(a.gate) + row * a.gate_stride + (int64_t)h * HD + d);
-            v *= 1.0f / (1.0f + expf(-g));
-        }
-        store_f32(static_cast<T *>(a.out) + row * a.out_stride + (int64_t)h * HD + d, v);
+    auto add4 = [](float4 &z, const float4 &w, float f) {
+        if (f == 0.f) return;  // (saw no key: whatever stands there)
+        z.x = fmaf(w.x, f, z.x), z.y = fmaf(w.y, f, z.y), z.z = fmaf(w.z, f, z.z), z.w = fmaf(w.w, f, z.w);
     };
-    for (int x = threadIdx.x; x < kKvAttnRows * HD; x += kThreads) {
-        const int r = x / HD, d = x % HD;
-        float m = -INFINITY, o = 0.f, t = 0.f;
+    for (int x = threadIdx.x; x < kKvAttnRows * HD / 4; x += kThreads) {
+        const int r = x / (HD / 4), c = x % (HD / 4);
+        float m = -INFINITY, t = 0.f;
 #pragma unroll
         for (int y = 0; y < kKvAttnWarps; ++y) m = fmaxf(m, s_m[y][r]);
+        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int y = 0; y < kKvAttnWarps; ++y) {
             const float f = part_factor(s_m[y][r], s_l[y][r], m);
-            o += f == 0.f ? 0.f : so[(y * kKvAttnRows + r) * HD + d] * f;
-            t += f == 0.f ? 0.f : s_l[y][r] * f;
+            add4(z, *reinterpret_cast<const float4 *>(so_at(y, r, c)), f);
+            if (f != 0.f) t = fmaf(s_l[y][r], f, t);
         }
-        if (a.splits == 1) {
-            finish(r, d, o, t);
-        } else {
-            float *p = a.part + ((group * a.splits + split) * kKvAttnRows + r) * PR;
-            p[d] = o;
-            if (d == 0) {
-                p[HD] = m;
-                p[HD + 1] = t;
+        *reinterpret_cast<float4 *>(so_at(0, r, c)) = z;  // (read by this thread alone so far)
+        if (c == 0) {
+            c_m[r] = m;
+            c_l[r] = t;
+        }
+    }
+    auto finish = [&](int r, int c, const float4 &z, float total) {
+        const int gr = rg * kKvAttnRows + r;
+        if (gr >= q_len * G) return;
+        const int64_t row = row0 + gr / G;
+        const int d = (kh * G + gr % G) * HD + 4 * c;
+        const float inv = total == 0.f ? 0.f : 1.0f / total;  // a row that sees no key: zeros
+        float v[4] = {z.x * inv, z.y * inv, z.z * inv, z.w * inv};
+        if (a.gate != nullptr) {
+            const T *g = static_cast<const T *>(a.gate) + row * a.gate_stride + d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] *= 1.0f / (1.0f + expf(-load_f32<T>(g + i)));
+        }
+        T *o = static_cast<T *>(a.out) + row * a.out_stride + d;
+        if (a.vec) {
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+            } else {
+                __nv_bfloat162 w[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+                *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<uint2 *>(w);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) store_f32(o + i, v[i]);
+        }
+    };
+    if (a.splits == 1) {
+        __syncthreads();
+        for (int x = threadIdx.x; x < kKvAttnRows * HD / 4; x += kThreads) {
+            const int r = x / (HD / 4), c = x % (HD / 4);
+            finish(r, c, *reinterpret_cast<const float4 *>(so_at(0, r, c)), c_l[r]);
+        }
+        return;
+    }
+    // cluster: rank k of n finishes rows k 8 / n .. from every CTA's shared memory
+    cg::cluster_group cl = cg::this_cluster();
+    const int n_cta = a.cluster, rank = split % n_cta, rows = kKvAttnRows / n_cta, r0 = rank * rows;
+    const int clusters = a.splits / n_cta, cluster = split / n_cta;
+    cl.sync();
+    const int64_t group = ((int64_t)seq * a.row_groups + rg) * a.c.kv_heads + kh;
+    constexpr int PR = HD + 4;  // a partial's row: sums, maximum, total
+    for (int x = threadIdx.x; x < rows * HD / 4; x += kThreads) {
+        const int r = r0 + x / (HD / 4), c = x % (HD / 4);
+        float pm[8], pl[8], m = -INFINITY, t = 0.f;
+        float4 w[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y)
+            if (y < n_cta) {
+                pm[y] = *cl.map_shared_rank(&c_m[r], y);
+                pl[y] = *cl.map_shared_rank(&c_l[r], y);
+                w[y] = *reinterpret_cast<const float4 *>(cl.map_shared_rank(so_at(0, r, c), y));
+                m = fmaxf(m, pm[y]);
+            }
+        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int y = 0; y < 8; ++y)
+            if (y < n_cta) {
+                const float f = part_factor(pm[y], pl[y], m);
+                add4(z, w[y], f);
+                if (f != 0.f) t = fmaf(pl[y], f, t);
+            }
+        if (clusters == 1) {
+            finish(r, c, z, t);
+        } else {
+            float *p = a.part + ((group * clusters + cluster) * kKvAttnRows + r) * PR;
+            *reinterpret_cast<float4 *>(p + 4 * c) = z;
+            if (c == 0) *reinterpret_cast<float2 *>(p + HD) = make_float2(m, t);
         }
     }
-    if (a.splits == 1) return;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) s_last = atomicAdd(a.arrivals + group, 1u) == (unsigned)a.splits - 1;
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-    for (int x = threadIdx.x; x < kKvAttnRows * HD; x += kThreads) {
-        const int r = x / HD, d = x % HD;
-        const float *p = a.part + (group * a.splits * kKvAttnRows + r) * PR;
-        float m = -INFINITY, o = 0.f, t = 0.f;
-        for (int y = 0; y < a.splits; ++y) m = fmaxf(m, __ldcg(p + (int64_t)y * kKvAttnRows * PR + HD));
-        for (int y = 0; y < a.splits; ++y) {
-            const float *z = p + (int64_t)y * kKvAttnRows * PR;
-            const float pm = __ldcg(z + HD), pt = __ldcg(z + HD + 1);
-            const float f = part_factor(pm, pt, m);
-            o += f == 0.f ? 0.f : __ldcg(z + d) * f;
-            t += f == 0.f ? 0.f : pt * f;
+    __syncwarp();
+    cl.barrier_arrive();  // (waited for at the end: a CTA's shared memory is read until all have arrived)
+    if (clusters > 1) {
+        __threadfence();
+        __syncthreads();
+        unsigned *arrived = a.arrivals + group * kKvAttnRows + rank;
+        if (threadIdx.x == 0) s_last = atomicAdd(arrived, 1u) == (unsigned)clusters - 1;
+        __syncthreads();
+        if (s_last) {
+            __threadfence();
+            for (int x = threadIdx.x; x < rows * HD / 4; x += kThreads) {
+                const int r = r0 + x / (HD / 4), c = x % (HD / 4);
+                const float *p = a.part + (group * clusters * kKvAttnRows + r) * PR;
+                float m = -INFINITY, t = 0.f;
+                float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int y0 = 0; y0 < clusters; y0 += 8) {  // eight partials in flight
+                    float2 ml[8];
+                    float4 w[8];
+                    float mb = m;
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+                        if (y0 + y < clusters) {
+                            const float *g = p + (int64_t)(y0 + y) * kKvAttnRows * PR;
+                            ml[y] = __ldcg(reinterpret_cast<const float2 *>(g + HD));
+                            w[y] = __ldcg(reinterpret_cast<const float4 *>(g + 4 * c));
+                            mb = fmaxf(mb, ml[y].x);
+                        }
+                    const float f0 = m == -INFINITY ? (t == t ? 0.f : t) : ex2(m - mb);
+                    z.x *= f0, z.y *= f0, z.z *= f0, z.w *= f0, t *= f0;
+                    m = mb;
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+                        if (y0 + y < clusters) {
+                            const float f = part_factor(ml[y].x, ml[y].y, m);
+                            add4(z, w[y], f);
+                            if (f != 0.f) t = fmaf(ml[y].y, f, t);
+                        }
+                }
+                finish(r, c, z, t);
+            }
+            if (threadIdx.x == 0) *arrived = 0;
         }
-        finish(r, d, o, t);
     }
-    if (threadIdx.x == 0) a.arrivals[group] = 0;
+    __syncwarp();
+    cl.barrier_wait();
 }
 
 template <typename T, int HD>
@@ -551,8 +671,17 @@ cudaError_t launch_hd(const Kv8AttnArgs &a, cudaStream_t s) {
     const int smem = kKvAttnWarps * stages(HD) * 2 * kKvBlock * HD + HD / 16 * 32 * 16;
     cudaError_t e = cudaFuncSetAttribute(attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    attn_kernel<T, HD><<<dim3(a.splits, a.c.kv_heads * a.row_groups, a.c.n_seqs), kThreads, smem, s>>>(a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.splits, a.c.kv_heads * a.row_groups, a.c.n_seqs);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {(unsigned)a.cluster, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_kernel<T, HD>, a);
 }
 template <typename T>
 cudaError_t launch_t(const Kv8AttnArgs &a, cudaStream_t s) {
