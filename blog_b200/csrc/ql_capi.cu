@@ -7,6 +7,7 @@
 // into CUDA graphs), and a device error word for bounded waits that expired.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -1249,8 +1250,18 @@ Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs,
     const int64_t groups = (int64_t)n_seqs * kv_heads * s.row_groups;
     const int64_t slots = (int64_t)sms * kv8_attn_ctas_per_sm(head_dim);
     const int64_t blocks = (max_kv_len + kKvBlock - 1) / kKvBlock;
-    int64_t n = groups > 0 ? (slots + groups - 1) / groups : 1;
-    n = std::min<int64_t>(n, (blocks + kKvAttnWarps - 1) / kKvAttnWarps);
+    // CTAs per group.  Where one wave of CTAs has room, as many as it holds (a second wave costs the start's
+    // chain of loads again: 8 x 8192 tokens of 4 KV heads, 8 per group 19 us, 16 per group 32 us), but a block
+    // for every warp, and four where that leaves 8 CTAs (one sequence of 32768 tokens: 64 per group 16.2 us,
+    // 104 per group 20 us; of 1024: 8 per group 7.1 us, 2 per group 9.5 us).  Where there are several waves
+    // anyway, two or more per group even out unlike lengths, as long as a warp has 32 blocks (64 sequences of
+    // up to 8192 tokens, 8 KV heads: 2 per group 133 us, 1 per group 153 us).
+    int64_t n = 1;
+    if (groups > 0 && slots / groups >= 2)
+        n = std::min({slots / groups, (blocks + kKvAttnWarps - 1) / kKvAttnWarps,
+                      std::max<int64_t>(8, blocks / (4 * kKvAttnWarps))});
+    else
+        n = blocks / (32 * kKvAttnWarps);
     s.cluster = n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
     int64_t clusters = std::min<int64_t>(n / s.cluster, kKvAttnMaxClusters);
     if (groups * kKvAttnRows > kKvAttnCounters) clusters = 1;

@@ -25,6 +25,8 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "ql_kv8.cuh"
 
 namespace cg = cooperative_groups;
@@ -669,8 +671,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
 template <typename T, int HD>
 cudaError_t launch_hd(const Kv8AttnArgs &a, cudaStream_t s) {
     const int smem = kKvAttnWarps * stages(HD) * 2 * kKvBlock * HD + HD / 16 * 32 * 16;
-    cudaError_t e = cudaFuncSetAttribute(attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // (the attribute is the device's: set once for each)
+    static std::atomic<uint64_t> ready{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load() >> dev & 1)) {
+        if ((e = cudaFuncSetAttribute(attn_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess)
+            return e;
+        if (dev < 64) ready.fetch_or(1ull << dev);
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.splits, a.c.kv_heads * a.row_groups, a.c.n_seqs);
     cfg.blockDim = dim3(kThreads);
