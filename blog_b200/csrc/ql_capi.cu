@@ -1365,7 +1365,9 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         a.row_groups = sh.row_groups;
         a.arrivals = static_cast<unsigned *>(workspace_);
         a.part = reinterpret_cast<float *>(a.arrivals + kKvAttnCounters);
-        const cudaError_t e = kv8_attn_launch(a, type == QL_BF16, g_stream);
+        const bool prompt = kv8_prompt_takes(hd) && (int64_t)mq * (n_heads / a.c.kv_heads) >= 128;
+        const cudaError_t e = prompt ? kv8_prompt_launch(a, mq, type == QL_BF16, g_stream)
+                                     : kv8_attn_launch(a, type == QL_BF16, g_stream);
         ++t_launches;
         return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
     });

@@ -111,6 +111,9 @@ cudaError_t kv8_append_launch(const Kv8AppendArgs &a, bool bf16, cudaStream_t s)
 cudaError_t kv8_gather_launch(const Kv8View &c, const int *kv_len, const int *start, int count, void *k_out, void *v_out,
                               bool bf16, cudaStream_t s);
 cudaError_t kv8_attn_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s);
+// The tensor-core form for prompts (ql_kv8_prompt.cu).
+bool kv8_prompt_takes(int head_dim);
+cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, int max_q_len, bool bf16, cudaStream_t s);
 
 // CTAs of the attention's split kernel that one SM holds (the host sizes the split count by it).
 int kv8_attn_ctas_per_sm(int head_dim);

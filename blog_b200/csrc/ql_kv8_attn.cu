@@ -6,9 +6,10 @@
 //
 // Mathematics.  A code is an integer of 8 bits and so exact in f16: with q = 2^-e (qh + ql) in two f16 limbs
 // (22 bits) the products q . c are exact and summed in fp32, and one multiplication by sk_b scale 2^-e gives
-// the score.  Weights p = 2^(s - m) are multiplied by sv_b / vref (vref: the largest scale met, like the
-// running maximum m) and split into two f16 limbs in the same way, so the result is as exact as fp32 sums
-// make it.  The two limbs cost nothing: mma.m16n8k16 has 16 rows, the 8 rows' upper limbs and their lower
+// the score.  What meets V's codes is p sv_b, p = 2^(s - m): it is taken relative to the row's largest such
+// product so far (2^mh, a running maximum of s + log2 sv_b beside that of s) and split into two f16 limbs in
+// the same way, so the result is as exact as fp32 sums make it, however unlike the blocks' scales are.  The
+// two limbs cost nothing: mma.m16n8k16 has 16 rows, the 8 rows' upper limbs and their lower
 // ones, and the two halves of an accumulator fragment are added.
 //
 // Layout.  A CTA has 4 warps and 8 rows (query token, head of one KV head's group); each warp walks over
@@ -35,10 +36,10 @@ namespace ql {
 namespace {
 
 constexpr int kThreads = 32 * kKvAttnWarps;
-// Weights are 2^(s - m) sv_b / vref, m and vref being kept until a score passes m by kMHeadroom or a scale
-// vref by kVHeadroom (so the sums are seldom rescaled), times kPScale: at most 2^7 x 3.9 x 64 = 31949 in f16,
-// and limbs down to 2^-24 / 64 of a weight of one.
-constexpr float kPScale = 64.0f, kMHeadroom = 7.0f, kVHeadroom = 3.9f;
+// m and h are whole numbers, at or above the maxima they stand for when they are set, and kept until a value
+// passes them by kHeadroom (so the sums are seldom rescaled).  Weights are scaled by 2^kWBits: at most
+// 2^(7 + 8) in f16, and limbs down to 2^-24 / 2^8 of the row's largest.
+constexpr float kHeadroom = 7.0f, kWBits = 8.0f;
 
 __device__ __forceinline__ void cp16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -135,12 +136,25 @@ __device__ __forceinline__ float part_factor(float pm, float pt, float m) {
     return pt != pt ? pt : pm == -INFINITY ? 0.f : ex2(pm - m);
 }
 
+// 2^(kWBits - h), 0 while nothing but zeros has been met (h = -inf).
+__device__ __forceinline__ float weight_unit(float h) { return h == -INFINITY ? 0.f : ex2(kWBits - h); }
+// What turns sums of w 2^(s - m) sv code into sums of 2^(s - m) sv code: x 2^(h - kWBits), in two steps where
+// the power leaves the range.
+__device__ __forceinline__ float weight_undo(float x, float h) {
+    const float e = h - kWBits;
+    return h == -INFINITY ? x * 0.f : x * ex2(fmaxf(e, -120.f)) * ex2(fminf(e + 120.f, 0.f));  // (NaN stays)
+}
+// Below this h the weights' factor sv w leaves the range, and 2^(s - m) with it, where the weights themselves
+// do not (the row's heaviest keys have values of zero): they are computed from s - m - h then.
+constexpr float kDeep = -60.0f;
+
 // Running state of one warp: row g8 = lane / 4 in the first two floats of a fragment (upper limbs) and the
 // last two (lower limbs).
 template <int HD>
 struct Acc {
     float o[HD / 8][4];
-    float m, l, vref, inv;  // inv: kPScale / vref (0 while vref is)
+    float m, l;  // maximum of the scores, total of 2^(s - m)
+    float h, w;  // maximum of s - m + log2 of V's scale; 2^(kWBits - h): o holds sums of w 2^(s - m) sv code
 
     // Block's scores s[n][2] (base-2 logarithms) of row g8, columns 2 q4, 2 q4 + 1 of n-tile n, to weights:
     // returns the two limbs' A fragments.  vs: the scale of the block's values.
@@ -149,36 +163,52 @@ struct Acc {
         float t = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[n][0], s[n][1]));
-        const bool grown = vs > kVHeadroom * vref;  // warp-uniform; vref = 0 before the first block
-        // (m = -inf: any score passes it; the four lanes of a row agree after the shuffles)
-        if (__any_sync(0xffffffffu, t > m + kMHeadroom) || grown) {
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        const float lv = log2f(vs);  // (0: -inf, which never passes h; NaN neither)
+        if (__any_sync(0xffffffffu, t > m + kHeadroom || t - m + lv > h + kHeadroom)) {
+            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));  // the row's four lanes agree
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            float r = 1.0f;
             if (t > m) {
-                r = ex2(m - t);  // m = -inf: 0
-                m = t;
+                const float z = ceilf(t);
+                l *= ex2(m - z);  // m = -inf: 0
+                h -= z - m;       // (o's unit 2^(m + h) stays)
+                m = z;
             }
-            l *= r;
-            if (grown) {
-                const float v = fmaxf(vs, 1e-36f);  // (its reciprocal stays finite)
-                r *= vref / v;
-                vref = v;
-                inv = kPScale / v;
+            float r = 1.0f;
+            if (t - m + lv > h) {
+                const float z = ceilf(t - m + lv);
+                r = ex2(h - z);
+                h = z;
             }
+            w = weight_unit(h);
+            if (__any_sync(0xffffffffu, r != 1.0f)) {
 #pragma unroll
-            for (int n = 0; n < HD / 8; ++n)
+                for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[n][i] *= r;
+                    for (int i = 0; i < 4; ++i) o[n][i] *= r;
+            }
         }
-        const float f = vs * inv;
+        const float f = vs * w;
         const float base = m == -INFINITY ? 0.f : m;
+        // (x = -inf, a masked key: a NaN scale must not reach its weight)
+        if (__any_sync(0xffffffffu, h < kDeep)) {
+            const float lift = h == -INFINITY ? 0.f : h, g = h == -INFINITY ? f : vs * ex2(kWBits);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float p0 = ex2(s[n][0] - base), p1 = ex2(s[n][1] - base);
-            l += p0 + p1;
-            // (a NaN scale must not reach the weights of masked keys)
-            split_f16(s[n][0] == -INFINITY ? 0.f : p0 * f, s[n][1] == -INFINITY ? 0.f : p1 * f, hi[n], lo[n]);
+            for (int n = 0; n < NT; ++n) {
+                float x[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    l += ex2(s[n][e] - base);
+                    x[e] = s[n][e] == -INFINITY ? 0.f : ex2(fminf(s[n][e] - base - lift, 126.f)) * g;
+                }
+                split_f16(x[0], x[1], hi[n], lo[n]);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float p0 = ex2(s[n][0] - base), p1 = ex2(s[n][1] - base);
+                l += p0 + p1;
+                split_f16(s[n][0] == -INFINITY ? 0.f : p0 * f, s[n][1] == -INFINITY ? 0.f : p1 * f, hi[n], lo[n]);
+            }
         }
     }
 };
@@ -296,8 +326,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
         for (int i = 0; i < 4; ++i) acc.o[n][i] = 0.f;
     acc.m = -INFINITY;
     acc.l = 0.f;
-    acc.vref = 0.f;
-    acc.inv = 0.f;
+    acc.h = -INFINITY;
+    acc.w = 0.f;
 
     for (int i = 0; i < n_blocks; ++i) {
         const int pg = __shfl_sync(0xffffffffu, page, i & 31);
@@ -513,16 +543,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
         return so + (y * kKvAttnRows + r) * HD + (pow2 ? chunk ^ ((chunk / (HD / 16) * 2 + (r & 1)) & 7) : chunk) * 4;
     };
     {
-        const float f = acc.vref * (1.0f / kPScale);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int n = 0; n < HD / 8; n += 4) {
                 float4 z;
-                z.x = (acc.o[n][e] + acc.o[n][e + 2]) * f;
-                z.y = (acc.o[n + 1][e] + acc.o[n + 1][e + 2]) * f;
-                z.z = (acc.o[n + 2][e] + acc.o[n + 2][e + 2]) * f;
-                z.w = (acc.o[n + 3][e] + acc.o[n + 3][e + 2]) * f;
+                z.x = weight_undo(acc.o[n][e] + acc.o[n][e + 2], acc.h);
+                z.y = weight_undo(acc.o[n + 1][e] + acc.o[n + 1][e + 2], acc.h);
+                z.z = weight_undo(acc.o[n + 2][e] + acc.o[n + 2][e + 2], acc.h);
+                z.w = weight_undo(acc.o[n + 3][e] + acc.o[n + 3][e + 2], acc.h);
                 *reinterpret_cast<float4 *>(so_at(warp, g8, (2 * q4 + e) * (HD / 32) + n / 4)) = z;
             }
         if (q4 == 0) {

@@ -1,0 +1,838 @@
+// Attention over the 8-bit KV cache for prompts: the same function as ql_kv8_attn.cu's, on the 5th-generation
+// tensor cores.
+//
+// A CTA takes 256 rows (query token, head of one KV head's group; the group's heads share every key) as two
+// tiles of 128 and walks over the keys 128 at a time with a running maximum and total per row:
+//   S = Q K^T       tcgen05.mma, Q and K in shared memory, S (fp32) in TMEM
+//   P = 2^(S f - m) one thread per row; f: the block's scale of K x the row's scale; P (f16) over S in TMEM
+//   O += P V        tcgen05.mma, P from TMEM, V in shared memory, O (fp32) in TMEM
+// Codes are exact in f16.  bf16 rows: q scaled by a power of two is exact in f16 too, P is rounded to f16's 11
+// bits (its result is rounded to 8).  f32 rows: q and P in two f16 limbs, twice the products, fp32 results.
+// The scale of V's block is multiplied into P relative to the row's largest such product, as in the split
+// kernel, and O is rescaled only when one passes that by 2^7.
+//
+// Roles, 16 warps: 0-3 and 4-7 a thread per row of tile 0 and 1 (S from TMEM, P to TMEM, the result); 8-11 codes
+// from global memory through registers to f16 in the layout the MMA reads (128-byte swizzle; K with the head
+// dimension contiguous and V too, as the transposed operand), a tile ahead; 12 issues the MMAs.  While one tile's
+// threads exponentiate, the tensor cores run the other tile's products.
+// The rows of the block that is not full make a last tile of 64 keys: their upper f16 limbs, then their lower.
+//
+// Bound: the tensor cores (4 head_dim flops per row and key, twice that for f32), with the exponentials (16 per
+// clock and SM) close behind.
+#include <cuda_fp16.h>
+
+#include <atomic>
+
+#include "ql_kv8.cuh"
+
+namespace ql {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kKeys = 128;   // keys per tile: 4 blocks
+constexpr int kTileBlocks = kKeys / kKvBlock;
+constexpr int kRows = 256;   // rows per CTA: two MMA tiles
+constexpr float kHeadroom = 7.0f, kWBits = 8.0f;  // as in the split kernel
+
+// Registers per thread of the roles; 16 warps launch with 128 each.
+template <int LIMBS>
+struct Regs {
+    static constexpr int softmax = LIMBS == 2 ? 208 : 184, convert = LIMBS == 2 ? 64 : 104, issue = LIMBS == 2 ? 32 : 40;
+    static_assert(2 * softmax + convert + issue == 4 * 128, "the block's registers at launch");
+};
+
+template <int HD, int LIMBS>
+struct Layout {
+    static constexpr int A = HD / 64;                        // 128-byte columns of a row
+    static constexpr int ST = LIMBS == 2 && HD == 128 ? 1 : 2;  // K and V stages
+    static constexpr int QT = A * 128 * 128;                 // one limb of one tile of Q
+    static constexpr int KV = A * kKeys * 128;               // one stage of K or of V
+    static constexpr int q = 0, k = q + 2 * LIMBS * QT, v = k + ST * KV, end = v + ST * KV;
+    static constexpr int bytes = 1024 + end + 512;
+};
+
+__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// 32 lanes x 32 columns; the registers are valid after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+// Shared-memory matrix descriptors, 128-byte swizzle.  K-major: 8-row atoms of 1024 B (stride byte offset).
+// MN-major (V, the head dimension contiguous): 64 x 8 atoms of 1024 B, the next 8 keys 1024 B on (stride byte
+// offset), the next 64 dimensions `lead` bytes on (leading byte offset).
+__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
+    return ((a >> 4) & 0x3FFFull) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t a, uint32_t lead) {
+    return ((a >> 4) & 0x3FFFull) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+// Instruction descriptor: f32 accumulator, f16 operands, M 128; bit 16: B is MN-major.
+constexpr uint32_t idesc(int n, bool b_mn) {
+    return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// As in the split kernel: 2^(kWBits - h), 0 while nothing but zeros has been met (h = -inf).
+__device__ __forceinline__ float weight_unit(float h) { return h == -INFINITY ? 0.f : ex2(kWBits - h); }
+// What turns sums of w 2^(s - m) sv code into sums of 2^(s - m) sv code: x 2^(h - kWBits), in two steps where
+// the power leaves the range.
+__device__ __forceinline__ float weight_undo(float x, float h) {
+    const float e = h - kWBits;
+    return h == -INFINITY ? x * 0.f : x * ex2(fmaxf(e, -120.f)) * ex2(fminf(e + 120.f, 0.f));  // (NaN stays)
+}
+// Below this h the weights' factor sv w leaves the range, and 2^(s - m) with it, where the weights themselves
+// do not (the row's heaviest keys have values of zero): they are computed from s - m - h then.
+constexpr float kDeep = -60.0f;
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
+__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t &hi, uint32_t &lo) {
+    hi = pack_f16(x0, x1);
+    const float2 h = unpack_f16(hi);
+    lo = pack_f16(x0 - h.x, x1 - h.y);
+}
+__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t sel) {
+    uint32_t r = __byte_perm(w, 0x64646464u, sel);
+    const uint32_t bias = 0x64806480u;  // 1152, 1152
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(bias));
+    return r;
+}
+__device__ __forceinline__ float limb_scale(float amax, float &inv) {  // as in the split kernel
+    const int e = (int)(__float_as_uint(amax) >> 23) & 0xFF;
+    const int f = min(max(264 - e, 1), 253);
+    inv = __uint_as_float((uint32_t)(254 - f) << 23);
+    return __uint_as_float((uint32_t)f << 23);
+}
+template <typename T>
+__device__ __forceinline__ void load8(float *x, const T *p, bool vec) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+            const uint4 z = *reinterpret_cast<const uint4 *>(p);
+            const uint32_t w[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(T) == 4)
+                x[i] = p[i];
+            else
+                x[i] = __bfloat162float(p[i]);
+        }
+    }
+}
+
+struct Bars {
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], open_max, done;
+    uint32_t tmem;
+    int abort;
+    // Scales of the tile's blocks (K's < 0: no such block), a ring: when the scores of the tile ST before have been
+    // computed, its rows may still have to read them, so ST + 1 tiles are in use.
+    float ks[4][kTileBlocks], vs[4][kTileBlocks];
+    unsigned bad;                                  // tokens of the open block that hold NaN or infinity
+};
+static_assert(sizeof(Bars) <= 512, "Bars at the end of shared memory");
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    constexpr int LIMBS = sizeof(T) == 4 ? 2 : 1;
+    using L = Layout<HD, LIMBS>;
+    constexpr int A = L::A, ST = L::ST;
+    constexpr uint32_t kS = 0, kO = kKeys, kTile = 256;  // TMEM columns of a tile: S (then P), O
+    extern __shared__ uint8_t sm_raw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
+    Bars &b = *reinterpret_cast<Bars *>(sm + L::end);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = a.n_heads / a.c.kv_heads;
+    const int kh = blockIdx.x, seq = blockIdx.y, r_base = (gridDim.z - 1 - blockIdx.z) * kRows;  // longest first
+    int row0, q_len;
+    kv8_rows_of(a.r, seq, row0, q_len);
+    const int n_rows = q_len * G;
+    if (r_base >= n_rows) return;
+    int kv_len = a.r.kv_len[seq];
+    if ((kv_len + kKvBlock - 1) / kKvBlock > a.c.max_pages) {
+        if (threadIdx.x == 0) atomicExch(a.c.err, kErrKvPage);
+        kv_len = 0;
+    }
+    // tiles of keys that each tile of rows needs; the open block's, where it is needed, is tile n_closed
+    const int blocks = kv_len / kKvBlock, open0 = blocks * kKvBlock, n_closed = (blocks + kTileBlocks - 1) / kTileBlocks;
+    int n_tiles[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r1 = min(r_base + 128 * (i + 1), n_rows) - 1;  // the tile's last row
+        const int keys = r_base + 128 * i < n_rows ? max(0, min(kv_len, kv_len - q_len + r1 / G + 1)) : 0;
+        const int bl = min((keys + kKvBlock - 1) / kKvBlock, blocks);
+        n_tiles[i] = (bl + kTileBlocks - 1) / kTileBlocks + (keys > open0 ? 1 : 0);
+    }
+    const int n_all = max(n_tiles[0], n_tiles[1]);
+    auto tile_blocks = [&](int j) { return j < n_closed ? min(kTileBlocks, blocks - j * kTileBlocks) : 2; };
+
+    if (threadIdx.x == 0) {
+        mbar_init(&b.q_full, kRows);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&b.k_full[i], 4), mbar_init(&b.k_empty[i], 1), mbar_init(&b.v_full[i], 4), mbar_init(&b.v_empty[i], 1);
+            mbar_init(&b.s_full[i], 1), mbar_init(&b.p_full[i], 4), mbar_init(&b.o_full[i], 1);
+        }
+        mbar_init(&b.open_max, 4);
+        mbar_init(&b.done, 1);
+        b.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) tmem_alloc(&b.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = b.tmem;
+    volatile int *abort_flag = &b.abort;
+    // Bounded wait: false (and everybody told) when it ran out or another role gave up.
+    auto wait = [&](uint64_t *bar, int phase) {
+        if (*abort_flag || !mbar_wait(bar, (uint32_t)phase & 1u, a.c.err, kErrWaitFull)) {
+            *abort_flag = 1;
+            return false;
+        }
+        return true;
+    };
+
+    if (warp < 8) {
+        // ------------------------------------ a thread per row ------------------------------------
+        reg_inc<Regs<LIMBS>::softmax>();
+        const int i = warp >> 2, r = threadIdx.x & 127, gr = r_base + 128 * i + r;
+        const bool live = gr < n_rows;
+        const int tok = live ? gr / G : 0, head = kh * G + (live ? gr % G : 0);
+        const int pos = live ? kv_len - q_len + tok : -1;  // the last key that the row sees
+        float row_scale;
+        {
+            const T *q = static_cast<const T *>(a.q) + (int64_t)(row0 + tok) * a.q_stride + (int64_t)head * HD;
+            float amax = 0.f, inv;
+            for (int d = 0; d < HD; d += 8) {
+                float x[8];
+                load8<T>(x, q + d, a.vec);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+            }
+            // (a negative softmax scale: its sign goes to q, so that scores and products order alike)
+            const float f = copysignf(limb_scale(amax, inv), a.scale_log2);
+            row_scale = fabsf(a.scale_log2) * inv;
+#pragma unroll 2
+            for (int d = 0; d < HD; d += 8) {
+                float x[8];
+                load8<T>(x, q + d, a.vec);
+                uint4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = live ? x[e] * f : 0.f;
+                split_f16(x[0], x[1], hi.x, lo.x);
+                split_f16(x[2], x[3], hi.y, lo.y);
+                split_f16(x[4], x[5], hi.z, lo.z);
+                split_f16(x[6], x[7], hi.w, lo.w);
+                uint8_t *p = sm + L::q + i * L::QT + d / 64 * (128 * 128) + r * 128 + ((d / 8 & 7) ^ (r & 7)) * 16;
+                *reinterpret_cast<uint4 *>(p) = hi;
+                if (LIMBS == 2) *reinterpret_cast<uint4 *>(p + 2 * L::QT) = lo;
+            }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&b.q_full);
+
+        const uint32_t tS = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + i * kTile + kS, tO = tS - kS + kO;
+        float m = -INFINITY, l = 0.f, h = -INFINITY, wf = 0.f;  // (as in the split kernel; wf: its w)
+        const int n = n_tiles[i];
+        bool ok = true;
+        float acc[LIMBS == 2 ? HD : 1];  // f32 rows: the sum over tiles, see below
+        if constexpr (LIMBS == 2) {
+#pragma unroll
+            for (int e = 0; e < HD; ++e) acc[e] = 0.f;
+        }
+        // The tensor cores truncate when they accumulate, so a sum over thousands of keys in TMEM would lose
+        // bits in one direction.  For f32 rows a tile's product starts from zero and is added here, rounded.
+        auto add_tile = [&]() {
+            if constexpr (LIMBS == 2) {
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(tO + 32 * c, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) acc[32 * c + e] += __uint_as_float(o[e]);
+                }
+            }
+        };
+        for (int j = 0; j < n; ++j) {
+            // (k_full too: the scales are the converters' writes)
+            ok = __all_sync(0xffffffffu, wait(&b.k_full[j % ST], j / ST) && wait(&b.s_full[i], j));
+            if (!ok) break;
+            tc_fence_after();  // (S full: the earlier products into O have completed too)
+            const bool open = j == n_closed;
+            const int key0 = open ? open0 : j * kKeys;
+            float ks[kTileBlocks], f[kTileBlocks], vs[kTileBlocks];
+            bool holes = false;  // blocks whose page is not there
+#pragma unroll
+            for (int c = 0; c < kTileBlocks; ++c) {
+                ks[c] = b.ks[j & 3][c];
+                f[c] = ks[c] * row_scale;
+                vs[c] = b.vs[j & 3][c];
+                holes |= f[c] < 0.f;
+            }
+            // (per warp) some row hides a key, or the tile is out of the ordinary
+            const bool masked = __any_sync(0xffffffffu, key0 + kKeys - 1 > pos || holes || open);
+            const unsigned bad = open ? b.bad : 0;
+            auto hidden = [&](int c, int e) { return key0 + 32 * c + e > pos || f[c] < 0.f; };
+            // the largest of block c's 32 scores, in units of log2
+            auto largest = [&](int c, const uint32_t *s) {
+                float t = -INFINITY;
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (!hidden(c, e) && !(bad >> e & 1)) t = fmaxf(t, __uint_as_float(s[e]));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) t = fmaxf(t, __uint_as_float(s[e]));
+                }
+                return t == -INFINITY ? t : t * f[c];
+            };
+            // The blocks' largest scores: the factor of the sums so far.
+            auto settle = [&](const float (&t)[kTileBlocks]) {
+                const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+                auto heaviest = [&]() {
+                    float x = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < kTileBlocks; ++c) x = fmaxf(x, t[c] - m + log2f(vs[c]));
+                    return x;
+                };
+                float z = 1.f;
+                if (__any_sync(0xffffffffu, top > m + kHeadroom || heaviest() > h + kHeadroom)) {
+                    if (top > m) {
+                        const float x = ceilf(top);
+                        l *= ex2(m - x);
+                        h -= x - m;
+                        m = x;
+                    }
+                    const float u = ceilf(heaviest());
+                    if (u > h) {
+                        z = ex2(h - u);
+                        h = u;
+                    }
+                    wf = weight_unit(h);
+                }
+                return z;
+            };
+            // Block c's products s to weights, two at a time to put(e, x0, x1), and the sum of 2^(score - m) to part.
+            // The score less m is one rounding: m by the fma; for f32 rows the scale's own rounding is added back.
+            auto weigh32 = [&](int c, const uint32_t *s, float (&part)[2], auto &&put) {
+                const float base = m == -INFINITY ? 0.f : m;
+                const float f_lo = LIMBS == 2 ? fmaf(ks[c], row_scale, -f[c]) : 0.f;
+                const bool deep = __any_sync(0xffffffffu, h < kDeep);
+                if (!masked && !deep) {
+                    const float g = vs[c] * wf;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float p[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float v = __uint_as_float(s[e + k]);
+                            float d = fmaf(v, f[c], -base);
+                            if (LIMBS == 2) d = fmaf(v, f_lo, d);
+                            p[k] = ex2(d);
+                            part[k] += p[k];
+                        }
+                        put(e, p[0] * g, p[1] * g);
+                    }
+                    return;
+                }
+                const float lift = deep && h != -INFINITY ? h : 0.f;
+                const float g = vs[c] * (deep && h != -INFINITY ? ex2(kWBits) : wf);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float x[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float v = __uint_as_float(s[e + k]);
+                        float d = fmaf(v, f[c], -base);
+                        if (LIMBS == 2) d = fmaf(v, f_lo, d);
+                        if (masked && (bad >> (e + k) & 1)) d = __int_as_float(0x7FC00000);
+                        float p = ex2(d);
+                        float z = p * g;
+                        if (deep) z = ex2(fminf(d - lift, 126.f)) * g;
+                        if (masked && hidden(c, e + k)) p = z = 0.f;  // (nor may a NaN scale reach it)
+                        part[k] += p;
+                        x[k] = z;
+                    }
+                    put(e, x[0], x[1]);
+                }
+            };
+            if constexpr (LIMBS == 2) {
+                if (j > 0) add_tile();
+                float t[kTileBlocks] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                const int parts = open ? 1 : kTileBlocks;
+                auto raw = [&](int c, uint32_t *s) {  // 32 products: of the open block, the two limbs' sums
+                    tmem_ld32(tS + 32 * c, s);
+                    if (open) {
+                        uint32_t s1[32];
+                        tmem_ld32(tS + 32, s1);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(s1[e]));
+                    } else {
+                        tmem_wait_ld();
+                    }
+                };
+#pragma unroll
+                for (int c = 0; c < kTileBlocks; ++c)
+                    if (c < parts) {
+                        uint32_t s[32];
+                        raw(c, s);
+                        t[c] = largest(c, s);
+                    }
+                const float z = settle(t);
+                if (__any_sync(0xffffffffu, z != 1.f)) {
+#pragma unroll
+                    for (int e = 0; e < HD; ++e) acc[e] *= z;
+                }
+                float l_tile = 0.f;
+                // the weights' limbs take the place of their scores: per 32 keys 16 columns of each
+#pragma unroll
+                for (int c = 0; c < kTileBlocks; ++c)
+                    if (c < parts) {
+                        uint32_t s[32], w[32];
+                        raw(c, s);
+                        float part[2] = {0.f, 0.f};
+                        weigh32(c, s, part, [&](int e, float x0, float x1) { split_f16(x0, x1, w[e / 2], w[16 + e / 2]); });
+                        l_tile += part[0] + part[1];
+                        tmem_st32(tS + 32 * c, w);
+                        if (open) tmem_st32(tS + 32, w);  // (the values' lower limbs)
+                    }
+                l += l_tile;
+            } else {
+                uint32_t s[kKeys];
+#pragma unroll
+                for (int c = 0; c < kTileBlocks; ++c) tmem_ld32(tS + 32 * c, s + 32 * c);
+                tmem_wait_ld();
+                if (open) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(s[32 + e]));
+                }
+                float t[kTileBlocks] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < kTileBlocks; ++c)
+                    if (c == 0 || !open) t[c] = largest(c, s + 32 * c);
+                const float z = settle(t);
+                if (j > 0 && __any_sync(0xffffffffu, z != 1.f)) {
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + 32 * c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * z);
+                        tmem_st32(tO + 32 * c, o);
+                    }
+                }
+                float l_tile = 0.f;
+                // 64 keys at a time: their weights take the place of the first half of their scores
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int c = 2 * u; c < 2 * u + 2; ++c) {
+                        uint32_t *wc = w + (c & 1) * 16;
+                        if (open && c > 0) {  // the values' lower limbs: the same weights; nothing beyond
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) wc[e] = c == 1 ? w[e] : 0u;
+                        } else {
+                            float part[2] = {0.f, 0.f};
+                            weigh32(c, s + 32 * c, part, [&](int e, float x0, float x1) { wc[e / 2] = pack_f16(x0, x1); });
+                            l_tile += part[0] + part[1];
+                        }
+                    }
+                    tmem_st32(tS + 32 * u, w);
+                }
+                l += l_tile;
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.p_full[i]);
+        }
+        if (n > 0) {
+            ok = __all_sync(0xffffffffu, ok && wait(&b.o_full[i], 0));
+            tc_fence_after();
+            add_tile();
+        }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;  // (a row that sees no key: zeros)
+        T *out = static_cast<T *>(a.out) + (int64_t)(row0 + tok) * a.out_stride + (int64_t)head * HD;
+        const T *gate = a.gate == nullptr ? nullptr
+                                          : static_cast<const T *>(a.gate) + (int64_t)(row0 + tok) * a.gate_stride + (int64_t)head * HD;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            if constexpr (LIMBS == 2) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(acc[32 * c + e]);
+            } else if (n > 0) {
+                tmem_ld32(tO + 32 * c, o);
+                tmem_wait_ld();
+            }
+            if (!live || !ok) continue;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = l == 0.f ? 0.f : weight_undo(__uint_as_float(o[e + k]), h) * inv;
+                if (gate != nullptr) {
+                    float g[8];
+                    load8<T>(g, gate + 32 * c + e, false);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] *= 1.0f / (1.0f + expf(-g[k]));
+                }
+                T *p = out + 32 * c + e;
+                if (a.vec) {
+                    if constexpr (sizeof(T) == 4) {
+                        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    } else {
+                        __nv_bfloat162 w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+                        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<uint4 *>(w);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        if constexpr (sizeof(T) == 4)
+                            p[k] = v[k];
+                        else
+                            p[k] = __float2bfloat16_rn(v[k]);
+                    }
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ------------------------------------ codes to f16 ------------------------------------
+        reg_dec<Regs<LIMBS>::convert>();
+        const int w = warp - 8;
+        // pieces of 16 codes: the 8 lanes of a store phase hold four pieces of two rows, whose 16-byte chunks
+        // the swizzle puts on distinct banks
+        constexpr int RPI = 8 / A;                  // rows per warp access
+        constexpr int U = kKeys / (4 * RPI);        // accesses per warp, operand and tile
+        const int pc = lane & 3, at = (lane >> 3) % A, rl = ((lane >> 2) & 1) + 2 * ((lane >> 3) / A);
+        const int src = (at * 4 + pc) * 16;
+        auto row_of = [&](int u) { return (u * 4 + w) * RPI + rl; };
+        auto store16 = [&](uint8_t *tile, int row, const uint32_t (&h)[8]) {
+            uint8_t *p = tile + at * (kKeys * 128) + row * 128;
+            *reinterpret_cast<uint4 *>(p + ((2 * pc) ^ (row & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4 *>(p + ((2 * pc + 1) ^ (row & 7)) * 16) = make_uint4(h[4], h[5], h[6], h[7]);
+        };
+        int pg[kTileBlocks];
+        auto pages = [&](int j) {
+#pragma unroll
+            for (int c = 0; c < kTileBlocks; ++c)
+                pg[c] = j < n_closed && j * kTileBlocks + c < blocks ? kv8_page(a.c, seq, j * kTileBlocks + c) : -1;
+        };
+        uint4 raw[U];
+        auto load = [&](const uint8_t *codes) {  // of the tile whose pages are in pg
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int row = row_of(u), p = pg[u * 4 * RPI / kKvBlock];
+                raw[u] = p >= 0 ? *reinterpret_cast<const uint4 *>(codes + kv8_codes_at(a.c, p, kh) + (row & 31) * HD + src)
+                                : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            }
+        };
+        auto convert = [&](uint8_t *tile) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t z[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                uint32_t h[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h[2 * e] = codes2(z[e], 0x4140);
+                    h[2 * e + 1] = codes2(z[e], 0x4342);
+                }
+                store16(tile, row_of(u), h);
+            }
+        };
+        static_assert(4 * RPI <= kKvBlock, "one access of the four warps lies in one block");
+        bool ok = true;
+        auto full = [&](uint64_t *bar) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        auto empty = [&](uint64_t *bar, int j) {  // the stage's former tile has been read
+            return j < ST || __all_sync(0xffffffffu, wait(bar, j / ST - 1));
+        };
+        const int n_c = min(n_all, n_closed);
+        if (n_c > 0) {
+            pages(0);
+            load(a.c.k_codes);
+        }
+        for (int j = 0; j < n_c && ok; ++j) {
+            const int st = j % ST;
+            if (!(ok = empty(&b.k_empty[st], j))) break;
+            if (w == 0 && lane < kTileBlocks) {
+                const int c = j * kTileBlocks + lane < blocks ? kv8_page(a.c, seq, j * kTileBlocks + lane) : -1;
+                const int64_t z = (int64_t)c * a.c.kv_heads + kh;
+                // no such block: its keys (masked by their position, or by the sign) give nothing
+                b.ks[j & 3][lane] = c >= 0 ? a.c.k_scale[z] : -1.f;
+                b.vs[j & 3][lane] = c >= 0 ? a.c.v_scale[z] : 0.f;
+            }
+            convert(sm + L::k + st * L::KV);
+            full(&b.k_full[st]);
+            load(a.c.v_codes);
+            if (!(ok = empty(&b.v_empty[st], j))) break;
+            convert(sm + L::v + st * L::KV);
+            full(&b.v_full[st]);
+            if (j + 1 < n_c) {
+                pages(j + 1);
+                load(a.c.k_codes);
+            }
+        }
+        if (ok && n_all > n_closed) {  // the open block: upper limbs in rows 0..31, lower in 32..63
+            const int j = n_closed, st = j % ST, there = kv_len - open0, slot = kv8_slot(a.c, seq);
+            __shared__ float s_max[2][4];
+            __shared__ unsigned s_bad[4];
+            // a thread per 16 values of a row
+            constexpr int PPR = HD / 16, RP = 128 / PPR;  // pieces per row, rows per step
+            const int tid = threadIdx.x - 256, piece = tid % PPR;
+            unsigned bad = 0;
+            float amax[2] = {0.f, 0.f};
+            auto piece_of = [&](int op, int t, float (&x)[16]) {
+                const float *p = (op ? a.c.v_open : a.c.k_open) + kv8_open_at(a.c, max(slot, 0), open0 / kKvBlock, kh) +
+                                 t * HD + piece * 16;
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4 z = slot >= 0 && t < there ? *reinterpret_cast<const float4 *>(p + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[e] = z.x, x[e + 1] = z.y, x[e + 2] = z.z, x[e + 3] = z.w;
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!(fabsf(x[e]) < INFINITY)) {
+                        bad |= 1u << t;
+                        x[e] = 0.f;
+                    }
+            };
+            for (int op = 0; op < 2; ++op)
+                for (int t = tid / PPR; t < kKvBlock; t += RP) {
+                    float x[16];
+                    piece_of(op, t, x);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) amax[op] = fmaxf(amax[op], fabsf(x[e]));
+                }
+            bad = __reduce_or_sync(0xffffffffu, bad);
+#pragma unroll
+            for (int op = 0; op < 2; ++op) {
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) amax[op] = fmaxf(amax[op], __shfl_xor_sync(0xffffffffu, amax[op], o));
+                if (lane == 0) s_max[op][w] = amax[op];
+            }
+            if (lane == 0) s_bad[w] = bad;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.open_max);
+            ok = __all_sync(0xffffffffu, wait(&b.open_max, 0));
+            float scale[2], inv[2];
+#pragma unroll
+            for (int op = 0; op < 2; ++op)
+                scale[op] = limb_scale(fmaxf(fmaxf(s_max[op][0], s_max[op][1]), fmaxf(s_max[op][2], s_max[op][3])), inv[op]);
+            ok = ok && empty(&b.k_empty[st], j);
+            if (ok && tid == 0) {
+                b.bad = slot >= 0 ? s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3] : 0;
+                b.ks[j & 3][0] = slot >= 0 ? inv[0] : 0.f;
+                b.vs[j & 3][0] = slot >= 0 ? inv[1] : 0.f;
+                for (int c = 1; c < kTileBlocks; ++c) b.ks[j & 3][c] = b.vs[j & 3][c] = 0.f;
+            }
+            for (int op = 0; op < 2 && ok; ++op) {
+                if (op == 1 && !(ok = empty(&b.v_empty[st], j))) break;
+                uint8_t *tile = sm + (op ? L::v : L::k) + st * L::KV;
+                for (int t = tid / PPR; t < kKvBlock; t += RP) {
+                    float x[16];
+                    piece_of(op, t, x);
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) split_f16(x[2 * e] * scale[op], x[2 * e + 1] * scale[op], hi[e], lo[e]);
+                    uint8_t *p = tile + piece / 4 * (kKeys * 128);
+                    const int c0 = (piece & 3) * 2;
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const uint32_t(&h)[8] = z ? lo : hi;
+                        const int row = t + 32 * z;
+                        *reinterpret_cast<uint4 *>(p + row * 128 + (c0 ^ (row & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4 *>(p + row * 128 + ((c0 + 1) ^ (row & 7)) * 16) = make_uint4(h[4], h[5], h[6], h[7]);
+                    }
+                }
+                full(op ? &b.v_full[st] : &b.k_full[st]);
+            }
+        }
+    } else {
+        // ------------------------------------ MMA issue ------------------------------------
+        reg_dec<Regs<LIMBS>::issue>();
+        if (warp == 12 && lane == 0) {
+            const uint32_t sq = smem_u32(sm + L::q), sk = smem_u32(sm + L::k), sv = smem_u32(sm + L::v);
+            auto scores = [&](int i, int j) {
+                uint32_t acc = 0;
+#pragma unroll 1
+                for (int z = LIMBS - 1; z >= 0; --z)  // (lower limbs first: fewer additions to a full-sized sum)
+#pragma unroll 1
+                    for (int at = 0; at < A; ++at)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            mma_ss(tmem + i * kTile + kS, desc_k(sq + (2 * z + i) * L::QT + at * (128 * 128) + 32 * k),
+                                   desc_k(sk + j % ST * L::KV + at * (kKeys * 128) + 32 * k), idesc(kKeys, false), acc);
+                            acc = 1;
+                        }
+                mma_commit(&b.s_full[i]);
+            };
+            auto values = [&](int i, int j) {
+                const int steps = 2 * tile_blocks(j);
+                uint32_t add = LIMBS == 2 ? 0u : (uint32_t)(j > 0);  // f32 rows: each tile's product by itself
+#pragma unroll 1
+                for (int z = LIMBS - 1; z >= 0; --z)
+#pragma unroll 1
+                    for (int k = 0; k < steps; ++k) {
+                        // 16 keys are 8 columns of P; two limbs: per 32 keys 16 columns of the upper, 16 of the lower
+                        mma_ts(tmem + i * kTile + kO, tmem + i * kTile + kS + (LIMBS == 2 ? k / 2 * 32 + k % 2 * 8 + 16 * z : 8 * k),
+                               desc_mn(sv + j % ST * L::KV + k * 2048, kKeys * 128), idesc(HD, true), add);
+                        add = 1;
+                    }
+            };
+            bool ok = n_all == 0 || (wait(&b.q_full, 0) && wait(&b.k_full[0], 0));
+            if (ok && n_all > 0) {
+                tc_fence_after();
+                for (int i = 0; i < 2; ++i)
+                    if (n_tiles[i] > 0) scores(i, 0);
+                mma_commit(&b.k_empty[0]);
+            }
+            for (int j = 0; j < n_all && ok; ++j) {
+                bool v = false, k = false;
+                for (int i = 0; i < 2 && ok; ++i) {
+                    if (j >= n_tiles[i]) continue;
+                    ok = wait(&b.p_full[i], j) && (v || wait(&b.v_full[j % ST], j / ST));
+                    if (!ok) break;
+                    v = true;
+                    tc_fence_after();
+                    values(i, j);
+                    if (j + 1 < n_tiles[i]) {
+                        ok = k || wait(&b.k_full[(j + 1) % ST], (j + 1) / ST);
+                        if (!ok) break;
+                        k = true;
+                        tc_fence_after();
+                        scores(i, j + 1);
+                    } else {
+                        mma_commit(&b.o_full[i]);
+                    }
+                }
+                mma_commit(&b.v_empty[j % ST]);
+                if (j + 1 < n_all) mma_commit(&b.k_empty[(j + 1) % ST]);
+            }
+            // every MMA has completed before TMEM is freed
+            mma_commit(&b.done);
+            mbar_wait(&b.done, 0u, a.c.err, kErrWaitFull);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int HD>
+cudaError_t launch_hd(const Kv8AttnArgs &a, int max_q_len, cudaStream_t s) {
+    constexpr int smem = Layout<HD, sizeof(T) == 4 ? 2 : 1>::bytes;
+    static_assert(smem <= 232448, "shared memory of one SM");
+    static std::atomic<uint64_t> ready{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load() >> dev & 1)) {
+        if ((e = cudaFuncSetAttribute(prompt_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess)
+            return e;
+        if (dev < 64) ready.fetch_or(1ull << dev);
+    }
+    const int64_t rows = (int64_t)max_q_len * (a.n_heads / a.c.kv_heads);
+    prompt_kernel<T, HD><<<dim3(a.c.kv_heads, a.c.n_seqs, (unsigned)((rows + kRows - 1) / kRows)), kThreads, smem, s>>>(a);
+    return cudaGetLastError();
+}
+}  // namespace
+
+bool kv8_prompt_takes(int head_dim) { return head_dim == 64 || head_dim == 128; }
+
+cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, int max_q_len, bool bf16, cudaStream_t s) {
+    if (a.c.head_dim == 64)
+        return bf16 ? launch_hd<__nv_bfloat16, 64>(a, max_q_len, s) : launch_hd<float, 64>(a, max_q_len, s);
+    return bf16 ? launch_hd<__nv_bfloat16, 128>(a, max_q_len, s) : launch_hd<float, 128>(a, max_q_len, s);
+}
+
+}  // namespace ql

@@ -81,3 +81,22 @@ def logits_rules(x, history=(), prompt_len=0, repetition=None, frequency=0.0, pr
         y[~allowed] = -np.inf
     z = np.where(np.isnan(y), -np.inf, y)
     return y, (int(np.argmax(z)) if z.max() > -np.inf else -1)
+
+
+def attend_rows(q, k, v, pos0, scale, gate=None):
+    """Rows q [n][nh][hd] at positions pos0, pos0 + 1, ..; k and v [kvh][keys][hd]."""
+    n, nh, hd = q.shape
+    g = nh // k.shape[0]
+    out = np.zeros((n, nh, hd))
+    pos = pos0 + np.arange(n)
+    seen = np.arange(k.shape[1])[None] <= pos[:, None]
+    for h in range(nh):
+        s = q[:, h].astype(np.float64) @ k[h // g].T * scale
+        s = np.where(seen, s, -np.inf)
+        m = s.max(1, keepdims=True)
+        p = np.exp(s - np.where(np.isfinite(m), m, 0))
+        t = p.sum(1, keepdims=True)
+        out[:, h] = p @ v[h // g] / np.where(t > 0, t, 1)
+    if gate is not None:
+        out = out / (1 + np.exp(-gate.astype(np.float64)))
+    return out

@@ -367,6 +367,85 @@ def test_attend_ragged_queries(nh, kvh, hd, t):
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("nh,kvh,hd", [(28, 4, 128), (14, 2, 64), (16, 2, 128), (3, 3, 64), (64, 2, 64), (8, 1, 256)])
+@pytest.mark.parametrize("gate", [False, True])
+def test_attend_prompts(nh, kvh, hd, t, gate):
+    """Prompts and later chunks of hundreds of tokens beside single tokens and a sequence without rows: full tiles of
+    keys, tiles that end inside one, an open block of 1 to 31 tokens or none, rows that end inside a tile."""
+    q_len = [300, 1, 0, 257, 129, 32, 64]
+    lens = [300, 1000, 64, 700, 129 + 96, 32, 1088]
+    c, stands = _filled(lens, 1100, kvh, hd, seed=hd + 3)
+    rng = np.random.default_rng(hd + 4)
+    starts = np.concatenate([[0], np.cumsum(q_len)])
+    qd, q = _dev(rng.standard_normal((starts[-1], nh * hd)) * 1.5, t)
+    gd, g = _dev(rng.standard_normal((starts[-1], nh * hd)), t)
+    got = _attend(c, t, qd, nh, _i32(lens), _i32(starts), max(q_len), max(lens), gate=gd if gate else None)
+    for s in range(len(lens)):
+        r = slice(starts[s], starts[s + 1])
+        if q_len[s] == 0:
+            continue
+        want = U.attend_rows(q[r].reshape(-1, nh, hd), *stands[s], lens[s] - q_len[s], hd ** -0.5,
+                             g[r].reshape(-1, nh, hd) if gate else None).reshape(-1, nh * hd)
+        for i in range(q_len[s]):
+            assert rel_l2(got[r][i], want[i]) < TOL[t], (s, i)
+    Q.check_device()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attend_prompt_scores_of_every_size_and_signs(hd):
+    """Scores of +-1e3, equal scores, tiny and huge queries, values whose scales lie 1e12 apart, a block of zeros, and a
+    negative softmax scale, in a prompt."""
+    nh, kvh, n = 8, 1, 300
+    c = Cache(1, n, kvh, hd, seed=41)
+    rng = np.random.default_rng(42)
+    k, v = rng.standard_normal((2, n, kvh, hd))
+    v[:64] *= 1e-6
+    v[64:96] *= 1e6
+    v[96:128] = 0
+    k[128:160] = 0
+    stands = [z.transpose(1, 0, 2) for z in c.set(0, k, v)]
+    q = rng.standard_normal((n, nh, hd)).astype(np.float32)
+    q[:, 1] *= 100
+    q[:, 2] = 0
+    q[:, 3] *= 1e-30
+    q[:, 4] = -q[:, 1]
+    for scale in (hd ** -0.5, -hd ** -0.5):
+        got = _attend(c, "f32", dev(q.reshape(n, -1)), nh, _i32([n]), _i32([0, n]), n, n, scale=scale).reshape(n, nh, hd)
+        want = U.attend_rows(q, *stands, 0, scale)
+        for h in range(nh):
+            s = np.abs(stands[0][0] @ q[:, h].T.astype(np.float64)).max() * hd ** -0.5
+            for i in range(n):
+                assert rel_l2(got[i, h], want[i, h]) < 2e-6 + s * 2.0 ** -21, (h, i)
+    Q.check_device()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_attend_prompt_nan_and_infinity(hd, t):
+    """As for the few rows below: what is not finite reaches exactly the rows that see it, in a prompt."""
+    nh, kvh = 4, 2
+    lens, q_len = [207, 207, 207, 207], [200, 200, 200, 200]
+    c, stands = _filled(lens, 224, kvh, hd, seed=43)
+    c.ko[int(c.slot[0]), 0, :, 10, 3] = float("nan")   # token 202
+    c.vo[int(c.slot[1]), 0, :, 10, 3] = float("-inf")  # token 202
+    c.vs[int(c.table[2, 1])] = float("nan")            # tokens 32 .. 63
+    c.ks[int(c.table[3, 5])] = float("nan")            # tokens 160 .. 191
+    c.ko[int(c.slot[3]), 0, :, 15:] = float("nan")     # past the end
+    c.vo[int(c.slot[3]), 0, :, 15:] = float("inf")
+    rng = np.random.default_rng(44)
+    starts = np.concatenate([[0], np.cumsum(q_len)])
+    qd, q = _dev(rng.standard_normal((800, nh * hd)), t)
+    got = _attend(c, t, qd, nh, _i32(lens), _i32(starts), 200, 207)
+    for s, first_bad in enumerate([202, 202, 32, 160]):
+        want = U.attend_rows(q[starts[s]:starts[s + 1]].reshape(-1, nh, hd), *stands[s], 7, hd ** -0.5).reshape(-1, nh * hd)
+        for i in range(200):
+            if 7 + i >= first_bad:
+                assert np.isnan(got[starts[s] + i]).all(), (s, i)
+            else:
+                assert rel_l2(got[starts[s] + i], want[i]) < TOL[t], (s, i)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_attend_long_cache(t):
     """20011 tokens of one sequence: many key splits, merged in a fixed order (twice the same bits)."""
     import torch
