@@ -22,6 +22,7 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "ql_kv8.cuh"
 
@@ -104,6 +105,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *v) {
         "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 template <int N>
@@ -136,12 +145,6 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // As in the split kernel: 2^(kWBits - h), 0 while nothing but zeros has been met (h = -inf).
 __device__ __forceinline__ float weight_unit(float h) { return h == -INFINITY ? 0.f : ex2(kWBits - h); }
-// What turns sums of w 2^(s - m) sv code into sums of 2^(s - m) sv code: x 2^(h - kWBits), in two steps where
-// the power leaves the range.
-__device__ __forceinline__ float weight_undo(float x, float h) {
-    const float e = h - kWBits;
-    return h == -INFINITY ? x * 0.f : x * ex2(fmaxf(e, -120.f)) * ex2(fminf(e + 120.f, 0.f));  // (NaN stays)
-}
 // Below this h the weights' factor sv w leaves the range, and 2^(s - m) with it, where the weights themselves
 // do not (the row's heaviest keys have values of zero): they are computed from s - m - h then.
 constexpr float kDeep = -60.0f;
@@ -169,6 +172,10 @@ __device__ __forceinline__ float limb_scale(float amax, float &inv) {  // as in 
     inv = __uint_as_float((uint32_t)(254 - f) << 23);
     return __uint_as_float((uint32_t)f << 23);
 }
+__device__ __forceinline__ float2 ffma2_of(float2 a, float2 b, float2 c) {
+    ffma2(c, a, b);
+    return c;
+}
 template <typename T>
 __device__ __forceinline__ void load8(float *x, const T *p, bool vec) {
     if (vec) {
@@ -195,6 +202,32 @@ __device__ __forceinline__ void load8(float *x, const T *p, bool vec) {
     }
 }
 
+// V (2 or 4) elements of one lane's part of a row, as loaded.
+template <int V, typename T>
+struct Few {
+    using P = typename std::conditional<V * sizeof(T) == 16, uint4,
+                                        typename std::conditional<V * sizeof(T) == 8, uint2, uint32_t>::type>::type;
+    P raw;
+    __device__ __forceinline__ void load(const T *p, bool vec, bool there) {
+        T e[V];
+        if (!there) {
+            memset(&raw, 0, sizeof(raw));
+        } else if (vec) {
+            raw = *reinterpret_cast<const P *>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) e[i] = p[i];
+            memcpy(&raw, e, sizeof(raw));
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[V]) const {
+        T e[V];
+        memcpy(e, &raw, sizeof(raw));
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = (float)e[i];
+    }
+};
+
 struct Bars {
     uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], open_max, done;
     uint32_t tmem;
@@ -202,7 +235,8 @@ struct Bars {
     // Scales of the tile's blocks (K's < 0: no such block), a ring: when the scores of the tile ST before have been
     // computed, its rows may still have to read them, so ST + 1 tiles are in use.
     float ks[4][kTileBlocks], vs[4][kTileBlocks];
-    unsigned bad;                                  // tokens of the open block that hold NaN or infinity
+    int plain[4];   // every block of the tile is there, its scales positive and finite
+    unsigned bad;   // tokens of the open block that hold NaN or infinity
 };
 static_assert(sizeof(Bars) <= 512, "Bars at the end of shared memory");
 
@@ -273,34 +307,42 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const int i = warp >> 2, r = threadIdx.x & 127, gr = r_base + 128 * i + r;
         const bool live = gr < n_rows;
         const int tok = live ? gr / G : 0, head = kh * G + (live ? gr % G : 0);
-        const int pos = live ? kv_len - q_len + tok : -1;  // the last key that the row sees
-        float row_scale;
+        // the last key that the row sees (past the rows' end: a row of zeros, kept on the others' paths)
+        const int pos = live ? kv_len - q_len + tok : kv_len - 1;
+        float row_scale = 0.f;
         {
-            const T *q = static_cast<const T *>(a.q) + (int64_t)(row0 + tok) * a.q_stride + (int64_t)head * HD;
-            float amax = 0.f, inv;
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                load8<T>(x, q + d, a.vec);
+            // Q: the warp's 32 rows one after another, a row over the lanes, 16 rows' loads in flight
+            constexpr int V = HD / 32, B = 16;
+            const int64_t mine = (int64_t)(row0 + tok) * a.q_stride + (int64_t)head * HD;
+#pragma unroll 1
+            for (int k0 = 0; k0 < 32; k0 += B) {
+                Few<V, T> raw[B];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-            }
-            // (a negative softmax scale: its sign goes to q, so that scores and products order alike)
-            const float f = copysignf(limb_scale(amax, inv), a.scale_log2);
-            row_scale = fabsf(a.scale_log2) * inv;
-#pragma unroll 2
-            for (int d = 0; d < HD; d += 8) {
-                float x[8];
-                load8<T>(x, q + d, a.vec);
-                uint4 hi, lo;
+                for (int k = 0; k < B; ++k) {
+                    const T *q = static_cast<const T *>(a.q) + __shfl_sync(0xffffffffu, mine, k0 + k) + lane * V;
+                    raw[k].load(q, a.vec, r_base + 128 * i + 32 * (warp & 3) + k0 + k < n_rows);
+                }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = live ? x[e] * f : 0.f;
-                split_f16(x[0], x[1], hi.x, lo.x);
-                split_f16(x[2], x[3], hi.y, lo.y);
-                split_f16(x[4], x[5], hi.z, lo.z);
-                split_f16(x[6], x[7], hi.w, lo.w);
-                uint8_t *p = sm + L::q + i * L::QT + d / 64 * (128 * 128) + r * 128 + ((d / 8 & 7) ^ (r & 7)) * 16;
-                *reinterpret_cast<uint4 *>(p) = hi;
-                if (LIMBS == 2) *reinterpret_cast<uint4 *>(p + 2 * L::QT) = lo;
+                for (int k = 0; k < B; ++k) {
+                    float x[V], inv;
+                    raw[k].get(x);
+                    uint32_t bits = 0;  // (magnitudes order like their bits; NaN above all)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) bits = max(bits, __float_as_uint(fabsf(x[e])));
+                    const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, bits));
+                    // (a negative softmax scale: its sign goes to q, so that scores and products order alike)
+                    const float f = copysignf(limb_scale(amax, inv), a.scale_log2);
+                    if (lane == k0 + k) row_scale = fabsf(a.scale_log2) * (amax > 0.f ? inv : 1.f);
+                    const int rr = 32 * (warp & 3) + k0 + k, d = lane * V;
+                    uint8_t *p = sm + L::q + i * L::QT + d / 64 * (128 * 128) + rr * 128 + ((d / 8 & 7) ^ (rr & 7)) * 16 + d % 8 * 2;
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) {
+                        uint32_t hi, lo;
+                        split_f16(x[2 * e] * f, x[2 * e + 1] * f, hi, lo);
+                        reinterpret_cast<uint32_t *>(p)[e] = hi;
+                        if (LIMBS == 2) reinterpret_cast<uint32_t *>(p + 2 * L::QT)[e] = lo;
+                    }
+                }
             }
         }
         fence_proxy_async_smem();
@@ -325,7 +367,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     tmem_ld32(tO + 32 * c, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) acc[32 * c + e] += __uint_as_float(o[e]);
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 z = fadd2(make_float2(acc[32 * c + e], acc[32 * c + e + 1]),
+                                               make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])));
+                        acc[32 * c + e] = z.x, acc[32 * c + e + 1] = z.y;
+                    }
                 }
             }
         };
@@ -334,192 +380,229 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             ok = __all_sync(0xffffffffu, wait(&b.k_full[j % ST], j / ST) && wait(&b.s_full[i], j));
             if (!ok) break;
             tc_fence_after();  // (S full: the earlier products into O have completed too)
+            if (LIMBS == 2 && j > 0) add_tile();
             const bool open = j == n_closed;
-            const int key0 = open ? open0 : j * kKeys;
-            float ks[kTileBlocks], f[kTileBlocks], vs[kTileBlocks];
-            bool holes = false;  // blocks whose page is not there
-#pragma unroll
-            for (int c = 0; c < kTileBlocks; ++c) {
-                ks[c] = b.ks[j & 3][c];
-                f[c] = ks[c] * row_scale;
-                vs[c] = b.vs[j & 3][c];
-                holes |= f[c] < 0.f;
+            // the last key of the tile that the row sees (a closed tile ends with the closed blocks)
+            const int see = open ? pos - open0 : min(pos, open0 - 1) - j * kKeys;
+            const float *ks = b.ks[j & 3], *vs = b.vs[j & 3];
+            // (per warp) ordinary: all of the tile's scales are positive and finite
+            const bool masked = __any_sync(0xffffffffu, see < kKeys - 1);
+            bool plain = b.plain[j & 3] && a.scale_log2 != 0.f;
+            if (plain && masked) {  // hidden scores have to end far below the others
+                const float least = fminf(fminf(ks[0], ks[1]), fminf(ks[2], ks[3])) * row_scale;
+                plain = __all_sync(0xffffffffu, least > 1e-30f);
             }
-            // (per warp) some row hides a key, or the tile is out of the ordinary
-            const bool masked = __any_sync(0xffffffffu, key0 + kKeys - 1 > pos || holes || open);
+
+            // Largest score of each block.
+            float t[kTileBlocks] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            // 32 products as they came; the open block's: the two limbs' sums
+            auto raw = [&](int c, uint32_t *s) {
+                tmem_ld32(tS + 32 * c, s);
+                if (open) {
+                    uint32_t s1[32];
+                    tmem_ld32(tS + 32, s1);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(s1[e]));
+                } else {
+                    tmem_wait_ld();
+                }
+            };
+            auto hide = [&](int c, uint32_t *s) {  // keys that the row does not see: the lowest finite (x f below: plain)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (32 * c + e > see) s[e] = 0xFF7FFFFFu;
+            };
+            auto top32 = [](const uint32_t *s) {
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(s[e]));
+                return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            };
+            const int parts = open ? 1 : kTileBlocks;
             const unsigned bad = open ? b.bad : 0;
-            auto hidden = [&](int c, int e) { return key0 + 32 * c + e > pos || f[c] < 0.f; };
-            // the largest of block c's 32 scores, in units of log2
-            auto largest = [&](int c, const uint32_t *s) {
-                float t = -INFINITY;
-                if (masked) {
+            if (plain) {
+                // (loops kept rolled: the roles share the instruction cache)
+#pragma unroll 1
+                for (int c = 0; c < kTileBlocks; c += 2) {
+                    uint32_t s[64];
+                    tmem_ld32(tS + 32 * c, s);
+                    tmem_ld32(tS + 32 * c + 32, s + 32);
+                    tmem_wait_ld();
+                    if (masked) {
+                        hide(c, s);
+                        hide(c + 1, s + 32);
+                    }
+                    float x0 = top32(s) * (ks[c] * row_scale), x1 = top32(s + 32) * (ks[c + 1] * row_scale);
+                    if (32 * c > see) x0 = -INFINITY;
+                    if (32 * c + 32 > see) x1 = -INFINITY;
+                    if (c == 0)
+                        t[0] = x0, t[1] = x1;
+                    else
+                        t[2] = x0, t[3] = x1;
+                }
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < parts; ++c) {
+                    uint32_t s[32];
+                    raw(c, s);
+                    float x = -INFINITY;
+                    const float f = ks[c] * row_scale;
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
-                        if (!hidden(c, e) && !(bad >> e & 1)) t = fmaxf(t, __uint_as_float(s[e]));
-                } else {
+                        if (32 * c + e <= see && !(bad >> e & 1)) x = fmaxf(x, __uint_as_float(s[e]));
+                    x = x == -INFINITY || f < 0.f ? -INFINITY : x * f;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) t = fmaxf(t, __uint_as_float(s[e]));
+                    for (int k = 0; k < kTileBlocks; ++k)
+                        if (k == c) t[k] = x;
                 }
-                return t == -INFINITY ? t : t * f[c];
-            };
-            // The blocks' largest scores: the factor of the sums so far.
-            auto settle = [&](const float (&t)[kTileBlocks]) {
+            }
+            // The factor of the sums so far.
+            float z = 1.f;
+            {
                 const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-                auto heaviest = [&]() {
-                    float x = -INFINITY;
+                float u = -INFINITY;  // log2 of the heaviest weight x scale, m aside
 #pragma unroll
-                    for (int c = 0; c < kTileBlocks; ++c) x = fmaxf(x, t[c] - m + log2f(vs[c]));
-                    return x;
-                };
-                float z = 1.f;
-                if (__any_sync(0xffffffffu, top > m + kHeadroom || heaviest() > h + kHeadroom)) {
+                for (int c = 0; c < kTileBlocks; ++c) u = fmaxf(u, t[c] + __log2f(vs[c]));
+                if (__any_sync(0xffffffffu, top > m + kHeadroom || u - m > h + kHeadroom)) {
                     if (top > m) {
                         const float x = ceilf(top);
                         l *= ex2(m - x);
                         h -= x - m;
                         m = x;
                     }
-                    const float u = ceilf(heaviest());
+                    u = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < kTileBlocks; ++c) u = fmaxf(u, t[c] - m + __log2f(vs[c]));
+                    u = ceilf(u);
                     if (u > h) {
                         z = ex2(h - u);
                         h = u;
                     }
                     wf = weight_unit(h);
-                }
-                return z;
-            };
-            // Block c's products s to weights, two at a time to put(e, x0, x1), and the sum of 2^(score - m) to part.
-            // The score less m is one rounding: m by the fma; for f32 rows the scale's own rounding is added back.
-            auto weigh32 = [&](int c, const uint32_t *s, float (&part)[2], auto &&put) {
-                const float base = m == -INFINITY ? 0.f : m;
-                const float f_lo = LIMBS == 2 ? fmaf(ks[c], row_scale, -f[c]) : 0.f;
-                const bool deep = __any_sync(0xffffffffu, h < kDeep);
-                if (!masked && !deep) {
-                    const float g = vs[c] * wf;
+                    if (__any_sync(0xffffffffu, z != 1.f)) {
+                        if constexpr (LIMBS == 2) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float p[2];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const float v = __uint_as_float(s[e + k]);
-                            float d = fmaf(v, f[c], -base);
-                            if (LIMBS == 2) d = fmaf(v, f_lo, d);
-                            p[k] = ex2(d);
-                            part[k] += p[k];
-                        }
-                        put(e, p[0] * g, p[1] * g);
-                    }
-                    return;
-                }
-                const float lift = deep && h != -INFINITY ? h : 0.f;
-                const float g = vs[c] * (deep && h != -INFINITY ? ex2(kWBits) : wf);
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float x[2];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float v = __uint_as_float(s[e + k]);
-                        float d = fmaf(v, f[c], -base);
-                        if (LIMBS == 2) d = fmaf(v, f_lo, d);
-                        if (masked && (bad >> (e + k) & 1)) d = __int_as_float(0x7FC00000);
-                        float p = ex2(d);
-                        float z = p * g;
-                        if (deep) z = ex2(fminf(d - lift, 126.f)) * g;
-                        if (masked && hidden(c, e + k)) p = z = 0.f;  // (nor may a NaN scale reach it)
-                        part[k] += p;
-                        x[k] = z;
-                    }
-                    put(e, x[0], x[1]);
-                }
-            };
-            if constexpr (LIMBS == 2) {
-                if (j > 0) add_tile();
-                float t[kTileBlocks] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                const int parts = open ? 1 : kTileBlocks;
-                auto raw = [&](int c, uint32_t *s) {  // 32 products: of the open block, the two limbs' sums
-                    tmem_ld32(tS + 32 * c, s);
-                    if (open) {
-                        uint32_t s1[32];
-                        tmem_ld32(tS + 32, s1);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(s1[e]));
-                    } else {
-                        tmem_wait_ld();
-                    }
-                };
-#pragma unroll
-                for (int c = 0; c < kTileBlocks; ++c)
-                    if (c < parts) {
-                        uint32_t s[32];
-                        raw(c, s);
-                        t[c] = largest(c, s);
-                    }
-                const float z = settle(t);
-                if (__any_sync(0xffffffffu, z != 1.f)) {
-#pragma unroll
-                    for (int e = 0; e < HD; ++e) acc[e] *= z;
-                }
-                float l_tile = 0.f;
-                // the weights' limbs take the place of their scores: per 32 keys 16 columns of each
-#pragma unroll
-                for (int c = 0; c < kTileBlocks; ++c)
-                    if (c < parts) {
-                        uint32_t s[32], w[32];
-                        raw(c, s);
-                        float part[2] = {0.f, 0.f};
-                        weigh32(c, s, part, [&](int e, float x0, float x1) { split_f16(x0, x1, w[e / 2], w[16 + e / 2]); });
-                        l_tile += part[0] + part[1];
-                        tmem_st32(tS + 32 * c, w);
-                        if (open) tmem_st32(tS + 32, w);  // (the values' lower limbs)
-                    }
-                l += l_tile;
-            } else {
-                uint32_t s[kKeys];
-#pragma unroll
-                for (int c = 0; c < kTileBlocks; ++c) tmem_ld32(tS + 32 * c, s + 32 * c);
-                tmem_wait_ld();
-                if (open) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(s[32 + e]));
-                }
-                float t[kTileBlocks] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < kTileBlocks; ++c)
-                    if (c == 0 || !open) t[c] = largest(c, s + 32 * c);
-                const float z = settle(t);
-                if (j > 0 && __any_sync(0xffffffffu, z != 1.f)) {
+                            for (int e = 0; e < HD; ++e) acc[e] *= z;
+                        } else if (j > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < HD / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(tO + 32 * c, o);
-                        tmem_wait_ld();
+                            for (int c = 0; c < HD / 32; ++c) {
+                                uint32_t o[32];
+                                tmem_ld32(tO + 32 * c, o);
+                                tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * z);
-                        tmem_st32(tO + 32 * c, o);
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * z);
+                                tmem_st32(tO + 32 * c, o);
+                            }
+                        }
                     }
                 }
-                float l_tile = 0.f;
-                // 64 keys at a time: their weights take the place of the first half of their scores
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+            const bool deep = __any_sync(0xffffffffu, h < kDeep && h != -INFINITY);
+            float2 sum = make_float2(0.f, 0.f);
+            // Weights take the place of scores: one limb, 16 columns per 32 keys from column 16 c; two limbs, 16 of
+            // the upper and 16 of the lower from column 32 c.
+            if (plain && !deep) {
+                auto weigh = [&](int c, const uint32_t *s) {
+                    const float f = ks[c] * row_scale, g = vs[c] * wf;
+                    // (the scale's own rounding is added back for f32 rows)
+                    const float f_lo = LIMBS == 2 ? fmaf(ks[c], row_scale, -f) : 0.f;
+                    const float2 f2 = make_float2(f, f), fl2 = make_float2(f_lo, f_lo), b2 = make_float2(-base, -base);
+                    const float2 g2 = make_float2(g, g);
                     uint32_t w[32];
 #pragma unroll
-                    for (int c = 2 * u; c < 2 * u + 2; ++c) {
-                        uint32_t *wc = w + (c & 1) * 16;
-                        if (open && c > 0) {  // the values' lower limbs: the same weights; nothing beyond
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 v = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                        float2 d = ffma2_of(v, f2, b2);
+                        if (LIMBS == 2) d = ffma2_of(v, fl2, d);
+                        const float2 p = make_float2(ex2(d.x), ex2(d.y));
+                        sum = fadd2(sum, p);
+                        const float2 x = fmul2(p, g2);
+                        if (LIMBS == 2)
+                            split_f16(x.x, x.y, w[e / 2], w[16 + e / 2]);
+                        else
+                            w[e / 2] = pack_f16(x.x, x.y);
+                    }
+                    if (LIMBS == 2)
+                        tmem_st32(tS + 32 * c, w);
+                    else
+                        tmem_st16(tS + 16 * c, w);
+                };
+                if constexpr (LIMBS == 2) {
+#pragma unroll 1
+                    for (int c = 0; c < kTileBlocks; ++c) {
+                        uint32_t s[32];
+                        tmem_ld32(tS + 32 * c, s);
+                        tmem_wait_ld();
+                        if (masked) hide(c, s);
+                        weigh(c, s);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < kTileBlocks; c += 2) {
+                        uint32_t s[64];
+                        tmem_ld32(tS + 32 * c, s);
+                        tmem_ld32(tS + 32 * c + 32, s + 32);
+                        tmem_wait_ld();
+                        if (masked) {
+                            hide(c, s);
+                            hide(c + 1, s + 32);
+                        }
+                        weigh(c, s);
+                        weigh(c + 1, s + 32);
+                    }
+                }
+            } else {
+                // (the open block, scales of zero or NaN, pages that are not there, rows whose heaviest keys have no value)
+#pragma unroll 1
+                for (int c = 0; c < parts; ++c) {
+                    uint32_t s[32], w[32];
+                    raw(c, s);
+                    const float f = ks[c] * row_scale, f_lo = LIMBS == 2 ? fmaf(ks[c], row_scale, -f) : 0.f;
+                    const float g = vs[c] * wf, nan = __int_as_float(0x7FC00000);
+                    const int last = f < 0.f ? -1 : see - 32 * c;
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) wc[e] = c == 1 ? w[e] : 0u;
-                        } else {
-                            float part[2] = {0.f, 0.f};
-                            weigh32(c, s + 32 * c, part, [&](int e, float x0, float x1) { wc[e / 2] = pack_f16(x0, x1); });
-                            l_tile += part[0] + part[1];
+                    for (int e = 0; e < 32; ++e) {
+                        float d = fmaf(__uint_as_float(s[e]), f, -base);
+                        if (LIMBS == 2) d = fmaf(__uint_as_float(s[e]), f_lo, d);
+                        if (bad >> e & 1) d = nan;
+                        s[e] = __float_as_uint(e <= last ? d : -INFINITY);
+                    }
+                    if (!deep) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float p = ex2(__uint_as_float(s[e]));
+                            sum.x += p;
+                            s[e] = __float_as_uint(e <= last ? p * g : 0.f);  // (nor may a NaN scale reach others)
+                        }
+                    } else {
+                        const bool lift = h != -INFINITY;
+                        const float gl = lift ? vs[c] * ex2(kWBits) : g, up = lift ? h : 0.f;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float d = __uint_as_float(s[e]);
+                            sum.x += ex2(d);
+                            s[e] = __float_as_uint(e <= last ? ex2(fminf(d - up, 126.f)) * gl : 0.f);
                         }
                     }
-                    tmem_st32(tS + 32 * u, w);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        if (LIMBS == 2)
+                            split_f16(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), w[e / 2], w[16 + e / 2]);
+                        else
+                            w[e / 2] = pack_f16(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                    }
+                    if (LIMBS == 2) {
+                        tmem_st32(tS + 32 * c, w);
+                        if (open) tmem_st32(tS + 32, w);  // the values' lower limbs: the same weights
+                    } else {
+                        tmem_st16(tS + 16 * c, w);
+                        if (open) tmem_st16(tS + 16, w);
+                    }
                 }
-                l += l_tile;
             }
+            l += sum.x + sum.y;
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -530,7 +613,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             tc_fence_after();
             add_tile();
         }
-        const float inv = l == 0.f ? 0.f : 1.0f / l;  // (a row that sees no key: zeros)
+        // sums to the result: x 2^(h - kWBits) / l, the power in two steps where it leaves the range
+        const float e0 = h - kWBits, u0 = h == -INFINITY ? 0.f : ex2(fmaxf(e0, -120.f));
+        const float u1 = (l == 0.f ? 0.f : 1.0f / l) * (h == -INFINITY ? 1.f : ex2(fminf(e0 + 120.f, 0.f)));
         T *out = static_cast<T *>(a.out) + (int64_t)(row0 + tok) * a.out_stride + (int64_t)head * HD;
         const T *gate = a.gate == nullptr ? nullptr
                                           : static_cast<const T *>(a.gate) + (int64_t)(row0 + tok) * a.gate_stride + (int64_t)head * HD;
@@ -549,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             for (int e = 0; e < 32; e += 8) {
                 float v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = l == 0.f ? 0.f : weight_undo(__uint_as_float(o[e + k]), h) * inv;
+                for (int k = 0; k < 8; ++k) v[k] = l == 0.f ? 0.f : __uint_as_float(o[e + k]) * u0 * u1;  // (sees no key: zeros)
                 if (gate != nullptr) {
                     float g[8];
                     load8<T>(g, gate + 32 * c + e, false);
@@ -594,14 +679,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             *reinterpret_cast<uint4 *>(p + ((2 * pc) ^ (row & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<uint4 *>(p + ((2 * pc + 1) ^ (row & 7)) * 16) = make_uint4(h[4], h[5], h[6], h[7]);
         };
+        constexpr bool kBoth = LIMBS == 1;  // registers for both operands' next tile (f32: one at a time, twice the time)
         int pg[kTileBlocks];
         auto pages = [&](int j) {
 #pragma unroll
             for (int c = 0; c < kTileBlocks; ++c)
                 pg[c] = j < n_closed && j * kTileBlocks + c < blocks ? kv8_page(a.c, seq, j * kTileBlocks + c) : -1;
         };
-        uint4 raw[U];
-        auto load = [&](const uint8_t *codes) {  // of the tile whose pages are in pg
+        uint4 raw_k[U], raw_v[kBoth ? U : 1];
+        auto load = [&](uint4 *raw, const uint8_t *codes) {  // of the tile whose pages are in pg
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int row = row_of(u), p = pg[u * 4 * RPI / kKvBlock];
@@ -609,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                                 : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
             }
         };
-        auto convert = [&](uint8_t *tile) {
+        auto convert = [&](const uint4 *raw, uint8_t *tile) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t z[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
@@ -623,6 +709,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
         };
         static_assert(4 * RPI <= kKvBlock, "one access of the four warps lies in one block");
+        // scales of a tile's blocks (lanes 0 .. 3 of the first warp)
+        float next_ks = -1.f, next_vs = 0.f;
+        auto scales = [&](int j) {
+            if (w != 0 || lane >= kTileBlocks) return;
+            if (j * kTileBlocks + lane >= blocks) {  // past the closed blocks: all of its keys are hidden by their position
+                next_ks = next_vs = 1.f;
+                return;
+            }
+            const int c = kv8_page(a.c, seq, j * kTileBlocks + lane);
+            const int64_t z = (int64_t)c * a.c.kv_heads + kh;
+            // (no such page: its keys are hidden by the sign)
+            next_ks = c >= 0 ? a.c.k_scale[z] : -1.f;
+            next_vs = c >= 0 ? a.c.v_scale[z] : 0.f;
+        };
         bool ok = true;
         auto full = [&](uint64_t *bar) {
             fence_proxy_async_smem();
@@ -635,27 +735,42 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const int n_c = min(n_all, n_closed);
         if (n_c > 0) {
             pages(0);
-            load(a.c.k_codes);
+            load(raw_k, a.c.k_codes);
+            if (kBoth) load(raw_v, a.c.v_codes);
+            scales(0);
+            if (kBoth) pages(1);
         }
         for (int j = 0; j < n_c && ok; ++j) {
             const int st = j % ST;
             if (!(ok = empty(&b.k_empty[st], j))) break;
-            if (w == 0 && lane < kTileBlocks) {
-                const int c = j * kTileBlocks + lane < blocks ? kv8_page(a.c, seq, j * kTileBlocks + lane) : -1;
-                const int64_t z = (int64_t)c * a.c.kv_heads + kh;
-                // no such block: its keys (masked by their position, or by the sign) give nothing
-                b.ks[j & 3][lane] = c >= 0 ? a.c.k_scale[z] : -1.f;
-                b.vs[j & 3][lane] = c >= 0 ? a.c.v_scale[z] : 0.f;
+            if (w == 0) {
+                const bool good = next_ks > 0.f && next_ks < INFINITY && next_vs > 0.f && next_vs < INFINITY;
+                if (lane < kTileBlocks) {
+                    b.ks[j & 3][lane] = next_ks;
+                    b.vs[j & 3][lane] = next_vs;
+                }
+                const unsigned all = __ballot_sync(0xffffffffu, good);
+                if (lane == 0) b.plain[j & 3] = (all & 15u) == 15u;
             }
-            convert(sm + L::k + st * L::KV);
+            convert(raw_k, sm + L::k + st * L::KV);
             full(&b.k_full[st]);
-            load(a.c.v_codes);
+            if (kBoth) {
+                if (j + 1 < n_c) load(raw_k, a.c.k_codes);
+            } else {
+                load(raw_k, a.c.v_codes);
+            }
+            if (j + 1 < n_c) scales(j + 1);
             if (!(ok = empty(&b.v_empty[st], j))) break;
-            convert(sm + L::v + st * L::KV);
+            convert(kBoth ? raw_v : raw_k, sm + L::v + st * L::KV);
             full(&b.v_full[st]);
             if (j + 1 < n_c) {
-                pages(j + 1);
-                load(a.c.k_codes);
+                if (kBoth) {
+                    load(raw_v, a.c.v_codes);
+                    pages(j + 2);
+                } else {
+                    pages(j + 1);
+                    load(raw_k, a.c.k_codes);
+                }
             }
         }
         if (ok && n_all > n_closed) {  // the open block: upper limbs in rows 0..31, lower in 32..63
@@ -710,6 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 b.ks[j & 3][0] = slot >= 0 ? inv[0] : 0.f;
                 b.vs[j & 3][0] = slot >= 0 ? inv[1] : 0.f;
                 for (int c = 1; c < kTileBlocks; ++c) b.ks[j & 3][c] = b.vs[j & 3][c] = 0.f;
+                b.plain[j & 3] = 0;
             }
             for (int op = 0; op < 2 && ok; ++op) {
                 if (op == 1 && !(ok = empty(&b.v_empty[st], j))) break;
