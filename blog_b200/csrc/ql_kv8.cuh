@@ -51,7 +51,7 @@ struct Kv8AttnArgs {
     float scale_log2;  // softmax scale x log2(e)
     bool vec;          // q and out: every row starts on 16 bytes
     int splits;        // CTAs over the keys of one (sequence, KV head, row group): clusters of `cluster`
-    int cluster;       // 1, 2, 4 or 8
+    int cluster;       // 1, 2, 4 or 8 (prompts: 1 to 8, all of the splits)
     int row_groups;    // groups of 8 (query token, head of the KV head's group) rows per sequence
     unsigned *arrivals;  // [n_seqs x kv_heads x row_groups][8] zero between calls (several clusters)
     float *part;         // [...][clusters][8][head_dim + 4]
@@ -113,6 +113,7 @@ cudaError_t kv8_gather_launch(const Kv8View &c, const int *kv_len, const int *st
 cudaError_t kv8_attn_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s);
 // The tensor-core form for prompts (ql_kv8_prompt.cu).
 bool kv8_prompt_takes(int head_dim);
+unsigned kv8_prompt_row_tiles(int max_q_len, int group);  // CTAs over one (sequence, KV head)'s rows
 cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, int max_q_len, bool bf16, cudaStream_t s);
 
 // CTAs of the attention's split kernel that one SM holds (the host sizes the split count by it).

@@ -17,14 +17,20 @@
 // threads exponentiate, the tensor cores run the other tile's products.
 // The rows of the block that is not full make a last tile of 64 keys: their upper f16 limbs, then their lower.
 //
+// Where the tiles of rows alone would leave SMs idle, the keys are split over the CTAs of a cluster, and their
+// sums are joined through distributed shared memory, each CTA finishing its share of the rows.
+//
 // Bound: the tensor cores (4 head_dim flops per row and key, twice that for f32), with the exponentials (16 per
 // clock and SM) close behind.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include <atomic>
 #include <type_traits>
 
 #include "ql_kv8.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace ql {
 namespace {
@@ -38,7 +44,7 @@ constexpr float kHeadroom = 7.0f, kWBits = 8.0f;  // as in the split kernel
 // Registers per thread of the roles; 16 warps launch with 128 each.
 template <int LIMBS>
 struct Regs {
-    static constexpr int softmax = LIMBS == 2 ? 208 : 184, convert = LIMBS == 2 ? 64 : 104, issue = LIMBS == 2 ? 32 : 40;
+    static constexpr int softmax = LIMBS == 2 ? 200 : 184, convert = LIMBS == 2 ? 80 : 104, issue = LIMBS == 2 ? 32 : 40;
     static_assert(2 * softmax + convert + issue == 4 * 128, "the block's registers at launch");
 };
 
@@ -91,6 +97,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *v) {
           "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
           "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t *v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr)
         : "memory");
 }
@@ -246,13 +261,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     using L = Layout<HD, LIMBS>;
     constexpr int A = L::A, ST = L::ST;
     constexpr uint32_t kS = 0, kO = kKeys, kTile = 256;  // TMEM columns of a tile: S (then P), O
+    constexpr int kPitch = HD + 4;                       // floats of a row's sums in shared memory at the end
+    static_assert(kRows * kPitch * 4 <= L::end, "the sums take the operands' place");
     extern __shared__ uint8_t sm_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     Bars &b = *reinterpret_cast<Bars *>(sm + L::end);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.n_heads / a.c.kv_heads;
-    const int kh = blockIdx.x, seq = blockIdx.y, r_base = (gridDim.z - 1 - blockIdx.z) * kRows;  // longest first
+    const int split = blockIdx.x % a.cluster, kh = blockIdx.x / a.cluster, seq = blockIdx.y, r_base = (gridDim.z - 1 - blockIdx.z) * kRows;  // longest first
     int row0, q_len;
     kv8_rows_of(a.r, seq, row0, q_len);
     const int n_rows = q_len * G;
@@ -272,8 +289,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const int bl = min((keys + kKvBlock - 1) / kKvBlock, blocks);
         n_tiles[i] = (bl + kTileBlocks - 1) / kTileBlocks + (keys > open0 ? 1 : 0);
     }
+    // this CTA's of them: tiles j0 + jj, jj < n_tiles[i]
+    const int n_total = max(n_tiles[0], n_tiles[1]), per = (n_total + a.cluster - 1) / a.cluster, j0 = split * per;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) n_tiles[i] = max(0, min(n_tiles[i], j0 + per) - j0);
     const int n_all = max(n_tiles[0], n_tiles[1]);
-    auto tile_blocks = [&](int j) { return j < n_closed ? min(kTileBlocks, blocks - j * kTileBlocks) : 2; };
+    auto tile_blocks = [&](int jj) { return j0 + jj < n_closed ? min(kTileBlocks, blocks - (j0 + jj) * kTileBlocks) : 2; };
 
     if (threadIdx.x == 0) {
         mbar_init(&b.q_full, kRows);
@@ -375,15 +396,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
             }
         };
+#pragma unroll 1
         for (int j = 0; j < n; ++j) {
             // (k_full too: the scales are the converters' writes)
             ok = __all_sync(0xffffffffu, wait(&b.k_full[j % ST], j / ST) && wait(&b.s_full[i], j));
             if (!ok) break;
             tc_fence_after();  // (S full: the earlier products into O have completed too)
             if (LIMBS == 2 && j > 0) add_tile();
-            const bool open = j == n_closed;
+            const bool open = j0 + j == n_closed;
             // the last key of the tile that the row sees (a closed tile ends with the closed blocks)
-            const int see = open ? pos - open0 : min(pos, open0 - 1) - j * kKeys;
+            const int see = open ? pos - open0 : min(pos, open0 - 1) - (j0 + j) * kKeys;
             const float *ks = b.ks[j & 3], *vs = b.vs[j & 3];
             // (per warp) ordinary: all of the tile's scales are positive and finite
             const bool masked = __any_sync(0xffffffffu, see < kKeys - 1);
@@ -395,23 +417,30 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
             // Largest score of each block.
             float t[kTileBlocks] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            // 32 products as they came; the open block's: the two limbs' sums
-            auto raw = [&](int c, uint32_t *s) {
-                tmem_ld32(tS + 32 * c, s);
+            // GR products from column GR u, as they came; the open block's: the two limbs' sums
+            constexpr int GR = LIMBS == 2 ? 16 : 32;
+            auto raw = [&](int u, uint32_t *s) {
+                auto ld = [](uint32_t at, uint32_t *v) {
+                    if constexpr (GR == 16)
+                        tmem_ld16(at, v);
+                    else
+                        tmem_ld32(at, v);
+                };
+                ld(tS + GR * u, s);
                 if (open) {
-                    uint32_t s1[32];
-                    tmem_ld32(tS + 32, s1);
+                    uint32_t s1[GR];
+                    ld(tS + 32 + GR * u, s1);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(s1[e]));
+                    for (int e = 0; e < GR; ++e) s[e] = __float_as_uint(__uint_as_float(s[e]) + __uint_as_float(s1[e]));
                 } else {
                     tmem_wait_ld();
                 }
             };
-            auto hide = [&](int c, uint32_t *s) {  // keys that the row does not see: the lowest finite (x f below: plain)
+            auto hide = [&](int first, int count, uint32_t *s) {  // keys not seen: the lowest finite (x f below: plain)
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                    if (32 * c + e > see) s[e] = 0xFF7FFFFFu;
+                    if (e < count && first + e > see) s[e] = 0xFF7FFFFFu;
             };
             auto top32 = [](const uint32_t *s) {
                 float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -419,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 for (int e = 0; e < 32; ++e) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(s[e]));
                 return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
             };
-            const int parts = open ? 1 : kTileBlocks;
+            const int grains = (open ? kKvBlock : kKeys) / GR;
             const unsigned bad = open ? b.bad : 0;
             if (plain) {
                 // (loops kept rolled: the roles share the instruction cache)
@@ -430,8 +459,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     tmem_ld32(tS + 32 * c + 32, s + 32);
                     tmem_wait_ld();
                     if (masked) {
-                        hide(c, s);
-                        hide(c + 1, s + 32);
+                        hide(32 * c, 32, s);
+                        hide(32 * c + 32, 32, s + 32);
                     }
                     float x0 = top32(s) * (ks[c] * row_scale), x1 = top32(s + 32) * (ks[c + 1] * row_scale);
                     if (32 * c > see) x0 = -INFINITY;
@@ -443,18 +472,19 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
             } else {
 #pragma unroll 1
-                for (int c = 0; c < parts; ++c) {
-                    uint32_t s[32];
-                    raw(c, s);
-                    float x = -INFINITY;
+                for (int u = 0; u < grains; ++u) {
+                    uint32_t s[GR];
+                    raw(u, s);
+                    const int c = u * GR / 32;
                     const float f = ks[c] * row_scale;
+                    float x = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (32 * c + e <= see && !(bad >> e & 1)) x = fmaxf(x, __uint_as_float(s[e]));
+                    for (int e = 0; e < GR; ++e)
+                        if (GR * u + e <= see && !(bad >> (GR * u + e & 31) & 1)) x = fmaxf(x, __uint_as_float(s[e]));
                     x = x == -INFINITY || f < 0.f ? -INFINITY : x * f;
 #pragma unroll
                     for (int k = 0; k < kTileBlocks; ++k)
-                        if (k == c) t[k] = x;
+                        if (k == c) t[k] = fmaxf(t[k], x);
                 }
             }
             // The factor of the sums so far.
@@ -501,18 +531,23 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const float base = m == -INFINITY ? 0.f : m;
             const bool deep = __any_sync(0xffffffffu, h < kDeep && h != -INFINITY);
             float2 sum = make_float2(0.f, 0.f);
-            // Weights take the place of scores: one limb, 16 columns per 32 keys from column 16 c; two limbs, 16 of
-            // the upper and 16 of the lower from column 32 c.
+            // Weights take the place of scores: one limb, 16 columns per 32 keys from column 16 c; two limbs, 8 of the
+            // upper and 8 of the lower per 16 keys from column 16 u.
+            auto put = [&](int u, const uint32_t *w) {
+                tmem_st16(tS + 16 * u, w);
+                if (open) tmem_st16(tS + (GR == 16 ? 32 : 16) + 16 * u, w);  // the values' lower limbs: the same weights
+            };
             if (plain && !deep) {
-                auto weigh = [&](int c, const uint32_t *s) {
+                auto weigh = [&](int u, const uint32_t *s) {
+                    const int c = u * GR / 32;
                     const float f = ks[c] * row_scale, g = vs[c] * wf;
                     // (the scale's own rounding is added back for f32 rows)
                     const float f_lo = LIMBS == 2 ? fmaf(ks[c], row_scale, -f) : 0.f;
                     const float2 f2 = make_float2(f, f), fl2 = make_float2(f_lo, f_lo), b2 = make_float2(-base, -base);
                     const float2 g2 = make_float2(g, g);
-                    uint32_t w[32];
+                    uint32_t w[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
+                    for (int e = 0; e < GR; e += 2) {
                         const float2 v = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                         float2 d = ffma2_of(v, f2, b2);
                         if (LIMBS == 2) d = ffma2_of(v, fl2, d);
@@ -520,58 +555,49 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         sum = fadd2(sum, p);
                         const float2 x = fmul2(p, g2);
                         if (LIMBS == 2)
-                            split_f16(x.x, x.y, w[e / 2], w[16 + e / 2]);
+                            split_f16(x.x, x.y, w[e / 2], w[8 + e / 2]);
                         else
                             w[e / 2] = pack_f16(x.x, x.y);
                     }
-                    if (LIMBS == 2)
-                        tmem_st32(tS + 32 * c, w);
-                    else
-                        tmem_st16(tS + 16 * c, w);
+                    tmem_st16(tS + 16 * u, w);
                 };
-                if constexpr (LIMBS == 2) {
 #pragma unroll 1
-                    for (int c = 0; c < kTileBlocks; ++c) {
-                        uint32_t s[32];
-                        tmem_ld32(tS + 32 * c, s);
-                        tmem_wait_ld();
-                        if (masked) hide(c, s);
-                        weigh(c, s);
+                for (int u = 0; u < kKeys / GR; u += 2) {
+                    uint32_t s[2 * GR];
+                    if constexpr (GR == 16) {
+                        tmem_ld32(tS + 16 * u, s);
+                    } else {
+                        tmem_ld32(tS + 32 * u, s);
+                        tmem_ld32(tS + 32 * u + 32, s + 32);
                     }
-                } else {
-#pragma unroll 1
-                    for (int c = 0; c < kTileBlocks; c += 2) {
-                        uint32_t s[64];
-                        tmem_ld32(tS + 32 * c, s);
-                        tmem_ld32(tS + 32 * c + 32, s + 32);
-                        tmem_wait_ld();
-                        if (masked) {
-                            hide(c, s);
-                            hide(c + 1, s + 32);
-                        }
-                        weigh(c, s);
-                        weigh(c + 1, s + 32);
+                    tmem_wait_ld();
+                    if (masked) {
+                        hide(GR * u, GR, s);
+                        hide(GR * u + GR, GR, s + GR);
                     }
+                    weigh(u, s);
+                    weigh(u + 1, s + GR);
                 }
             } else {
                 // (the open block, scales of zero or NaN, pages that are not there, rows whose heaviest keys have no value)
 #pragma unroll 1
-                for (int c = 0; c < parts; ++c) {
-                    uint32_t s[32], w[32];
-                    raw(c, s);
+                for (int u = 0; u < grains; ++u) {
+                    uint32_t s[GR], w[16];
+                    raw(u, s);
+                    const int c = u * GR / 32;
                     const float f = ks[c] * row_scale, f_lo = LIMBS == 2 ? fmaf(ks[c], row_scale, -f) : 0.f;
                     const float g = vs[c] * wf, nan = __int_as_float(0x7FC00000);
-                    const int last = f < 0.f ? -1 : see - 32 * c;
+                    const int last = f < 0.f ? -1 : see - GR * u;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
+                    for (int e = 0; e < GR; ++e) {
                         float d = fmaf(__uint_as_float(s[e]), f, -base);
                         if (LIMBS == 2) d = fmaf(__uint_as_float(s[e]), f_lo, d);
-                        if (bad >> e & 1) d = nan;
+                        if (bad >> (GR * u + e & 31) & 1) d = nan;
                         s[e] = __float_as_uint(e <= last ? d : -INFINITY);
                     }
                     if (!deep) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
+                        for (int e = 0; e < GR; ++e) {
                             const float p = ex2(__uint_as_float(s[e]));
                             sum.x += p;
                             s[e] = __float_as_uint(e <= last ? p * g : 0.f);  // (nor may a NaN scale reach others)
@@ -580,26 +606,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         const bool lift = h != -INFINITY;
                         const float gl = lift ? vs[c] * ex2(kWBits) : g, up = lift ? h : 0.f;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
+                        for (int e = 0; e < GR; ++e) {
                             const float d = __uint_as_float(s[e]);
                             sum.x += ex2(d);
                             s[e] = __float_as_uint(e <= last ? ex2(fminf(d - up, 126.f)) * gl : 0.f);
                         }
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
+                    for (int e = 0; e < GR; e += 2) {
                         if (LIMBS == 2)
-                            split_f16(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), w[e / 2], w[16 + e / 2]);
+                            split_f16(__uint_as_float(s[e]), __uint_as_float(s[e + 1]), w[e / 2], w[8 + e / 2]);
                         else
                             w[e / 2] = pack_f16(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                     }
-                    if (LIMBS == 2) {
-                        tmem_st32(tS + 32 * c, w);
-                        if (open) tmem_st32(tS + 32, w);  // the values' lower limbs: the same weights
-                    } else {
-                        tmem_st16(tS + 16 * c, w);
-                        if (open) tmem_st16(tS + 16, w);
-                    }
+                    put(u, w);
                 }
             }
             l += sum.x + sum.y;
@@ -613,12 +633,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             tc_fence_after();
             add_tile();
         }
-        // sums to the result: x 2^(h - kWBits) / l, the power in two steps where it leaves the range
+        // Every product of the CTA has been computed: Q, K and V make way for the rows' sums, x 2^(h - kWBits) (the
+        // power in two steps where it leaves the range), their maxima and totals.
+        ok = __all_sync(0xffffffffu, wait(&b.done, 0) && ok);
         const float e0 = h - kWBits, u0 = h == -INFINITY ? 0.f : ex2(fmaxf(e0, -120.f));
-        const float u1 = (l == 0.f ? 0.f : 1.0f / l) * (h == -INFINITY ? 1.f : ex2(fminf(e0 + 120.f, 0.f)));
-        T *out = static_cast<T *>(a.out) + (int64_t)(row0 + tok) * a.out_stride + (int64_t)head * HD;
-        const T *gate = a.gate == nullptr ? nullptr
-                                          : static_cast<const T *>(a.gate) + (int64_t)(row0 + tok) * a.gate_stride + (int64_t)head * HD;
+        const float u1 = h == -INFINITY ? 1.f : ex2(fminf(e0 + 120.f, 0.f));
+        float *row = reinterpret_cast<float *>(sm) + (128 * i + r) * kPitch;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
             uint32_t o[32];
@@ -629,40 +649,17 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 tmem_ld32(tO + 32 * c, o);
                 tmem_wait_ld();
             }
-            if (!live || !ok) continue;
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-                float v[8];
+            for (int e = 0; e < 32; e += 4) {
+                float v[4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = l == 0.f ? 0.f : __uint_as_float(o[e + k]) * u0 * u1;  // (sees no key: zeros)
-                if (gate != nullptr) {
-                    float g[8];
-                    load8<T>(g, gate + 32 * c + e, false);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] *= 1.0f / (1.0f + expf(-g[k]));
-                }
-                T *p = out + 32 * c + e;
-                if (a.vec) {
-                    if constexpr (sizeof(T) == 4) {
-                        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-                        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                    } else {
-                        __nv_bfloat162 w[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) w[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-                        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<uint4 *>(w);
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        if constexpr (sizeof(T) == 4)
-                            p[k] = v[k];
-                        else
-                            p[k] = __float2bfloat16_rn(v[k]);
-                    }
-                }
+                for (int k = 0; k < 4; ++k) v[k] = n > 0 ? __uint_as_float(o[e + k]) * u0 * u1 : 0.f;
+                *reinterpret_cast<float4 *>(row + 32 * c + e) = make_float4(v[0], v[1], v[2], v[3]);
             }
         }
+        row[HD] = m;
+        row[HD + 1] = l;
+        reg_dec<128>();  // (as launched: the roles meet)
     } else if (warp < 12) {
         // ------------------------------------ codes to f16 ------------------------------------
         reg_dec<Regs<LIMBS>::convert>();
@@ -680,11 +677,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             *reinterpret_cast<uint4 *>(p + ((2 * pc + 1) ^ (row & 7)) * 16) = make_uint4(h[4], h[5], h[6], h[7]);
         };
         constexpr bool kBoth = LIMBS == 1;  // registers for both operands' next tile (f32: one at a time, twice the time)
+        const int n_c = max(0, min(n_all, n_closed - j0));  // closed tiles
         int pg[kTileBlocks];
-        auto pages = [&](int j) {
+        auto pages = [&](int jj) {
+            const int b0 = (j0 + jj) * kTileBlocks;
 #pragma unroll
-            for (int c = 0; c < kTileBlocks; ++c)
-                pg[c] = j < n_closed && j * kTileBlocks + c < blocks ? kv8_page(a.c, seq, j * kTileBlocks + c) : -1;
+            for (int c = 0; c < kTileBlocks; ++c) pg[c] = jj < n_c && b0 + c < blocks ? kv8_page(a.c, seq, b0 + c) : -1;
         };
         uint4 raw_k[U], raw_v[kBoth ? U : 1];
         auto load = [&](uint4 *raw, const uint8_t *codes) {  // of the tile whose pages are in pg
@@ -713,11 +711,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         float next_ks = -1.f, next_vs = 0.f;
         auto scales = [&](int j) {
             if (w != 0 || lane >= kTileBlocks) return;
-            if (j * kTileBlocks + lane >= blocks) {  // past the closed blocks: all of its keys are hidden by their position
+            const int block = (j0 + j) * kTileBlocks + lane;
+            if (block >= blocks) {  // past the closed blocks: all of its keys are hidden by their position
                 next_ks = next_vs = 1.f;
                 return;
             }
-            const int c = kv8_page(a.c, seq, j * kTileBlocks + lane);
+            const int c = kv8_page(a.c, seq, block);
             const int64_t z = (int64_t)c * a.c.kv_heads + kh;
             // (no such page: its keys are hidden by the sign)
             next_ks = c >= 0 ? a.c.k_scale[z] : -1.f;
@@ -732,7 +731,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         auto empty = [&](uint64_t *bar, int j) {  // the stage's former tile has been read
             return j < ST || __all_sync(0xffffffffu, wait(bar, j / ST - 1));
         };
-        const int n_c = min(n_all, n_closed);
         if (n_c > 0) {
             pages(0);
             load(raw_k, a.c.k_codes);
@@ -773,8 +771,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
             }
         }
-        if (ok && n_all > n_closed) {  // the open block: upper limbs in rows 0..31, lower in 32..63
-            const int j = n_closed, st = j % ST, there = kv_len - open0, slot = kv8_slot(a.c, seq);
+        if (ok && n_all > n_c) {  // the open block: upper limbs in rows 0..31, lower in 32..63
+            const int j = n_c, st = j % ST, there = kv_len - open0, slot = kv8_slot(a.c, seq);
             __shared__ float s_max[2][4];
             __shared__ unsigned s_bad[4];
             // a thread per 16 values of a row
@@ -849,6 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 full(op ? &b.v_full[st] : &b.k_full[st]);
             }
         }
+        reg_inc<128>();
     } else {
         // ------------------------------------ MMA issue ------------------------------------
         reg_dec<Regs<LIMBS>::issue>();
@@ -875,8 +874,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 for (int z = LIMBS - 1; z >= 0; --z)
 #pragma unroll 1
                     for (int k = 0; k < steps; ++k) {
-                        // 16 keys are 8 columns of P; two limbs: per 32 keys 16 columns of the upper, 16 of the lower
-                        mma_ts(tmem + i * kTile + kO, tmem + i * kTile + kS + (LIMBS == 2 ? k / 2 * 32 + k % 2 * 8 + 16 * z : 8 * k),
+                        // 16 keys are 8 columns of P; two limbs: 8 of the upper, then 8 of the lower
+                        mma_ts(tmem + i * kTile + kO, tmem + i * kTile + kS + (LIMBS == 2 ? 16 * k + 8 * z : 8 * k),
                                desc_mn(sv + j % ST * L::KV + k * 2048, kKeys * 128), idesc(HD, true), add);
                         add = 1;
                     }
@@ -915,6 +914,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             mbar_wait(&b.done, 0u, a.c.err, kErrWaitFull);
         }
         __syncwarp();
+        reg_inc<128>();
     }
     tc_fence_before();
     __syncthreads();
@@ -922,6 +922,61 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    // This CTA's share of the rows from every CTA of the cluster, consecutive threads along a row.
+    cg::cluster_group cl = cg::this_cluster();
+    if (a.cluster > 1) cl.sync();
+    const int share = (kRows + a.cluster - 1) / a.cluster, r0 = split * share, r1 = min(min(r0 + share, kRows), n_rows - r_base);
+    if (*abort_flag == 0) {
+        const float *sums = reinterpret_cast<const float *>(sm);
+        for (int x = threadIdx.x; x < (r1 - r0) * (HD / 4); x += kThreads) {
+            const int r = r0 + x / (HD / 4), c = x % (HD / 4), gr = r_base + r;
+            float m = -INFINITY, l = 0.f;
+            float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (a.cluster == 1) {
+                l = sums[r * kPitch + HD + 1];
+                z = *reinterpret_cast<const float4 *>(sums + r * kPitch + 4 * c);
+            } else {
+                for (int y = 0; y < a.cluster; ++y) m = fmaxf(m, *cl.map_shared_rank(sums + r * kPitch + HD, y));
+                for (int y = 0; y < a.cluster; ++y) {
+                    const float *p = cl.map_shared_rank(sums + r * kPitch, y);
+                    const float pm = p[HD], pl = p[HD + 1];
+                    const float4 w = *reinterpret_cast<const float4 *>(p + 4 * c);
+                    // 0 where the CTA saw no key, NaN where its total is one (its maximum then says nothing)
+                    const float f = pl != pl ? pl : pm == -INFINITY ? 0.f : ex2(pm - m);
+                    if (f == 0.f) continue;
+                    z.x = fmaf(w.x, f, z.x), z.y = fmaf(w.y, f, z.y), z.z = fmaf(w.z, f, z.z), z.w = fmaf(w.w, f, z.w);
+                    l = fmaf(pl, f, l);
+                }
+            }
+            const float inv = l == 0.f ? 0.f : 1.0f / l;  // a row that sees no key: zeros
+            float v[4] = {z.x * inv, z.y * inv, z.z * inv, z.w * inv};
+            const int64_t row = row0 + gr / G;
+            const int d = (kh * G + gr % G) * HD + 4 * c;
+            if (a.gate != nullptr) {
+                const T *g = static_cast<const T *>(a.gate) + row * a.gate_stride + d;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] *= 1.0f / (1.0f + expf(-(float)g[k]));
+            }
+            T *o = static_cast<T *>(a.out) + row * a.out_stride + d;
+            if (a.vec) {
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    __nv_bfloat162 w[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+                    *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<uint2 *>(w);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (sizeof(T) == 4)
+                        o[k] = v[k];
+                    else
+                        o[k] = __float2bfloat16_rn(v[k]);
+                }
+            }
+        }
+    }
+    if (a.cluster > 1) cl.sync();  // (its shared memory is read until all have arrived)
 }
 
 template <typename T, int HD>
@@ -937,12 +992,23 @@ cudaError_t launch_hd(const Kv8AttnArgs &a, int max_q_len, cudaStream_t s) {
             return e;
         if (dev < 64) ready.fetch_or(1ull << dev);
     }
-    const int64_t rows = (int64_t)max_q_len * (a.n_heads / a.c.kv_heads);
-    prompt_kernel<T, HD><<<dim3(a.c.kv_heads, a.c.n_seqs, (unsigned)((rows + kRows - 1) / kRows)), kThreads, smem, s>>>(a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.c.kv_heads * a.cluster, a.c.n_seqs, kv8_prompt_row_tiles(max_q_len, a.n_heads / a.c.kv_heads));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {(unsigned)a.cluster, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prompt_kernel<T, HD>, a);
 }
 }  // namespace
 
+unsigned kv8_prompt_row_tiles(int max_q_len, int group) {
+    return (unsigned)(((int64_t)max_q_len * group + kRows - 1) / kRows);
+}
 bool kv8_prompt_takes(int head_dim) { return head_dim == 64 || head_dim == 128; }
 
 cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, int max_q_len, bool bf16, cudaStream_t s) {
