@@ -1370,7 +1370,6 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
             const int64_t base = (int64_t)a.c.n_seqs * a.c.kv_heads * kv8_prompt_row_tiles(mq, n_heads / a.c.kv_heads);
             const int64_t tiles = (max_kv_len + 127) / 128;
             a.cluster = (int)std::max<int64_t>(1, std::min<int64_t>({ws->sms / base, tiles / 4, 8}));
-            if (const char *v = getenv("QLC")) a.cluster = atoi(v);
         }
         const cudaError_t e = prompt ? kv8_prompt_launch(a, mq, type == QL_BF16, g_stream)
                                      : kv8_attn_launch(a, type == QL_BF16, g_stream);
