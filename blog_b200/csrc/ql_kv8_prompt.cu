@@ -11,9 +11,10 @@
 // The scale of V's block is multiplied into P relative to the row's largest such product, as in the split
 // kernel, and O is rescaled only when one passes that by 2^7.
 //
-// Roles, 16 warps: 0-3 and 4-7 a thread per row of tile 0 and 1 (S from TMEM, P to TMEM, the result); 8-11 codes
-// from global memory through registers to f16 in the layout the MMA reads (128-byte swizzle; K with the head
-// dimension contiguous and V too, as the transposed operand), a tile ahead; 12 issues the MMAs.  While one tile's
+// Roles, 16 warps: 0-3 and 4-7 a thread per row of tile 0 and 1 (S from TMEM, P to TMEM, the result); 13 copies
+// the pages' codes into shared memory (one bulk copy per block and operand), 8-11 turn them into f16 in the layout
+// the MMA reads (128-byte swizzle; K with the head dimension contiguous and V too, as the transposed operand), a
+// tile ahead; 12 issues the MMAs.  While one tile's
 // threads exponentiate, the tensor cores run the other tile's products.
 // The rows of the block that is not full make a last tile of 64 keys: their upper f16 limbs, then their lower.
 //
@@ -42,11 +43,8 @@ constexpr int kRows = 256;   // rows per CTA: two MMA tiles
 constexpr float kHeadroom = 7.0f, kWBits = 8.0f;  // as in the split kernel
 
 // Registers per thread of the roles; 16 warps launch with 128 each.
-template <int LIMBS>
-struct Regs {
-    static constexpr int softmax = LIMBS == 2 ? 200 : 184, convert = LIMBS == 2 ? 80 : 104, issue = LIMBS == 2 ? 32 : 40;
-    static_assert(2 * softmax + convert + issue == 4 * 128, "the block's registers at launch");
-};
+constexpr int kSoftmaxRegs = 168, kConvertRegs = 96, kIssueRegs = 80;
+static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs == 4 * 128, "the block's registers at launch");
 
 template <int HD, int LIMBS>
 struct Layout {
@@ -54,7 +52,8 @@ struct Layout {
     static constexpr int ST = LIMBS == 2 && HD == 128 ? 1 : 2;  // K and V stages
     static constexpr int QT = A * 128 * 128;                 // one limb of one tile of Q
     static constexpr int KV = A * kKeys * 128;               // one stage of K or of V
-    static constexpr int q = 0, k = q + 2 * LIMBS * QT, v = k + ST * KV, end = v + ST * KV;
+    static constexpr int RAW = kKeys * HD;                   // a tile's codes of K or of V
+    static constexpr int q = 0, k = q + 2 * LIMBS * QT, v = k + ST * KV, raw = v + ST * KV, end = raw + 2 * RAW;
     static constexpr int bytes = 1024 + end + 512;
 };
 
@@ -68,20 +67,29 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Upper words of the operand descriptors: 128-byte swizzle, the next 8 rows (K-major) or keys (MN-major) 1024
+// bytes on.  The lower words: address / 16, and in the upper half the leading byte offset / 16.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// D (+)= A B, A and B in shared memory.
+template <bool ADD>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "n"(ADD ? 1 : 0), "r"(kDescHi)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// The same with A in tensor memory.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(kDescHi)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
@@ -130,6 +138,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// One contiguous copy, global to shared memory, its bytes counted on bar (addresses and size multiples of 16).
+__device__ __forceinline__ void bulk_copy(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
 template <int N>
 __device__ __forceinline__ void reg_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
@@ -138,16 +152,10 @@ template <int N>
 __device__ __forceinline__ void reg_inc() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
-// Shared-memory matrix descriptors, 128-byte swizzle.  K-major: 8-row atoms of 1024 B (stride byte offset).
-// MN-major (V, the head dimension contiguous): 64 x 8 atoms of 1024 B, the next 8 keys 1024 B on (stride byte
-// offset), the next 64 dimensions `lead` bytes on (leading byte offset).
-__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
-    return ((a >> 4) & 0x3FFFull) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t a, uint32_t lead) {
-    return ((a >> 4) & 0x3FFFull) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
-}
+// Lower descriptor words.  K-major: 8-row atoms of 1024 B, the leading byte offset unused (1).  MN-major (V, the
+// head dimension contiguous): 64 x 8 atoms of 1024 B, the next 64 dimensions `lead` bytes on.
+__device__ __forceinline__ uint32_t desc_k(uint32_t a) { return ((a >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t a, uint32_t lead) { return ((a >> 4) & 0x3FFFu) | ((lead >> 4) << 16); }
 // Instruction descriptor: f32 accumulator, f16 operands, M 128; bit 16: B is MN-major.
 constexpr uint32_t idesc(int n, bool b_mn) {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
@@ -244,7 +252,7 @@ struct Few {
 };
 
 struct Bars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], open_max, done;
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], raw_full[2], raw_empty[2], open_max, done;
     uint32_t tmem;
     int abort;
     // Scales of the tile's blocks (K's < 0: no such block), a ring: when the scores of the tile ST before have been
@@ -294,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll
     for (int i = 0; i < 2; ++i) n_tiles[i] = max(0, min(n_tiles[i], j0 + per) - j0);
     const int n_all = max(n_tiles[0], n_tiles[1]);
+    const int n_c = max(0, min(n_all, n_closed - j0));  // closed tiles among them
     auto tile_blocks = [&](int jj) { return j0 + jj < n_closed ? min(kTileBlocks, blocks - (j0 + jj) * kTileBlocks) : 2; };
 
     if (threadIdx.x == 0) {
@@ -301,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b.k_full[i], 4), mbar_init(&b.k_empty[i], 1), mbar_init(&b.v_full[i], 4), mbar_init(&b.v_empty[i], 1);
             mbar_init(&b.s_full[i], 1), mbar_init(&b.p_full[i], 4), mbar_init(&b.o_full[i], 1);
+            mbar_init(&b.raw_full[i], 1), mbar_init(&b.raw_empty[i], 4);
         }
         mbar_init(&b.open_max, 4);
         mbar_init(&b.done, 1);
@@ -324,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
     if (warp < 8) {
         // ------------------------------------ a thread per row ------------------------------------
-        reg_inc<Regs<LIMBS>::softmax>();
+        reg_inc<kSoftmaxRegs>();
         const int i = warp >> 2, r = threadIdx.x & 127, gr = r_base + 128 * i + r;
         const bool live = gr < n_rows;
         const int tok = live ? gr / G : 0, head = kh * G + (live ? gr % G : 0);
@@ -451,24 +461,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const int grains = (open ? kKvBlock : kKeys) / GR;
             const unsigned bad = open ? b.bad : 0;
             if (plain) {
-                // (loops kept rolled: the roles share the instruction cache)
+                // (loops kept rolled: the roles share the instruction cache; f32 rows have registers for one block)
+                constexpr int NB = LIMBS == 2 ? 1 : 2;
 #pragma unroll 1
-                for (int c = 0; c < kTileBlocks; c += 2) {
-                    uint32_t s[64];
-                    tmem_ld32(tS + 32 * c, s);
-                    tmem_ld32(tS + 32 * c + 32, s + 32);
+                for (int c = 0; c < kTileBlocks; c += NB) {
+                    uint32_t s[32 * NB];
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) tmem_ld32(tS + 32 * (c + k), s + 32 * k);
                     tmem_wait_ld();
-                    if (masked) {
-                        hide(32 * c, 32, s);
-                        hide(32 * c + 32, 32, s + 32);
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) {
+                        if (masked) hide(32 * (c + k), 32, s + 32 * k);
+                        const float x = 32 * (c + k) > see ? -INFINITY : top32(s + 32 * k) * (ks[c + k] * row_scale);
+#pragma unroll
+                        for (int z = k; z < kTileBlocks; z += NB)
+                            if (z == c + k) t[z] = x;
                     }
-                    float x0 = top32(s) * (ks[c] * row_scale), x1 = top32(s + 32) * (ks[c + 1] * row_scale);
-                    if (32 * c > see) x0 = -INFINITY;
-                    if (32 * c + 32 > see) x1 = -INFINITY;
-                    if (c == 0)
-                        t[0] = x0, t[1] = x1;
-                    else
-                        t[2] = x0, t[3] = x1;
                 }
             } else {
 #pragma unroll 1
@@ -563,20 +571,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 };
 #pragma unroll 1
                 for (int u = 0; u < kKeys / GR; u += 2) {
-                    uint32_t s[2 * GR];
                     if constexpr (GR == 16) {
-                        tmem_ld32(tS + 16 * u, s);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            uint32_t s[16];
+                            tmem_ld16(tS + 16 * (u + k), s);
+                            tmem_wait_ld();
+                            if (masked) hide(16 * (u + k), 16, s);
+                            weigh(u + k, s);
+                        }
                     } else {
+                        uint32_t s[64];
                         tmem_ld32(tS + 32 * u, s);
                         tmem_ld32(tS + 32 * u + 32, s + 32);
+                        tmem_wait_ld();
+                        if (masked) {
+                            hide(32 * u, 32, s);
+                            hide(32 * u + 32, 32, s + 32);
+                        }
+                        weigh(u, s);
+                        weigh(u + 1, s + 32);
                     }
-                    tmem_wait_ld();
-                    if (masked) {
-                        hide(GR * u, GR, s);
-                        hide(GR * u + GR, GR, s + GR);
-                    }
-                    weigh(u, s);
-                    weigh(u + 1, s + GR);
                 }
             } else {
                 // (the open block, scales of zero or NaN, pages that are not there, rows whose heaviest keys have no value)
@@ -659,54 +674,56 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         }
         row[HD] = m;
         row[HD + 1] = l;
-        reg_dec<128>();  // (as launched: the roles meet)
+        reg_dec<128>();  // as launched: the others take theirs back when all rows' warps have come here
     } else if (warp < 12) {
         // ------------------------------------ codes to f16 ------------------------------------
-        reg_dec<Regs<LIMBS>::convert>();
+        reg_dec<kConvertRegs>();
         const int w = warp - 8;
-        // pieces of 16 codes: the 8 lanes of a store phase hold four pieces of two rows, whose 16-byte chunks
-        // the swizzle puts on distinct banks
-        constexpr int RPI = 8 / A;                  // rows per warp access
-        constexpr int U = kKeys / (4 * RPI);        // accesses per warp, operand and tile
-        const int pc = lane & 3, at = (lane >> 3) % A, rl = ((lane >> 2) & 1) + 2 * ((lane >> 3) / A);
-        const int src = (at * 4 + pc) * 16;
+        // Pieces of 16 codes, 32 to a warp access.  A phase's 8 lanes hold four pieces of two rows: of different
+        // halves of the rows where these are 128 bytes, so that the reads meet distinct banks, and the rows'
+        // swizzles differ, so that the writes do.
+        constexpr int RPI = 8 / A;            // rows per warp access
+        constexpr int U = kKeys / (4 * RPI);  // accesses per warp, operand and tile
+        const int pc = lane & 3, rb = (lane >> 2) & 1, at = (lane >> 3) % A ^ (A == 2 ? rb : 0), rl = rb + 2 * ((lane >> 3) / A);
         auto row_of = [&](int u) { return (u * 4 + w) * RPI + rl; };
-        auto store16 = [&](uint8_t *tile, int row, const uint32_t (&h)[8]) {
-            uint8_t *p = tile + at * (kKeys * 128) + row * 128;
-            *reinterpret_cast<uint4 *>(p + ((2 * pc) ^ (row & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4 *>(p + ((2 * pc + 1) ^ (row & 7)) * 16) = make_uint4(h[4], h[5], h[6], h[7]);
+        bool ok = true;
+        auto full = [&](uint64_t *bar) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
         };
-        constexpr bool kBoth = LIMBS == 1;  // registers for both operands' next tile (f32: one at a time, twice the time)
-        const int n_c = max(0, min(n_all, n_closed - j0));  // closed tiles
-        int pg[kTileBlocks];
-        auto pages = [&](int jj) {
-            const int b0 = (j0 + jj) * kTileBlocks;
-#pragma unroll
-            for (int c = 0; c < kTileBlocks; ++c) pg[c] = jj < n_c && b0 + c < blocks ? kv8_page(a.c, seq, b0 + c) : -1;
+        auto empty = [&](uint64_t *bar, int j) {  // the stage's former tile has been read
+            return j < ST || __all_sync(0xffffffffu, wait(bar, j / ST - 1));
         };
-        uint4 raw_k[U], raw_v[kBoth ? U : 1];
-        auto load = [&](uint4 *raw, const uint8_t *codes) {  // of the tile whose pages are in pg
+        auto convert = [&](int op, int j, uint64_t *stage_empty, uint8_t *tile) {
+            if (!__all_sync(0xffffffffu, wait(&b.raw_full[op], j))) return false;
+            const uint8_t *src = sm + L::raw + op * L::RAW + (at * 4 + pc) * 16;
+            uint8_t *p = tile + at * (kKeys * 128);
+            if (!empty(stage_empty, j)) return false;
+            constexpr int H = U / 2;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int row = row_of(u), p = pg[u * 4 * RPI / kKvBlock];
-                raw[u] = p >= 0 ? *reinterpret_cast<const uint4 *>(codes + kv8_codes_at(a.c, p, kh) + (row & 31) * HD + src)
-                                : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-            }
-        };
-        auto convert = [&](const uint4 *raw, uint8_t *tile) {
+            for (int u0 = 0; u0 < U; u0 += H) {
+                uint4 raw[H];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t z[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-                uint32_t h[8];
+                for (int u = 0; u < H; ++u) raw[u] = *reinterpret_cast<const uint4 *>(src + row_of(u0 + u) * HD);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    h[2 * e] = codes2(z[e], 0x4140);
-                    h[2 * e + 1] = codes2(z[e], 0x4342);
+                for (int u = 0; u < H; ++u) {
+                    const uint32_t z[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                    uint32_t h[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        h[2 * e] = codes2(z[e], 0x4140);
+                        h[2 * e + 1] = codes2(z[e], 0x4342);
+                    }
+                    const int row = row_of(u0 + u);
+                    *reinterpret_cast<uint4 *>(p + row * 128 + ((2 * pc) ^ (row & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(p + row * 128 + ((2 * pc + 1) ^ (row & 7)) * 16) = make_uint4(h[4], h[5], h[6], h[7]);
                 }
-                store16(tile, row_of(u), h);
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.raw_empty[op]);
+            return true;
         };
-        static_assert(4 * RPI <= kKvBlock, "one access of the four warps lies in one block");
         // scales of a tile's blocks (lanes 0 .. 3 of the first warp)
         float next_ks = -1.f, next_vs = 0.f;
         auto scales = [&](int j) {
@@ -722,25 +739,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             next_ks = c >= 0 ? a.c.k_scale[z] : -1.f;
             next_vs = c >= 0 ? a.c.v_scale[z] : 0.f;
         };
-        bool ok = true;
-        auto full = [&](uint64_t *bar) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-        };
-        auto empty = [&](uint64_t *bar, int j) {  // the stage's former tile has been read
-            return j < ST || __all_sync(0xffffffffu, wait(bar, j / ST - 1));
-        };
-        if (n_c > 0) {
-            pages(0);
-            load(raw_k, a.c.k_codes);
-            if (kBoth) load(raw_v, a.c.v_codes);
-            scales(0);
-            if (kBoth) pages(1);
-        }
+        if (n_c > 0) scales(0);
         for (int j = 0; j < n_c && ok; ++j) {
             const int st = j % ST;
-            if (!(ok = empty(&b.k_empty[st], j))) break;
+            if (!(ok = convert(0, j, &b.k_empty[st], sm + L::k + st * L::KV))) break;
             if (w == 0) {
                 const bool good = next_ks > 0.f && next_ks < INFINITY && next_vs > 0.f && next_vs < INFINITY;
                 if (lane < kTileBlocks) {
@@ -749,58 +751,43 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 const unsigned all = __ballot_sync(0xffffffffu, good);
                 if (lane == 0) b.plain[j & 3] = (all & 15u) == 15u;
+                if (j + 1 < n_c) scales(j + 1);
             }
-            convert(raw_k, sm + L::k + st * L::KV);
             full(&b.k_full[st]);
-            if (kBoth) {
-                if (j + 1 < n_c) load(raw_k, a.c.k_codes);
-            } else {
-                load(raw_k, a.c.v_codes);
-            }
-            if (j + 1 < n_c) scales(j + 1);
-            if (!(ok = empty(&b.v_empty[st], j))) break;
-            convert(kBoth ? raw_v : raw_k, sm + L::v + st * L::KV);
+            if (!(ok = convert(1, j, &b.v_empty[st], sm + L::v + st * L::KV))) break;
             full(&b.v_full[st]);
-            if (j + 1 < n_c) {
-                if (kBoth) {
-                    load(raw_v, a.c.v_codes);
-                    pages(j + 2);
-                } else {
-                    pages(j + 1);
-                    load(raw_k, a.c.k_codes);
-                }
-            }
         }
         if (ok && n_all > n_c) {  // the open block: upper limbs in rows 0..31, lower in 32..63
             const int j = n_c, st = j % ST, there = kv_len - open0, slot = kv8_slot(a.c, seq);
             __shared__ float s_max[2][4];
             __shared__ unsigned s_bad[4];
-            // a thread per 16 values of a row
-            constexpr int PPR = HD / 16, RP = 128 / PPR;  // pieces per row, rows per step
+            // a thread per 8 values of a row
+            constexpr int PPR = HD / 8, RP = 128 / PPR;  // pieces per row, rows per step
             const int tid = threadIdx.x - 256, piece = tid % PPR;
             unsigned bad = 0;
             float amax[2] = {0.f, 0.f};
-            auto piece_of = [&](int op, int t, float (&x)[16]) {
+            auto piece_of = [&](int op, int t, float (&x)[8]) {
                 const float *p = (op ? a.c.v_open : a.c.k_open) + kv8_open_at(a.c, max(slot, 0), open0 / kKvBlock, kh) +
-                                 t * HD + piece * 16;
+                                 t * HD + piece * 8;
 #pragma unroll
-                for (int e = 0; e < 16; e += 4) {
+                for (int e = 0; e < 8; e += 4) {
                     const float4 z = slot >= 0 && t < there ? *reinterpret_cast<const float4 *>(p + e) : make_float4(0.f, 0.f, 0.f, 0.f);
                     x[e] = z.x, x[e + 1] = z.y, x[e + 2] = z.z, x[e + 3] = z.w;
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
+                for (int e = 0; e < 8; ++e)
                     if (!(fabsf(x[e]) < INFINITY)) {
                         bad |= 1u << t;
                         x[e] = 0.f;
                     }
             };
             for (int op = 0; op < 2; ++op)
+#pragma unroll 1
                 for (int t = tid / PPR; t < kKvBlock; t += RP) {
-                    float x[16];
+                    float x[8];
                     piece_of(op, t, x);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) amax[op] = fmaxf(amax[op], fabsf(x[e]));
+                    for (int e = 0; e < 8; ++e) amax[op] = fmaxf(amax[op], fabsf(x[e]));
                 }
             bad = __reduce_or_sync(0xffffffffu, bad);
 #pragma unroll
@@ -828,57 +815,69 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             for (int op = 0; op < 2 && ok; ++op) {
                 if (op == 1 && !(ok = empty(&b.v_empty[st], j))) break;
                 uint8_t *tile = sm + (op ? L::v : L::k) + st * L::KV;
+#pragma unroll 1
                 for (int t = tid / PPR; t < kKvBlock; t += RP) {
-                    float x[16];
+                    float x[8];
                     piece_of(op, t, x);
-                    uint32_t hi[8], lo[8];
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) split_f16(x[2 * e] * scale[op], x[2 * e + 1] * scale[op], hi[e], lo[e]);
-                    uint8_t *p = tile + piece / 4 * (kKeys * 128);
-                    const int c0 = (piece & 3) * 2;
+                    for (int e = 0; e < 4; ++e) split_f16(x[2 * e] * scale[op], x[2 * e + 1] * scale[op], hi[e], lo[e]);
+                    uint8_t *p = tile + piece / 8 * (kKeys * 128);
 #pragma unroll
                     for (int z = 0; z < 2; ++z) {
-                        const uint32_t(&h)[8] = z ? lo : hi;
+                        const uint32_t(&h)[4] = z ? lo : hi;
                         const int row = t + 32 * z;
-                        *reinterpret_cast<uint4 *>(p + row * 128 + (c0 ^ (row & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4 *>(p + row * 128 + ((c0 + 1) ^ (row & 7)) * 16) = make_uint4(h[4], h[5], h[6], h[7]);
+                        *reinterpret_cast<uint4 *>(p + row * 128 + ((piece & 7) ^ (row & 7)) * 16) = make_uint4(h[0], h[1], h[2], h[3]);
                     }
                 }
                 full(op ? &b.v_full[st] : &b.k_full[st]);
             }
         }
-        reg_inc<128>();
     } else {
         // ------------------------------------ MMA issue ------------------------------------
-        reg_dec<Regs<LIMBS>::issue>();
+        reg_dec<kIssueRegs>();
         if (warp == 12 && lane == 0) {
             const uint32_t sq = smem_u32(sm + L::q), sk = smem_u32(sm + L::k), sv = smem_u32(sm + L::v);
+            // (one thread issues 32 or 64 MMAs a tile: descriptors are sums of constants, the loops unrolled)
+            const uint32_t dq = desc_k(sq), dk = desc_k(sk), dv = desc_mn(sv, kKeys * 128);
             auto scores = [&](int i, int j) {
-                uint32_t acc = 0;
-#pragma unroll 1
+                const uint32_t qb = dq + (i * L::QT >> 4), kb = dk + ((ST == 1 ? 0 : j % ST) * L::KV >> 4);
+                const uint32_t d = tmem + i * kTile + kS;
+#pragma unroll
                 for (int z = LIMBS - 1; z >= 0; --z)  // (lower limbs first: fewer additions to a full-sized sum)
-#pragma unroll 1
+#pragma unroll
                     for (int at = 0; at < A; ++at)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            mma_ss(tmem + i * kTile + kS, desc_k(sq + (2 * z + i) * L::QT + at * (128 * 128) + 32 * k),
-                                   desc_k(sk + j % ST * L::KV + at * (kKeys * 128) + 32 * k), idesc(kKeys, false), acc);
-                            acc = 1;
+                            const uint32_t qa = qb + ((2 * z * L::QT + at * (128 * 128) + 32 * k) >> 4);
+                            const uint32_t ka = kb + ((at * (kKeys * 128) + 32 * k) >> 4);
+                            if (z == LIMBS - 1 && at == 0 && k == 0)
+                                mma_ss<false>(d, qa, ka, idesc(kKeys, false));
+                            else
+                                mma_ss<true>(d, qa, ka, idesc(kKeys, false));
                         }
                 mma_commit(&b.s_full[i]);
             };
             auto values = [&](int i, int j) {
+                const uint32_t vb = dv + ((ST == 1 ? 0 : j % ST) * L::KV >> 4);
+                const uint32_t d = tmem + i * kTile + kO, p = tmem + i * kTile + kS;
+                const uint32_t first = LIMBS == 2 ? 0u : (uint32_t)(j > 0);  // f32 rows: each tile's product by itself
+                // 16 keys are 8 columns of P; two limbs: 8 of the upper, then 8 of the lower
+                auto step = [&](int z, int k, uint32_t add) {
+                    mma_ts(d, p + (LIMBS == 2 ? 16 * k + 8 * z : 8 * k), vb + (k * 2048 >> 4), idesc(HD, true), add);
+                };
                 const int steps = 2 * tile_blocks(j);
-                uint32_t add = LIMBS == 2 ? 0u : (uint32_t)(j > 0);  // f32 rows: each tile's product by itself
+                if (steps == 2 * kTileBlocks) {
+#pragma unroll
+                    for (int z = LIMBS - 1; z >= 0; --z)
+#pragma unroll
+                        for (int k = 0; k < 2 * kTileBlocks; ++k) step(z, k, z == LIMBS - 1 && k == 0 ? first : 1u);
+                } else {
 #pragma unroll 1
-                for (int z = LIMBS - 1; z >= 0; --z)
+                    for (int z = LIMBS - 1; z >= 0; --z)
 #pragma unroll 1
-                    for (int k = 0; k < steps; ++k) {
-                        // 16 keys are 8 columns of P; two limbs: 8 of the upper, then 8 of the lower
-                        mma_ts(tmem + i * kTile + kO, tmem + i * kTile + kS + (LIMBS == 2 ? 16 * k + 8 * z : 8 * k),
-                               desc_mn(sv + j % ST * L::KV + k * 2048, kKeys * 128), idesc(HD, true), add);
-                        add = 1;
-                    }
+                        for (int k = 0; k < steps; ++k) step(z, k, z == LIMBS - 1 && k == 0 ? first : 1u);
+                }
             };
             bool ok = n_all == 0 || (wait(&b.q_full, 0) && wait(&b.k_full[0], 0));
             if (ok && n_all > 0) {
@@ -912,12 +911,42 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             // every MMA has completed before TMEM is freed
             mma_commit(&b.done);
             mbar_wait(&b.done, 0u, a.c.err, kErrWaitFull);
+        } else if (warp == 13 && lane == 0) {
+            // ------------------------------------ pages to shared memory ------------------------------------
+            constexpr uint32_t kBytes = kKvBlock * HD;
+            int issued[2] = {0, 0};
+            bool ok = true;
+            for (int j = 0; j < n_c && ok; ++j) {
+                int page[kTileBlocks], count = 0;
+#pragma unroll
+                for (int c = 0; c < kTileBlocks; ++c) {
+                    const int block = (j0 + j) * kTileBlocks + c;
+                    page[c] = block < blocks ? kv8_page(a.c, seq, block) : -1;
+                    count += page[c] >= 0;
+                }
+#pragma unroll
+                for (int op = 0; op < 2; ++op) {
+                    if (!(ok = ok && (j == 0 || wait(&b.raw_empty[op], j - 1)))) break;
+                    // (where no page is, what stood there stays: its keys are hidden, its values not multiplied)
+                    mbar_arrive_expect_tx(&b.raw_full[op], count * kBytes);
+#pragma unroll
+                    for (int c = 0; c < kTileBlocks; ++c)
+                        if (page[c] >= 0)
+                            bulk_copy(sm + L::raw + op * L::RAW + c * kBytes,
+                                      (op ? a.c.v_codes : a.c.k_codes) + kv8_codes_at(a.c, page[c], kh), kBytes, &b.raw_full[op]);
+                    issued[op] = j + 1;
+                }
+            }
+            // never leave with copies in flight
+#pragma unroll
+            for (int op = 0; op < 2; ++op)
+                if (issued[op] > 0) mbar_wait(&b.raw_full[op], (uint32_t)(issued[op] - 1) & 1u, nullptr, 0);
         }
         __syncwarp();
-        reg_inc<128>();
     }
     tc_fence_before();
     __syncthreads();
+    if (warp >= 8) reg_inc<128>();
     if (warp == 12) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
