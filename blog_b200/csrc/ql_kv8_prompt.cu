@@ -2,10 +2,12 @@
 // tensor cores.
 //
 // A CTA takes 256 rows (query token, head of one KV head's group; the group's heads share every key) as two
-// tiles of 128 and walks over the keys 128 at a time with a running maximum and total per row:
+// tiles of 128 and walks over the keys 64 at a time with a running maximum and total per row:
 //   S = Q K^T       tcgen05.mma, Q and K in shared memory, S (fp32) in TMEM
 //   P = 2^(S f - m) one thread per row; f: the block's scale of K x the row's scale; P (f16) over S in TMEM
 //   O += P V        tcgen05.mma, P from TMEM, V in shared memory, O (fp32) in TMEM
+// S has two buffers, so that a row tile's next scores are computed while it exponentiates these: 2 x (2 x 64 + 128)
+// columns are all of TMEM.
 // Codes are exact in f16.  bf16 rows: q scaled by a power of two is exact in f16 too, P is rounded to f16's 11
 // bits (its result is rounded to 8).  f32 rows: q and P in two f16 limbs, twice the products, fp32 results.
 // The scale of V's block is multiplied into P relative to the row's largest such product, as in the split
@@ -14,8 +16,7 @@
 // Roles, 16 warps: 0-3 and 4-7 a thread per row of tile 0 and 1 (S from TMEM, P to TMEM, the result); 13 copies
 // the pages' codes into shared memory (one bulk copy per block and operand), 8-11 turn them into f16 in the layout
 // the MMA reads (128-byte swizzle; K with the head dimension contiguous and V too, as the transposed operand), a
-// tile ahead; 12 issues the MMAs.  While one tile's
-// threads exponentiate, the tensor cores run the other tile's products.
+// tile ahead; 12 issues the MMAs.
 // The rows of the block that is not full make a last tile of 64 keys: their upper f16 limbs, then their lower.
 //
 // Where the tiles of rows alone would leave SMs idle, the keys are split over the CTAs of a cluster, and their
@@ -37,7 +38,7 @@ namespace ql {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kKeys = 128;   // keys per tile: 4 blocks
+constexpr int kKeys = 64;    // keys per tile: 2 blocks
 constexpr int kTileBlocks = kKeys / kKvBlock;
 constexpr int kRows = 256;   // rows per CTA: two MMA tiles
 constexpr float kHeadroom = 7.0f, kWBits = 8.0f;  // as in the split kernel
@@ -49,11 +50,11 @@ static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs == 4 * 128, "the bloc
 template <int HD, int LIMBS>
 struct Layout {
     static constexpr int A = HD / 64;                        // 128-byte columns of a row
-    static constexpr int ST = LIMBS == 2 && HD == 128 ? 1 : 2;  // K and V stages
+    static constexpr int ST = 2;                             // K and V stages, and of their codes
     static constexpr int QT = A * 128 * 128;                 // one limb of one tile of Q
     static constexpr int KV = A * kKeys * 128;               // one stage of K or of V
     static constexpr int RAW = kKeys * HD;                   // a tile's codes of K or of V
-    static constexpr int q = 0, k = q + 2 * LIMBS * QT, v = k + ST * KV, raw = v + ST * KV, end = raw + 2 * RAW;
+    static constexpr int q = 0, k = q + 2 * LIMBS * QT, v = k + ST * KV, raw = v + ST * KV, end = raw + 2 * ST * RAW;
     static constexpr int bytes = 1024 + end + 512;
 };
 
@@ -143,6 +144,16 @@ __device__ __forceinline__ void bulk_copy(void *dst, const void *src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
                  "l"(src), "r"(bytes), "r"(smem_u32(bar))
                  : "memory");
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e != 0;
 }
 template <int N>
 __device__ __forceinline__ void reg_dec() {
@@ -251,13 +262,19 @@ struct Few {
     }
 };
 
+// Hand-overs.  No waiter may fall two phases behind its barrier: what is handed from tile to tile by roles that
+// run ahead of one another has a ring.
 struct Bars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], raw_full[2], raw_empty[2], open_max, done;
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t raw_full[2][2], raw_empty[2][2];  // [operand][stage]
+    uint64_t s_full[2][2], p_full[2][2];       // [tile of rows][S buffer]
+    uint64_t o_full[2];                        // a tile's product with V has been added
+    uint64_t scales[4], open_max, done;
     uint32_t tmem;
     int abort;
-    // Scales of the tile's blocks (K's < 0: no such block), a ring: when the scores of the tile ST before have been
-    // computed, its rows may still have to read them, so ST + 1 tiles are in use.
-    float ks[4][kTileBlocks], vs[4][kTileBlocks];
+    // A tile's scales (K's < 0: no such block).  When they are written the scores two tiles before are done, which
+    // their rows may be about to read, and no earlier ones: four are in use at most.
+    float ks[4][kTileBlocks], vs[4][kTileBlocks], lv[4][kTileBlocks];  // lv: log2 of vs
     int plain[4];   // every block of the tile is there, its scales positive and finite
     unsigned bad;   // tokens of the open block that hold NaN or infinity
 };
@@ -268,14 +285,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     constexpr int LIMBS = sizeof(T) == 4 ? 2 : 1;
     using L = Layout<HD, LIMBS>;
     constexpr int A = L::A, ST = L::ST;
-    constexpr uint32_t kS = 0, kO = kKeys, kTile = 256;  // TMEM columns of a tile: S (then P), O
+    constexpr uint32_t kS = 0, kO = 2 * kKeys, kTile = 256;  // TMEM columns of a tile of rows: S (then P) twice, O
     constexpr int kPitch = HD + 4;                       // floats of a row's sums in shared memory at the end
     static_assert(kRows * kPitch * 4 <= L::end, "the sums take the operands' place");
     extern __shared__ uint8_t sm_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     Bars &b = *reinterpret_cast<Bars *>(sm + L::end);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (values of the whole warp pass a shuffle, which tells the compiler so: the MMA's operands are uniform registers)
+    auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+    const int warp = uni(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int G = a.n_heads / a.c.kv_heads;
     const int split = blockIdx.x % a.cluster, kh = blockIdx.x / a.cluster, seq = blockIdx.y, r_base = (gridDim.z - 1 - blockIdx.z) * kRows;  // longest first
     int row0, q_len;
@@ -303,15 +322,18 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     for (int i = 0; i < 2; ++i) n_tiles[i] = max(0, min(n_tiles[i], j0 + per) - j0);
     const int n_all = max(n_tiles[0], n_tiles[1]);
     const int n_c = max(0, min(n_all, n_closed - j0));  // closed tiles among them
-    auto tile_blocks = [&](int jj) { return j0 + jj < n_closed ? min(kTileBlocks, blocks - (j0 + jj) * kTileBlocks) : 2; };
 
     if (threadIdx.x == 0) {
         mbar_init(&b.q_full, kRows);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b.k_full[i], 4), mbar_init(&b.k_empty[i], 1), mbar_init(&b.v_full[i], 4), mbar_init(&b.v_empty[i], 1);
-            mbar_init(&b.s_full[i], 1), mbar_init(&b.p_full[i], 4), mbar_init(&b.o_full[i], 1);
-            mbar_init(&b.raw_full[i], 1), mbar_init(&b.raw_empty[i], 4);
+            for (int k = 0; k < 2; ++k) {
+                mbar_init(&b.s_full[i][k], 1), mbar_init(&b.p_full[i][k], 4);
+                mbar_init(&b.raw_full[i][k], 1), mbar_init(&b.raw_empty[i][k], 4);
+            }
+            mbar_init(&b.o_full[i], 1);
         }
+        for (int k = 0; k < 4; ++k) mbar_init(&b.scales[k], 1);
         mbar_init(&b.open_max, 4);
         mbar_init(&b.done, 1);
         b.abort = 0;
@@ -321,13 +343,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = b.tmem;
+    const uint32_t tmem = uni(b.tmem);
     volatile int *abort_flag = &b.abort;
-    // Bounded wait: false (and everybody told) when it ran out or another role gave up.
+    // Bounded wait (about 2 s): false, and everybody told, when it ran out or another role gave up.  The limit is by
+    // the SM's own clock: a read of the global timer at every hand-over would cost more than the hand-over.
     auto wait = [&](uint64_t *bar, int phase) {
-        if (*abort_flag || !mbar_wait(bar, (uint32_t)phase & 1u, a.c.err, kErrWaitFull)) {
-            *abort_flag = 1;
-            return false;
+        if (mbar_try_wait(bar, (uint32_t)phase & 1u)) return true;
+        const long long t0 = clock64();
+        while (!mbar_try_wait(bar, (uint32_t)phase & 1u)) {
+            if (*abort_flag) return false;
+            if (clock64() - t0 > 4000000000ll) {
+                atomicExch(a.c.err, kErrWaitFull);
+                *abort_flag = 1;
+                return false;
+            }
         }
         return true;
     };
@@ -379,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         fence_proxy_async_smem();
         mbar_arrive(&b.q_full);
 
-        const uint32_t tS = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + i * kTile + kS, tO = tS - kS + kO;
+        const uint32_t tS0 = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + i * kTile + kS, tO = tS0 - kS + kO;
         float m = -INFINITY, l = 0.f, h = -INFINITY, wf = 0.f;  // (as in the split kernel; wf: its w)
         const int n = n_tiles[i];
         bool ok = true;
@@ -390,8 +419,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         }
         // The tensor cores truncate when they accumulate, so a sum over thousands of keys in TMEM would lose
         // bits in one direction.  For f32 rows a tile's product starts from zero and is added here, rounded.
-        auto add_tile = [&]() {
+        auto add_tile = [&](float z) {  // z: the unit of the rows' weights has changed since
             if constexpr (LIMBS == 2) {
+                const float2 z2 = make_float2(z, z);
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) {
                     uint32_t o[32];
@@ -399,34 +429,34 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float2 z = fadd2(make_float2(acc[32 * c + e], acc[32 * c + e + 1]),
-                                               make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])));
-                        acc[32 * c + e] = z.x, acc[32 * c + e + 1] = z.y;
+                        const float2 x = ffma2_of(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), z2,
+                                                  make_float2(acc[32 * c + e], acc[32 * c + e + 1]));
+                        acc[32 * c + e] = x.x, acc[32 * c + e + 1] = x.y;
                     }
                 }
             }
         };
 #pragma unroll 1
         for (int j = 0; j < n; ++j) {
-            // (k_full too: the scales are the converters' writes)
-            ok = __all_sync(0xffffffffu, wait(&b.k_full[j % ST], j / ST) && wait(&b.s_full[i], j));
+            const uint32_t tS = tS0 + (j & 1) * kKeys;
+            ok = __all_sync(0xffffffffu, wait(&b.scales[j & 3], j >> 2) && wait(&b.s_full[i][j & 1], j >> 1));
             if (!ok) break;
-            tc_fence_after();  // (S full: the earlier products into O have completed too)
-            if (LIMBS == 2 && j > 0) add_tile();
+            tc_fence_after();
             const bool open = j0 + j == n_closed;
             // the last key of the tile that the row sees (a closed tile ends with the closed blocks)
             const int see = open ? pos - open0 : min(pos, open0 - 1) - (j0 + j) * kKeys;
-            const float *ks = b.ks[j & 3], *vs = b.vs[j & 3];
+            const float *ks = b.ks[j & 3], *vs = b.vs[j & 3], *lv = b.lv[j & 3];
             // (per warp) ordinary: all of the tile's scales are positive and finite
             const bool masked = __any_sync(0xffffffffu, see < kKeys - 1);
             bool plain = b.plain[j & 3] && a.scale_log2 != 0.f;
             if (plain && masked) {  // hidden scores have to end far below the others
-                const float least = fminf(fminf(ks[0], ks[1]), fminf(ks[2], ks[3])) * row_scale;
+                const float least = fminf(ks[0], ks[1]) * row_scale;
                 plain = __all_sync(0xffffffffu, least > 1e-30f);
             }
 
             // Largest score of each block.
-            float t[kTileBlocks] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float t[kTileBlocks] = {-INFINITY, -INFINITY};
+            uint32_t held[LIMBS == 1 ? kKeys : 1];  // bf16 rows have registers for all of them
             // GR products from column GR u, as they came; the open block's: the two limbs' sums
             constexpr int GR = LIMBS == 2 ? 16 : 32;
             auto raw = [&](int u, uint32_t *s) {
@@ -461,22 +491,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const int grains = (open ? kKvBlock : kKeys) / GR;
             const unsigned bad = open ? b.bad : 0;
             if (plain) {
-                // (loops kept rolled: the roles share the instruction cache; f32 rows have registers for one block)
-                constexpr int NB = LIMBS == 2 ? 1 : 2;
-#pragma unroll 1
-                for (int c = 0; c < kTileBlocks; c += NB) {
-                    uint32_t s[32 * NB];
+                if constexpr (LIMBS == 1) {
 #pragma unroll
-                    for (int k = 0; k < NB; ++k) tmem_ld32(tS + 32 * (c + k), s + 32 * k);
+                    for (int c = 0; c < kTileBlocks; ++c) tmem_ld32(tS + 32 * c, held + 32 * c);
                     tmem_wait_ld();
+                }
 #pragma unroll
-                    for (int k = 0; k < NB; ++k) {
-                        if (masked) hide(32 * (c + k), 32, s + 32 * k);
-                        const float x = 32 * (c + k) > see ? -INFINITY : top32(s + 32 * k) * (ks[c + k] * row_scale);
-#pragma unroll
-                        for (int z = k; z < kTileBlocks; z += NB)
-                            if (z == c + k) t[z] = x;
+                for (int c = 0; c < kTileBlocks; ++c) {
+                    uint32_t own[32], *s = LIMBS == 1 ? held + 32 * c : own;
+                    if constexpr (LIMBS == 2) {
+                        tmem_ld32(tS + 32 * c, s);
+                        tmem_wait_ld();
                     }
+                    if (masked) hide(32 * c, 32, s);
+                    t[c] = 32 * c > see ? -INFINITY : top32(s) * (ks[c] * row_scale);
                 }
             } else {
 #pragma unroll 1
@@ -497,41 +525,36 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
             // The factor of the sums so far.
             float z = 1.f;
-            {
-                const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-                float u = -INFINITY;  // log2 of the heaviest weight x scale, m aside
+            const float top = fmaxf(t[0], t[1]);
+            if (__any_sync(0xffffffffu, top > m + kHeadroom || fmaxf(t[0] + lv[0], t[1] + lv[1]) - m > h + kHeadroom)) {
+                if (top > m) {
+                    const float x = ceilf(top);
+                    l *= ex2(m - x);
+                    h -= x - m;
+                    m = x;
+                }
+                const float u = ceilf(fmaxf(t[0] - m + lv[0], t[1] - m + lv[1]));  // of the heaviest weight x scale
+                if (u > h) {
+                    z = ex2(h - u);
+                    h = u;
+                }
+                wf = weight_unit(h);
+                if (__any_sync(0xffffffffu, z != 1.f)) {
+                    if constexpr (LIMBS == 2) {
 #pragma unroll
-                for (int c = 0; c < kTileBlocks; ++c) u = fmaxf(u, t[c] + __log2f(vs[c]));
-                if (__any_sync(0xffffffffu, top > m + kHeadroom || u - m > h + kHeadroom)) {
-                    if (top > m) {
-                        const float x = ceilf(top);
-                        l *= ex2(m - x);
-                        h -= x - m;
-                        m = x;
-                    }
-                    u = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < kTileBlocks; ++c) u = fmaxf(u, t[c] - m + __log2f(vs[c]));
-                    u = ceilf(u);
-                    if (u > h) {
-                        z = ex2(h - u);
-                        h = u;
-                    }
-                    wf = weight_unit(h);
-                    if (__any_sync(0xffffffffu, z != 1.f)) {
-                        if constexpr (LIMBS == 2) {
-#pragma unroll
-                            for (int e = 0; e < HD; ++e) acc[e] *= z;
-                        } else if (j > 0) {
+                        for (int e = 0; e < HD; ++e) acc[e] *= z;
+                    } else if (j > 0) {  // (the product before is the last so far: this tile's waits for its weights)
+                        ok = __all_sync(0xffffffffu, wait(&b.o_full[i], j - 1));
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll 1
-                            for (int c = 0; c < HD / 32; ++c) {
-                                uint32_t o[32];
-                                tmem_ld32(tO + 32 * c, o);
-                                tmem_wait_ld();
+                        for (int c = 0; c < HD / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(tO + 32 * c, o);
+                            tmem_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * z);
-                                tmem_st32(tO + 32 * c, o);
-                            }
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * z);
+                            tmem_st32(tO + 32 * c, o);
                         }
                     }
                 }
@@ -569,9 +592,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     }
                     tmem_st16(tS + 16 * u, w);
                 };
+                if constexpr (LIMBS == 1) {
+#pragma unroll
+                    for (int c = 0; c < kTileBlocks; ++c) weigh(c, held + 32 * c);
+                } else {
 #pragma unroll 1
-                for (int u = 0; u < kKeys / GR; u += 2) {
-                    if constexpr (GR == 16) {
+                    for (int u = 0; u < kKeys / 16; u += 2) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             uint32_t s[16];
@@ -580,17 +606,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                             if (masked) hide(16 * (u + k), 16, s);
                             weigh(u + k, s);
                         }
-                    } else {
-                        uint32_t s[64];
-                        tmem_ld32(tS + 32 * u, s);
-                        tmem_ld32(tS + 32 * u + 32, s + 32);
-                        tmem_wait_ld();
-                        if (masked) {
-                            hide(32 * u, 32, s);
-                            hide(32 * u + 32, 32, s + 32);
-                        }
-                        weigh(u, s);
-                        weigh(u + 1, s + 32);
                     }
                 }
             } else {
@@ -638,15 +653,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
             }
             l += sum.x + sum.y;
+            if (LIMBS == 2 && j > 0) {  // the tile before's product, ere this one's takes its place
+                ok = __all_sync(0xffffffffu, wait(&b.o_full[i], j - 1));
+                if (!ok) break;
+                tc_fence_after();
+                add_tile(z);
+            }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.p_full[i]);
+            if (lane == 0) mbar_arrive(&b.p_full[i][j & 1]);
         }
         if (n > 0) {
-            ok = __all_sync(0xffffffffu, ok && wait(&b.o_full[i], 0));
+            ok = __all_sync(0xffffffffu, ok && wait(&b.o_full[i], n - 1));
             tc_fence_after();
-            add_tile();
+            add_tile(1.f);
         }
         // Every product of the CTA has been computed: Q, K and V make way for the rows' sums, x 2^(h - kWBits) (the
         // power in two steps where it leaves the range), their maxima and totals.
@@ -696,11 +717,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             return j < ST || __all_sync(0xffffffffu, wait(bar, j / ST - 1));
         };
         auto convert = [&](int op, int j, uint64_t *stage_empty, uint8_t *tile) {
-            if (!__all_sync(0xffffffffu, wait(&b.raw_full[op], j))) return false;
-            const uint8_t *src = sm + L::raw + op * L::RAW + (at * 4 + pc) * 16;
+            if (!__all_sync(0xffffffffu, wait(&b.raw_full[op][j % ST], j / ST))) return false;
+            const uint8_t *src = sm + L::raw + (op * ST + j % ST) * L::RAW + (at * 4 + pc) * 16;
             uint8_t *p = tile + at * (kKeys * 128);
             if (!empty(stage_empty, j)) return false;
-            constexpr int H = U / 2;
+            constexpr int H = U < 4 ? U : 4;
 #pragma unroll
             for (int u0 = 0; u0 < U; u0 += H) {
                 uint4 raw[H];
@@ -721,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b.raw_empty[op]);
+            if (lane == 0) mbar_arrive(&b.raw_empty[op][j % ST]);
             return true;
         };
         // scales of a tile's blocks (lanes 0 .. 3 of the first warp)
@@ -739,22 +760,33 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             next_ks = c >= 0 ? a.c.k_scale[z] : -1.f;
             next_vs = c >= 0 ? a.c.v_scale[z] : 0.f;
         };
-        if (n_c > 0) scales(0);
-        for (int j = 0; j < n_c && ok; ++j) {
+        // K two tiles ahead of V, as the MMAs take them: the scores of tile j + 2 follow the values of tile j.
+        auto convert_k = [&](int j) {
             const int st = j % ST;
-            if (!(ok = convert(0, j, &b.k_empty[st], sm + L::k + st * L::KV))) break;
+            if (j >= n_c) return true;
+            if (!convert(0, j, &b.k_empty[st], sm + L::k + st * L::KV)) return false;
+            full(&b.k_full[st]);
             if (w == 0) {
                 const bool good = next_ks > 0.f && next_ks < INFINITY && next_vs > 0.f && next_vs < INFINITY;
+                const unsigned all = __ballot_sync(0xffffffffu, good || lane >= kTileBlocks);
                 if (lane < kTileBlocks) {
                     b.ks[j & 3][lane] = next_ks;
                     b.vs[j & 3][lane] = next_vs;
+                    b.lv[j & 3][lane] = log2f(next_vs);
                 }
-                const unsigned all = __ballot_sync(0xffffffffu, good);
-                if (lane == 0) b.plain[j & 3] = (all & 15u) == 15u;
+                if (lane == 0) b.plain[j & 3] = all == 0xffffffffu;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b.scales[j & 3]);
                 if (j + 1 < n_c) scales(j + 1);
             }
-            full(&b.k_full[st]);
-            if (!(ok = convert(1, j, &b.v_empty[st], sm + L::v + st * L::KV))) break;
+            return true;
+        };
+        if (n_c > 0) scales(0);
+        ok = convert_k(0) && convert_k(1);
+#pragma unroll 1
+        for (int j = 0; j < n_c && ok; ++j) {
+            const int st = j % ST;
+            if (!(ok = convert_k(j + 2) && convert(1, j, &b.v_empty[st], sm + L::v + st * L::KV))) break;
             full(&b.v_full[st]);
         }
         if (ok && n_all > n_c) {  // the open block: upper limbs in rows 0..31, lower in 32..63
@@ -809,8 +841,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 b.bad = slot >= 0 ? s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3] : 0;
                 b.ks[j & 3][0] = slot >= 0 ? inv[0] : 0.f;
                 b.vs[j & 3][0] = slot >= 0 ? inv[1] : 0.f;
-                for (int c = 1; c < kTileBlocks; ++c) b.ks[j & 3][c] = b.vs[j & 3][c] = 0.f;
+                b.lv[j & 3][0] = log2f(b.vs[j & 3][0]);
+                b.ks[j & 3][1] = b.vs[j & 3][1] = 0.f;
+                b.lv[j & 3][1] = -INFINITY;
                 b.plain[j & 3] = 0;
+                mbar_arrive(&b.scales[j & 3]);
             }
             for (int op = 0; op < 2 && ok; ++op) {
                 if (op == 1 && !(ok = empty(&b.v_empty[st], j))) break;
@@ -836,13 +871,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     } else {
         // ------------------------------------ MMA issue ------------------------------------
         reg_dec<kIssueRegs>();
-        if (warp == 12 && lane == 0) {
+        if (warp == 12) {
+            // The whole warp goes along, one elected lane issues: 24 or 48 MMAs a tile, descriptors sums of constants.
             const uint32_t sq = smem_u32(sm + L::q), sk = smem_u32(sm + L::k), sv = smem_u32(sm + L::v);
-            // (one thread issues 32 or 64 MMAs a tile: descriptors are sums of constants, the loops unrolled)
             const uint32_t dq = desc_k(sq), dk = desc_k(sk), dv = desc_mn(sv, kKeys * 128);
+            const int nt0 = uni(n_tiles[0]), nt1 = uni(n_tiles[1]), nt = max(nt0, nt1), closed = uni(n_closed - j0);
+            const int last_blocks = uni(blocks - (n_closed - 1) * kTileBlocks);  // of the last closed tile
+            auto all_wait = [&](uint64_t *bar, int phase) { return __all_sync(0xffffffffu, wait(bar, phase)); };
             auto scores = [&](int i, int j) {
-                const uint32_t qb = dq + (i * L::QT >> 4), kb = dk + ((ST == 1 ? 0 : j % ST) * L::KV >> 4);
-                const uint32_t d = tmem + i * kTile + kS;
+                const uint32_t qb = dq + (i * L::QT >> 4), kb = dk + (j % ST * L::KV >> 4);
+                const uint32_t d = tmem + i * kTile + kS + (j & 1) * kKeys;
 #pragma unroll
                 for (int z = LIMBS - 1; z >= 0; --z)  // (lower limbs first: fewer additions to a full-sized sum)
 #pragma unroll
@@ -856,67 +894,69 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                             else
                                 mma_ss<true>(d, qa, ka, idesc(kKeys, false));
                         }
-                mma_commit(&b.s_full[i]);
+                mma_commit(&b.s_full[i][j & 1]);
             };
             auto values = [&](int i, int j) {
-                const uint32_t vb = dv + ((ST == 1 ? 0 : j % ST) * L::KV >> 4);
-                const uint32_t d = tmem + i * kTile + kO, p = tmem + i * kTile + kS;
+                const uint32_t vb = dv + (j % ST * L::KV >> 4);
+                const uint32_t d = tmem + i * kTile + kO, p = tmem + i * kTile + kS + (j & 1) * kKeys;
                 const uint32_t first = LIMBS == 2 ? 0u : (uint32_t)(j > 0);  // f32 rows: each tile's product by itself
                 // 16 keys are 8 columns of P; two limbs: 8 of the upper, then 8 of the lower
                 auto step = [&](int z, int k, uint32_t add) {
                     mma_ts(d, p + (LIMBS == 2 ? 16 * k + 8 * z : 8 * k), vb + (k * 2048 >> 4), idesc(HD, true), add);
                 };
-                const int steps = 2 * tile_blocks(j);
-                if (steps == 2 * kTileBlocks) {
+                const bool half = j == closed - 1 && last_blocks == 1;  // one block in the tile
 #pragma unroll
-                    for (int z = LIMBS - 1; z >= 0; --z)
+                for (int z = LIMBS - 1; z >= 0; --z)
 #pragma unroll
-                        for (int k = 0; k < 2 * kTileBlocks; ++k) step(z, k, z == LIMBS - 1 && k == 0 ? first : 1u);
-                } else {
-#pragma unroll 1
-                    for (int z = LIMBS - 1; z >= 0; --z)
-#pragma unroll 1
-                        for (int k = 0; k < steps; ++k) step(z, k, z == LIMBS - 1 && k == 0 ? first : 1u);
-                }
+                    for (int k = 0; k < 2 * kTileBlocks; ++k)
+                        if (k < 2 || !half) step(z, k, z == LIMBS - 1 && k == 0 ? first : 1u);
+                mma_commit(&b.o_full[i]);
             };
-            bool ok = n_all == 0 || (wait(&b.q_full, 0) && wait(&b.k_full[0], 0));
-            if (ok && n_all > 0) {
+            bool ok = nt == 0 || all_wait(&b.q_full, 0);
+            for (int j = 0; j < 2 && j < nt && ok; ++j) {
+                if (!(ok = all_wait(&b.k_full[j % ST], j / ST))) break;
                 tc_fence_after();
-                for (int i = 0; i < 2; ++i)
-                    if (n_tiles[i] > 0) scores(i, 0);
-                mma_commit(&b.k_empty[0]);
-            }
-            for (int j = 0; j < n_all && ok; ++j) {
-                bool v = false, k = false;
-                for (int i = 0; i < 2 && ok; ++i) {
-                    if (j >= n_tiles[i]) continue;
-                    ok = wait(&b.p_full[i], j) && (v || wait(&b.v_full[j % ST], j / ST));
-                    if (!ok) break;
-                    v = true;
-                    tc_fence_after();
-                    values(i, j);
-                    if (j + 1 < n_tiles[i]) {
-                        ok = k || wait(&b.k_full[(j + 1) % ST], (j + 1) / ST);
-                        if (!ok) break;
-                        k = true;
-                        tc_fence_after();
-                        scores(i, j + 1);
-                    } else {
-                        mma_commit(&b.o_full[i]);
-                    }
+                if (elect_one()) {
+                    if (j < nt0) scores(0, j);
+                    if (j < nt1) scores(1, j);
+                    mma_commit(&b.k_empty[j % ST]);
                 }
-                mma_commit(&b.v_empty[j % ST]);
-                if (j + 1 < n_all) mma_commit(&b.k_empty[(j + 1) % ST]);
+                __syncwarp();
+            }
+#pragma unroll 1
+            for (int j = 0; j < nt && ok; ++j) {
+                if (!(ok = all_wait(&b.v_full[j % ST], j / ST))) break;
+                const bool more = j + 2 < nt;
+                if (more && !(ok = all_wait(&b.k_full[j % ST], (j + 2) / ST))) break;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int n_i = i ? nt1 : nt0;
+                    if (j >= n_i || !ok) continue;
+                    if (!(ok = all_wait(&b.p_full[i][j & 1], j >> 1))) continue;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        values(i, j);
+                        if (j + 2 < n_i) scores(i, j + 2);  // into the buffer of the weights just multiplied, after them
+                    }
+                    __syncwarp();
+                }
+                if (ok && elect_one()) {
+                    mma_commit(&b.v_empty[j % ST]);
+                    if (more) mma_commit(&b.k_empty[j % ST]);
+                }
+                __syncwarp();
             }
             // every MMA has completed before TMEM is freed
-            mma_commit(&b.done);
-            mbar_wait(&b.done, 0u, a.c.err, kErrWaitFull);
+            if (elect_one()) mma_commit(&b.done);
+            __syncwarp();
+            wait(&b.done, 0);
         } else if (warp == 13 && lane == 0) {
             // ------------------------------------ pages to shared memory ------------------------------------
             constexpr uint32_t kBytes = kKvBlock * HD;
             int issued[2] = {0, 0};
-            bool ok = true;
-            for (int j = 0; j < n_c && ok; ++j) {
+            auto load = [&](int op, int j) {
+                if (j >= n_c) return true;
+                const int st = j % ST;
                 int page[kTileBlocks], count = 0;
 #pragma unroll
                 for (int c = 0; c < kTileBlocks; ++c) {
@@ -924,23 +964,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     page[c] = block < blocks ? kv8_page(a.c, seq, block) : -1;
                     count += page[c] >= 0;
                 }
+                if (j >= ST && !wait(&b.raw_empty[op][st], j / ST - 1)) return false;
+                // (where no page is, what stood there stays: its keys are hidden, its values not multiplied)
+                mbar_arrive_expect_tx(&b.raw_full[op][st], count * kBytes);
 #pragma unroll
-                for (int op = 0; op < 2; ++op) {
-                    if (!(ok = ok && (j == 0 || wait(&b.raw_empty[op], j - 1)))) break;
-                    // (where no page is, what stood there stays: its keys are hidden, its values not multiplied)
-                    mbar_arrive_expect_tx(&b.raw_full[op], count * kBytes);
-#pragma unroll
-                    for (int c = 0; c < kTileBlocks; ++c)
-                        if (page[c] >= 0)
-                            bulk_copy(sm + L::raw + op * L::RAW + c * kBytes,
-                                      (op ? a.c.v_codes : a.c.k_codes) + kv8_codes_at(a.c, page[c], kh), kBytes, &b.raw_full[op]);
-                    issued[op] = j + 1;
-                }
-            }
+                for (int c = 0; c < kTileBlocks; ++c)
+                    if (page[c] >= 0)
+                        bulk_copy(sm + L::raw + (op * ST + st) * L::RAW + c * kBytes,
+                                  (op ? a.c.v_codes : a.c.k_codes) + kv8_codes_at(a.c, page[c], kh), kBytes, &b.raw_full[op][st]);
+                issued[op] = j + 1;
+                return true;
+            };
+            bool ok = load(0, 0) && load(0, 1);
+            for (int j = 0; j < n_c && ok; ++j) ok = load(1, j) && load(0, j + 2);
             // never leave with copies in flight
 #pragma unroll
             for (int op = 0; op < 2; ++op)
-                if (issued[op] > 0) mbar_wait(&b.raw_full[op], (uint32_t)(issued[op] - 1) & 1u, nullptr, 0);
+                for (int j = max(0, issued[op] - ST); j < issued[op]; ++j)
+                    mbar_wait(&b.raw_full[op][j % ST], (uint32_t)(j / ST) & 1u, nullptr, 0);
         }
         __syncwarp();
     }
