@@ -44,7 +44,7 @@ constexpr int kRows = 256;   // rows per CTA: two MMA tiles
 constexpr float kHeadroom = 7.0f, kWBits = 8.0f;  // as in the split kernel
 
 // Registers per thread of the roles; 16 warps launch with 128 each.
-constexpr int kSoftmaxRegs = 168, kConvertRegs = 96, kIssueRegs = 80;
+constexpr int kSoftmaxRegs = 200, kConvertRegs = 64, kIssueRegs = 48;
 static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs == 4 * 128, "the block's registers at launch");
 
 template <int HD, int LIMBS>
@@ -456,7 +456,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
             // Largest score of each block.
             float t[kTileBlocks] = {-INFINITY, -INFINITY};
-            uint32_t held[LIMBS == 1 ? kKeys : 1];  // bf16 rows have registers for all of them
             // GR products from column GR u, as they came; the open block's: the two limbs' sums
             constexpr int GR = LIMBS == 2 ? 16 : 32;
             auto raw = [&](int u, uint32_t *s) {
@@ -490,23 +489,105 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             };
             const int grains = (open ? kKvBlock : kKeys) / GR;
             const unsigned bad = open ? b.bad : 0;
-            if (plain) {
-                if constexpr (LIMBS == 1) {
-#pragma unroll
-                    for (int c = 0; c < kTileBlocks; ++c) tmem_ld32(tS + 32 * c, held + 32 * c);
-                    tmem_wait_ld();
+            // Whether a score, or a score and log2 of its value's scale, has passed what the weights stand in relation to
+            // by more than the headroom, in some row of the warp; and if so, the new relation and z, the factor of the
+            // sums so far.
+            float z = 1.f;
+            auto exceeds = [&]() {
+                return __any_sync(0xffffffffu, fmaxf(t[0], t[1]) > m + kHeadroom ||
+                                                   fmaxf(t[0] + lv[0], t[1] + lv[1]) - m > h + kHeadroom);
+            };
+            auto settle = [&]() {
+                const float top = fmaxf(t[0], t[1]);
+                if (top > m) {
+                    const float x = ceilf(top);
+                    l *= ex2(m - x);
+                    h -= x - m;
+                    m = x;
                 }
+                const float u = ceilf(fmaxf(t[0] - m + lv[0], t[1] - m + lv[1]));  // of the heaviest weight x scale
+                if (u > h) {
+                    z = ex2(h - u);
+                    h = u;
+                }
+                wf = weight_unit(h);
+                if (!__any_sync(0xffffffffu, z != 1.f)) return true;
+                if constexpr (LIMBS == 2) {
+#pragma unroll
+                    for (int e = 0; e < HD; ++e) acc[e] *= z;
+                } else if (j > 0) {  // (the product before is the last so far: this tile's waits for its weights)
+                    if (!__all_sync(0xffffffffu, wait(&b.o_full[i], j - 1))) return false;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + 32 * c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * z);
+                        tmem_st32(tO + 32 * c, o);
+                    }
+                }
+                return true;
+            };
+            auto is_deep = [&]() { return __any_sync(0xffffffffu, h < kDeep && h != -INFINITY); };
+            bool weighed = false;
+            if constexpr (LIMBS == 1) {
+                if (plain && !is_deep()) {
+                    // bf16 rows: all 64 scores in registers, their weights computed in the relation that stands, their
+                    // maxima beside; seldom, when these exceed it, once more.
+                    uint32_t s[kKeys];
+#pragma unroll
+                    for (int c = 0; c < kTileBlocks; ++c) tmem_ld32(tS + 32 * c, s + 32 * c);
+                    tmem_wait_ld();
+                    if (masked) {
+                        hide(0, 32, s);
+                        hide(32, 32, s + 32);
+                    }
+#pragma unroll 1
+                    for (int again = 0; again < 2; ++again) {
+                        uint32_t w[kKeys / 2];
+                        float2 sum = make_float2(0.f, 0.f);
+                        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                        for (int c = 0; c < kTileBlocks; ++c) {
+                            const float f = ks[c] * row_scale, g = vs[c] * wf;
+                            const float2 f2 = make_float2(f, f), b2 = make_float2(-base, -base), g2 = make_float2(g, g);
+                            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                const float2 v = make_float2(__uint_as_float(s[32 * c + e]), __uint_as_float(s[32 * c + e + 1]));
+                                const float2 d = ffma2_of(v, f2, b2), p = make_float2(ex2(d.x), ex2(d.y));
+                                top[0] = fmaxf(top[0], v.x), top[1] = fmaxf(top[1], v.y);
+                                sum = fadd2(sum, p);
+                                const float2 x = fmul2(p, g2);
+                                w[16 * c + e / 2] = pack_f16(x.x, x.y);
+                            }
+                            t[c] = 32 * c > see ? -INFINITY : fmaxf(top[0], top[1]) * f;
+                        }
+                        if (!exceeds()) {
+                            tmem_st32(tS, w);
+                            l += sum.x + sum.y;
+                            weighed = true;
+                            break;
+                        }
+                        if (!(ok = settle()) || is_deep()) break;
+                    }
+                }
+                if (!ok) break;
+            }
+            if (!weighed) {
+            if (LIMBS == 2 && plain) {
 #pragma unroll
                 for (int c = 0; c < kTileBlocks; ++c) {
-                    uint32_t own[32], *s = LIMBS == 1 ? held + 32 * c : own;
-                    if constexpr (LIMBS == 2) {
-                        tmem_ld32(tS + 32 * c, s);
-                        tmem_wait_ld();
-                    }
+                    uint32_t s[32];
+                    tmem_ld32(tS + 32 * c, s);
+                    tmem_wait_ld();
                     if (masked) hide(32 * c, 32, s);
                     t[c] = 32 * c > see ? -INFINITY : top32(s) * (ks[c] * row_scale);
                 }
             } else {
+                t[0] = t[1] = -INFINITY;
 #pragma unroll 1
                 for (int u = 0; u < grains; ++u) {
                     uint32_t s[GR];
@@ -523,44 +604,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         if (k == c) t[k] = fmaxf(t[k], x);
                 }
             }
-            // The factor of the sums so far.
-            float z = 1.f;
-            const float top = fmaxf(t[0], t[1]);
-            if (__any_sync(0xffffffffu, top > m + kHeadroom || fmaxf(t[0] + lv[0], t[1] + lv[1]) - m > h + kHeadroom)) {
-                if (top > m) {
-                    const float x = ceilf(top);
-                    l *= ex2(m - x);
-                    h -= x - m;
-                    m = x;
-                }
-                const float u = ceilf(fmaxf(t[0] - m + lv[0], t[1] - m + lv[1]));  // of the heaviest weight x scale
-                if (u > h) {
-                    z = ex2(h - u);
-                    h = u;
-                }
-                wf = weight_unit(h);
-                if (__any_sync(0xffffffffu, z != 1.f)) {
-                    if constexpr (LIMBS == 2) {
-#pragma unroll
-                        for (int e = 0; e < HD; ++e) acc[e] *= z;
-                    } else if (j > 0) {  // (the product before is the last so far: this tile's waits for its weights)
-                        ok = __all_sync(0xffffffffu, wait(&b.o_full[i], j - 1));
-                        if (!ok) break;
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < HD / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(tO + 32 * c, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * z);
-                            tmem_st32(tO + 32 * c, o);
-                        }
-                    }
-                }
-            }
+            if (exceeds() && !(ok = settle())) break;
             const float base = m == -INFINITY ? 0.f : m;
-            const bool deep = __any_sync(0xffffffffu, h < kDeep && h != -INFINITY);
+            const bool deep = is_deep();
             float2 sum = make_float2(0.f, 0.f);
             // Weights take the place of scores: one limb, 16 columns per 32 keys from column 16 c; two limbs, 8 of the
             // upper and 8 of the lower per 16 keys from column 16 u.
@@ -568,44 +614,29 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 tmem_st16(tS + 16 * u, w);
                 if (open) tmem_st16(tS + (GR == 16 ? 32 : 16) + 16 * u, w);  // the values' lower limbs: the same weights
             };
-            if (plain && !deep) {
-                auto weigh = [&](int u, const uint32_t *s) {
-                    const int c = u * GR / 32;
-                    const float f = ks[c] * row_scale, g = vs[c] * wf;
-                    // (the scale's own rounding is added back for f32 rows)
-                    const float f_lo = LIMBS == 2 ? fmaf(ks[c], row_scale, -f) : 0.f;
+            if (LIMBS == 2 && plain && !deep) {
+#pragma unroll 1
+                for (int c = 0; c < kTileBlocks; ++c) {
+                    uint32_t s[32];
+                    tmem_ld32(tS + 32 * c, s);
+                    const float f = ks[c] * row_scale, g = vs[c] * wf, f_lo = fmaf(ks[c], row_scale, -f);
                     const float2 f2 = make_float2(f, f), fl2 = make_float2(f_lo, f_lo), b2 = make_float2(-base, -base);
                     const float2 g2 = make_float2(g, g);
-                    uint32_t w[16];
+                    tmem_wait_ld();
+                    if (masked) hide(32 * c, 32, s);
 #pragma unroll
-                    for (int e = 0; e < GR; e += 2) {
-                        const float2 v = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-                        float2 d = ffma2_of(v, f2, b2);
-                        if (LIMBS == 2) d = ffma2_of(v, fl2, d);
-                        const float2 p = make_float2(ex2(d.x), ex2(d.y));
-                        sum = fadd2(sum, p);
-                        const float2 x = fmul2(p, g2);
-                        if (LIMBS == 2)
+                    for (int u = 0; u < 32; u += 16) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const float2 v = make_float2(__uint_as_float(s[u + e]), __uint_as_float(s[u + e + 1]));
+                            // (the scale's own rounding is added back)
+                            const float2 d = ffma2_of(v, fl2, ffma2_of(v, f2, b2)), p = make_float2(ex2(d.x), ex2(d.y));
+                            sum = fadd2(sum, p);
+                            const float2 x = fmul2(p, g2);
                             split_f16(x.x, x.y, w[e / 2], w[8 + e / 2]);
-                        else
-                            w[e / 2] = pack_f16(x.x, x.y);
-                    }
-                    tmem_st16(tS + 16 * u, w);
-                };
-                if constexpr (LIMBS == 1) {
-#pragma unroll
-                    for (int c = 0; c < kTileBlocks; ++c) weigh(c, held + 32 * c);
-                } else {
-#pragma unroll 1
-                    for (int u = 0; u < kKeys / 16; u += 2) {
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            uint32_t s[16];
-                            tmem_ld16(tS + 16 * (u + k), s);
-                            tmem_wait_ld();
-                            if (masked) hide(16 * (u + k), 16, s);
-                            weigh(u + k, s);
                         }
+                        tmem_st16(tS + 32 * c + u, w);
                     }
                 }
             } else {
@@ -653,6 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
             }
             l += sum.x + sum.y;
+            }
             if (LIMBS == 2 && j > 0) {  // the tile before's product, ere this one's takes its place
                 ok = __all_sync(0xffffffffu, wait(&b.o_full[i], j - 1));
                 if (!ok) break;
