@@ -8,6 +8,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -1270,6 +1271,25 @@ Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs,
     if (clusters > 1) s.bytes += sizeof(float) * (size_t)groups * clusters * kKvAttnRows * (head_dim + 4);
     return s;
 }
+// Split keys (mma.sync), or tiles of 256 rows on tcgen05: whichever should take less
+// time.  The terms are fits (us) of both kernels over 180 shapes of 1 and 8 sequences, 4 to 400 tokens each over 0 to
+// 8192 earlier ones, 14/2/64, 28/4/128 and 64/8/128 heads, f32 and bf16; the choice they make costs 2 % over the
+// better of the two on average.  At the two ends: 4 tokens over 8192 (28/4/128, f32) split 17 us, tiles 50 us; 400
+// tokens over 8192 split 414 us, tiles 133 us.
+bool kv8_prefers_prompt(int rows, int group, int kv_heads, int head_dim, int n_seqs, int max_q_len, int max_kv_len,
+                        bool f32, int sms, int &cluster) {
+    const double keys = std::max(1.0, (double)max_kv_len - max_q_len / 2.0), wide = head_dim / 128.0;
+    const double groups = kv_heads * std::max<double>(n_seqs, (double)rows * group / kKvAttnRows);
+    const double split = 9.0 + 0.0059 * groups * keys / 128.0 * wide + 0.00028 * keys;
+    const double ctas = kv_heads * std::max<double>(n_seqs, std::ceil((double)rows * group / 256.0));
+    // keys of a CTA over a cluster while that fits the SMs at once and leaves a CTA 512 keys
+    const int share = (int)std::max(1.0, std::min({std::floor(sms / ctas), std::floor(max_kv_len / 512.0), 8.0}));
+    const double waves = std::max(1.0, ctas * share / sms);
+    const double tiles = (waves > 1.0 ? keys : max_kv_len) / 64.0 / share;
+    if (1.0 + waves * (13.0 + (f32 ? 2.8 : 1.8) * (head_dim == 64 ? 0.9 : 1.0) * tiles) >= split) return false;
+    cluster = share;
+    return true;
+}
 }  // namespace
 
 int ql_kv8_append(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
@@ -1365,12 +1385,9 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         a.row_groups = sh.row_groups;
         a.arrivals = static_cast<unsigned *>(workspace_);
         a.part = reinterpret_cast<float *>(a.arrivals + kKvAttnCounters);
-        const bool prompt = kv8_prompt_takes(hd) && (int64_t)mq * (n_heads / a.c.kv_heads) >= 128;
-        if (prompt) {
-            const int64_t base = (int64_t)a.c.n_seqs * a.c.kv_heads * kv8_prompt_row_tiles(mq, n_heads / a.c.kv_heads);
-            const int64_t tiles = (max_kv_len + 127) / 128;
-            a.cluster = (int)std::max<int64_t>(1, std::min<int64_t>({ws->sms / base, tiles / 4, 8}));
-        }
+        const bool prompt = kv8_prompt_takes(hd) &&
+                            kv8_prefers_prompt(rows, n_heads / a.c.kv_heads, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len,
+                                               type == QL_F32, ws->sms, a.cluster);
         const cudaError_t e = prompt ? kv8_prompt_launch(a, mq, type == QL_BF16, g_stream)
                                      : kv8_attn_launch(a, type == QL_BF16, g_stream);
         ++t_launches;

@@ -944,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         if (k < 2 || !half) step(z, k, z == LIMBS - 1 && k == 0 ? first : 1u);
                 mma_commit(&b.o_full[i]);
             };
-            bool ok = nt == 0 || all_wait(&b.q_full, 0);
+            bool ok = all_wait(&b.q_full, 0);  // (a CTA without keys too: the rows' sums take Q's place after `done`)
             for (int j = 0; j < 2 && j < nt && ok; ++j) {
                 if (!(ok = all_wait(&b.k_full[j % ST], j / ST))) break;
                 tc_fence_after();
