@@ -1273,7 +1273,7 @@ Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs,
 }
 // Split keys (mma.sync), or tiles of 256 rows on tcgen05: whichever should take less
 // time.  The terms are fits (us) of both kernels over 180 shapes of 1 and 8 sequences, 4 to 400 tokens each over 0 to
-// 8192 earlier ones, 14/2/64, 28/4/128 and 64/8/128 heads, f32 and bf16; the choice they make costs 2 % over the
+// 8192 earlier ones, 14/2/64, 28/4/128 and 64/8/128 heads, f32 and bf16 (and 36 of 16/4/256, bf16); the choice they make costs 2 % over the
 // better of the two on average.  At the two ends: 4 tokens over 8192 (28/4/128, f32) split 17 us, tiles 50 us; 400
 // tokens over 8192 split 414 us, tiles 133 us.
 bool kv8_prefers_prompt(int rows, int group, int kv_heads, int head_dim, int n_seqs, int max_q_len, int max_kv_len,
@@ -1281,12 +1281,13 @@ bool kv8_prefers_prompt(int rows, int group, int kv_heads, int head_dim, int n_s
     const double keys = std::max(1.0, (double)max_kv_len - max_q_len / 2.0), wide = head_dim / 128.0;
     const double groups = kv_heads * std::max<double>(n_seqs, (double)rows * group / kKvAttnRows);
     const double split = 9.0 + 0.0059 * groups * keys / 128.0 * wide + 0.00028 * keys;
-    const double ctas = kv_heads * std::max<double>(n_seqs, std::ceil((double)rows * group / 256.0));
+    const double ctas = kv_heads * std::max<double>(n_seqs, std::ceil((double)rows * group / kv8_prompt_rows(head_dim, f32)));
     // keys of a CTA over a cluster while that fits the SMs at once and leaves a CTA 512 keys
     const int share = (int)std::max(1.0, std::min({std::floor(sms / ctas), std::floor(max_kv_len / 512.0), 8.0}));
     const double waves = std::max(1.0, ctas * share / sms);
     const double tiles = (waves > 1.0 ? keys : max_kv_len) / 64.0 / share;
-    if (1.0 + waves * (13.0 + (f32 ? 2.8 : 1.8) * (head_dim == 64 ? 0.9 : 1.0) * tiles) >= split) return false;
+    const double tile = f32 ? 2.8 : head_dim == 256 ? 2.9 : 1.8;  // us per 64 keys
+    if (1.0 + waves * (13.0 + tile * (head_dim == 64 ? 0.9 : 1.0) * tiles) >= split) return false;
     cluster = share;
     return true;
 }
@@ -1385,7 +1386,7 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         a.row_groups = sh.row_groups;
         a.arrivals = static_cast<unsigned *>(workspace_);
         a.part = reinterpret_cast<float *>(a.arrivals + kKvAttnCounters);
-        const bool prompt = kv8_prompt_takes(hd) &&
+        const bool prompt = kv8_prompt_rows(hd, type == QL_F32) > 0 &&
                             kv8_prefers_prompt(rows, n_heads / a.c.kv_heads, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len,
                                                type == QL_F32, ws->sms, a.cluster);
         const cudaError_t e = prompt ? kv8_prompt_launch(a, mq, type == QL_BF16, g_stream)

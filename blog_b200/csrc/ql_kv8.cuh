@@ -112,8 +112,7 @@ cudaError_t kv8_gather_launch(const Kv8View &c, const int *kv_len, const int *st
                               bool bf16, cudaStream_t s);
 cudaError_t kv8_attn_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s);
 // The tensor-core form for prompts (ql_kv8_prompt.cu).
-bool kv8_prompt_takes(int head_dim);
-unsigned kv8_prompt_row_tiles(int max_q_len, int group);  // CTAs over one (sequence, KV head)'s rows
+int kv8_prompt_rows(int head_dim, bool f32);  // rows per CTA, 0: not taken
 cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, int max_q_len, bool bf16, cudaStream_t s);
 
 // CTAs of the attention's split kernel that one SM holds (the host sizes the split count by it).

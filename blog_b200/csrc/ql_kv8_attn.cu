@@ -147,22 +147,33 @@ __device__ __forceinline__ float weight_undo(float x, float h) {
 // Below this h the weights' factor sv w leaves the range, and 2^(s - m) with it, where the weights themselves
 // do not (the row's heaviest keys have values of zero): they are computed from s - m - h then.
 constexpr float kDeep = -60.0f;
+// Beyond this |m| a score is rounded before m is taken off it: m is a rounded score then, and what one rounding
+// of the difference would keep is larger than the range of the weights.
+constexpr float kHuge = 1e6f;
 
 // Running state of one warp: row g8 = lane / 4 in the first two floats of a fragment (upper limbs) and the
 // last two (lower limbs).
-template <int HD>
+template <int HD, bool EXACT>
 struct Acc {
     float o[HD / 8][4];
     float m, l;  // maximum of the scores, total of 2^(s - m)
     float h, w;  // maximum of s - m + log2 of V's scale; 2^(kWBits - h): o holds sums of w 2^(s - m) sv code
 
-    // Block's scores s[n][2] (base-2 logarithms) of row g8, columns 2 q4, 2 q4 + 1 of n-tile n, to weights:
-    // returns the two limbs' A fragments.  vs: the scale of the block's values.
+    // Block's products s[n][2] of row g8, columns 2 q4, 2 q4 + 1 of n-tile n (-inf: a masked key), to weights:
+    // returns the two limbs' A fragments.  The score (a base-2 logarithm) is s k r, r >= 0 the row's scale and k the
+    // block's; less m it is one rounding, and f32 rows add back that of k r.  vs: the scale of the block's values.
+    static __device__ __forceinline__ float less_m(float s, float kr, float kr_lo, float m) {
+        const float d = fmaf(s, kr, -m);
+        return EXACT ? fmaf(s, kr_lo, d) : d;
+    }
     template <int NT>
-    __device__ __forceinline__ void weights(const float (&s)[NT][2], float vs, uint32_t (&hi)[NT], uint32_t (&lo)[NT]) {
+    __device__ __forceinline__ void weights(const float (&s)[NT][2], float k, float r_, float vs, uint32_t (&hi)[NT],
+                                            uint32_t (&lo)[NT]) {
+        const float kr = k * r_, kr_lo = EXACT ? fmaf(k, r_, -kr) : 0.f;
         float t = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n) t = fmaxf(t, fmaxf(s[n][0], s[n][1]));
+        if (t != -INFINITY) t *= kr;
         const float lv = log2f(vs);  // (0: -inf, which never passes h; NaN neither)
         if (__any_sync(0xffffffffu, t > m + kHeadroom || t - m + lv > h + kHeadroom)) {
             t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));  // the row's four lanes agree
@@ -189,25 +200,30 @@ struct Acc {
         }
         const float f = vs * w;
         const float base = m == -INFINITY ? 0.f : m;
-        // (x = -inf, a masked key: a NaN scale must not reach its weight)
-        if (__any_sync(0xffffffffu, h < kDeep)) {
+        // (a masked key: a NaN scale must not reach its weight)
+        if (__any_sync(0xffffffffu, h < kDeep || fabsf(base) > kHuge)) {
+            const bool huge = fabsf(base) > kHuge;
             const float lift = h == -INFINITY ? 0.f : h, g = h == -INFINITY ? f : vs * ex2(kWBits);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float x[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    l += ex2(s[n][e] - base);
-                    x[e] = s[n][e] == -INFINITY ? 0.f : ex2(fminf(s[n][e] - base - lift, 126.f)) * g;
+                    const bool seen = s[n][e] != -INFINITY;
+                    const float d = huge ? __fsub_rn(__fmul_rn(s[n][e], kr), base) : less_m(s[n][e], kr, kr_lo, base);
+                    l += seen ? ex2(d) : 0.f;
+                    x[e] = seen ? ex2(fminf(d - lift, 126.f)) * g : 0.f;
                 }
                 split_f16(x[0], x[1], hi[n], lo[n]);
             }
         } else {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float p0 = ex2(s[n][0] - base), p1 = ex2(s[n][1] - base);
+                const bool s0 = s[n][0] != -INFINITY, s1 = s[n][1] != -INFINITY;
+                const float p0 = s0 ? ex2(less_m(s[n][0], kr, kr_lo, base)) : 0.f;
+                const float p1 = s1 ? ex2(less_m(s[n][1], kr, kr_lo, base)) : 0.f;
                 l += p0 + p1;
-                split_f16(s[n][0] == -INFINITY ? 0.f : p0 * f, s[n][1] == -INFINITY ? 0.f : p1 * f, hi[n], lo[n]);
+                split_f16(s0 ? p0 * f : 0.f, s1 ? p1 * f : 0.f, hi[n], lo[n]);
             }
         }
     }
@@ -306,8 +322,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float inv;
-        const float f = limb_scale(amax, inv);
-        if (q4 == 0) s_q[g8] = a.scale_log2 * inv;
+        // (a negative softmax scale: its sign goes to q, so that products order like scores)
+        const float f = copysignf(limb_scale(amax, inv), a.scale_log2);
+        if (q4 == 0) s_q[g8] = fabsf(a.scale_log2) * inv;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             uint4 u;
@@ -319,7 +336,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     __syncthreads();
     const float row_scale = s_q[g8];
 
-    Acc<HD> acc;
+    constexpr bool EXACT = sizeof(T) == 4;
+    Acc<HD, EXACT> acc;
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
@@ -389,12 +407,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
             }
         }
         const int key0 = (w + i * W) * kKvBlock;
-        const float f = bk * row_scale;
         float s[4][2];
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) s[n][e] = (c[n][e] + c[n][e + 2]) * f;
+            for (int e = 0; e < 2; ++e) s[n][e] = c[n][e] + c[n][e + 2];
         if (key0 + kKvBlock > keys_all) {  // some row does not see the whole block
 #pragma unroll
             for (int n = 0; n < 4; ++n)
@@ -403,44 +420,67 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
                     if (key0 + 8 * n + 2 * q4 + e > pos) s[n][e] = -INFINITY;
         }
         uint32_t hi[4], lo[4];
-        acc.weights(s, bv, hi, lo);
+        acc.weights(s, bk, row_scale, bv, hi, lo);
 
-        // values: n-tile n's column g8 is dimension g8 * HD / 8 + n; the k-step's tokens are those of two
-        // score n-tiles, so the weights are already the A fragment
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            const uint32_t af[4] = {hi[2 * kk], lo[2 * kk], hi[2 * kk + 1], lo[2 * kk + 1]};
+        // values: n-tile n's column g8 is dimension g8 * HD / 8 + n; a k-step's tokens are those of two score
+        // n-tiles, so the weights are already the A fragment.  The tensor cores truncate when they accumulate: f32
+        // rows start each block's products from zero and add them here, rounded.
+        constexpr int WD = HD / 32;  // 4-byte words per lane and row
+        constexpr int WC = EXACT ? (WD % 2 == 0 ? 2 : 1) : WD % 4 == 0 ? 4 : WD % 2 == 0 ? 2 : 1;
+        auto rows4 = [&](int kk, int x, uint32_t (&r)[4][WC]) {  // rows t0, t0 + 1, t0 + 8, t0 + 9 of the k-step
             const int t0 = 16 * kk + 2 * q4;
-            constexpr int WD = HD / 32;  // 4-byte words per lane and row
-            constexpr int WC = WD % 4 == 0 ? 4 : WD % 2 == 0 ? 2 : 1;
 #pragma unroll
-            for (int x = 0; x < WD; x += WC) {
-                uint32_t r[4][WC];  // rows t0, t0 + 1, t0 + 8, t0 + 9
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int t = t0 + (y & 1) + (y >> 1) * 8, byte = g8 * (HD / 8) + 4 * x;
-                    const uint8_t *p = vt + t * HD + v_chunk<HD>(byte / 16, t) * 16 + byte % 16;
-                    if constexpr (WC == 4) {
-                        const uint4 z = *reinterpret_cast<const uint4 *>(p);
-                        r[y][0] = z.x, r[y][1] = z.y, r[y][2] = z.z, r[y][3] = z.w;
-                    } else if constexpr (WC == 2) {
-                        const uint2 z = *reinterpret_cast<const uint2 *>(p);
-                        r[y][0] = z.x, r[y][1] = z.y;
-                    } else {
-                        r[y][0] = *reinterpret_cast<const uint32_t *>(p);
-                    }
-                }
-#pragma unroll
-                for (int z = 0; z < WC; ++z) {
-                    const uint32_t a01 = __byte_perm(r[0][z], r[1][z], 0x5140), a23 = __byte_perm(r[0][z], r[1][z], 0x7362);
-                    const uint32_t b01 = __byte_perm(r[2][z], r[3][z], 0x5140), b23 = __byte_perm(r[2][z], r[3][z], 0x7362);
-                    const int n = 4 * (x + z);
-                    mma16816(acc.o[n], af, codes2(a01, 0x4140), codes2(b01, 0x4140));
-                    mma16816(acc.o[n + 1], af, codes2(a01, 0x4342), codes2(b01, 0x4342));
-                    mma16816(acc.o[n + 2], af, codes2(a23, 0x4140), codes2(b23, 0x4140));
-                    mma16816(acc.o[n + 3], af, codes2(a23, 0x4342), codes2(b23, 0x4342));
+            for (int y = 0; y < 4; ++y) {
+                const int t = t0 + (y & 1) + (y >> 1) * 8, byte = g8 * (HD / 8) + 4 * x;
+                const uint8_t *p = vt + t * HD + v_chunk<HD>(byte / 16, t) * 16 + byte % 16;
+                if constexpr (WC == 4) {
+                    const uint4 z = *reinterpret_cast<const uint4 *>(p);
+                    r[y][0] = z.x, r[y][1] = z.y, r[y][2] = z.z, r[y][3] = z.w;
+                } else if constexpr (WC == 2) {
+                    const uint2 z = *reinterpret_cast<const uint2 *>(p);
+                    r[y][0] = z.x, r[y][1] = z.y;
+                } else {
+                    r[y][0] = *reinterpret_cast<const uint32_t *>(p);
                 }
             }
+        };
+        auto product = [&](float (&d)[4][4], const uint32_t (&r)[4][WC], int z, int kk) {  // four n-tiles
+            const uint32_t af[4] = {hi[2 * kk], lo[2 * kk], hi[2 * kk + 1], lo[2 * kk + 1]};
+            const uint32_t a01 = __byte_perm(r[0][z], r[1][z], 0x5140), a23 = __byte_perm(r[0][z], r[1][z], 0x7362);
+            const uint32_t b01 = __byte_perm(r[2][z], r[3][z], 0x5140), b23 = __byte_perm(r[2][z], r[3][z], 0x7362);
+            mma16816(d[0], af, codes2(a01, 0x4140), codes2(b01, 0x4140));
+            mma16816(d[1], af, codes2(a01, 0x4342), codes2(b01, 0x4342));
+            mma16816(d[2], af, codes2(a23, 0x4140), codes2(b23, 0x4140));
+            mma16816(d[3], af, codes2(a23, 0x4342), codes2(b23, 0x4342));
+        };
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int x = 0; x < WD; x += WC) {
+                uint32_t r0[4][WC], r1[4][WC];
+                rows4(0, x, r0);
+                rows4(1, x, r1);
+#pragma unroll
+                for (int z = 0; z < WC; ++z) {
+                    float d[4][4] = {};
+                    product(d, r0, z, 0);
+                    product(d, r1, z, 1);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc.o[4 * (x + z) + n][e] += d[n][e];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int x = 0; x < WD; x += WC) {
+                    uint32_t r[4][WC];
+                    rows4(kk, x, r);
+#pragma unroll
+                    for (int z = 0; z < WC; ++z)
+                        product(*reinterpret_cast<float(*)[4][4]>(&acc.o[4 * (x + z)]), r, z, kk);
+                }
         }
     }
     cp_wait<0>();
@@ -514,13 +554,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int t = 2 * q4 + e;
-            // (q times 2^10 .. 2^11 and k too: the product of the two inverse scales may leave the range)
-            s[0][e] = (c[e] + c[e + 2]) * kinv * row_scale;
+            s[0][e] = c[e] + c[e + 2];
             if (bad >> t & 1) s[0][e] = __int_as_float(0x7FC00000);
             if (key0 + t > pos) s[0][e] = -INFINITY;
         }
         uint32_t hi[1], lo[1];
-        acc.weights(s, vinv, hi, lo);
+        acc.weights(s, kinv, row_scale, vinv, hi, lo);
         const uint32_t af[4] = {hi[0], lo[0], 0u, 0u};
 #pragma unroll
         for (int n = 0; n < HD / 8; ++n) {

@@ -1,7 +1,7 @@
 // Attention over the 8-bit KV cache for prompts: the same function as ql_kv8_attn.cu's, on the 5th-generation
 // tensor cores.
 //
-// A CTA takes 256 rows (query token, head of one KV head's group; the group's heads share every key) as two
+// A CTA takes 256 rows (head_dim 256: 128) (query token, head of one KV head's group; the group's heads share every key) as two
 // tiles of 128 and walks over the keys 64 at a time with a running maximum and total per row:
 //   S = Q K^T       tcgen05.mma, Q and K in shared memory, S (fp32) in TMEM
 //   P = 2^(S f - m) one thread per row; f: the block's scale of K x the row's scale; P (f16) over S in TMEM
@@ -40,7 +40,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kKeys = 64;    // keys per tile: 2 blocks
 constexpr int kTileBlocks = kKeys / kKvBlock;
-constexpr int kRows = 256;   // rows per CTA: two MMA tiles
+// Tiles of 128 rows per CTA: two, or one where O takes 256 columns of TMEM.
+constexpr int row_tiles(int hd) { return hd <= 128 ? 2 : 1; }
 constexpr float kHeadroom = 7.0f, kWBits = 8.0f;  // as in the split kernel
 
 // Registers per thread of the roles; 16 warps launch with 128 each.
@@ -50,11 +51,12 @@ static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs == 4 * 128, "the bloc
 template <int HD, int LIMBS>
 struct Layout {
     static constexpr int A = HD / 64;                        // 128-byte columns of a row
-    static constexpr int ST = 2;                             // K and V stages, and of their codes
+    static constexpr int MT = row_tiles(HD), ROWS = 128 * MT;
+    static constexpr int ST = HD <= 128 ? 2 : 1;             // K and V stages, and of their codes
     static constexpr int QT = A * 128 * 128;                 // one limb of one tile of Q
     static constexpr int KV = A * kKeys * 128;               // one stage of K or of V
     static constexpr int RAW = kKeys * HD;                   // a tile's codes of K or of V
-    static constexpr int q = 0, k = q + 2 * LIMBS * QT, v = k + ST * KV, raw = v + ST * KV, end = raw + 2 * ST * RAW;
+    static constexpr int q = 0, k = q + MT * LIMBS * QT, v = k + ST * KV, raw = v + ST * KV, end = raw + 2 * ST * RAW;
     static constexpr int bytes = 1024 + end + 512;
 };
 
@@ -182,6 +184,9 @@ __device__ __forceinline__ float weight_unit(float h) { return h == -INFINITY ? 
 // Below this h the weights' factor sv w leaves the range, and 2^(s - m) with it, where the weights themselves
 // do not (the row's heaviest keys have values of zero): they are computed from s - m - h then.
 constexpr float kDeep = -60.0f;
+// Beyond this |m| a score is rounded before m is taken off it: m is a rounded score then, and what one rounding
+// of the difference would keep is larger than the range of the weights.
+constexpr float kHuge = 1e6f;
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     uint32_t r;
@@ -284,10 +289,10 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ Kv8AttnArgs a) {
     constexpr int LIMBS = sizeof(T) == 4 ? 2 : 1;
     using L = Layout<HD, LIMBS>;
-    constexpr int A = L::A, ST = L::ST;
+    constexpr int A = L::A, ST = L::ST, MT = L::MT, ROWS = L::ROWS;
     constexpr uint32_t kS = 0, kO = 2 * kKeys, kTile = 256;  // TMEM columns of a tile of rows: S (then P) twice, O
     constexpr int kPitch = HD + 4;                       // floats of a row's sums in shared memory at the end
-    static_assert(kRows * kPitch * 4 <= L::end, "the sums take the operands' place");
+    static_assert(ROWS * kPitch * 4 <= L::end, "the sums take the operands' place");
     extern __shared__ uint8_t sm_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     Bars &b = *reinterpret_cast<Bars *>(sm + L::end);
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
     const int warp = uni(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int G = a.n_heads / a.c.kv_heads;
-    const int split = blockIdx.x % a.cluster, kh = blockIdx.x / a.cluster, seq = blockIdx.y, r_base = (gridDim.z - 1 - blockIdx.z) * kRows;  // longest first
+    const int split = blockIdx.x % a.cluster, kh = blockIdx.x / a.cluster, seq = blockIdx.y, r_base = (gridDim.z - 1 - blockIdx.z) * ROWS;  // longest first
     int row0, q_len;
     kv8_rows_of(a.r, seq, row0, q_len);
     const int n_rows = q_len * G;
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r1 = min(r_base + 128 * (i + 1), n_rows) - 1;  // the tile's last row
-        const int keys = r_base + 128 * i < n_rows ? max(0, min(kv_len, kv_len - q_len + r1 / G + 1)) : 0;
+        const int keys = i < MT && r_base + 128 * i < n_rows ? max(0, min(kv_len, kv_len - q_len + r1 / G + 1)) : 0;
         const int bl = min((keys + kKvBlock - 1) / kKvBlock, blocks);
         n_tiles[i] = (bl + kTileBlocks - 1) / kTileBlocks + (keys > open0 ? 1 : 0);
     }
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const int n_c = max(0, min(n_all, n_closed - j0));  // closed tiles among them
 
     if (threadIdx.x == 0) {
-        mbar_init(&b.q_full, kRows);
+        mbar_init(&b.q_full, ROWS);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b.k_full[i], 4), mbar_init(&b.k_empty[i], 1), mbar_init(&b.v_full[i], 4), mbar_init(&b.v_empty[i], 1);
             for (int k = 0; k < 2; ++k) {
@@ -364,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     if (warp < 8) {
         // ------------------------------------ a thread per row ------------------------------------
         reg_inc<kSoftmaxRegs>();
+        if (warp < 4 * MT) {
         const int i = warp >> 2, r = threadIdx.x & 127, gr = r_base + 128 * i + r;
         const bool live = gr < n_rows;
         const int tok = live ? gr / G : 0, head = kh * G + (live ? gr % G : 0);
@@ -400,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         uint32_t hi, lo;
                         split_f16(x[2 * e] * f, x[2 * e + 1] * f, hi, lo);
                         reinterpret_cast<uint32_t *>(p)[e] = hi;
-                        if (LIMBS == 2) reinterpret_cast<uint32_t *>(p + 2 * L::QT)[e] = lo;
+                        if (LIMBS == 2) reinterpret_cast<uint32_t *>(p + MT * L::QT)[e] = lo;
                     }
                 }
             }
@@ -530,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 return true;
             };
-            auto is_deep = [&]() { return __any_sync(0xffffffffu, h < kDeep && h != -INFINITY); };
+            auto is_deep = [&]() { return __any_sync(0xffffffffu, (h < kDeep || m > kHuge || m < -kHuge) && h != -INFINITY); };
             bool weighed = false;
             if constexpr (LIMBS == 1) {
                 if (plain && !is_deep()) {
@@ -649,10 +655,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     const float f = ks[c] * row_scale, f_lo = LIMBS == 2 ? fmaf(ks[c], row_scale, -f) : 0.f;
                     const float g = vs[c] * wf, nan = __int_as_float(0x7FC00000);
                     const int last = f < 0.f ? -1 : see - GR * u;
+                    const bool huge = fabsf(base) > kHuge;
 #pragma unroll
                     for (int e = 0; e < GR; ++e) {
-                        float d = fmaf(__uint_as_float(s[e]), f, -base);
-                        if (LIMBS == 2) d = fmaf(__uint_as_float(s[e]), f_lo, d);
+                        const float v = __uint_as_float(s[e]);
+                        float d = huge ? __fsub_rn(__fmul_rn(v, f), base) : fmaf(v, f, -base);
+                        if (LIMBS == 2 && !huge) d = fmaf(v, f_lo, d);
                         if (bad >> (GR * u + e & 31) & 1) d = nan;
                         s[e] = __float_as_uint(e <= last ? d : -INFINITY);
                     }
@@ -727,6 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         }
         row[HD] = m;
         row[HD + 1] = l;
+        }
         reg_dec<128>();  // as launched: the others take theirs back when all rows' warps have come here
     } else if (warp < 12) {
         // ------------------------------------ codes to f16 ------------------------------------
@@ -737,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         // swizzles differ, so that the writes do.
         constexpr int RPI = 8 / A;            // rows per warp access
         constexpr int U = kKeys / (4 * RPI);  // accesses per warp, operand and tile
-        const int pc = lane & 3, rb = (lane >> 2) & 1, at = (lane >> 3) % A ^ (A == 2 ? rb : 0), rl = rb + 2 * ((lane >> 3) / A);
+        const int pc = lane & 3, rb = (lane >> 2) & 1, at = (lane >> 3) % A ^ (A >= 2 ? rb : 0), rl = rb + 2 * ((lane >> 3) / A);
         auto row_of = [&](int u) { return (u * 4 + w) * RPI + rl; };
         bool ok = true;
         auto full = [&](uint64_t *bar) {
@@ -919,7 +928,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     for (int at = 0; at < A; ++at)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            const uint32_t qa = qb + ((2 * z * L::QT + at * (128 * 128) + 32 * k) >> 4);
+                            const uint32_t qa = qb + ((MT * z * L::QT + at * (128 * 128) + 32 * k) >> 4);
                             const uint32_t ka = kb + ((at * (kKeys * 128) + 32 * k) >> 4);
                             if (z == LIMBS - 1 && at == 0 && k == 0)
                                 mma_ss<false>(d, qa, ka, idesc(kKeys, false));
@@ -959,7 +968,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             for (int j = 0; j < nt && ok; ++j) {
                 if (!(ok = all_wait(&b.v_full[j % ST], j / ST))) break;
                 const bool more = j + 2 < nt;
-                if (more && !(ok = all_wait(&b.k_full[j % ST], (j + 2) / ST))) break;
+                bool k = false;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int n_i = i ? nt1 : nt0;
@@ -968,13 +977,20 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     tc_fence_after();
                     if (elect_one()) {
                         values(i, j);
-                        if (j + 2 < n_i) scores(i, j + 2);  // into the buffer of the weights just multiplied, after them
+                        if (MT == 1) mma_commit(&b.v_empty[j % ST]);  // (the next values may precede the next K)
                     }
+                    __syncwarp();
+                    if (j + 2 >= n_i) continue;
+                    // (only now: with one stage the converters need these values done before they come to K)
+                    if (!(ok = k || all_wait(&b.k_full[(j + 2) % ST], (j + 2) / ST))) continue;
+                    k = true;
+                    tc_fence_after();
+                    if (elect_one()) scores(i, j + 2);  // into the buffer of the weights just multiplied, after them
                     __syncwarp();
                 }
                 if (ok && elect_one()) {
-                    mma_commit(&b.v_empty[j % ST]);
-                    if (more) mma_commit(&b.k_empty[j % ST]);
+                    if (MT == 2) mma_commit(&b.v_empty[j % ST]);
+                    if (more) mma_commit(&b.k_empty[(j + 2) % ST]);
                 }
                 __syncwarp();
             }
@@ -1027,7 +1043,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     // This CTA's share of the rows from every CTA of the cluster, consecutive threads along a row.
     cg::cluster_group cl = cg::this_cluster();
     if (a.cluster > 1) cl.sync();
-    const int share = (kRows + a.cluster - 1) / a.cluster, r0 = split * share, r1 = min(min(r0 + share, kRows), n_rows - r_base);
+    const int share = (ROWS + a.cluster - 1) / a.cluster, r0 = split * share, r1 = min(min(r0 + share, ROWS), n_rows - r_base);
     if (*abort_flag == 0) {
         const float *sums = reinterpret_cast<const float *>(sm);
         for (int x = threadIdx.x; x < (r1 - r0) * (HD / 4); x += kThreads) {
@@ -1095,7 +1111,9 @@ cudaError_t launch_hd(const Kv8AttnArgs &a, int max_q_len, cudaStream_t s) {
         if (dev < 64) ready.fetch_or(1ull << dev);
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.c.kv_heads * a.cluster, a.c.n_seqs, kv8_prompt_row_tiles(max_q_len, a.n_heads / a.c.kv_heads));
+    constexpr int rows = 128 * row_tiles(HD);
+    cfg.gridDim = dim3(a.c.kv_heads * a.cluster, a.c.n_seqs,
+                       (unsigned)(((int64_t)max_q_len * (a.n_heads / a.c.kv_heads) + rows - 1) / rows));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -1108,12 +1126,13 @@ cudaError_t launch_hd(const Kv8AttnArgs &a, int max_q_len, cudaStream_t s) {
 }
 }  // namespace
 
-unsigned kv8_prompt_row_tiles(int max_q_len, int group) {
-    return (unsigned)(((int64_t)max_q_len * group + kRows - 1) / kRows);
+// (f32 rows of 256 would need 256 registers for their sums)
+int kv8_prompt_rows(int head_dim, bool f32) {
+    return head_dim == 64 || head_dim == 128 || (head_dim == 256 && !f32) ? 128 * row_tiles(head_dim) : 0;
 }
-bool kv8_prompt_takes(int head_dim) { return head_dim == 64 || head_dim == 128; }
 
 cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, int max_q_len, bool bf16, cudaStream_t s) {
+    if (a.c.head_dim == 256) return launch_hd<__nv_bfloat16, 256>(a, max_q_len, s);
     if (a.c.head_dim == 64)
         return bf16 ? launch_hd<__nv_bfloat16, 64>(a, max_q_len, s) : launch_hd<float, 64>(a, max_q_len, s);
     return bf16 ? launch_hd<__nv_bfloat16, 128>(a, max_q_len, s) : launch_hd<float, 128>(a, max_q_len, s);
