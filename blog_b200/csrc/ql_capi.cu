@@ -635,7 +635,7 @@ int ql_check_device(void) {
         if (h >= kErrKvPage)
             return fail(QL_EDEVICE, std::string(h == kErrKvPage       ? "a page outside the KV cache"
                                                 : h == kErrKvSlot     ? "a slot outside the KV cache's open rows"
-                                                : h == kErrKvLength   ? "more rows than the sequence has tokens"
+                                                : h == kErrKvLength   ? "more rows than the sequence has tokens, or than max_q_len"
                                                 : h == kErrKvPosition ? "a position past the rotation table"
                                                                       : "a mask row outside the masks") +
                                         " (device error code " + std::to_string(h) + ")");
@@ -1239,11 +1239,10 @@ int kv8_operand(const void *p, int64_t stride, int64_t width, int32_t type, cons
     return QL_OK;
 }
 
-// Launch shape of the attention over split keys, from the caller's bounds alone (so the workspace can be
-// sized before the call and a captured launch fits every length).
+// Launch shape of the attention over split keys, from the caller's bounds alone (a captured launch fits every
+// length).
 struct Kv8AttnShape {
     int row_groups, splits, cluster;
-    size_t bytes;
 };
 Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs, int max_q_len, int max_kv_len, int sms) {
     Kv8AttnShape s{};
@@ -1256,24 +1255,27 @@ Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs,
     // for every warp, and four where that leaves 8 CTAs (one sequence of 32768 tokens: 64 per group 16.2 us,
     // 104 per group 20 us; of 1024: 8 per group 7.1 us, 2 per group 9.5 us).  Where there are several waves
     // anyway, two or more per group even out unlike lengths, as long as a warp has 32 blocks (64 sequences of
-    // up to 8192 tokens, 8 KV heads: 2 per group 133 us, 1 per group 153 us).
+    // up to 8192 tokens, 8 KV heads: 2 per group 133 us, 1 per group 153 us); they stay one cluster, so that only
+    // one wave's groups have partials in the workspace.
     int64_t n = 1;
     if (groups > 0 && slots / groups >= 2)
         n = std::min({slots / groups, (blocks + kKvAttnWarps - 1) / kKvAttnWarps,
                       std::max<int64_t>(8, blocks / (4 * kKvAttnWarps))});
     else
-        n = blocks / (32 * kKvAttnWarps);
+        n = std::min<int64_t>(8, blocks / (32 * kKvAttnWarps));
     s.cluster = n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
-    int64_t clusters = std::min<int64_t>(n / s.cluster, kKvAttnMaxClusters);
-    if (groups * kKvAttnRows > kKvAttnCounters) clusters = 1;
-    s.splits = s.cluster * (int)std::max<int64_t>(clusters, 1);
-    s.bytes = sizeof(unsigned) * kKvAttnCounters;
-    if (clusters > 1) s.bytes += sizeof(float) * (size_t)groups * clusters * kKvAttnRows * (head_dim + 4);
+    s.splits = s.cluster * (int)std::clamp<int64_t>(n / s.cluster, 1, kKvAttnMaxClusters);
     return s;
 }
-// Split keys (mma.sync), or tiles of 256 rows on tcgen05: whichever should take less
-// time.  The terms are fits (us) of both kernels over 180 shapes of 1 and 8 sequences, 4 to 400 tokens each over 0 to
-// 8192 earlier ones, 14/2/64, 28/4/128 and 64/8/128 heads, f32 and bf16 (and 36 of 16/4/256, bf16); the choice they make costs 2 % over the
+// Counters (a group's 8 ranks), and the partials of several clusters per group: there are those only where all
+// groups' CTAs fit the SMs at once, so this holds for calls of any size.
+size_t kv8_attn_workspace_bytes(int head_dim, int sms) {
+    const size_t clusters = (size_t)sms * kv8_attn_ctas_per_sm(head_dim) / 8;
+    return sizeof(unsigned) * kKvAttnRows * clusters + sizeof(float) * clusters * kKvAttnRows * (head_dim + 4);
+}
+// Split keys (mma.sync), or tiles of 256 rows on tcgen05: whichever should take less time.  The terms are fits (us)
+// of both kernels over 180 shapes of 1 and 8 sequences, 4 to 400 tokens each over 0 to 8192 earlier ones, 14/2/64,
+// 28/4/128 and 64/8/128 heads, f32 and bf16 (and 36 of 16/4/256, bf16); the choice they make costs 2 % over the
 // better of the two on average.  At the two ends: 4 tokens over 8192 (28/4/128, f32) split 17 us, tiles 50 us; 400
 // tokens over 8192 split 414 us, tiles 133 us.
 bool kv8_prefers_prompt(int rows, int group, int kv_heads, int head_dim, int n_seqs, int max_q_len, int max_kv_len,
@@ -1342,7 +1344,7 @@ size_t ql_kv8_attend_workspace(int n_heads, int kv_heads, int head_dim, int n_se
     int st;
     Workspace *ws = workspace(&st);
     if (!ws) return 0;
-    return kv8_attn_shape(n_heads, kv_heads, head_dim, n_seqs, max_q_len, max_kv_len, ws->sms).bytes;
+    return kv8_attn_workspace_bytes(head_dim, ws->sms);
 }
 
 int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *gate,
@@ -1367,10 +1369,11 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         if (!ws) return st;
         const int mq = q_start ? max_q_len : 1;
         const Kv8AttnShape sh = kv8_attn_shape(n_heads, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len, ws->sms);
-        if ((int64_t)sh.row_groups * a.c.kv_heads > 65535)
+        if ((int64_t)sh.splits * sh.row_groups * a.c.kv_heads > INT32_MAX)
             return fail(QL_EINVAL, what + ": max_q_len x n_heads too large for one call");
-        if (!workspace_ || workspace_bytes < sh.bytes || reinterpret_cast<uintptr_t>(workspace_) % 16)
-            return fail(QL_EINVAL, what + ": the workspace must be 16-byte aligned and hold " + std::to_string(sh.bytes) +
+        const size_t need = kv8_attn_workspace_bytes(hd, ws->sms);
+        if (!workspace_ || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace_) % 16)
+            return fail(QL_EINVAL, what + ": the workspace must be 16-byte aligned and hold " + std::to_string(need) +
                                        " bytes (ql_kv8_attend_workspace)");
         a.c.err = ws->err;
         a.q = q, a.gate = gate, a.out = out;
@@ -1385,7 +1388,7 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         a.cluster = sh.cluster;
         a.row_groups = sh.row_groups;
         a.arrivals = static_cast<unsigned *>(workspace_);
-        a.part = reinterpret_cast<float *>(a.arrivals + kKvAttnCounters);
+        a.part = reinterpret_cast<float *>(a.arrivals + ws->sms * kv8_attn_ctas_per_sm(hd) / 8 * kKvAttnRows);
         const bool prompt = kv8_prompt_rows(hd, type == QL_F32) > 0 &&
                             kv8_prefers_prompt(rows, n_heads / a.c.kv_heads, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len,
                                                type == QL_F32, ws->sms, a.cluster);

@@ -120,6 +120,5 @@ int kv8_attn_ctas_per_sm(int head_dim);
 constexpr int kKvAttnWarps = 4;           // warps per CTA, each with key blocks of its own
 constexpr int kKvAttnRows = 8;            // rows per CTA: query tokens x heads of one KV head's group
 constexpr int kKvAttnMaxClusters = 16;
-constexpr int kKvAttnCounters = 16384;    // arrival counters at the head of the workspace
 
 }  // namespace ql

@@ -7,10 +7,12 @@
 // Mathematics.  A code is an integer of 8 bits and so exact in f16: with q = 2^-e (qh + ql) in two f16 limbs
 // (22 bits) the products q . c are exact and summed in fp32, and one multiplication by sk_b scale 2^-e gives
 // the score.  What meets V's codes is p sv_b, p = 2^(s - m): it is taken relative to the row's largest such
-// product so far (2^mh, a running maximum of s + log2 sv_b beside that of s) and split into two f16 limbs in
+// product so far (2^h, a running maximum of s - m + log2 sv_b beside that of s) and split into two f16 limbs in
 // the same way, so the result is as exact as fp32 sums make it, however unlike the blocks' scales are.  The
 // two limbs cost nothing: mma.m16n8k16 has 16 rows, the 8 rows' upper limbs and their lower
-// ones, and the two halves of an accumulator fragment are added.
+// ones, and the two halves of an accumulator fragment are added.  The MMA truncates as it accumulates (about
+// 3e-8 of the sum, always downwards, per step of 16), so f32 results are summed per block there and added up
+// with rounding outside.
 //
 // Layout.  A CTA has 4 warps and 8 rows (query token, head of one KV head's group); each warp walks over
 // key blocks of its own (32 tokens x head_dim codes of K and of V, two contiguous pieces of a page) through
@@ -22,7 +24,10 @@
 // a cluster's CTAs through distributed shared memory (each finishes its share of the rows), and clusters by
 // the last to arrive, always in split order: the result does not depend on which that is.
 //
-// Bound: HBM for the codes (2 head_dim bytes per token and KV head).
+// Bound: HBM for the codes (2 head_dim bytes per token and KV head) where the keys are many: 64 sequences of 4096 to
+// 8192 tokens, 64/8/128 heads, bf16, 681 MB in 133 us, 5.1 TB/s (0.79 of a copy's).  Below that the chain of one
+// CTA's loads, products and merges: one sequence of 28/4/128 heads, f32, 16.2 us at 32768 tokens (2.1 TB/s) and
+// 6.8 us at 200.  Tiles of 8 rows and not of 16: a group of 7 or 8 heads fills them, and a single token has no more.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -237,7 +242,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     constexpr int KS = HD / 16;                          // k-steps of q . k
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
     const int G = a.n_heads / a.c.kv_heads;
-    const int split = blockIdx.x, kh = blockIdx.y % a.c.kv_heads, rg = blockIdx.y / a.c.kv_heads, seq = blockIdx.z;
+    const int split = blockIdx.x % a.splits, at = blockIdx.x / a.splits;
+    const int kh = at % a.c.kv_heads, rg = at / a.c.kv_heads, seq = blockIdx.y;
     uint8_t *ring = sm + warp * (ST * 2 * BLK);
     uint4 *qf = reinterpret_cast<uint4 *>(sm + kKvAttnWarps * ST * 2 * BLK);  // [KS][32] A fragments of q
     __shared__ float s_m[kKvAttnWarps][kKvAttnRows], s_l[kKvAttnWarps][kKvAttnRows], s_q[kKvAttnRows];
@@ -247,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     int row0, q_len;
     kv8_rows_of(a.r, seq, row0, q_len);
     int kv_len = a.r.kv_len[seq];
+    if (threadIdx.x == 0 && rg == 0 && q_len * G > a.row_groups * kKvAttnRows) atomicExch(a.c.err, kErrKvLength);
     if (rg * kKvAttnRows >= q_len * G) return;  // (uniform: every split of the group leaves here)
     if ((kv_len + kKvBlock - 1) / kKvBlock > a.c.max_pages) {
         if (threadIdx.x == 0) atomicExch(a.c.err, kErrKvPage);
@@ -490,14 +497,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     for (int u = W - 1 - w; u < open_units; u += W) {
         const int slot = kv8_slot(a.c, seq);
         if (slot < 0) break;
-        const int64_t at = kv8_open_at(a.c, slot, open0 / kKvBlock, kh) + (int64_t)u * 8 * HD;
+        const int64_t rows_at = kv8_open_at(a.c, slot, open0 / kKvBlock, kh) + (int64_t)u * 8 * HD;
         const int key0 = open0 + 8 * u, there = min(8, kv_len - key0);
         unsigned bad = 0;
         float c[4] = {0.f, 0.f, 0.f, 0.f};
         float kinv;
         {
             float x[KS][4], amax = 0.f;
-            const float *k = a.c.k_open + at + g8 * HD;
+            const float *k = a.c.k_open + rows_at + g8 * HD;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const int d = s < 4 * G64 ? s / 4 * 64 + 16 * q4 + s % 4 * 4 : 64 * G64 + 8 * q4 + (s - 4 * G64) * 4;
@@ -527,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
             }
         }
         float v[2][HD / 8], vmax = 0.f, vinv;
-        const float *vp = a.c.v_open + at + g8 * (HD / 8);
+        const float *vp = a.c.v_open + rows_at + g8 * (HD / 8);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
             const int t = 2 * q4 + y;
@@ -750,7 +757,7 @@ cudaError_t launch_hd(const Kv8AttnArgs &a, cudaStream_t s) {
         if (dev < 64) ready.fetch_or(1ull << dev);
     }
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.splits, a.c.kv_heads * a.row_groups, a.c.n_seqs);
+    cfg.gridDim = dim3((unsigned)(a.splits * a.c.kv_heads * a.row_groups), a.c.n_seqs);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;

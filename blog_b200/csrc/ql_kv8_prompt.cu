@@ -1,8 +1,8 @@
 // Attention over the 8-bit KV cache for prompts: the same function as ql_kv8_attn.cu's, on the 5th-generation
 // tensor cores.
 //
-// A CTA takes 256 rows (head_dim 256: 128) (query token, head of one KV head's group; the group's heads share every key) as two
-// tiles of 128 and walks over the keys 64 at a time with a running maximum and total per row:
+// A CTA takes 256 rows (query token, head of one KV head's group; the group's heads share every key) as two tiles
+// of 128, or one tile at head_dim 256, and walks over the keys 64 at a time with a running maximum and total per row:
 //   S = Q K^T       tcgen05.mma, Q and K in shared memory, S (fp32) in TMEM
 //   P = 2^(S f - m) one thread per row; f: the block's scale of K x the row's scale; P (f16) over S in TMEM
 //   O += P V        tcgen05.mma, P from TMEM, V in shared memory, O (fp32) in TMEM
@@ -22,8 +22,12 @@
 // Where the tiles of rows alone would leave SMs idle, the keys are split over the CTAs of a cluster, and their
 // sums are joined through distributed shared memory, each CTA finishing its share of the rows.
 //
-// Bound: the tensor cores (4 head_dim flops per row and key, twice that for f32), with the exponentials (16 per
-// clock and SM) close behind.
+// Bound: the softmax threads (reading S, one exponential per row and key at 16 per clock and SM, weighing, writing
+// P), 3000 clocks per 64 keys of two tiles in bf16 and 5300 in f32, where the products take 1024 and 2048 of the
+// tensor cores: 28/4/128 heads, 8192 tokens in bf16 641 us (750 TFLOP/s of 4 head_dim flops per row and key, 0.45
+// of a library matrix product's), 2048 tokens in f32 95 us (317 TFLOP/s, twice that with both limbs).  Two row tiles,
+// so that one's products run under the other's softmax; tiles of 64 keys, so that S has two buffers (tiles of 128 with
+// one: 714 and 110 us).
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -305,6 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     int row0, q_len;
     kv8_rows_of(a.r, seq, row0, q_len);
     const int n_rows = q_len * G;
+    if (threadIdx.x == 0 && r_base == 0 && n_rows > (int)gridDim.z * ROWS) atomicExch(a.c.err, kErrKvLength);
     if (r_base >= n_rows) return;
     int kv_len = a.r.kv_len[seq];
     if ((kv_len + kKvBlock - 1) / kKvBlock > a.c.max_pages) {

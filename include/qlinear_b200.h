@@ -285,7 +285,7 @@ QL_API int ql_full_attention_attend_batch(const float *q, const float *gate, con
  * What a serving step does between the q/k/v projection and the attention's output, over a paged
  * cache of one byte per value.  A page holds QL_KV8_BLOCK tokens of every KV head; a full page has one
  * f32 scale per KV head for K and one for V:
- *   scale = max|x| / 127 over the page's tokens and the head's dimensions, byte = rint(x / scale) + 128
+ *   scale = max|x| / 127 over the page's tokens and the head's dimensions (>= 0), byte = rint(x / scale) + 128
  * (scale 0: bytes 128; a page that holds NaN or infinity has a NaN scale).  The tokens of a sequence's
  * last, unfinished page are exact: their rows stand in f32 in the "open" rows, from which the page is
  * quantised once, when it is full.  So the bytes do not depend on how a sequence was cut into calls, and
@@ -326,10 +326,11 @@ QL_API int ql_kv8_append(const ql_kv8_cache *cache, int32_t type, const void *q,
  *   out_h = softmax_j(scale q_h . k_j) . v_j [* sigmoid(gate_h)],  j = 0 .. the row's position,
  * query head h reads KV head h / (n_heads / kv_heads).  gate == NULL: none.  A row that sees no key gets
  * zeros; one that sees a NaN or infinity gets NaN.  f32: fp32 results (1e-6); bf16: operands and weights of
- * 16 bits, sums of 32.  max_q_len and max_kv_len bound the lengths on the device (a longer sequence is
- * read whole all the same; they size the launch).  The workspace, ql_kv8_attend_workspace bytes, 16-byte
- * aligned, is zeroed by the caller before its first use and left usable by every call; calls that may
- * overlap on the GPU need one each. */
+ * 16 bits, sums of 32.  max_q_len and max_kv_len bound the lengths on the device and size the launch (more
+ * cached tokens are read all the same; rows beyond max_q_len are not computed, and reported).  The workspace,
+ * ql_kv8_attend_workspace bytes (they depend on head_dim alone: one serves calls of any size), 16-byte aligned,
+ * is zeroed by the caller before its first use and left usable by every call; calls that may overlap on the GPU
+ * need one each. */
 QL_API size_t ql_kv8_attend_workspace(int n_heads, int kv_heads, int head_dim, int n_seqs, int rows, int max_q_len,
                                       int max_kv_len);
 QL_API int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *gate,

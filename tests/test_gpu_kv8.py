@@ -445,6 +445,47 @@ def test_attend_prompt_nan_and_infinity(hd, t):
                 assert rel_l2(got[starts[s] + i], want[i]) < TOL[t], (s, i)
 
 
+@pytest.mark.parametrize("nh,kvh,hd,n", [(64, 64, 32, 8200), (64, 8, 128, 8200), (16, 4, 256, 5000)])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_attend_many_rows(nh, kvh, hd, n, t):
+    """One call of more row groups than a grid dimension of 65535 holds, and prompts over thousands of keys (rows at
+    both ends and at tile edges): K and V by ql_kv8_append, read back by ql_kv8_gather for the restatement."""
+    import torch
+    c = Cache(1, n, kvh, hd, seed=51)
+    g = torch.Generator(device="cuda:0").manual_seed(52)
+    dt = torch.float32 if t == "f32" else torch.bfloat16
+    x = torch.randn(n, 2 * kvh * hd, generator=g, device="cuda:0").to(dt)
+    _append(c, t, x, 0, None, _i32([n]), _i32([0, n]), n)
+    k, v = (z[0].transpose(1, 0, 2).astype(np.float64) for z in _gather(c, "f32", None, n, _i32([n])))
+    q = (torch.randn(n, nh * hd, generator=g, device="cuda:0") * 1.5).to(dt)
+    got = _attend(c, t, q, nh, _i32([n]), _i32([0, n]), n, n)
+    qh = host(q.float())
+    for i in (0, 31, 32, 63, 64, 127, 1000, n // 2 + 1, n - 33, n - 2, n - 1):
+        want = U.attend(qh[i].reshape(nh, hd), k, v, i, hd ** -0.5)
+        assert rel_l2(got[i], want.ravel()) < TOL[t], i
+    Q.check_device()
+
+
+@pytest.mark.parametrize("n_seqs,kvh,max_kv", [(64, 8, 1 << 17), (2, 2, 1 << 20), (37, 6, 1 << 20)])
+def test_attend_under_wide_bounds(n_seqs, kvh, max_kv):
+    """Bounds far above the lengths, with few and many groups of rows: nothing is written behind the workspace, whose
+    size the bounds do not change, and it is left zeroed where the next call counts."""
+    import torch
+    nh, hd = 2 * kvh, 128
+    lens = [40 + 3 * s for s in range(n_seqs)]
+    c, stands = _filled(lens, max(lens), kvh, hd, seed=53)
+    q = torch.randn((n_seqs, nh * hd), device="cuda:0", generator=torch.Generator(device="cuda:0").manual_seed(54))
+    n = Q.kv8_attend_workspace(nh, kvh, hd, n_seqs, n_seqs, 1, max_kv)
+    assert n == Q.kv8_attend_workspace(nh, kvh, hd, 1, 1, 1, 64)
+    room = torch.cat([torch.zeros(n, dtype=torch.uint8), torch.full((1 << 24,), 91, dtype=torch.uint8)]).to("cuda:0")
+    for _ in range(2):
+        got = _attend(c, "f32", q, nh, _i32(lens), None, 1, max_kv, ws=room[:n])
+        for s in range(0, n_seqs, 7):
+            want = U.attend(host(q)[s].reshape(nh, hd), *stands[s], lens[s] - 1, hd ** -0.5)
+            assert rel_l2(got[s], want.ravel()) < TOL["f32"], s
+    assert bool((room[n:] == 91).all())
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_attend_long_cache(t):
     """20011 tokens of one sequence: many key splits, merged in a fixed order (twice the same bits)."""
@@ -613,6 +654,12 @@ def test_what_lies_outside_the_cache_is_reported():
     run(bad_slot, "slot")
     run(lambda c, kv, rope: (c, _i32([65, 41]), rope), "page")
     run(lambda c, kv, rope: (c, kv, rope[:40]), "position")
+    for lens in ([41, 3], [1800, 200]):  # rows beyond max_q_len, in both forms of the kernel
+        c, _ = _filled(lens, max(lens), kvh, hd, seed=36)
+        q = torch.randn((sum(lens), nh * hd), device="cuda:0")
+        _attend(c, "f32", q, nh, _i32(lens), _i32([0, lens[0], sum(lens)]), sum(lens) // 2, max(lens))
+        with pytest.raises(Q.QLError, match="more rows"):
+            Q.check_device()
     c, _ = _filled([10], 64, kvh, hd, seed=34)
     _append(c, "f32", torch.randn((20, 2 * kvh * hd), device="cuda:0"), 0, None, _i32([10]), _i32([0, 20]), 20)
     with pytest.raises(Q.QLError, match="more rows"):
