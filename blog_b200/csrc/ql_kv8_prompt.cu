@@ -24,8 +24,8 @@
 //
 // Bound: the softmax threads (reading S, one exponential per row and key at 16 per clock and SM, weighing, writing
 // P), 3000 clocks per 64 keys of two tiles in bf16 and 5300 in f32, where the products take 1024 and 2048 of the
-// tensor cores: 28/4/128 heads, 8192 tokens in bf16 641 us (750 TFLOP/s of 4 head_dim flops per row and key, 0.45
-// of a library matrix product's), 2048 tokens in f32 95 us (317 TFLOP/s, twice that with both limbs).  Two row tiles,
+// tensor cores: 28/4/128 heads, 8192 tokens in bf16 643 us (749 TFLOP/s of 4 head_dim flops per row and key, 0.45
+// of a library matrix product's), 2048 tokens in f32 100 us (301 TFLOP/s, twice that with both limbs).  Two row tiles,
 // so that one's products run under the other's softmax; tiles of 64 keys, so that S has two buffers (tiles of 128 with
 // one: 714 and 110 us).
 #include <cooperative_groups.h>
@@ -309,7 +309,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     int row0, q_len;
     kv8_rows_of(a.r, seq, row0, q_len);
     const int n_rows = q_len * G;
-    if (threadIdx.x == 0 && r_base == 0 && n_rows > (int)gridDim.z * ROWS) atomicExch(a.c.err, kErrKvLength);
     if (r_base >= n_rows) return;
     int kv_len = a.r.kv_len[seq];
     if ((kv_len + kKvBlock - 1) / kKvBlock > a.c.max_pages) {
@@ -1035,6 +1034,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             for (int op = 0; op < 2; ++op)
                 for (int j = max(0, issued[op] - ST); j < issued[op]; ++j)
                     mbar_wait(&b.raw_full[op][j % ST], (uint32_t)(j / ST) & 1u, nullptr, 0);
+        } else if (warp == 14 && lane == 0 && r_base == 0 && n_rows > (int)gridDim.z * ROWS) {
+            atomicExch(a.c.err, kErrKvLength);  // rows that no CTA takes (an idle warp's check: at the top it cost 7 %)
         }
         __syncwarp();
     }
