@@ -1243,6 +1243,7 @@ int kv8_operand(const void *p, int64_t stride, int64_t width, int32_t type, cons
 // length).
 struct Kv8AttnShape {
     int row_groups, splits, cluster;
+    bool longest_first;
 };
 Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs, int max_q_len, int max_kv_len, int sms) {
     Kv8AttnShape s{};
@@ -1254,14 +1255,17 @@ Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs,
     // chain of loads again: 8 x 8192 tokens of 4 KV heads, 8 per group 19 us, 16 per group 32 us), but a block
     // for every warp, and four where that leaves 8 CTAs (one sequence of 32768 tokens: 64 per group 16.2 us,
     // 104 per group 20 us; of 1024: 8 per group 7.1 us, 2 per group 9.5 us).  Where there are several waves
-    // anyway, two or more per group even out unlike lengths, as long as a warp has 32 blocks (64 sequences of
-    // up to 8192 tokens, 8 KV heads: 2 per group 133 us, 1 per group 153 us); they stay one cluster, so that only
-    // one wave's groups have partials in the workspace.
+    // anyway, unlike lengths leave SMs idle at the end.  Up to 16384 tokens the longest sequences start first, one
+    // CTA per group (64 sequences of up to 8192 tokens, 8 KV heads: 121 us, in the sequences' order 153 us; with 2 per
+    // group 136 us in either).  Else two or more per group even out, as long as a warp has 32 blocks (60 of up to 32000:
+    // 408 us, longest first 421 us; at 20000 it is 283 and 271 us, but a long sequence among short ones should not wait
+    // for one CTA).  They stay one cluster, so that only one wave's groups have partials in the workspace.
+    s.longest_first = n_seqs > 1 && n_seqs <= kKvAttnSorted && groups >= slots && blocks <= 512;
     int64_t n = 1;
     if (groups > 0 && slots / groups >= 2)
         n = std::min({slots / groups, (blocks + kKvAttnWarps - 1) / kKvAttnWarps,
                       std::max<int64_t>(8, blocks / (4 * kKvAttnWarps))});
-    else
+    else if (!s.longest_first)
         n = std::min<int64_t>(8, blocks / (32 * kKvAttnWarps));
     s.cluster = n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
     s.splits = s.cluster * (int)std::clamp<int64_t>(n / s.cluster, 1, kKvAttnMaxClusters);
@@ -1387,6 +1391,7 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         a.splits = sh.splits;
         a.cluster = sh.cluster;
         a.row_groups = sh.row_groups;
+        a.longest_first = sh.longest_first;
         a.arrivals = static_cast<unsigned *>(workspace_);
         a.part = reinterpret_cast<float *>(a.arrivals + ws->sms * kv8_attn_ctas_per_sm(hd) / 8 * kKvAttnRows);
         const bool prompt = kv8_prompt_rows(hd, type == QL_F32) > 0 &&

@@ -52,6 +52,7 @@ struct Kv8AttnArgs {
     bool vec;          // q and out: every row starts on 16 bytes
     int splits;        // CTAs over the keys of one (sequence, KV head, row group): clusters of `cluster`
     int cluster;       // 1, 2, 4 or 8 (prompts: 1 to 8, all of the splits)
+    bool longest_first;  // CTAs start by their sequences' lengths, at most kKvAttnSorted sequences
     int row_groups;    // groups of 8 (query token, head of the KV head's group) rows per sequence
     unsigned *arrivals;  // [n_seqs x kv_heads x row_groups][8] zero between calls (several clusters)
     float *part;         // [...][clusters][8][head_dim + 4]
@@ -120,5 +121,6 @@ int kv8_attn_ctas_per_sm(int head_dim);
 constexpr int kKvAttnWarps = 4;           // warps per CTA, each with key blocks of its own
 constexpr int kKvAttnRows = 8;            // rows per CTA: query tokens x heads of one KV head's group
 constexpr int kKvAttnMaxClusters = 16;
+constexpr int kKvAttnSorted = 32 * kKvAttnWarps;  // sequences that a CTA ranks, one per thread
 
 }  // namespace ql

@@ -25,13 +25,14 @@
 // the last to arrive, always in split order: the result does not depend on which that is.
 //
 // Bound: HBM for the codes (2 head_dim bytes per token and KV head) where the keys are many: 64 sequences of 4096 to
-// 8192 tokens, 64/8/128 heads, bf16, 681 MB in 136 us, 5.0 TB/s (0.77 of a copy's).  Below that the chain of one
-// CTA's loads, products and merges: one sequence of 28/4/128 heads, f32, 17.3 us at 32768 tokens (1.9 TB/s) and
-// 7.4 us at 200.  Tiles of 8 rows and not of 16: a group of 7 or 8 heads fills them, and a single token has no more.
+// 8192 tokens, 64/8/128 heads, bf16, 681 MB in 121 us, 5.6 TB/s (0.87 of a copy's).  Below that the chain of one
+// CTA's loads, products and merges: one sequence of 28/4/128 heads, f32, 17.6 us at 32768 tokens (1.9 TB/s) and
+// 7.6 us at 200.  Tiles of 8 rows and not of 16: a group of 7 or 8 heads fills them, and a single token has no more.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <climits>
 
 #include "ql_kv8.cuh"
 
@@ -243,7 +244,27 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, q4 = lane & 3;
     const int G = a.n_heads / a.c.kv_heads;
     const int split = blockIdx.x % a.splits, at = blockIdx.x / a.splits;
-    const int kh = at % a.c.kv_heads, rg = at / a.c.kv_heads, seq = blockIdx.y;
+    const int kh = at % a.c.kv_heads, rg = at / a.c.kv_heads;
+    int seq = blockIdx.y;
+    if (a.longest_first) {  // the sequence of this rank by length, a thread per sequence (equals: in their order)
+        __shared__ int4 s_len[kThreads / 4];
+        __shared__ int s_seq;
+        const int n = a.c.n_seqs, me = threadIdx.x, mine = me < n ? a.r.kv_len[me] : INT_MIN;
+        reinterpret_cast<int *>(s_len)[me] = mine;
+        __syncthreads();
+        int rank = 0;
+#pragma unroll 1
+        for (int j = 0; j < n; j += 4) {
+            const int4 x = s_len[j / 4];
+            rank += x.x > mine || (x.x == mine && j < me);
+            rank += x.y > mine || (x.y == mine && j + 1 < me);
+            rank += x.z > mine || (x.z == mine && j + 2 < me);
+            rank += x.w > mine || (x.w == mine && j + 3 < me);
+        }
+        if (me < n && rank == seq) s_seq = me;
+        __syncthreads();
+        seq = s_seq;
+    }
     uint8_t *ring = sm + warp * (ST * 2 * BLK);
     uint4 *qf = reinterpret_cast<uint4 *>(sm + kKvAttnWarps * ST * 2 * BLK);  // [KS][32] A fragments of q
     __shared__ float s_m[kKvAttnWarps][kKvAttnRows], s_l[kKvAttnWarps][kKvAttnRows], s_q[kKvAttnRows];

@@ -486,6 +486,33 @@ def test_attend_under_wide_bounds(n_seqs, kvh, max_kv):
     assert bool((room[n:] == 91).all())
 
 
+@pytest.mark.parametrize("n_seqs", [2, 127, 128, 129])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attend_waves_of_unlike_lengths(n_seqs, ragged):
+    """More CTAs than run at once, lengths in no order with many equal ones and idle sequences: every row is its own
+    sequence's, whichever starts first."""
+    import torch
+    kvh, hd, nh = 16, 64, 32
+    rng = np.random.default_rng(55)
+    lens = [int(x) for x in rng.choice([0, 1, 33, 64, 64, 150, 300], n_seqs)]
+    lens[-1] = 300
+    q_len = [min(n, int(x)) for n, x in zip(lens, rng.integers(0, 6, n_seqs))] if ragged else [1] * n_seqs
+    q_len[-1] = 5 if ragged else 1
+    starts = np.concatenate([[0], np.cumsum(q_len)])
+    c, stands = _filled(lens, 300, kvh, hd, seed=56)
+    q = torch.randn((int(starts[-1]), nh * hd), device="cuda:0", generator=torch.Generator(device="cuda:0").manual_seed(57))
+    got = _attend(c, "f32", q, nh, _i32(lens), _i32(starts) if ragged else None, 5 if ragged else 1, 300)
+    for s in range(n_seqs):
+        for i in range(q_len[s]):
+            row = got[starts[s] + i]
+            if lens[s] == 0:
+                assert not row.any(), s
+                continue
+            want = U.attend(host(q)[starts[s] + i].reshape(nh, hd), *stands[s], lens[s] - q_len[s] + i, hd ** -0.5)
+            assert rel_l2(row, want.ravel()) < TOL["f32"], (s, i)
+    Q.check_device()
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_attend_long_cache(t):
     """20011 tokens of one sequence: many key splits, merged in a fixed order (twice the same bits)."""
