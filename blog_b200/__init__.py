@@ -66,6 +66,7 @@ SIGNATURES = {
     "ql_kv8_append": (I, [P, I32, P, I64, P, I64, P, I64, P, I64, I, P, P, F, P, I, I, P, P, I, I]),
     "ql_kv8_attend_workspace": (SZ, [I, I, I, I, I, I, I]),
     "ql_kv8_attend": (I, [P, I32, P, I64, P, I64, P, I64, I, F, P, P, I, I, I, P, SZ]),
+    "ql_kv8_attend_form": (I, [P]),
     "ql_kv8_gather": (I, [P, I32, P, P, P, I, P]),
     "ql_logits_apply": (I, [P, I64, P, I64, I, I, P, P, P, SZ]),
     "ql_moe_swiglu_grouped": (I, [I32, P, P, SZ, SZ, SZ, SZ, P, I64, P, I, I, P, I, I, I, I]),
@@ -393,6 +394,15 @@ def kv8_attend(cache, t, q, q_stride, gate, gate_stride, out, out_stride, n_head
                max_q_len, max_kv_len, workspace, workspace_bytes):
     _call("ql_kv8_attend", C.byref(cache), t, q, q_stride, gate, gate_stride, out, out_stride, n_heads, scale, kv_len,
           q_start, rows, max_q_len, max_kv_len, workspace, workspace_bytes)
+
+
+KV8_FORM_SPLIT, KV8_FORM_TILES = 1, 2
+
+
+def kv8_attend_form():
+    """(form, CTAs that shared a row's keys) of this thread's last kv8_attend (see include/qlinear_b200.h)."""
+    ctas = C.c_int(0)
+    return int(lib().ql_kv8_attend_form(C.byref(ctas))), ctas.value
 
 
 def kv8_gather(cache, t, k_out, v_out, start, count, kv_len):

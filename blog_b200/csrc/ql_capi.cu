@@ -86,6 +86,7 @@ Workspace g_ws[kMaxDevices];
 cudaStream_t g_stream = nullptr;
 thread_local std::string t_err;
 thread_local int t_launches = 0;
+thread_local int t_kv8_form = 0, t_kv8_ctas = 0;  // of this thread's last ql_kv8_attend
 
 int fail(int code, const std::string &msg) {
     t_err = msg;
@@ -1357,6 +1358,7 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
     return guarded([&] {
         const std::string what = "ql_kv8_attend";
         t_launches = 0;
+        t_kv8_form = t_kv8_ctas = 0;
         Kv8AttnArgs a{};
         int st;
         if ((st = kv8_view(cache, type, a.c, what)) || (st = kv8_rows(a.c, kv_len, q_start, rows, max_q_len, a.r, what)))
@@ -1400,8 +1402,17 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         const cudaError_t e = prompt ? kv8_prompt_launch(a, mq, type == QL_BF16, g_stream)
                                      : kv8_attn_launch(a, type == QL_BF16, g_stream);
         ++t_launches;
+        if (e == cudaSuccess) {
+            t_kv8_form = prompt ? QL_KV8_FORM_TILES : QL_KV8_FORM_SPLIT;
+            t_kv8_ctas = prompt ? a.cluster : a.splits;
+        }
         return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
     });
+}
+
+int ql_kv8_attend_form(int *ctas) {
+    if (ctas) *ctas = t_kv8_ctas;
+    return t_kv8_form;
 }
 
 int ql_kv8_gather(const ql_kv8_cache *cache, int32_t type, void *k_out, void *v_out, const int32_t *start, int count,

@@ -337,6 +337,11 @@ QL_API int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q,
                          int64_t gate_stride, void *out, int64_t out_stride, int n_heads, float scale,
                          const int32_t *kv_len, const int32_t *q_start, int rows, int max_q_len, int max_kv_len,
                          void *workspace, size_t workspace_bytes);
+/* Which kernel this thread's last ql_kv8_attend launched: QL_KV8_FORM_SPLIT (rows of 8, split over the keys),
+ * QL_KV8_FORM_TILES (tiles of rows on tcgen05), 0 none.  ctas (nullable): the CTAs that shared the keys of a row. */
+#define QL_KV8_FORM_SPLIT 1
+#define QL_KV8_FORM_TILES 2
+QL_API int ql_kv8_attend_form(int *ctas);
 /* The cache's values back: k_out and v_out [n_seqs][count][kv_heads][head_dim] of `type` (either may be
  * NULL), positions start[s] .. start[s] + count - 1 of sequence s (start == NULL: from 0), zeros where the
  * sequence has none.  E.g. to move a sequence to the bf16 cache of ql_full_attention_attend. */

@@ -1,0 +1,216 @@
+"""ql_kv8_attend by the kernel that takes the call: each case is sized for the tiles on tcgen05 or for the split over the
+keys and asserts which of the two ran, so that a change of the rule between them cannot move a case to the other.
+
+Tolerances as in test_gpu_kv8.py; a score of size S carries an error of 2^-22 S into the exponent, so extreme scores
+add S 2^-21."""
+import numpy as np
+import pytest
+
+import blog_b200 as Q
+import kv8_util as U
+from gpu_util import dev, host, rel_l2
+from test_gpu_kv8 import TOL, Cache, _attend, _dev, _filled, _i32
+
+pytestmark = pytest.mark.gpu
+WIDTHS = [("f32", 64), ("f32", 128), ("bf16", 64), ("bf16", 128), ("bf16", 256)]  # that the tiles take
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _stream():
+    import torch
+    torch.cuda.init()
+    Q.init(0)
+    Q.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield
+    Q.check_device()
+
+
+def _tiles(ctas=None):
+    form, n = Q.kv8_attend_form()
+    assert form == Q.KV8_FORM_TILES
+    assert ctas is None or n == ctas, n
+
+
+def _starts(q_len):
+    return np.concatenate([[0], np.cumsum(q_len)])
+
+
+def _check_rows(got, q, stands, lens, q_len, nh, tol, scale=None, rows=None):
+    """Every row (or those for which rows(s, i) holds) against the restatement."""
+    st, hd = _starts(q_len), q.shape[1] // nh
+    for s in range(len(lens)):
+        r = slice(st[s], st[s + 1])
+        if q_len[s] == 0:
+            continue
+        want = U.attend_rows(q[r].reshape(-1, nh, hd), *stands[s], lens[s] - q_len[s],
+                             hd ** -0.5 if scale is None else scale).reshape(-1, nh * hd)
+        for i in range(q_len[s]):
+            if rows is None or rows(s, i):
+                assert rel_l2(got[r][i], want[i]) < tol, (s, i)
+
+
+@pytest.mark.parametrize("t,hd,nh,kvh,q_len,past,ctas", [
+    ("f32", 64, 28, 4, 300, 1030, 2), ("f32", 64, 14, 2, 513, 1030, 3), ("f32", 64, 14, 2, 300, 2100, 4),
+    ("f32", 64, 8, 1, 400, 2600, 5), ("f32", 64, 14, 2, 200, 3100, 6), ("f32", 64, 32, 2, 64, 3650, 7),
+    ("f32", 64, 28, 4, 64, 4200, 8), ("f32", 128, 14, 2, 200, 1500, 3), ("f32", 128, 32, 2, 64, 2100, 4),
+    ("f32", 128, 8, 1, 200, 2600, 5), ("f32", 128, 14, 2, 100, 3100, 6), ("f32", 128, 8, 1, 150, 3650, 7),
+    ("f32", 128, 16, 1, 64, 4200, 8), ("bf16", 64, 8, 1, 513, 1500, 3), ("bf16", 64, 14, 2, 150, 2600, 5),
+    ("bf16", 64, 28, 4, 64, 3100, 6), ("bf16", 64, 8, 1, 200, 3650, 7), ("bf16", 128, 8, 1, 400, 1030, 2),
+    ("bf16", 128, 32, 2, 64, 1500, 3), ("bf16", 128, 8, 1, 150, 2600, 5), ("bf16", 128, 16, 1, 64, 3100, 6),
+    ("bf16", 128, 8, 1, 100, 3650, 7), ("bf16", 128, 8, 1, 100, 4200, 8), ("bf16", 256, 8, 1, 300, 1030, 2),
+    ("bf16", 256, 14, 2, 100, 1500, 3), ("bf16", 256, 16, 1, 64, 2100, 4), ("bf16", 256, 14, 2, 64, 2600, 5),
+    ("bf16", 256, 8, 1, 100, 3100, 6), ("bf16", 256, 8, 1, 100, 3650, 7), ("bf16", 256, 8, 1, 64, 4200, 8)])
+def test_keys_over_clusters_of_every_size(t, hd, nh, kvh, q_len, past, ctas):
+    """A chunk over a long cache, its keys split over 2 to 8 CTAs (shares of 256 or 128 rows that do not divide), and a
+    short one beside it, most of whose CTAs have no tiles."""
+    q_lens, lens = [q_len, q_len // 3], [past + q_len, 17 + q_len // 3]
+    c, stands = _filled(lens, max(lens), kvh, hd, seed=61)
+    qd, q = _dev(np.random.default_rng(62).standard_normal((sum(q_lens), nh * hd)) * 1.5, t)
+    got = _attend(c, t, qd, nh, _i32(lens), _i32(_starts(q_lens)), q_len, max(lens))
+    _tiles(ctas)
+    _check_rows(got, q, stands, lens, q_lens, nh, TOL[t])
+    Q.check_device()
+
+
+@pytest.mark.parametrize("t,hd", WIDTHS)
+def test_tiles_where_the_heaviest_keys_have_no_value(t, hd):
+    """Keys 60 to 80 nats above all others with values of zero: what is left of the others is 1e-26 and less, and still
+    relatively right (weights below the range of a 2^(s - m))."""
+    nh, kvh, n = 64, 1, 700
+    c = Cache(1, n, kvh, hd, seed=65)
+    rng = np.random.default_rng(66)
+    k, v = rng.standard_normal((2, n, kvh, hd)) * 0.5
+    u = np.sign(rng.standard_normal(hd))
+    k[32:64] = 4 * u
+    v[32:64] = 0
+    stands = [z.transpose(1, 0, 2) for z in c.set(0, k, v)]
+    q = rng.standard_normal((n, nh, hd)) * 0.1 + (15 + 5 * rng.random((n, nh, 1))) * u / 4 / hd * hd ** 0.5
+    q *= 4
+    qd, q = _dev(q.reshape(n, -1), t)
+    q = q.reshape(n, nh, hd)
+    got = _attend(c, t, qd, nh, _i32([n]), _i32([0, n]), n, n).reshape(n, nh, hd)
+    _tiles(1)
+    want = U.attend_rows(q, *stands, 0, hd ** -0.5)
+    s = np.abs(np.einsum("ihd,kd->ihk", q[::50].astype(np.float64), stands[0][0])).max() * hd ** -0.5
+    assert 40 < s < 200
+    for i in range(n):
+        for h in (0, 31, 63):
+            if 32 <= i < 64:  # (these see the block's first tokens: nothing but what lies under them)
+                assert np.abs(want[i, h]).max() < 1e-10
+            assert rel_l2(got[i, h], want[i, h]) < TOL[t] + s * 2.0 ** -21, (i, h)
+    Q.check_device()
+
+
+@pytest.mark.parametrize("t,hd", WIDTHS)
+def test_tiles_nan_and_infinity(t, hd):
+    """What is not finite, in open rows or as a page's scale, reaches exactly the rows that see it; past the end, none."""
+    nh, kvh = 32, 2
+    lens, q_len = [847] * 4, [800] * 4
+    c, stands = _filled(lens, 864, kvh, hd, seed=67)
+    c.ko[int(c.slot[0]), 0, :, 10, 3] = float("nan")   # token 842
+    c.vo[int(c.slot[1]), 0, :, 10, 3] = float("-inf")  # token 842
+    c.vs[int(c.table[2, 3])] = float("nan")            # tokens 96 .. 127
+    c.ks[int(c.table[3, 20])] = float("nan")           # tokens 640 .. 671
+    c.ko[int(c.slot[3]), 0, :, 15:] = float("nan")     # past the end
+    c.vo[int(c.slot[3]), 0, :, 15:] = float("inf")
+    qd, q = _dev(np.random.default_rng(68).standard_normal((3200, nh * hd)), t)
+    got = _attend(c, t, qd, nh, _i32(lens), _i32(_starts(q_len)), 800, 847)
+    _tiles()
+    first_bad = [842, 842, 96, 640]
+    _check_rows(got, q, stands, lens, q_len, nh, TOL[t], rows=lambda s, i: 47 + i < first_bad[s])
+    for s in range(4):
+        assert np.isnan(got[800 * s + first_bad[s] - 47:800 * s + 800]).all(), s
+    Q.check_device()
+
+
+@pytest.mark.parametrize("t,hd", WIDTHS)
+def test_tiles_report_what_lies_outside_the_cache(t, hd):
+    """A page, a slot, a length out of range and rows beyond max_q_len: reported, the other sequences' rows are right."""
+    nh, kvh = 32, 2
+    lens, q_len = [607, 607, 602, 607], [400, 450, 400, 400]
+    rng = np.random.default_rng(69)
+    qd, q = _dev(rng.standard_normal((sum(q_len), nh * hd)), t)
+
+    def run(change, expect, max_q=450):
+        c, stands = _filled(lens, 608, kvh, hd, seed=70)
+        kv = _i32(lens)
+        change(c, kv)
+        got = _attend(c, t, qd, nh, kv, _i32(_starts(q_len)), max_q, 607)
+        _tiles()
+        with pytest.raises(Q.QLError) as e:
+            Q.check_device()
+        assert e.value.status == Q.QL_EDEVICE and expect in str(e.value)
+        _check_rows(got, q, stands, lens, q_len, nh, TOL[t], rows=lambda s, i: s != 1 and i % 7 == 0)
+
+    run(lambda c, kv: c.td.__setitem__((1, 5), c.pages), "page")
+    run(lambda c, kv: c.td.__setitem__((1, 5), -1), "page")
+    run(lambda c, kv: c.sd.__setitem__(1, -1), "slot")
+    run(lambda c, kv: kv.__setitem__(1, 609), "page")
+    run(lambda c, kv: None, "more rows", max_q=413)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("tiles", [False, True])
+def test_lengths_above_the_bound_are_read(t, tiles):
+    """max_kv_len sizes the launch; longer sequences are read to their ends all the same."""
+    nh, kvh, hd = 64, 8, 128
+    q_len, lens = ([256, 100], [700, 1300]) if tiles else ([1, 3], [700, 2000])
+    c, stands = _filled(lens, max(lens), kvh, hd, seed=71)
+    qd, q = _dev(np.random.default_rng(72).standard_normal((sum(q_len), nh * hd)) * 1.5, t)
+    for bound in (256, 0):
+        got = _attend(c, t, qd, nh, _i32(lens), _i32(_starts(q_len)), max(q_len), bound)
+        if bound:
+            assert Q.kv8_attend_form()[0] == (Q.KV8_FORM_TILES if tiles else Q.KV8_FORM_SPLIT)
+        _check_rows(got, q, stands, lens, q_len, nh, TOL[t])
+    Q.check_device()
+
+
+def test_overlapping_calls_with_a_workspace_each():
+    """Two streams, each with its workspace, over and over: the bits of the calls alone."""
+    import torch
+    nh, kvh, hd, n = 14, 2, 128, 12000
+    c, stands = _filled([n], n, kvh, hd, seed=73)
+    rng = np.random.default_rng(74)
+    q = [dev(rng.standard_normal((1, nh * hd)).astype(np.float32)) for _ in range(2)]
+    kv = _i32([n])
+    size = Q.kv8_attend_workspace(nh, kvh, hd, 1, 1, 1, n)
+    ws = [torch.zeros(size, dtype=torch.uint8, device="cuda:0") for _ in range(2)]
+    alone = [_attend(c, "f32", x, nh, kv, None, 1, n, ws=ws[0]) for x in q]
+    form, ctas = Q.kv8_attend_form()
+    assert form == Q.KV8_FORM_SPLIT and ctas > 8  # (several clusters: partials and counters in the workspace)
+    outs = torch.full((2, 40, nh * hd), float("nan"), device="cuda:0")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    try:
+        for i in range(40):
+            for j, s in enumerate(streams):
+                Q.set_stream(s.cuda_stream)
+                Q.kv8_attend(c.view, Q.F32, q[j].data_ptr(), nh * hd, None, 0, outs[j, i].data_ptr(), nh * hd, nh, hd ** -0.5,
+                             kv.data_ptr(), None, 1, 1, n, ws[j].data_ptr(), size)
+        torch.cuda.synchronize()
+    finally:
+        Q.set_stream(torch.cuda.current_stream().cuda_stream)
+    got = host(outs)
+    for j in range(2):
+        assert rel_l2(alone[j][0], U.attend(host(q[j]).reshape(nh, hd), *stands[0], n - 1, hd ** -0.5).ravel()) < TOL["f32"]
+        assert (got[j] == alone[j][0]).all()
+
+
+@pytest.mark.parametrize("nh,kvh,hd,n_seqs", [(16, 2, 64, 1), (16, 2, 128, 1)])
+def test_tiles_one_heavy_key_over_many_light_ones(nh, kvh, hd, n_seqs):
+    """One key 23.2 nats above 32799 others whose values all point the other way: each weighs 2^-33 of it, their sum
+    3e-6.  Sums are fp32 and go tile by tile of 64 keys: one rounding of 2^-24 of the sum for each tile at most, in the
+    sums and in the total, beside a weight's own 2^-32 of the heaviest."""
+    n, rows = 32800, 1280
+    c = Cache(1, n, kvh, hd, seed=75)
+    k, v = np.zeros((2, n, kvh, hd))
+    u = np.sign(np.random.default_rng(76).standard_normal(hd))
+    k[0], v[0], v[1:] = 4 * u, u, -u
+    stands = [z.transpose(1, 0, 2) for z in c.set(0, k, v)]
+    q = np.tile(23.2 / 4 * hd ** -0.5 * u, (rows, nh)).astype(np.float32)
+    got = _attend(c, "f32", dev(q), nh, _i32([n]), _i32([0, rows]), rows, n)
+    _tiles(1)
+    for i in (0, 700, rows - 1):
+        want = U.attend(q[i].reshape(nh, hd), *stands, n - rows + i, hd ** -0.5)
+        assert rel_l2(got[i], want.ravel()) < 2e-6 + n / 64 * 2.0 ** -23 + n * 2.0 ** -32, i
+    Q.check_device()
