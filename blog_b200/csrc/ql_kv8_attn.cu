@@ -210,6 +210,8 @@ struct Acc {
         if (__any_sync(0xffffffffu, h < kDeep || fabsf(base) > kHuge)) {
             const bool huge = fabsf(base) > kHuge;
             const float lift = h == -INFINITY ? 0.f : h, g = h == -INFINITY ? f : vs * ex2(kWBits);
+            // (huge scores: h says nothing of the values' scale any more, so their product is kept in f16 by itself; NaN stays)
+            const float most = fminf(126.f, kHeadroom + 0.9f - lv);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float x[2];
@@ -218,7 +220,7 @@ struct Acc {
                     const bool seen = s[n][e] != -INFINITY;
                     const float d = huge ? __fsub_rn(__fmul_rn(s[n][e], kr), base) : less_m(s[n][e], kr, kr_lo, base);
                     l += seen ? ex2(d) : 0.f;
-                    x[e] = seen ? ex2(fminf(d - lift, 126.f)) * g : 0.f;
+                    x[e] = seen ? ex2(fminf(d - lift, most)) * g : 0.f;
                 }
                 split_f16(x[0], x[1], hi[n], lo[n]);
             }

@@ -678,11 +678,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     } else {
                         const bool lift = h != -INFINITY;
                         const float gl = lift ? vs[c] * ex2(kWBits) : g, up = lift ? h : 0.f;
+                        // (huge scores: h says nothing of the values' scale any more, so their product is kept in f16 by
+                        // itself; NaN stays)
+                        const float most = fminf(126.f, kHeadroom + 0.9f - lv[c]);
 #pragma unroll
                         for (int e = 0; e < GR; ++e) {
                             const float d = __uint_as_float(s[e]);
                             sum.x += ex2(d);
-                            s[e] = __float_as_uint(e <= last ? ex2(fminf(d - up, 126.f)) * gl : 0.f);
+                            s[e] = __float_as_uint(e <= last ? ex2(fminf(d - up, most)) * gl : 0.f);
                         }
                     }
 #pragma unroll

@@ -73,6 +73,68 @@ def test_keys_over_clusters_of_every_size(t, hd, nh, kvh, q_len, past, ctas):
 
 
 @pytest.mark.parametrize("t,hd", WIDTHS)
+def test_tiles_scores_of_every_size_and_signs(t, hd):
+    """Scores of +-1e3 and 1e30, equal scores, tiny and huge queries, values whose scales lie 1e12 apart, blocks of zeros
+    (K, V), positive and negative softmax scales."""
+    nh, kvh, n = 64, 1, 700
+    c = Cache(1, n, kvh, hd, seed=63)
+    rng = np.random.default_rng(64)
+    k, v = rng.standard_normal((2, n, kvh, hd))
+    v[:64] *= 1e-6
+    v[64:96] *= 1e6
+    v[96:128] = 0
+    k[128:160] = 0
+    stands = [z.transpose(1, 0, 2) for z in c.set(0, k, v)]
+    q = rng.standard_normal((n, nh, hd))
+    q[:, 1] *= 100
+    q[:, 2] = 0
+    q[:, 3] *= 1e-30
+    q[:, 4] = -q[:, 1]
+    q[:, 5] *= 1e30
+    qd, q = _dev(q.reshape(n, -1), t)
+    q = q.reshape(n, nh, hd)
+    for scale in (hd ** -0.5, -hd ** -0.5):
+        got = _attend(c, t, qd, nh, _i32([n]), _i32([0, n]), n, n, scale=scale).reshape(n, nh, hd)
+        _tiles(1)
+        want = U.attend_rows(q, *stands, 0, scale)
+        for h in (0, 1, 2, 3, 4, 5, 40, 63):
+            s = np.abs(stands[0][0] @ q[:, h].T.astype(np.float64)).max() * hd ** -0.5
+            tol = TOL[t] + (0 if s > 1e6 else s * 2.0 ** -21)
+            for i in range(n):
+                assert rel_l2(got[i, h], want[i, h]) < tol, (h, i)
+    Q.check_device()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [64, 96, 256])
+def test_split_scores_of_every_size_where_the_heaviest_keys_have_no_value(hd, t):
+    """The same in few rows, eight blocks to a warp: blocks of zero and of large values among keys whose
+    scores lie 0 to 1e30 apart."""
+    nh, kvh, n = 8, 1, 1000
+    c = Cache(1, n, kvh, hd, seed=77)
+    rng = np.random.default_rng(78)
+    k, v = rng.standard_normal((2, n, kvh, hd))
+    v[640:] *= 1e6
+    v[320:640] = 0
+    stands = [z.transpose(1, 0, 2) for z in c.set(0, k, v)]
+    q = rng.standard_normal((16, nh, hd)) * 10.0 ** np.asarray([0, 1, 2, 4, 7, 12, 20, 30])[None, :, None]
+    qd, q = _dev(q.reshape(16, -1), t)
+    q = q.reshape(16, nh, hd)
+    got = _attend(c, t, qd, nh, _i32([n]), _i32([0, 16]), 16, 32).reshape(16, nh, hd)  # (a short bound: one CTA)
+    assert Q.kv8_attend_form() == (Q.KV8_FORM_SPLIT, 1)
+    want = U.attend_rows(q, *stands, n - 16, hd ** -0.5)
+    for h in range(nh):
+        s = np.abs(stands[0][0] @ q[:, h].T.astype(np.float64)).max() * hd ** -0.5
+        for i in range(16):
+            if s < 1e6:
+                assert rel_l2(got[i, h], want[i, h]) < TOL[t] + s * 2.0 ** -21, (h, i)
+            else:  # (one key has it all: its value, or zeros)
+                top = np.argmax(stands[0][0][:n - 15 + i] @ q[i, h].astype(np.float64))
+                assert rel_l2(got[i, h], stands[1][0][top]) < TOL[t], (h, i)
+    Q.check_device()
+
+
+@pytest.mark.parametrize("t,hd", WIDTHS)
 def test_tiles_where_the_heaviest_keys_have_no_value(t, hd):
     """Keys 60 to 80 nats above all others with values of zero: what is left of the others is 1e-26 and less, and still
     relatively right (weights below the range of a 2^(s - m))."""
