@@ -5,7 +5,7 @@
 //   n = x / sqrt(mean(x^2) + eps) * gamma,   (a, b) -> (a cos - b sin, b cos + a sin)
 // for the pairs (i, i + rotary_dim / 2) of the first rotary_dim elements, and k and v go to the cache:
 //   a block of 32 tokens that is full is stored as scale = max|x| / 127 over its 32 x head_dim values of
-//   one head and code = rint(x / scale) + 128 in a byte;
+//   one head and code = rint(x / scale) + 128 in a byte (x / scale within +-127);
 //   the rows of the last block and of the one before it are kept in f32 ("open" rows), so that a block
 //   is quantised once, from exact values, when its last token arrives.
 // The codes therefore do not depend on how a sequence was cut into calls, no code is ever re-scaled, and
@@ -211,7 +211,7 @@ __device__ void append_block(const Kv8AppendArgs &a, bool is_v, int seq, int slo
     // rint(x / scale): the quotient from the block's one reciprocal and a residual step, which rounds it
     // correctly (P. Markstein, 1990; ties of bf16 values are common and go by the last bit), then 1.5 x 2^23
     // added, which rounds to an integer, half to even, with the code in the low byte.  Scales near the ends of
-    // the range are divided by.
+    // the range are divided by, and the quotient kept within 127: a subnormal scale is too coarse to keep it there.
     const float inv = 1.0f / scale;
     const bool divide = !(scale > 1e-30f && scale < 1e30f);
 #pragma unroll
@@ -223,7 +223,8 @@ __device__ void append_block(const Kv8AppendArgs &a, bool is_v, int seq, int slo
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float r = x[u][i] * inv;
-            r = divide ? (scale > 0.f ? x[u][i] / scale : 0.f) : fmaf(fmaf(-r, scale, x[u][i]), inv, r);
+            r = divide ? (scale > 0.f ? fminf(fmaxf(x[u][i] / scale, -127.f), 127.f) : 0.f)
+                       : fmaf(fmaf(-r, scale, x[u][i]), inv, r);
             c[i] = __float_as_uint(r + 12582912.0f) ^ 0x80u;
         }
 #pragma unroll

@@ -286,7 +286,8 @@ QL_API int ql_full_attention_attend_batch(const float *q, const float *gate, con
  * cache of one byte per value.  A page holds QL_KV8_BLOCK tokens of every KV head; a full page has one
  * f32 scale per KV head for K and one for V:
  *   scale = max|x| / 127 over the page's tokens and the head's dimensions (>= 0), byte = rint(x / scale) + 128
- * (scale 0: bytes 128; a page that holds NaN or infinity has a NaN scale).  The tokens of a sequence's
+ * (x / scale kept within +-127, which a subnormal scale may pass; scale 0: bytes 128; a page that holds NaN or
+ * infinity has a NaN scale).  The tokens of a sequence's
  * last, unfinished page are exact: their rows stand in f32 in the "open" rows, from which the page is
  * quantised once, when it is full.  So the bytes do not depend on how a sequence was cut into calls, and
  * since the open rows hold the last two pages, kv_len may go back by up to QL_KV8_BLOCK tokens (rejected

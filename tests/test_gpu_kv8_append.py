@@ -1,0 +1,45 @@
+"""ql_kv8_append where its blocks, lengths or arguments are out of the ordinary."""
+import numpy as np
+import pytest
+
+import blog_b200 as Q
+from gpu_util import dev, host
+from test_gpu_kv8 import Cache, _append, _i32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _stream():
+    import torch
+    torch.cuda.init()
+    Q.init(0)
+    Q.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield
+    Q.check_device()
+
+
+def test_codes_of_the_smallest_blocks():
+    """Largest magnitudes of 1 to 2^20 units of 2^-149: a subnormal scale is rounded so coarsely that x / scale may pass
+    127, and the code stays at +-127."""
+    kvh, hd = 2, 64
+    most = [1, 2, 63, 64, 100, 127, 190, 191, 254, 318, 1330, 5000, 1 << 20]
+    n = 32 * len(most)
+    rng = np.random.default_rng(81)
+    x = np.concatenate([rng.integers(-m, m + 1, (32, 2, kvh, hd)) for m in most]).astype(np.float64)
+    for b, m in enumerate(most):
+        x[32 * b, :, :, 0], x[32 * b, :, :, 1] = m, -m
+    x = (x * 2.0 ** -149).astype(np.float32)
+    c = Cache(1, n, kvh, hd, seed=82)
+    _append(c, "f32", dev(x.reshape(n, -1)), 0, None, _i32([n]), _i32([0, n]), n)
+    for j, (codes, scales) in enumerate(((c.kc, c.ks), (c.vc, c.vs))):
+        codes, scales = host(codes), host(scales)
+        for b in range(len(most)):
+            for h in range(kvh):
+                z = x[32 * b:32 * b + 32, j, h]
+                scale = np.abs(z).max() / np.float32(127)
+                want = np.rint(z / scale).clip(-127, 127) + 128 if scale else np.full(z.shape, 128)
+                page = c.table[0, b]
+                assert scales[page, h] == scale
+                assert np.array_equal(codes[page, h], want), most[b]
+    Q.check_device()
