@@ -1273,10 +1273,12 @@ Kv8AttnShape kv8_attn_shape(int n_heads, int kv_heads, int head_dim, int n_seqs,
     return s;
 }
 // Counters (a group's 8 ranks), and the partials of several clusters per group: there are those only where all
-// groups' CTAs fit the SMs at once, so this holds for calls of any size.
+// groups' CTAs fit the SMs at once, so this holds for calls of any size.  The counters have the same place for every
+// head_dim: what one's calls leave in the partials never lies where another's calls count.
+size_t kv8_attn_counter_bytes(int sms) { return sizeof(unsigned) * kKvAttnRows * ((size_t)sms * kKvAttnMaxCtasPerSm / 8); }
 size_t kv8_attn_workspace_bytes(int head_dim, int sms) {
     const size_t clusters = (size_t)sms * kv8_attn_ctas_per_sm(head_dim) / 8;
-    return sizeof(unsigned) * kKvAttnRows * clusters + sizeof(float) * clusters * kKvAttnRows * (head_dim + 4);
+    return kv8_attn_counter_bytes(sms) + sizeof(float) * clusters * kKvAttnRows * (head_dim + 4);
 }
 // Split keys (mma.sync), or tiles of 256 rows on tcgen05: whichever should take less time.  The terms are fits (us)
 // of both kernels over 180 shapes of 1 and 8 sequences, 4 to 400 tokens each over 0 to 8192 earlier ones, 14/2/64,
@@ -1395,7 +1397,7 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         a.row_groups = sh.row_groups;
         a.longest_first = sh.longest_first;
         a.arrivals = static_cast<unsigned *>(workspace_);
-        a.part = reinterpret_cast<float *>(a.arrivals + ws->sms * kv8_attn_ctas_per_sm(hd) / 8 * kKvAttnRows);
+        a.part = reinterpret_cast<float *>(static_cast<char *>(workspace_) + kv8_attn_counter_bytes(ws->sms));
         const bool prompt = kv8_prompt_rows(hd, type == QL_F32) > 0 &&
                             kv8_prefers_prompt(rows, n_heads / a.c.kv_heads, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len,
                                                type == QL_F32, ws->sms, a.cluster);

@@ -118,6 +118,7 @@ cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, int max_q_len, bool bf16, cu
 
 // CTAs of the attention's split kernel that one SM holds (the host sizes the split count by it).
 int kv8_attn_ctas_per_sm(int head_dim);
+constexpr int kKvAttnMaxCtasPerSm = 4;    // of any head_dim
 constexpr int kKvAttnWarps = 4;           // warps per CTA, each with key blocks of its own
 constexpr int kKvAttnRows = 8;            // rows per CTA: query tokens x heads of one KV head's group
 constexpr int kKvAttnMaxClusters = 16;

@@ -119,6 +119,7 @@ __device__ __forceinline__ void store_f32(__nv_bfloat16 *p, float v) { *p = __fl
 // Ring stages per warp, and CTAs per SM, by head_dim: 64 head_dim bytes per stage, 4 warps, 227 KB per SM.
 constexpr int stages(int hd) { return hd <= 64 ? 3 : hd <= 128 ? 2 : 3; }
 constexpr int ctas_per_sm(int hd) { return hd <= 64 ? 4 : hd <= 128 ? 3 : 1; }
+static_assert(ctas_per_sm(32) <= kKvAttnMaxCtasPerSm, "the workspace's counters");
 
 // 16-byte chunk of a row at which chunk c of row t lies.  K: a load phase (8 lanes) reads 64 bytes of two
 // rows, which share their banks where a row is a multiple of 128 bytes: the odd row's halves are swapped.

@@ -329,8 +329,8 @@ QL_API int ql_kv8_append(const ql_kv8_cache *cache, int32_t type, const void *q,
  * zeros; one that sees a NaN or infinity gets NaN.  f32: fp32 results (1e-6); bf16: operands and weights of
  * 16 bits, sums of 32.  max_q_len and max_kv_len bound the lengths on the device and size the launch (more
  * cached tokens are read all the same; rows beyond max_q_len are not computed, and reported).  The workspace,
- * ql_kv8_attend_workspace bytes (they depend on head_dim alone: one serves calls of any size), 16-byte aligned,
- * is zeroed by the caller before its first use and left usable by every call; calls that may overlap on the GPU
+ * ql_kv8_attend_workspace bytes (they depend on head_dim alone: one serves calls of any size, and the largest of
+ * several head_dims serves them all), 16-byte aligned, is zeroed by the caller before its first use and left usable by every call; calls that may overlap on the GPU
  * need one each. */
 QL_API size_t ql_kv8_attend_workspace(int n_heads, int kv_heads, int head_dim, int n_seqs, int rows, int max_q_len,
                                       int max_kv_len);

@@ -276,3 +276,26 @@ def test_tiles_one_heavy_key_over_many_light_ones(nh, kvh, hd, n_seqs):
         want = U.attend(q[i].reshape(nh, hd), *stands, n - rows + i, hd ** -0.5)
         assert rel_l2(got[i], want.ravel()) < 2e-6 + n / 64 * 2.0 ** -23 + n * 2.0 ** -32, i
     Q.check_device()
+
+
+def test_one_workspace_serves_every_head_dim():
+    """Calls of head_dim 256, 128 and 64 with several key clusters each, in turn over one workspace that was zeroed once."""
+    import torch
+    bound = 1 << 16
+    calls = []
+    for hd, nh, kvh, n in ((256, 16, 4, 1), (128, 8, 1, 24), (64, 14, 2, 9), (256, 8, 2, 1), (128, 28, 4, 5), (64, 4, 1, 30)):
+        lens = [3000 - 97 * s for s in range(n)]
+        c, stands = _filled(lens, max(lens), kvh, hd, seed=79 + hd)
+        q = np.random.default_rng(hd).standard_normal((n, nh * hd)).astype(np.float32)
+        calls.append((hd, nh, kvh, n, lens, c, stands, q))
+    ws = torch.zeros(max(Q.kv8_attend_workspace(x[1], x[2], x[0], x[3], x[3], 1, bound) for x in calls), dtype=torch.uint8,
+                     device="cuda:0")
+    for _ in range(2):
+        for hd, nh, kvh, n, lens, c, stands, q in calls:
+            got = _attend(c, "f32", dev(q), nh, _i32(lens), None, 1, bound, ws=ws)
+            form, ctas = Q.kv8_attend_form()
+            assert form == Q.KV8_FORM_SPLIT and ctas >= 16  # (two clusters or more)
+            for s in range(n):
+                want = U.attend(q[s].reshape(nh, hd), *stands[s], lens[s] - 1, hd ** -0.5)
+                assert rel_l2(got[s], want.ravel()) < TOL["f32"], (hd, s)
+    Q.check_device()
