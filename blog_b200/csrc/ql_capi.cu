@@ -1375,7 +1375,8 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         if (gate && (st = kv8_operand(gate, gate_stride, width, type, "gate", what))) return st;
         Workspace *ws = workspace(&st);
         if (!ws) return st;
-        const int mq = q_start ? max_q_len : 1;
+        const int mq = q_start ? std::min(max_q_len, rows) : 1, group = n_heads / a.c.kv_heads;
+        if ((int64_t)rows * group > INT32_MAX - 256) return fail(QL_EINVAL, what + ": too many rows x heads for one call");
         const Kv8AttnShape sh = kv8_attn_shape(n_heads, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len, ws->sms);
         if ((int64_t)sh.splits * sh.row_groups * a.c.kv_heads > INT32_MAX)
             return fail(QL_EINVAL, what + ": max_q_len x n_heads too large for one call");
@@ -1398,10 +1399,14 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         a.longest_first = sh.longest_first;
         a.arrivals = static_cast<unsigned *>(workspace_);
         a.part = reinterpret_cast<float *>(static_cast<char *>(workspace_) + kv8_attn_counter_bytes(ws->sms));
-        const bool prompt = kv8_prompt_rows(hd, type == QL_F32) > 0 &&
-                            kv8_prefers_prompt(rows, n_heads / a.c.kv_heads, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len,
-                                               type == QL_F32, ws->sms, a.cluster);
-        const cudaError_t e = prompt ? kv8_prompt_launch(a, mq, type == QL_BF16, g_stream)
+        int ctas = 1;  // that share a row's keys in tiles
+        const int tile_rows = kv8_prompt_rows(hd, type == QL_F32);
+        const int64_t tiles = tile_rows > 0 ? ((int64_t)mq * group + tile_rows - 1) / tile_rows : 0;
+        const bool prompt = tiles > 0 &&
+                            kv8_prefers_prompt(rows, group, a.c.kv_heads, hd, a.c.n_seqs, mq, max_kv_len, type == QL_F32,
+                                               ws->sms, ctas);
+        if (prompt) a.cluster = ctas, a.row_groups = (int)tiles;
+        const cudaError_t e = prompt ? kv8_prompt_launch(a, type == QL_BF16, g_stream)
                                      : kv8_attn_launch(a, type == QL_BF16, g_stream);
         ++t_launches;
         if (e == cudaSuccess) {

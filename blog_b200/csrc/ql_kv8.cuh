@@ -53,7 +53,8 @@ struct Kv8AttnArgs {
     int splits;        // CTAs over the keys of one (sequence, KV head, row group): clusters of `cluster`
     int cluster;       // 1, 2, 4 or 8 (prompts: 1 to 8, all of the splits)
     bool longest_first;  // CTAs start by their sequences' lengths, at most kKvAttnSorted sequences
-    int row_groups;    // groups of 8 (query token, head of the KV head's group) rows per sequence
+    int row_groups;    // groups of 8 (query token, head of the KV head's group) rows per sequence (prompts: kv8_prompt_rows)
+    int tile0;         // prompts: the launch's first tile of rows, from the sequence's end
     unsigned *arrivals;  // [n_seqs x kv_heads x row_groups][8] zero between calls (several clusters)
     float *part;         // [...][clusters][8][head_dim + 4]
 };
@@ -114,7 +115,7 @@ cudaError_t kv8_gather_launch(const Kv8View &c, const int *kv_len, const int *st
 cudaError_t kv8_attn_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s);
 // The tensor-core form for prompts (ql_kv8_prompt.cu).
 int kv8_prompt_rows(int head_dim, bool f32);  // rows per CTA, 0: not taken
-cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, int max_q_len, bool bf16, cudaStream_t s);
+cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s);
 
 // CTAs of the attention's split kernel that one SM holds (the host sizes the split count by it).
 int kv8_attn_ctas_per_sm(int head_dim);

@@ -299,3 +299,36 @@ def test_one_workspace_serves_every_head_dim():
                 want = U.attend(q[s].reshape(nh, hd), *stands[s], lens[s] - 1, hd ** -0.5)
                 assert rel_l2(got[s], want.ravel()) < TOL["f32"], (hd, s)
     Q.check_device()
+
+
+@pytest.mark.parametrize("t,hd", WIDTHS)
+def test_tiles_under_a_wide_bound_of_rows(t, hd):
+    """max_q_len of 2^20 (more tiles of rows than a grid's second and third dimension hold) for a call of 600 rows."""
+    nh, kvh = 16, 1
+    q_len, lens = [500, 100], [900, 333]
+    c, stands = _filled(lens, max(lens), kvh, hd, seed=83)
+    qd, q = _dev(np.random.default_rng(84).standard_normal((600, nh * hd)), t)
+    got = _attend(c, t, qd, nh, _i32(lens), _i32(_starts(q_len)), 1 << 20, 1 << 20)
+    _tiles()
+    _check_rows(got, q, stands, lens, q_len, nh, TOL[t])
+    Q.check_device()
+
+
+def test_tiles_of_more_rows_than_a_grid_dimension():
+    """65600 tiles of rows in one call, all but the last of them before the cache's first token (zeros)."""
+    import torch
+    nh, kvh, hd, rows, n = 64, 1, 64, 262400, 900
+    c, stands = _filled([n], n, kvh, hd, seed=85)
+    g = torch.Generator(device="cuda:0").manual_seed(86)
+    q = torch.randn(rows, nh * hd, device="cuda:0", generator=g, dtype=torch.bfloat16)
+    out = torch.full_like(q, float("nan"))
+    ws = torch.zeros(Q.kv8_attend_workspace(nh, kvh, hd, 1, rows, rows, 300000), dtype=torch.uint8, device="cuda:0")
+    kv, st = _i32([n]), _i32([0, rows])
+    Q.kv8_attend(c.view, Q.BF16, q.data_ptr(), nh * hd, None, 0, out.data_ptr(), nh * hd, nh, hd ** -0.5, kv.data_ptr(),
+                 st.data_ptr(), rows, rows, 300000, ws.data_ptr(), ws.numel())
+    _tiles()
+    torch.cuda.synchronize()
+    assert not bool(out[:rows - n].any())
+    got, qh = host(out[rows - n:].float()), host(q[rows - n:].float())
+    _check_rows(got, qh, stands, [n], [n], nh, TOL["bf16"], rows=lambda s, i: i % 50 == 0 or i > n - 5)
+    Q.check_device()
