@@ -91,10 +91,22 @@ class Decoder:
         return logits
 
 
+def check_request(lens, steps, seqs, max_tokens):
+    """Raises ValueError for prompts of `lens` tokens and `steps` new ones that a Decoder's cache does not hold."""
+    if len(lens) != seqs or min(lens, default=0) < 1:
+        raise ValueError("need %d prompts of at least one token each" % seqs)
+    if steps < 2:
+        raise ValueError("need at least 2 tokens: the prompts' and one step's")
+    if max(lens) + steps - 1 > max_tokens:  # (the last token's key is never stored)
+        raise ValueError("%d prompt tokens and %d new ones do not fit a cache of %d" % (max(lens), steps, max_tokens))
+
+
 def generate(model, prompts, steps):
-    """Greedy tokens [sequences][steps] after the prompts (lists of ids), the logits of the last step, us per step."""
+    """Greedy tokens [sequences][steps] after the prompts (lists of ids), the logits of the last step, us per
+    replayed step (None: there was none)."""
     n, V = model.n, model.V
     lens = [len(q) for q in prompts]
+    check_request(lens, steps, n, model.max_tokens)
     room = max(lens) + steps
     history = torch.zeros(n, room, dtype=torch.int32, device=DEV)
     for i, q in enumerate(prompts):
@@ -158,23 +170,24 @@ def generate(model, prompts, steps):
         Q.set_stream(before)
     Q.check_device()
     out = [history[i, lens[i]:lens[i] + steps].tolist() for i in range(n)]
-    return out, raw, start.elapsed_time(end) * 1e3 / max(1, steps - 2)
+    return out, raw, start.elapsed_time(end) * 1e3 / (steps - 2) if steps > 2 else None
 
 
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--layers", type=int, default=4)
-    ap.add_argument("--tokens", type=int, default=64)
+    ap.add_argument("--tokens", type=int, default=64, help="new tokens per sequence (at least 2)")
     a = ap.parse_args()
     Q.init(0)
     Q.set_stream(torch.cuda.current_stream().cuda_stream)
-    model = Decoder(layers=a.layers)
+    model = Decoder(layers=a.layers, max_tokens=max(512, 100 + a.tokens))
     g = torch.Generator().manual_seed(0)
     prompts = [torch.randint(0, model.V, (k,), generator=g).tolist() for k in (100, 33, 7)]
     out, _, us = generate(model, prompts, a.tokens)
     for i, t in enumerate(out):
         print("sequence %d (%d prompt tokens): %s ..." % (i, len(prompts[i]), t[:12]))
-    print("%.0f us per step of %d sequences, %d layers" % (us, model.n, a.layers))
+    if us is not None:
+        print("%.0f us per step of %d sequences, %d layers" % (us, model.n, a.layers))
 
 
 if __name__ == "__main__":
