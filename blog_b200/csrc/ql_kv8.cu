@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, V <= 4 ? 5 : 3) append_kernel(const 
     int row0, q_len;
     kv8_rows_of(a.r, seq, row0, q_len);
     const int kv_len = a.r.kv_len[seq];
-    if (q_len <= 0 || kv_len <= 0) return;
+    if (q_len <= 0 || kv_len == 0) return;
     if (kv_len < q_len) {
         if (threadIdx.x == 0) atomicExch(a.c.err, kErrKvLength);
         return;

@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
     int kv_len = a.r.kv_len[seq];
     if (threadIdx.x == 0 && rg == 0 && q_len * G > a.row_groups * kKvAttnRows) atomicExch(a.c.err, kErrKvLength);
     if (rg * kKvAttnRows >= q_len * G) return;  // (uniform: every split of the group leaves here)
-    if ((kv_len + kKvBlock - 1) / kKvBlock > a.c.max_pages) {
+    if ((unsigned)kv_len > (unsigned)(a.c.max_pages * kKvBlock)) {  // (negative too; the host bounds max_pages)
         if (threadIdx.x == 0) atomicExch(a.c.err, kErrKvPage);
         kv_len = 0;
     }

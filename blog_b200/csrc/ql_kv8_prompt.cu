@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const int n_rows = q_len * G;
     if (r_base >= n_rows) return;
     int kv_len = a.r.kv_len[seq];
-    if ((kv_len + kKvBlock - 1) / kKvBlock > a.c.max_pages) {
+    if ((unsigned)kv_len > (unsigned)(a.c.max_pages * kKvBlock)) {  // (negative too; the host bounds max_pages)
         if (threadIdx.x == 0) atomicExch(a.c.err, kErrKvPage);
         kv_len = 0;
     }

@@ -43,3 +43,20 @@ def test_codes_of_the_smallest_blocks():
                 assert scales[page, h] == scale
                 assert np.array_equal(codes[page, h], want), most[b]
     Q.check_device()
+
+
+@pytest.mark.parametrize("bad,what", [(2 ** 31 - 1, "page"), (2 ** 31 - 32, "page"), (-1, "more rows"), (-2 ** 31, "more rows")])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_lengths_at_the_ends_of_their_type_are_reported(bad, what, ragged):
+    """Nothing of that sequence is stored, the other's token is."""
+    kvh, hd = 2, 64
+    c = Cache(2, 64, kvh, hd, seed=89)
+    c.ko.zero_()
+    x = np.random.default_rng(90).standard_normal((2, 2 * kvh * hd)).astype(np.float32)
+    _append(c, "f32", dev(x), 0, None, _i32([bad, 3]), _i32([0, 1, 2]) if ragged else None, 1)
+    with pytest.raises(Q.QLError, match=what):
+        Q.check_device()
+    want = np.zeros(c.ko.shape, np.float32)
+    want[c.slot[1], 0, :, 2] = x[1, :kvh * hd].reshape(kvh, hd)
+    assert np.array_equal(host(c.ko), want)
+    assert (host(c.kc) == 77).all()

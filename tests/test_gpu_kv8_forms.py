@@ -332,3 +332,19 @@ def test_tiles_of_more_rows_than_a_grid_dimension():
     got, qh = host(out[rows - n:].float()), host(q[rows - n:].float())
     _check_rows(got, qh, stands, [n], [n], nh, TOL["bf16"], rows=lambda s, i: i % 50 == 0 or i > n - 5)
     Q.check_device()
+
+
+@pytest.mark.parametrize("bad", [2 ** 31 - 1, 2 ** 31 - 32, -1, -40, -2 ** 31])
+@pytest.mark.parametrize("tiles", [False, True])
+def test_lengths_at_the_ends_of_their_type_are_reported(tiles, bad):
+    """A length no cache holds: no key is read (zeros), it is reported, and the other sequences' rows are right."""
+    nh, kvh, hd = 32, 2, 128
+    lens, q_len = ([607] * 4, [400] * 4) if tiles else ([607] * 4, [3] * 4)
+    c, stands = _filled(lens, 608, kvh, hd, seed=87)
+    qd, q = _dev(np.random.default_rng(88).standard_normal((sum(q_len), nh * hd)), "f32")
+    got = _attend(c, "f32", qd, nh, _i32([607, bad, 607, 607]), _i32(_starts(q_len)), max(q_len), 607)
+    assert Q.kv8_attend_form()[0] == (Q.KV8_FORM_TILES if tiles else Q.KV8_FORM_SPLIT)
+    with pytest.raises(Q.QLError, match="page"):
+        Q.check_device()
+    assert not got[q_len[0]:2 * q_len[0]].any()
+    _check_rows(got, q, stands, lens, q_len, nh, TOL["f32"], rows=lambda s, i: s != 1 and i % 7 == 0)
