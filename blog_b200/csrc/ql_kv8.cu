@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, V <= 4 ? 5 : 3) append_kernel(const 
     }
     const int pos0 = kv_len - q_len, first = pos0 / kKvBlock, last = (kv_len - 1) / kKvBlock;
     const int block = first + j;
-    if (block > last) return;
+    if (j < 0 || block > last) return;  // (j < 0: rows before q_start[0] are nobody's)
     if (last >= a.c.max_pages) {
         if (threadIdx.x == 0) atomicExch(a.c.err, kErrKvPage);
         return;

@@ -60,3 +60,16 @@ def test_lengths_at_the_ends_of_their_type_are_reported(bad, what, ragged):
     want[c.slot[1], 0, :, 2] = x[1, :kvh * hd].reshape(kvh, hd)
     assert np.array_equal(host(c.ko), want)
     assert (host(c.kc) == 77).all()
+
+
+def test_rows_before_the_first_sequence_are_nobodys():
+    """q_start[0] = 70 (it should be 0): the 70 rows' tiles touch no page, and the sequences' own rows are stored."""
+    kvh, hd = 2, 64
+    c = Cache(2, 64, kvh, hd, seed=91)
+    x = np.random.default_rng(92).standard_normal((75, 2 * kvh * hd)).astype(np.float32)
+    _append(c, "f32", dev(x), 0, None, _i32([2, 3]), _i32([70, 72, 75]), 70)
+    ko = host(c.ko)
+    for s, (row, n) in enumerate(((70, 2), (72, 3))):
+        assert np.array_equal(ko[c.slot[s], 0, :, :n], x[row:row + n, :kvh * hd].reshape(n, kvh, hd).transpose(1, 0, 2))
+    assert (host(c.kc) == 77).all()
+    Q.check_device()
