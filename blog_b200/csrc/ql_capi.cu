@@ -12,6 +12,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <string>
@@ -1198,6 +1199,12 @@ int ql_full_attention_attend_batch(const float *q, const float *gate, const void
 
 // ---- 8-bit KV cache, rules on logits -------------------------------------------------
 namespace {
+// Whether 32-bit device arrays (null: absent) start on 4 bytes.
+bool on_words(std::initializer_list<const void *> arrays) {
+    for (const void *p : arrays)
+        if (reinterpret_cast<uintptr_t>(p) % 4) return false;
+    return true;
+}
 int kv8_view(const ql_kv8_cache *c, int32_t type, Kv8View &v, const std::string &what) {
     if (type != QL_F32 && type != QL_BF16) return fail(QL_EINVAL, what + ": type must be QL_F32 or QL_BF16");
     if (!c) return fail(QL_EINVAL, what + ": null cache");
@@ -1213,8 +1220,7 @@ int kv8_view(const ql_kv8_cache *c, int32_t type, Kv8View &v, const std::string 
             if (!p) return fail(QL_EINVAL, what + ": null cache buffer");
         for (const void *p : {need[0], need[1], need[4], need[5]})
             if (reinterpret_cast<uintptr_t>(p) % 16) return fail(QL_EINVAL, what + ": cache buffers must be 16-byte aligned");
-        for (const void *p : {need[2], need[3], need[6], static_cast<const void *>(c->slots)})
-            if (reinterpret_cast<uintptr_t>(p) % 4) return fail(QL_EINVAL, what + ": misaligned cache buffer");
+        if (!on_words({need[2], need[3], need[6], c->slots})) return fail(QL_EINVAL, what + ": misaligned cache buffer");
     }
     v = Kv8View{c->k_codes, c->v_codes, c->k_scale, c->v_scale, c->k_open,    c->v_open,   c->page_table,
                 c->slots,   c->n_pages, c->n_slots, c->n_seqs,  c->max_pages, c->kv_heads, c->head_dim, nullptr};
@@ -1227,6 +1233,7 @@ int kv8_rows(const Kv8View &c, const int32_t *kv_len, const int32_t *q_start, in
         return fail(QL_EINVAL, what + ": without q_start there is one row per sequence (rows == n_seqs)");
     if (rows > 0 && c.n_seqs == 0) return fail(QL_EINVAL, what + ": rows without sequences");
     if (rows > 0 && !kv_len) return fail(QL_EINVAL, what + ": null kv_len");
+    if (!on_words({kv_len, q_start})) return fail(QL_EINVAL, what + ": misaligned kv_len or q_start");
     if (rows > 0 && max_q_len < (q_start ? (rows + c.n_seqs - 1) / c.n_seqs : 1))
         return fail(QL_EINVAL, what + ": max_q_len is less than the rows need");
     r = Kv8Rows{kv_len, q_start, rows};
@@ -1320,8 +1327,9 @@ int ql_kv8_append(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
             return fail(QL_EINVAL, what + ": rotary_dim must be a multiple of head_dim / 16, at most head_dim");
         if (!(eps >= 0.f)) return fail(QL_EINVAL, what + ": eps must not be negative");
         if (rows == 0) return (int)QL_OK;
-        if (rotary_dim > 0 && (!rope || max_positions <= 0 || reinterpret_cast<uintptr_t>(rope) % 4))
+        if (rotary_dim > 0 && (!rope || max_positions <= 0))
             return fail(QL_EINVAL, what + ": rotation needs a table of max_positions > 0 rows");
+        if (!on_words({rope, q_gamma, k_gamma})) return fail(QL_EINVAL, what + ": misaligned rope, q_gamma or k_gamma");
         if (n_heads > 0 && ((st = kv8_operand(q, q_stride, (int64_t)n_heads * hd, type, "q", what)) ||
                             (st = kv8_operand(q_out, q_out_stride, (int64_t)n_heads * hd, type, "q_out", what))))
             return st;
@@ -1433,6 +1441,7 @@ int ql_kv8_gather(const ql_kv8_cache *cache, int32_t type, void *k_out, void *v_
         if (count < 0) return fail(QL_EINVAL, what + ": count must not be negative");
         if (count == 0 || c.n_seqs == 0 || (!k_out && !v_out)) return (int)QL_OK;
         if (!kv_len) return fail(QL_EINVAL, what + ": null kv_len");
+        if (!on_words({kv_len, start})) return fail(QL_EINVAL, what + ": misaligned kv_len or start");
         if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16)
             return fail(QL_EINVAL, what + ": outputs must be 16-byte aligned");
         if ((int64_t)c.n_seqs * count * c.kv_heads * (c.head_dim / 16) / 256 >= INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
@@ -1458,8 +1467,10 @@ int ql_logits_apply(const float *logits, int64_t logits_stride, float *out, int6
         if (!logits || logits_stride < vocab) return fail(QL_EINVAL, what + ": null logits, or a stride below vocab");
         if (out && out_stride < vocab) return fail(QL_EINVAL, what + ": out's stride is below vocab");
         if (out == logits && out_stride != logits_stride) return fail(QL_EINVAL, what + ": in place the strides are the same");
-        if (reinterpret_cast<uintptr_t>(logits) % 4 || reinterpret_cast<uintptr_t>(out) % 4)
-            return fail(QL_EINVAL, what + ": misaligned logits or out");
+        if (!on_words({logits, out, token})) return fail(QL_EINVAL, what + ": misaligned logits, out or token");
+        if (!on_words({rules->history, rules->history_len, rules->prompt_len, rules->repetition, rules->frequency,
+                       rules->presence, rules->bias_ids, rules->bias_values, rules->bias_start, rules->mask, rules->mask_row}))
+            return fail(QL_EINVAL, what + ": misaligned rules");
         if (rules->history && (!rules->history_len || rules->history_stride < 0 ||
                                rules->history_stride > (int64_t)kLogitsMaxHistory))
             return fail(QL_EINVAL, what + ": a history needs history_len and a stride of at most 1048575 ids");
