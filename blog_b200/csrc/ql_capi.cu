@@ -1234,7 +1234,7 @@ int kv8_rows(const Kv8View &c, const int32_t *kv_len, const int32_t *q_start, in
     if (rows > 0 && c.n_seqs == 0) return fail(QL_EINVAL, what + ": rows without sequences");
     if (rows > 0 && !kv_len) return fail(QL_EINVAL, what + ": null kv_len");
     if (!on_words({kv_len, q_start})) return fail(QL_EINVAL, what + ": misaligned kv_len or q_start");
-    if (rows > 0 && max_q_len < (q_start ? (rows + c.n_seqs - 1) / c.n_seqs : 1))
+    if (rows > 0 && max_q_len < (q_start ? ((int64_t)rows + c.n_seqs - 1) / c.n_seqs : 1))
         return fail(QL_EINVAL, what + ": max_q_len is less than the rows need");
     r = Kv8Rows{kv_len, q_start, rows};
     return QL_OK;

@@ -53,6 +53,12 @@ def test_misaligned_rules():
         _refused(Q.logits_apply, *a.values())
 
 
+def test_the_largest_numbers_of_rows():
+    for rows in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30):
+        _refused(Q.kv8_append, *dict(APPEND, cache=_cache(), rows=rows).values())
+        _refused(Q.kv8_attend, *dict(ATTEND, cache=_cache(), rows=rows).values())
+
+
 def test_workspace_of_bad_sizes():
     for a in ((3, 2, 64, 1, 1, 1, 64), (0, 1, 64, 1, 1, 1, 64), (4, 2, 80, 1, 1, 1, 64), (4, 2, 64, -1, 1, 1, 64)):
         assert Q.kv8_attend_workspace(*a) == 0
