@@ -1356,10 +1356,13 @@ size_t ql_kv8_attend_workspace(int n_heads, int kv_heads, int head_dim, int n_se
     if (n_heads <= 0 || kv_heads <= 0 || n_heads % kv_heads || head_dim <= 0 || head_dim > kKvMaxHeadDim || head_dim % 32 ||
         n_seqs < 0 || rows < 0 || max_q_len < 0 || max_kv_len < 0)
         return 0;
-    int st;
-    Workspace *ws = workspace(&st);
-    if (!ws) return 0;
-    return kv8_attn_workspace_bytes(head_dim, ws->sms);
+    size_t bytes = 0;
+    guarded([&] {
+        int st;
+        if (Workspace *ws = workspace(&st)) bytes = kv8_attn_workspace_bytes(head_dim, ws->sms);
+        return (int)QL_OK;
+    });
+    return bytes;
 }
 
 int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *gate,
