@@ -287,11 +287,11 @@ QL_API int ql_full_attention_attend_batch(const float *q, const float *gate, con
  * f32 scale per KV head for K and one for V:
  *   scale = max|x| / 127 over the page's tokens and the head's dimensions (>= 0), byte = rint(x / scale) + 128
  * (x / scale kept within +-127, which a subnormal scale may pass; scale 0: bytes 128; a page that holds NaN or
- * infinity has a NaN scale).  The tokens of a sequence's
- * last, unfinished page are exact: their rows stand in f32 in the "open" rows, from which the page is
- * quantised once, when it is full.  So the bytes do not depend on how a sequence was cut into calls, and
- * since the open rows hold the last two pages, kv_len may go back by up to QL_KV8_BLOCK tokens (rejected
- * speculative tokens) between calls.
+ * infinity has a NaN scale).  The tokens of a sequence's last, unfinished page are exact: their rows stand in f32 in
+ * the "open" rows, from which the page is quantised once, when it is full.  So the bytes do not depend on how a
+ * sequence was cut into calls.  kv_len may go back between calls (rejected speculative tokens): to any length within
+ * the last two pages of the longest the sequence has been, whose rows the open rows hold (at least QL_KV8_BLOCK tokens
+ * less than the longest), and to any multiple of QL_KV8_BLOCK.
  * All buffers are the caller's device memory; every base is 16-byte aligned.  head_dim: a multiple of 32
  * up to 256; activations f32 (QL_F32) or bf16 (QL_BF16).  kv_len, q_start, page_table and slots are read
  * on the device, so a captured CUDA graph follows them.  A page, slot, length or position outside the
@@ -326,12 +326,21 @@ QL_API int ql_kv8_append(const ql_kv8_cache *cache, int32_t type, const void *q,
 /* Causal attention of the call's rows over the cache (after ql_kv8_append):
  *   out_h = softmax_j(scale q_h . k_j) . v_j [* sigmoid(gate_h)],  j = 0 .. the row's position,
  * query head h reads KV head h / (n_heads / kv_heads).  gate == NULL: none.  A row that sees no key gets
- * zeros; one that sees a NaN or infinity gets NaN.  f32: fp32 results (1e-6); bf16: operands and weights of
- * 16 bits, sums of 32.  max_q_len and max_kv_len bound the lengths on the device and size the launch (more
- * cached tokens are read all the same; rows beyond max_q_len are not computed, and reported).  The workspace,
- * ql_kv8_attend_workspace bytes (they depend on head_dim alone: one serves calls of any size, and the largest of
- * several head_dims serves them all), 16-byte aligned, is zeroed by the caller before its first use and left usable by every call; calls that may overlap on the GPU
- * need one each. */
+ * zeros; one that sees a NaN or infinity gets NaN.  Keys and values are read as they stand after the append: a token
+ * whose page the same call filled is read as bytes by every row of the call that sees it, while a row that came before
+ * the page was full read exact rows.  So the bytes of the cache do not depend on how tokens are cut into calls, but a
+ * row's result does, by the quantisation of its own page.
+ * f32: fp32 results (1e-6 relative).  q, weights and open rows go through the tensor cores in two f16 limbs, 22 bits (of
+ * the row's largest, the weight itself, and the largest of the open page); products are exact, sums fp32.  A weight below
+ * 2^-32 of the row's heaviest adds nothing to the values' sum, and the sums take a rounding of at most 2^-24 for every 64
+ * keys: one heavy key over n light ones that all agree is right to n 2^-29.  bf16: operands and weights of 16 bits
+ * (weights: f16), sums of 32.
+ * max_q_len and max_kv_len bound the lengths on the device; the launch, its split over the keys and the choice between
+ * the two kernels follow from them, so bounds near the lengths are faster (more cached tokens are read all the same;
+ * rows beyond max_q_len are not computed, and reported).  The workspace, ql_kv8_attend_workspace bytes (they depend on
+ * head_dim alone: one serves calls of any size, and the largest of several head_dims serves them all), 16-byte aligned,
+ * is zeroed by the caller before its first use and left usable by every call; calls that may overlap on the GPU need
+ * one each. */
 QL_API size_t ql_kv8_attend_workspace(int n_heads, int kv_heads, int head_dim, int n_seqs, int rows, int max_q_len,
                                       int max_kv_len);
 QL_API int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_t q_stride, const void *gate,

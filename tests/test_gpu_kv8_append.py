@@ -4,7 +4,7 @@ import pytest
 
 import blog_b200 as Q
 from gpu_util import dev, host
-from test_gpu_kv8 import Cache, _append, _i32
+from test_gpu_kv8 import Cache, _append, _check_cache, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -72,4 +72,40 @@ def test_rows_before_the_first_sequence_are_nobodys():
     for s, (row, n) in enumerate(((70, 2), (72, 3))):
         assert np.array_equal(ko[c.slot[s], 0, :, :n], x[row:row + n, :kvh * hd].reshape(n, kvh, hd).transpose(1, 0, 2))
     assert (host(c.kc) == 77).all()
+    Q.check_device()
+
+
+def test_speculative_cycles():
+    """Calls of up to 33 draft tokens of which some are taken back each time, over ten pages: as if the rejected ones
+    had never been."""
+    kvh, hd = 2, 64
+    rng = np.random.default_rng(93)
+    c = Cache(1, 400, kvh, hd, seed=94)
+    text, pos = np.zeros((0, 2 * kvh * hd), np.float32), 0
+    for step in range(60):
+        n = int(rng.integers(1, 34))
+        x = rng.standard_normal((n, 2 * kvh * hd)).astype(np.float32)
+        if pos + n > 400:
+            break
+        _append(c, "f32", dev(x), 0, None, _i32([pos + n]), _i32([0, n]), n)
+        keep = int(rng.integers(1, n + 1))
+        text, pos = np.concatenate([text, x[:keep]]), pos + keep
+        z = text.reshape(pos, 2, kvh, hd).astype(np.float64)
+        _check_cache(c, [z[:, 0]], [z[:, 1]], [pos], exact_bytes=True)
+    assert pos > 320
+    Q.check_device()
+
+
+@pytest.mark.parametrize("back", [0, 32, 64, 96, 129, 140, 150])
+def test_going_back_to_a_page_and_into_the_last_two(back):
+    """From 180 tokens to a multiple of 32 or into the last two pages (from 128 on), then 90 others."""
+    kvh, hd = 2, 64
+    rng = np.random.default_rng(95)
+    x = rng.standard_normal((180, 2 * kvh * hd)).astype(np.float32)
+    y = rng.standard_normal((90, 2 * kvh * hd)).astype(np.float32)
+    c = Cache(1, 300, kvh, hd, seed=96)
+    _append(c, "f32", dev(x), 0, None, _i32([180]), _i32([0, 180]), 180)
+    _append(c, "f32", dev(y), 0, None, _i32([back + 90]), _i32([0, 90]), 90)
+    z = np.concatenate([x[:back], y]).reshape(back + 90, 2, kvh, hd).astype(np.float64)
+    _check_cache(c, [z[:, 0]], [z[:, 1]], [back + 90], exact_bytes=True)
     Q.check_device()
