@@ -524,7 +524,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
         const int64_t rows_at = kv8_open_at(a.c, slot, open0 / kKvBlock, kh) + (int64_t)u * 8 * HD;
         const int key0 = open0 + 8 * u, there = min(8, kv_len - key0);
         unsigned bad = 0;
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        // f32 rows: three sums, every other step's upper limbs and the lower limbs.  (The MMA truncates products of two
+        // limbs of 11 bits as it aligns them to its sum: in one sum scores of head_dim 256 have an error of 7e-7, so 3e-7.)
+        constexpr int C1 = EXACT ? 1 : 0, C2 = EXACT ? 2 : 0;
+        float c[C2 + 1][4] = {};
         float kinv;
         {
             float x[KS][4], amax = 0.f;
@@ -553,8 +556,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
                 uint32_t h0, l0, h1, l1;
                 split_f16(x[s][0] * f, x[s][1] * f, h0, l0);
                 split_f16(x[s][2] * f, x[s][3] * f, h1, l1);
-                mma16816(c, af, h0, h1);
-                mma16816(c, af, l0, l1);
+                mma16816(c[s & C1], af, h0, h1);
+                mma16816(c[C2], af, l0, l1);
             }
         }
         float v[2][HD / 8], vmax = 0.f, vinv;
@@ -585,7 +588,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(HD)) attn_kernel(const _
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int t = 2 * q4 + e;
-            s[0][e] = c[e] + c[e + 2];
+            s[0][e] = c[0][e] + c[0][e + 2];
+            if (EXACT) s[0][e] = (c[0][e] + c[C1][e]) + ((c[0][e + 2] + c[C1][e + 2]) + (c[C2][e] + c[C2][e + 2]));
             if (bad >> t & 1) s[0][e] = __int_as_float(0x7FC00000);
             if (key0 + t > pos) s[0][e] = -INFINITY;
         }

@@ -348,3 +348,26 @@ def test_lengths_at_the_ends_of_their_type_are_reported(tiles, bad):
         Q.check_device()
     assert not got[q_len[0]:2 * q_len[0]].any()
     _check_rows(got, q, stands, lens, q_len, nh, TOL["f32"], rows=lambda s, i: s != 1 and i % 7 == 0)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_f32_scores_over_open_rows(hd):
+    """The scores themselves, from the weight that one token has against another of score 0, both in the open rows: two
+    limbs of 22 bits (2^-23 of the rows' largest, three times their size), eight truncating additions of 2^-25 and an
+    exponential of 2^-22 add up to less than 2^-21 of the scores' size, in the root of the mean square."""
+    nh, kvh, n = 64, 1, 2
+    rng = np.random.default_rng(hd + n)
+    c = Cache(1, n, kvh, hd, seed=3)
+    k, v = np.zeros((2, n, kvh, hd))
+    k[0], v[0] = rng.standard_normal((kvh, hd)), 1
+    stands = c.set(0, k, v)
+    q = (rng.standard_normal((nh, hd)) * 2).astype(np.float32)
+    got = _attend(c, "f32", dev(q.reshape(1, -1)), nh, _i32([n]), None, 1, n)[0].reshape(nh, hd)
+    assert Q.kv8_attend_form()[0] == Q.KV8_FORM_SPLIT
+    s = q.astype(np.float64) @ stands[0][0, 0] * hd ** -0.5
+    p = got.mean(-1).astype(np.float64)
+    good = (p > 0.002) & (p < 0.9)
+    assert good.sum() > 20
+    err = (np.log(p / (1 - p)) - s)[good]
+    assert np.sqrt((err ** 2).mean()) < 2.0 ** -21 * np.sqrt((s[good] ** 2).mean())
+    Q.check_device()
