@@ -29,12 +29,11 @@
 // CTA's loads, products and merges: one sequence of 28/4/128 heads, f32, 17.6 us at 32768 tokens (1.9 TB/s) and
 // 7.6 us at 200.  Tiles of 8 rows and not of 16: a group of 7 or 8 heads fills them, and a single token has no more.
 #include <cooperative_groups.h>
-#include <cuda_fp16.h>
 
 #include <atomic>
 #include <climits>
 
-#include "ql_kv8.cuh"
+#include "ql_kv8_limbs.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -42,10 +41,6 @@ namespace ql {
 namespace {
 
 constexpr int kThreads = 32 * kKvAttnWarps;
-// m and h are whole numbers, at or above the maxima they stand for when they are set, and kept until a value
-// passes them by kHeadroom (so the sums are seldom rescaled).  Weights are scaled by 2^kWBits: at most
-// 2^(7 + 8) in f16, and limbs down to 2^-24 / 2^8 of the row's largest.
-constexpr float kHeadroom = 7.0f, kWBits = 8.0f;
 
 __device__ __forceinline__ void cp16(void *dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -61,39 +56,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         "%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// Two codes (bytes sel of w) as f16: 0x6400 | u is 1024 + u, minus 1152 is exact.
-__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t sel) {
-    uint32_t r = __byte_perm(w, 0x64646464u, sel);
-    const uint32_t bias = 0x64806480u;  // 1152, 1152
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(bias));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
-// x = hi + lo in two f16 limbs, two values packed.
-__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t &hi, uint32_t &lo) {
-    hi = pack_f16(x0, x1);
-    const float2 h = unpack_f16(hi);
-    lo = pack_f16(x0 - h.x, x1 - h.y);
-}
-// 2^k with amax * 2^k in [2^10, 2^11) (within the normal range), and 2^-k.
-__device__ __forceinline__ float limb_scale(float amax, float &inv) {
-    const int e = (int)(__float_as_uint(amax) >> 23) & 0xFF;
-    const int f = min(max(264 - e, 1), 253);
-    inv = __uint_as_float((uint32_t)(254 - f) << 23);
-    return __uint_as_float((uint32_t)f << 23);
 }
 template <typename T>
 __device__ __forceinline__ float load_f32(const T *p);
@@ -143,20 +105,12 @@ __device__ __forceinline__ float part_factor(float pm, float pt, float m) {
     return pt != pt ? pt : pm == -INFINITY ? 0.f : ex2(pm - m);
 }
 
-// 2^(kWBits - h), 0 while nothing but zeros has been met (h = -inf).
-__device__ __forceinline__ float weight_unit(float h) { return h == -INFINITY ? 0.f : ex2(kWBits - h); }
 // What turns sums of w 2^(s - m) sv code into sums of 2^(s - m) sv code: x 2^(h - kWBits), in two steps where
 // the power leaves the range.
 __device__ __forceinline__ float weight_undo(float x, float h) {
     const float e = h - kWBits;
     return h == -INFINITY ? x * 0.f : x * ex2(fmaxf(e, -120.f)) * ex2(fminf(e + 120.f, 0.f));  // (NaN stays)
 }
-// Below this h the weights' factor sv w leaves the range, and 2^(s - m) with it, where the weights themselves
-// do not (the row's heaviest keys have values of zero): they are computed from s - m - h then.
-constexpr float kDeep = -60.0f;
-// Beyond this |m| a score is rounded before m is taken off it: m is a rounded score then, and what one rounding
-// of the difference would keep is larger than the range of the weights.
-constexpr float kHuge = 1e6f;
 
 // Running state of one warp: row g8 = lane / 4 in the first two floats of a fragment (upper limbs) and the
 // last two (lower limbs).

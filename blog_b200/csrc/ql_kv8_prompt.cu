@@ -29,13 +29,12 @@
 // so that one's products run under the other's softmax; tiles of 64 keys, so that S has two buffers (tiles of 128 with
 // one: 714 and 110 us).
 #include <cooperative_groups.h>
-#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
 
-#include "ql_kv8.cuh"
+#include "ql_kv8_limbs.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -48,7 +47,6 @@ constexpr int kKeys = 64;    // keys per tile: 2 blocks
 constexpr int kTileBlocks = kKeys / kKvBlock;
 // Tiles of 128 rows per CTA: two, or one where O takes 256 columns of TMEM.
 constexpr int row_tiles(int hd) { return hd <= 128 ? 2 : 1; }
-constexpr float kHeadroom = 7.0f, kWBits = 8.0f;  // as in the split kernel
 
 // Registers per thread of the roles; 16 warps launch with 128 each.
 constexpr int kSoftmaxRegs = 200, kConvertRegs = 64, kIssueRegs = 48;
@@ -180,43 +178,6 @@ constexpr uint32_t idesc(int n, bool b_mn) {
     return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// As in the split kernel: 2^(kWBits - h), 0 while nothing but zeros has been met (h = -inf).
-__device__ __forceinline__ float weight_unit(float h) { return h == -INFINITY ? 0.f : ex2(kWBits - h); }
-// Below this h the weights' factor sv w leaves the range, and 2^(s - m) with it, where the weights themselves
-// do not (the row's heaviest keys have values of zero): they are computed from s - m - h then.
-constexpr float kDeep = -60.0f;
-// Beyond this |m| a score is rounded before m is taken off it: m is a rounded score then, and what one rounding
-// of the difference would keep is larger than the range of the weights.
-constexpr float kHuge = 1e6f;
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
-__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t &hi, uint32_t &lo) {
-    hi = pack_f16(x0, x1);
-    const float2 h = unpack_f16(hi);
-    lo = pack_f16(x0 - h.x, x1 - h.y);
-}
-__device__ __forceinline__ uint32_t codes2(uint32_t w, uint32_t sel) {
-    uint32_t r = __byte_perm(w, 0x64646464u, sel);
-    const uint32_t bias = 0x64806480u;  // 1152, 1152
-    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(bias));
-    return r;
-}
-__device__ __forceinline__ float limb_scale(float amax, float &inv) {  // as in the split kernel
-    const int e = (int)(__float_as_uint(amax) >> 23) & 0xFF;
-    const int f = min(max(264 - e, 1), 253);
-    inv = __uint_as_float((uint32_t)(254 - f) << 23);
-    return __uint_as_float((uint32_t)f << 23);
-}
 __device__ __forceinline__ float2 ffma2_of(float2 a, float2 b, float2 c) {
     ffma2(c, a, b);
     return c;
