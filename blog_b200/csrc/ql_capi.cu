@@ -1289,9 +1289,10 @@ size_t kv8_attn_workspace_bytes(int head_dim, int sms) {
 }
 // Split keys (mma.sync), or tiles of 256 rows on tcgen05: whichever should take less time.  The terms are fits (us)
 // of both kernels over 180 shapes of 1 and 8 sequences, 4 to 400 tokens each over 0 to 8192 earlier ones, 14/2/64,
-// 28/4/128 and 64/8/128 heads, f32 and bf16 (and 36 of 16/4/256, bf16); the choice they make costs 2 % over the
-// better of the two on average.  At the two ends: 4 tokens over 8192 (28/4/128, f32) split 17 us, tiles 50 us; 400
-// tokens over 8192 split 414 us, tiles 133 us.
+// 28/4/128 and 64/8/128 heads, f32 and bf16 (and 36 of 16/4/256, bf16); the choice they make costs 3.4 % over the
+// better of the two on average.  At the two ends: 4 tokens over 8192 (28/4/128, f32) split 18.6 us, tiles 50 us; 400
+// tokens over 8192 split 450 us, tiles 135 us.  Short prompts with nothing before them are underestimated for the split
+// kernel, which pays each group of 8 rows its start (8 x 48 tokens of 16/4/256: 65 us, tiles 20 us).
 bool kv8_prefers_prompt(int rows, int group, int kv_heads, int head_dim, int n_seqs, int max_q_len, int max_kv_len,
                         bool f32, int sms, int &cluster) {
     const double keys = std::max(1.0, (double)max_kv_len - max_q_len / 2.0), wide = head_dim / 128.0;

@@ -14,8 +14,10 @@
 // Every value is read once and written once, so the bound is HBM bandwidth for prompts and the launch for
 // single tokens: one launch holds both kinds of work (CTAs of query heads, a warp per row and head, and
 // CTAs of one block, KV head and operand, 4 rows per warp in registers until the block's maximum is known).
-// 4096 tokens of 28/4/128 heads in f32, 147 MB: 36 us, 4.1 TB/s.  8 chunks of up to 1500 tokens of 64/8/128 heads in
-// bf16, 347 MB: 128 us, 2.7 TB/s, the instructions of norm and rotation (half the bytes per value).  One token: 4.4 us.
+// With the read-back of the rows it touched: 4096 tokens of 28/4/128 heads in f32, 147 MB: 36 us, 4.1 TB/s (the append by
+// itself 31 us).  8 chunks of up to 1500 tokens of 64/8/128 heads in bf16, 347 MB: 128 us, 2.7 TB/s (111 us): two thirds of
+// the issue slots go to norm, rotation and conversion (half the bytes per value), the rest waits for loads and shuffles.
+// One token: 4.4 us.
 #include "ql_kv8.cuh"
 
 namespace ql {

@@ -25,7 +25,7 @@
 // the last to arrive, always in split order: the result does not depend on which that is.
 //
 // Bound: HBM for the codes (2 head_dim bytes per token and KV head) where the keys are many: 64 sequences of 4096 to
-// 8192 tokens, 64/8/128 heads, bf16, 681 MB in 121 us, 5.6 TB/s (0.87 of a copy's).  Below that the chain of one
+// 8192 tokens, 64/8/128 heads, bf16, 681 MB in 122 us, 5.6 TB/s (0.87 of a copy's).  Below that the chain of one
 // CTA's loads, products and merges: one sequence of 28/4/128 heads, f32, 17.6 us at 32768 tokens (1.9 TB/s) and
 // 7.6 us at 200.  Tiles of 8 rows and not of 16: a group of 7 or 8 heads fills them, and a single token has no more.
 #include <cooperative_groups.h>

@@ -22,12 +22,13 @@
 // Where the tiles of rows alone would leave SMs idle, the keys are split over the CTAs of a cluster, and their
 // sums are joined through distributed shared memory, each CTA finishing its share of the rows.
 //
-// Bound: the softmax threads (reading S, one exponential per row and key at 16 per clock and SM, weighing, writing
-// P), 3000 clocks per 64 keys of two tiles in bf16 and 5300 in f32, where the products take 1024 and 2048 of the
-// tensor cores: 28/4/128 heads, 8192 tokens in bf16 643 us (749 TFLOP/s of 4 head_dim flops per row and key, 0.45
-// of a library matrix product's), 2048 tokens in f32 100 us (301 TFLOP/s, twice that with both limbs).  Two row tiles,
-// so that one's products run under the other's softmax; tiles of 64 keys, so that S has two buffers (tiles of 128 with
-// one: 714 and 110 us).
+// Bound: the latency of the softmax threads (reading S, one exponential per row and key at 16 per clock and SM, weighing,
+// writing P): 3000 clocks per 64 keys of two tiles in bf16 and 5300 in f32, where the products take 1024 and 2048 of the
+// tensor cores.  Two softmax warps per scheduler do not hide their own chain: at 2048 tokens 47 to 49 % of the issue slots
+// are used, the tensor pipe 31 % (f32) and 23 % (bf16), the exponential unit 18 and 30 %.  28/4/128 heads, 8192 tokens in
+// bf16 640 us (751 TFLOP/s of 4 head_dim flops per row and key, 0.45 of a library matrix product's), 2048 tokens in f32
+// 99 us (304 TFLOP/s, twice that with both limbs).  Two row tiles, so that one's products run under the other's softmax;
+// tiles of 64 keys, so that S has two buffers (tiles of 128 with one: 714 and 110 us).
 #include <cooperative_groups.h>
 
 #include <algorithm>
