@@ -3,8 +3,9 @@ import numpy as np
 import pytest
 
 import blog_b200 as Q
-from gpu_util import dev, host
-from test_gpu_kv8 import Cache, _append, _check_cache, _i32
+import kv8_util as U
+from gpu_util import dev, host, rel_l2
+from test_gpu_kv8 import TOL, Cache, _append, _check_cache, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -108,4 +109,48 @@ def test_going_back_to_a_page_and_into_the_last_two(back):
     _append(c, "f32", dev(y), 0, None, _i32([back + 90]), _i32([0, 90]), 90)
     z = np.concatenate([x[:back], y]).reshape(back + 90, 2, kvh, hd).astype(np.float64)
     _check_cache(c, [z[:, 0]], [z[:, 1]], [back + 90], exact_bytes=True)
+    Q.check_device()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_pages_beyond_4_gb(t):
+    """Pages on both sides of the 2^32nd byte of the codes: append, read-back, and both kernels of the attention."""
+    import torch
+    nh, kvh, hd, n = 64, 8, 128, 700
+    pages = (1 << 32) // (kvh * 32 * hd) + 200
+    per = (n + 31) // 32
+    rng = np.random.default_rng(97)
+    table = np.stack([rng.permutation(400)[:per] + pages - 400, rng.permutation(per)]).astype(np.int32)
+    kc, vc = (torch.zeros((pages, kvh, 32, hd), dtype=torch.uint8, device="cuda:0") for _ in range(2))
+    ks, vs = (torch.zeros((pages, kvh), device="cuda:0") for _ in range(2))
+    ko, vo = (torch.zeros((2, 2, kvh, 32, hd), device="cuda:0") for _ in range(2))
+    td = dev(table)
+    cache = Q.kv8_cache(*(x.data_ptr() for x in (kc, vc, ks, vs, ko, vo, td)), None, pages, 2, 2, per, kvh, hd)
+    el, code = (4, Q.F32) if t == "f32" else (2, Q.BF16)
+    x = torch.randn((2 * n, (nh + 2 * kvh) * hd), device="cuda:0", generator=torch.Generator(device="cuda:0").manual_seed(98))
+    x = x.to(torch.float32 if t == "f32" else torch.bfloat16)
+    w, p = x.shape[1], x.data_ptr()
+    kv, st = _i32([n, n]), _i32([0, n, 2 * n])
+    Q.kv8_append(cache, code, None, 0, p + nh * hd * el, w, p + (nh + kvh) * hd * el, w, None, 0, 0, None, None, 1e-6, None, 0,
+                 0, kv.data_ptr(), st.data_ptr(), 2 * n, n)
+    back = [torch.zeros((2, n, kvh, hd), device="cuda:0") for _ in range(2)]
+    Q.kv8_gather(cache, Q.F32, back[0].data_ptr(), back[1].data_ptr(), None, n, kv.data_ptr())
+    k, v = (host(b).astype(np.float64) for b in back)
+    raw = host(x.float()).reshape(2, n, nh + 2 * kvh, hd)
+    for got, at in ((k, nh), (v, nh + kvh)):
+        assert np.abs(got - raw[:, :, at:at + kvh]).max() < np.abs(raw).max() / 250
+    ws = torch.zeros(Q.kv8_attend_workspace(nh, kvh, hd, 2, 2 * n, n, n), dtype=torch.uint8, device="cuda:0")
+    out = torch.zeros((2 * n, nh * hd), dtype=x.dtype, device="cuda:0")
+    for rows, form in ((2 * n, Q.KV8_FORM_TILES), (2, Q.KV8_FORM_SPLIT)):
+        q_len = rows // 2
+        Q.kv8_attend(cache, code, p, w, None, 0, out.data_ptr(), nh * hd, nh, hd ** -0.5, kv.data_ptr(),
+                     st.data_ptr() if q_len > 1 else None, rows, q_len, n, ws.data_ptr(), ws.numel())
+        assert Q.kv8_attend_form()[0] == form
+        got = host(out.float())
+        for s in range(2):
+            for i in (0, q_len // 2, q_len - 1):
+                row = s * q_len + i
+                q = raw.reshape(2 * n, -1, hd)[row, :nh]
+                want = U.attend(q, k[s].transpose(1, 0, 2), v[s].transpose(1, 0, 2), n - q_len + i, hd ** -0.5)
+                assert rel_l2(got[row], want.ravel()) < TOL[t], (form, s, i)
     Q.check_device()

@@ -371,3 +371,37 @@ def test_f32_scores_over_open_rows(hd):
     err = (np.log(p / (1 - p)) - s)[good]
     assert np.sqrt((err ** 2).mean()) < 2.0 ** -21 * np.sqrt((s[good] ** 2).mean())
     Q.check_device()
+
+
+@pytest.mark.parametrize("t,hd", WIDTHS)
+@pytest.mark.parametrize("tiles", [False, True])
+def test_queries_that_are_not_finite_and_a_scale_of_zero(t, hd, tiles):
+    """NaN and infinity in a head of a query reach that head of that row alone; a softmax scale of zero gives the mean."""
+    nh, kvh = 32, 2
+    lens, q_len = ([640, 607], [450, 400]) if tiles else ([640, 607], [3, 2])
+    c, stands = _filled(lens, 640, kvh, hd, seed=99)
+    q = np.random.default_rng(100).standard_normal((sum(q_len), nh, hd))
+    bad = [(1, 3, np.nan), (2, 31, np.inf), (q_len[0], 16, -np.inf)]
+    for row, h, x in bad:
+        q[row, h, 5] = x
+    qd, q = _dev(q.reshape(len(q), -1), t)
+    for row, h, x in bad:  # (as they are, whatever the rounding makes of them)
+        qd[row, h * hd + 5] = float(x)
+    for scale in (hd ** -0.5, 0.0):
+        got = _attend(c, t, qd, nh, _i32(lens), _i32(_starts(q_len)), max(q_len), 640, scale=scale).reshape(-1, nh, hd)
+        assert Q.kv8_attend_form()[0] == (Q.KV8_FORM_TILES if tiles else Q.KV8_FORM_SPLIT)
+        z = q.reshape(-1, nh, hd).copy()
+        for row, h, _ in bad:
+            assert np.isnan(got[row, h]).all(), (row, h)
+            got[row, h] = z[row, h] = 0
+        st = _starts(q_len)
+        for s in range(2):
+            want = U.attend_rows(z[st[s]:st[s + 1]], *stands[s], lens[s] - q_len[s], scale)
+            for i in range(0, q_len[s], 7 if tiles else 1):
+                for h in range(nh):
+                    if not any(r == st[s] + i and b == h for r, b, _ in bad):
+                        # (the mean of random values is small beside them: relative to these, too)
+                        v = stands[s][1][h // 16][:lens[s] - q_len[s] + i + 1]
+                        size = np.linalg.norm(want[i, h]) + (np.linalg.norm(np.abs(v).mean(0)) * 2.0 ** -9 if t == "bf16" else 0)
+                        assert np.linalg.norm(got[st[s] + i, h] - want[i, h]) < 2 * TOL[t] * size, (scale, s, i, h)
+    Q.check_device()
