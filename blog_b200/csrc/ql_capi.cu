@@ -1420,7 +1420,7 @@ int ql_kv8_attend(const ql_kv8_cache *cache, int32_t type, const void *q, int64_
         if (prompt) a.cluster = ctas, a.row_groups = (int)tiles;
         const cudaError_t e = prompt ? kv8_prompt_launch(a, type == QL_BF16, g_stream)
                                      : kv8_attn_launch(a, type == QL_BF16, g_stream);
-        ++t_launches;
+        t_launches += prompt ? (int)((tiles + kKvMaxTiles - 1) / kKvMaxTiles) : 1;
         if (e == cudaSuccess) {
             t_kv8_form = prompt ? QL_KV8_FORM_TILES : QL_KV8_FORM_SPLIT;
             t_kv8_ctas = prompt ? a.cluster : a.splits;

@@ -114,6 +114,7 @@ cudaError_t kv8_gather_launch(const Kv8View &c, const int *kv_len, const int *st
                               bool bf16, cudaStream_t s);
 cudaError_t kv8_attn_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s);
 // The tensor-core form for prompts (ql_kv8_prompt.cu).
+constexpr int kKvMaxTiles = 65535;            // tiles of rows of one launch (the grid's z)
 int kv8_prompt_rows(int head_dim, bool f32);  // rows per CTA, 0: not taken
 cudaError_t kv8_prompt_launch(const Kv8AttnArgs &a, bool bf16, cudaStream_t s);
 

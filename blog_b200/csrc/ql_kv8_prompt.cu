@@ -43,7 +43,6 @@ namespace ql {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kMaxGrid = 65535;  // of a grid's z
 constexpr int kKeys = 64;    // keys per tile: 2 blocks
 constexpr int kTileBlocks = kKeys / kKvBlock;
 // Tiles of 128 rows per CTA: two, or one where O takes 256 columns of TMEM.
@@ -1097,8 +1096,8 @@ cudaError_t launch_hd(const Kv8AttnArgs &a, cudaStream_t s) {
     // The tiles of rows lie in the grid's z, one launch but for calls of millions of rows.  (All in x, by divisions, the
     // 2048 tokens in f32 take 101.2 us and four chunks of narrow heads 79.3, so 99.5 and 78.1.)
     Kv8AttnArgs b = a;
-    for (b.tile0 = 0; b.tile0 < a.row_groups; b.tile0 += kMaxGrid) {
-        cfg.gridDim = dim3(a.c.kv_heads * a.cluster, a.c.n_seqs, std::min(a.row_groups - b.tile0, kMaxGrid));
+    for (b.tile0 = 0; b.tile0 < a.row_groups; b.tile0 += kKvMaxTiles) {
+        cfg.gridDim = dim3(a.c.kv_heads * a.cluster, a.c.n_seqs, std::min(a.row_groups - b.tile0, kKvMaxTiles));
         if ((e = cudaLaunchKernelEx(&cfg, prompt_kernel<T, HD>, b)) != cudaSuccess) return e;
     }
     return cudaSuccess;

@@ -327,6 +327,7 @@ def test_tiles_of_more_rows_than_a_grid_dimension():
     Q.kv8_attend(c.view, Q.BF16, q.data_ptr(), nh * hd, None, 0, out.data_ptr(), nh * hd, nh, hd ** -0.5, kv.data_ptr(),
                  st.data_ptr(), rows, rows, 300000, ws.data_ptr(), ws.numel())
     _tiles()
+    assert Q.last_launch_count() == 2
     torch.cuda.synchronize()
     assert not bool(out[:rows - n].any())
     got, qh = host(out[rows - n:].float()), host(q[rows - n:].float())
