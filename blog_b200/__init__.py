@@ -69,6 +69,8 @@ SIGNATURES = {
     "ql_kv8_attend_form": (I, [P]),
     "ql_kv8_gather": (I, [P, I32, P, P, P, I, P]),
     "ql_logits_apply": (I, [P, I64, P, I64, I, I, P, P, P, SZ]),
+    "ql_add_rms_norm": (I, [I32, P, I64, P, I64, P, I64, P, F, P, I64, P, I, I, I, I]),
+    "ql_moe_route": (I, [P, I64, P, P, I, I, I, P]),
     "ql_moe_swiglu_grouped": (I, [I32, P, P, SZ, SZ, SZ, SZ, P, I64, P, I, I, P, I, I, I, I]),
     "ql_moe_down_grouped_accum_ordered": (I, [I32, P, SZ, SZ, P, P, I, I, P, P, I64, I, I, I, I]),
     "ql_quant_embedding": (I, [I32, P, P, P, SZ, I, I]),
@@ -428,6 +430,34 @@ def logits_rules(history=None, history_stride=0, history_len=None, prompt_len=No
 def logits_apply(logits, logits_stride, out, out_stride, rows, vocab, rules, token, workspace, workspace_bytes):
     _call("ql_logits_apply", logits, logits_stride, out, out_stride, rows, vocab, C.byref(rules), token, workspace,
           workspace_bytes)
+
+
+Q8_NONE, Q8_ROWS, Q8_MMQ = 0, 1, 2
+
+
+def add_rms_norm(t, x, x_stride, residual, residual_stride, sum_, sum_stride, gamma, eps, y, y_stride, xq, layout,
+                 store_raw_sum, rows, hidden):
+    """Residual addition, RMS norm and its Q8_1 rows in one launch (see include/qlinear_b200.h)."""
+    _call("ql_add_rms_norm", t, x, x_stride, residual, residual_stride, sum_, sum_stride, gamma, eps, y, y_stride, xq,
+          layout, int(store_raw_sum), rows, hidden)
+
+
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+
+
+class MoeRouteRule(C.Structure):
+    """ql_moe_route_rule (include/qlinear_b200.h)."""
+    _fields_ = [("score", C.c_int32), ("bias", C.c_void_p), ("n_groups", C.c_int32), ("top_groups", C.c_int32),
+                ("group_best", C.c_int32), ("renormalise", C.c_int32), ("scale", C.c_float)]
+
+
+def moe_route_rule(score, bias=None, n_groups=1, top_groups=1, group_best=1, renormalise=False, scale=1.0):
+    return MoeRouteRule(score, bias, n_groups, top_groups, group_best, int(renormalise), scale)
+
+
+def moe_route(logits, logits_stride, idx, w, tokens, n_experts, k, rule):
+    """The k experts of each token and their weights (see include/qlinear_b200.h)."""
+    _call("ql_moe_route", logits, logits_stride, idx, w, tokens, n_experts, k, C.byref(rule))
 
 
 def moe_swiglu_grouped(t, gw, uw, geb, ueb, grb, urb, x, x_stride, ids, expert_begin, n_experts, act, tokens, k,

@@ -26,6 +26,8 @@
 #include "ql_attn.cuh"
 #include "ql_kv8.cuh"
 #include "ql_logits.cuh"
+#include "ql_norm.cuh"
+#include "ql_route.cuh"
 #include "ql_q81.cuh"
 
 namespace ql {
@@ -1502,6 +1504,79 @@ int ql_logits_apply(const float *logits, int64_t logits_stride, float *out, int6
         a.done = reinterpret_cast<unsigned *>(a.keys + rows);
         a.err = ws->err;
         const cudaError_t e = logits_launch(a, ws->sms, g_stream);
+        ++t_launches;
+        return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
+    });
+}
+
+// ---- residual, norm and 8-bit rows; choice of experts --------------------------------
+int ql_add_rms_norm(int32_t type, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, void *sum,
+                    int64_t sum_stride, const float *gamma, float eps, void *y, int64_t y_stride, uint8_t *xq, int layout,
+                    int store_raw_sum, int rows, int hidden) {
+    return guarded([&] {
+        const std::string what = "ql_add_rms_norm";
+        t_launches = 0;
+        if (type != QL_F32 && type != QL_BF16) return fail(QL_EINVAL, what + ": type must be QL_F32 or QL_BF16");
+        if (rows < 0 || hidden <= 0 || hidden > kNormMaxHidden)
+            return fail(QL_EINVAL, what + ": need rows >= 0 and 0 < hidden <= " + std::to_string(kNormMaxHidden));
+        if (!(eps >= 0.f)) return fail(QL_EINVAL, what + ": eps must not be negative");
+        if (layout != QL_Q8_NONE && layout != QL_Q8_ROWS && layout != QL_Q8_MMQ)
+            return fail(QL_EINVAL, what + ": layout must be QL_Q8_NONE, QL_Q8_ROWS or QL_Q8_MMQ");
+        if (rows == 0) return (int)QL_OK;
+        int st;
+        if ((st = kv8_operand(x, x_stride, hidden, type, "x", what))) return st;
+        if (residual && (st = kv8_operand(residual, residual_stride, hidden, type, "residual", what))) return st;
+        if (sum && (st = kv8_operand(sum, sum_stride, hidden, type, "sum", what))) return st;
+        if (y && (st = kv8_operand(y, y_stride, hidden, type, "y", what))) return st;
+        if ((sum && ((sum == x && sum_stride != x_stride) || (sum == residual && sum_stride != residual_stride))) ||
+            (y && ((y == x && y_stride != x_stride) || (y == residual && y_stride != residual_stride) || y == sum)))
+            return fail(QL_EINVAL, what + ": in place the strides are the same, and y is not sum");
+        if ((layout != QL_Q8_NONE) != (xq != nullptr)) return fail(QL_EINVAL, what + ": xq goes with a layout");
+        if (!on_words({gamma, xq})) return fail(QL_EINVAL, what + ": gamma and xq must be 4-byte aligned");
+        Workspace *ws = workspace(&st);
+        if (!ws) return st;
+        AddNormArgs a{};
+        a.x = x, a.residual = residual, a.sum = sum, a.y = y;
+        a.x_stride = x_stride, a.residual_stride = residual_stride, a.sum_stride = sum_stride, a.y_stride = y_stride;
+        a.gamma = gamma, a.xq = xq, a.eps = eps;
+        a.rows = rows, a.hidden = hidden;
+        a.mmq = layout == QL_Q8_MMQ, a.raw_sum = store_raw_sum != 0;
+        const cudaError_t e = add_norm_launch(a, type == QL_BF16, ws->sms, g_stream);
+        ++t_launches;
+        return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
+    });
+}
+
+int ql_moe_route(const float *logits, int64_t logits_stride, int32_t *top_idx, float *top_w, int tokens, int n_experts, int k,
+                 const ql_moe_route_rule *rule) {
+    return guarded([&] {
+        const std::string what = "ql_moe_route";
+        t_launches = 0;
+        if (!rule) return fail(QL_EINVAL, what + ": null rule");
+        if (tokens < 0 || n_experts <= 0 || n_experts > kRouteMaxExperts || k <= 0 || k > kRouteMaxTop || k > n_experts)
+            return fail(QL_EINVAL, what + ": need tokens >= 0, n_experts in 1..1024, k in 1..min(32, n_experts)");
+        if (rule->score != QL_ROUTE_SOFTMAX && rule->score != QL_ROUTE_SIGMOID)
+            return fail(QL_EINVAL, what + ": score must be QL_ROUTE_SOFTMAX or QL_ROUTE_SIGMOID");
+        if (rule->n_groups <= 0 || rule->n_groups > kRouteMaxGroups || n_experts % rule->n_groups || rule->top_groups <= 0 ||
+            rule->top_groups > rule->n_groups || (rule->group_best != 1 && rule->group_best != 2))
+            return fail(QL_EINVAL, what + ": need n_groups in 1..32 that divide n_experts, 1 <= top_groups <= n_groups, group_best 1 or 2");
+        if (!(std::fabs(rule->scale) <= 3.4e38f)) return fail(QL_EINVAL, what + ": scale must be finite");
+        if (tokens == 0) return (int)QL_OK;
+        if (!logits || !top_idx || !top_w) return fail(QL_EINVAL, what + ": null pointer");
+        if (logits_stride < n_experts) return fail(QL_EINVAL, what + ": logits_stride is below n_experts");
+        if (!on_words({logits, top_idx, top_w, rule->bias}))
+            return fail(QL_EINVAL, what + ": misaligned logits, top_idx, top_w or bias");
+        int st;
+        Workspace *ws = workspace(&st);
+        if (!ws) return st;
+        RouteArgs a{};
+        a.logits = logits, a.logits_stride = logits_stride, a.bias = rule->bias;
+        a.top_idx = top_idx, a.top_w = top_w;
+        a.tokens = tokens, a.n_experts = n_experts, a.k = k;
+        a.sigmoid = rule->score == QL_ROUTE_SIGMOID, a.renorm = rule->renormalise != 0;
+        a.n_groups = rule->n_groups, a.top_groups = rule->top_groups, a.group_best = rule->group_best;
+        a.scale = rule->scale;
+        const cudaError_t e = route_launch(a, ws->sms, g_stream);
         ++t_launches;
         return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
     });

@@ -385,6 +385,43 @@ QL_API int ql_logits_apply(const float *logits, int64_t logits_stride, float *ou
                            int vocab, const ql_logits_rules *rules, int32_t *token, void *workspace,
                            size_t workspace_bytes);
 
+/* ---- residual, norm and 8-bit rows (no reference twin as one launch; the reference adds, normalises and quantises in
+ *      three, kernel.cu:112-183, 1679-1765) ---------------------------------------------------------------------------
+ *   v = x + residual, rounded to `type` (residual == NULL: x);   y = v / sqrt(mean(v^2) + eps) * gamma
+ * type: QL_F32 or QL_BF16, of x, residual, sum and y; gamma f32 (NULL: 1).  sum receives v (NULL: not stored) and may be
+ * x or residual (same stride); y (NULL: not stored) x or residual.  Strides in elements, at least hidden.
+ * xq receives y (before its rounding to type) as Q8_1 rows: layout QL_Q8_ROWS, the bytes that ql_quantize_q8_1 gives
+ * for y, rows ql_q8_1_row_bytes(hidden) apart, or QL_Q8_MMQ, those of ql_quantize_q8_1_mmq; QL_Q8_NONE: xq unused.
+ * hidden: any up to 32768 (a last block of fewer than 32 is filled with zeros).  fp32 sums; one launch. */
+#define QL_Q8_NONE 0
+#define QL_Q8_ROWS 1
+#define QL_Q8_MMQ 2
+QL_API int ql_add_rms_norm(int32_t type, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                           void *sum, int64_t sum_stride, const float *gamma, float eps, void *y, int64_t y_stride,
+                           uint8_t *xq, int layout, int store_raw_sum, int rows, int hidden);
+
+/* ---- choice of experts (ql_moe_router_topk is the reference's: softmax, 64 experts) --------------------------------
+ *   s_e = softmax over the token's logits, or 1 / (1 + exp(-logit));   c_e = s_e + bias[e]
+ *   n_groups > 1: of n_groups groups of n_experts / n_groups consecutive experts the top_groups best stay, each
+ *   counted by the sum of its group_best (1 or 2) largest c;
+ *   the k experts of largest c in them, by descending c; equal ones by the lower id (groups likewise);
+ *   w_e = s_e [renormalise: / sum of the chosen s, 0 where that is 0] * scale   (the bias is not in the weights)
+ * c is compared as 64-bit scores (without a bias, logits); weights are f32 within 2^-18 of the token's largest score (with renormalise of
+ * 1) times scale.  A logit that is not finite counts as -inf; such an expert, or one with a bias of -inf or NaN, is never chosen, nor is a
+ * group of none but them.  Where fewer than k are left the rest of top_idx is -1 with weight 0 (the grouped experts
+ * skip those).  n_experts <= 1024, k <= 32, n_groups <= 32; tokens' rows of logits are logits_stride floats apart. */
+#define QL_ROUTE_SOFTMAX 0
+#define QL_ROUTE_SIGMOID 1
+typedef struct ql_moe_route_rule {
+    int32_t score;
+    const float *bias; /* device, [n_experts]; NULL: none */
+    int32_t n_groups, top_groups, group_best;
+    int32_t renormalise;
+    float scale;
+} ql_moe_route_rule;
+QL_API int ql_moe_route(const float *logits, int64_t logits_stride, int32_t *top_idx, float *top_w, int tokens,
+                        int n_experts, int k, const ql_moe_route_rule *rule);
+
 /* ---- opt-in int8 activation path, Q8_1 (reference kernel.cuh:47-52) -------------------
  * Changes numerics (activations rounded to int8 per 32), as in the reference, which keeps it off
  * by default (TensorTool.cpp:159-161).  Bytes of one Q8_1 row of in_dim activations (36 per 32). */
