@@ -71,6 +71,7 @@ SIGNATURES = {
     "ql_logits_apply": (I, [P, I64, P, I64, I, I, P, P, P, SZ]),
     "ql_add_rms_norm": (I, [I32, P, I64, P, I64, P, I64, P, F, P, I64, P, I, I, I, I]),
     "ql_moe_route": (I, [P, I64, P, P, I, I, I, P]),
+    "ql_lora_add": (I, [P, P, I64, P, I64, P, I64, P, I, P, I]),
     "ql_moe_swiglu_grouped": (I, [I32, P, P, SZ, SZ, SZ, SZ, P, I64, P, I, I, P, I, I, I, I]),
     "ql_moe_down_grouped_accum_ordered": (I, [I32, P, SZ, SZ, P, P, I, I, P, P, I64, I, I, I, I]),
     "ql_quant_embedding": (I, [I32, P, P, P, SZ, I, I]),
@@ -458,6 +459,28 @@ def moe_route_rule(score, bias=None, n_groups=1, top_groups=1, group_best=1, ren
 def moe_route(logits, logits_stride, idx, w, tokens, n_experts, k, rule):
     """The k experts of each token and their weights (see include/qlinear_b200.h)."""
     _call("ql_moe_route", logits, logits_stride, idx, w, tokens, n_experts, k, C.byref(rule))
+
+
+class LoraPool(C.Structure):
+    """ql_lora_pool (include/qlinear_b200.h): slots of low-rank adapters for one to three projections of one input."""
+    _fields_ = [("type", C.c_int32), ("n_proj", C.c_int32), ("a", C.c_void_p * 3), ("b", C.c_void_p * 3),
+                ("out_dim", C.c_int32 * 3), ("in_dim", C.c_int32), ("n_adapters", C.c_int32), ("max_rank", C.c_int32),
+                ("rank", C.c_void_p), ("scale", C.c_void_p)]
+
+
+def lora_pool(t, a, b, out_dims, in_dim, n_adapters, max_rank, rank=None, scale=None):
+    """a, b and out_dims are Python sequences, one entry per projection (<= 3)."""
+    if not len(a) == len(b) == len(out_dims) or len(a) > 3:
+        raise ValueError("a, b and out_dims have one entry per projection, at most 3")
+    pool = LoraPool(type=t, n_proj=len(a), in_dim=in_dim, n_adapters=n_adapters, max_rank=max_rank, rank=rank, scale=scale)
+    for i in range(len(a)):
+        pool.a[i], pool.b[i], pool.out_dim[i] = a[i], b[i], out_dims[i]
+    return pool
+
+
+def lora_add(pool, x, x_stride, base, base_stride, y, y_stride, adapter, n_seqs, q_start, rows):
+    """y = base + the rows' adapters applied to x (see include/qlinear_b200.h)."""
+    _call("ql_lora_add", C.byref(pool), x, x_stride, base, base_stride, y, y_stride, adapter, n_seqs, q_start, rows)
 
 
 def moe_swiglu_grouped(t, gw, uw, geb, ueb, grb, urb, x, x_stride, ids, expert_begin, n_experts, act, tokens, k,

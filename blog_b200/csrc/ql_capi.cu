@@ -26,6 +26,7 @@
 #include "ql_attn.cuh"
 #include "ql_kv8.cuh"
 #include "ql_logits.cuh"
+#include "ql_lora.cuh"
 #include "ql_norm.cuh"
 #include "ql_route.cuh"
 #include "ql_q81.cuh"
@@ -641,7 +642,8 @@ int ql_check_device(void) {
                                                 : h == kErrKvSlot     ? "a slot outside the KV cache's open rows"
                                                 : h == kErrKvLength   ? "more rows than the sequence has tokens, or than max_q_len"
                                                 : h == kErrKvPosition ? "a position past the rotation table"
-                                                                      : "a mask row outside the masks") +
+                                                : h == kErrMaskRow    ? "a mask row outside the masks"
+                                                                      : "an adapter outside the pool, or a rank above its slots") +
                                         " (device error code " + std::to_string(h) + ")");
         return fail(QL_EDEVICE, "a kernel gave up a bounded wait (device error code " + std::to_string(h) + ")");
     }
@@ -1577,6 +1579,69 @@ int ql_moe_route(const float *logits, int64_t logits_stride, int32_t *top_idx, f
         a.n_groups = rule->n_groups, a.top_groups = rule->top_groups, a.group_best = rule->group_best;
         a.scale = rule->scale;
         const cudaError_t e = route_launch(a, ws->sms, g_stream);
+        ++t_launches;
+        return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
+    });
+}
+
+// ---- low-rank adapters -----------------------------------------------------------------
+int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, const float *base, int64_t base_stride, float *y,
+                int64_t y_stride, const int32_t *adapter, int n_seqs, const int32_t *q_start, int rows) {
+    return guarded([&] {
+        const std::string what = "ql_lora_add";
+        t_launches = 0;
+        if (!pool) return fail(QL_EINVAL, what + ": null pool");
+        if (pool->type != QL_F32 && pool->type != QL_F16 && pool->type != QL_BF16)
+            return fail(QL_EINVAL, what + ": type must be QL_F32, QL_F16 or QL_BF16");
+        if (pool->n_proj <= 0 || pool->n_proj > kLoraMaxProj) return fail(QL_EINVAL, what + ": need n_proj in 1..3");
+        if (pool->in_dim <= 0 || pool->in_dim % 32) return fail(QL_EINVAL, what + ": in_dim must be a positive multiple of 32");
+        if (pool->max_rank <= 0 || pool->max_rank % 8 || pool->max_rank > kLoraMaxRank || pool->n_adapters < 0)
+            return fail(QL_EINVAL, what + ": max_rank must be a multiple of 8 up to 256, n_adapters not negative");
+        if (rows < 0 || n_seqs < 0 || (!q_start && rows != n_seqs))
+            return fail(QL_EINVAL, what + ": need rows, n_seqs >= 0, and rows == n_seqs without q_start");
+        LoraArgs a{};
+        int64_t width = 0;
+        for (int p = 0; p < pool->n_proj; ++p) {
+            if (pool->out_dim[p] <= 0 || (width += pool->out_dim[p]) > INT32_MAX / 2)
+                return fail(QL_EINVAL, what + ": out_dim must be positive");
+            a.a[p] = pool->a[p], a.b[p] = pool->b[p];
+            if ((a.a[p] == nullptr) != (a.b[p] == nullptr)) return fail(QL_EINVAL, what + ": a and b go together");
+            if (reinterpret_cast<uintptr_t>(a.a[p]) % 16 || reinterpret_cast<uintptr_t>(a.b[p]) % 16)
+                return fail(QL_EINVAL, what + ": a and b must be 16-byte aligned");
+            if (pool->n_adapters == 0) a.a[p] = a.b[p] = nullptr;
+            a.out[p] = pool->out_dim[p];
+            a.col[p] = (int)(width - pool->out_dim[p]);
+        }
+        if (rows == 0 || n_seqs == 0) return (int)QL_OK;
+        if (!adapter) return fail(QL_EINVAL, what + ": null adapter");
+        if (!on_words({adapter, q_start, pool->rank, pool->scale}))
+            return fail(QL_EINVAL, what + ": misaligned adapter, q_start, rank or scale");
+        int st;
+        if ((st = kv8_operand(x, x_stride, pool->in_dim, QL_F32, "x", what)) ||
+            (st = kv8_operand(y, y_stride, width, QL_F32, "y", what)))
+            return st;
+        if (base && (st = kv8_operand(base, base_stride, width, QL_F32, "base", what))) return st;
+        if (base == y && base_stride != y_stride) return fail(QL_EINVAL, what + ": in place the strides are the same");
+        if (x == y) return fail(QL_EINVAL, what + ": x and y must not overlap");
+        Workspace *ws = workspace(&st);
+        if (!ws) return st;
+        a.n_proj = pool->n_proj, a.in_dim = pool->in_dim, a.n_adapters = pool->n_adapters, a.max_rank = pool->max_rank;
+        a.rank = pool->rank, a.scale = pool->scale;
+        a.x = x, a.base = base, a.y = y;
+        a.x_stride = x_stride, a.base_stride = base_stride, a.y_stride = y_stride;
+        a.adapter = adapter, a.q_start = q_start;
+        a.n_seqs = n_seqs, a.rows = rows;
+        a.x_vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_stride % 4 == 0;
+        a.err = ws->err;
+        // Tiles: n rows of d adapters make at most (n + d (tm - 1)) / tm.
+        const int distinct = std::min(n_seqs, pool->n_adapters + 1), tm = lora_tile_rows(rows, distinct);
+        const int chunk = std::min(rows, kLoraChunk), chunks = (rows + kLoraChunk - 1) / kLoraChunk;
+        a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (tm - 1)) / tm);
+        const int64_t tiles = (int64_t)chunks * a.chunk_tiles;
+        a.cluster = 8;
+        while (a.cluster > 1 && tiles * a.n_proj * a.cluster > 4 * ws->sms) a.cluster /= 2;
+        if (tiles * a.cluster > INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
+        const cudaError_t e = lora_launch(a, pool->type == QL_F32 ? 0 : pool->type == QL_F16 ? 1 : 2, tm, g_stream);
         ++t_launches;
         return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
     });

@@ -63,7 +63,8 @@ enum DevErr : int {
     kErrKvSlot = 17,      // a slot outside the open rows
     kErrKvLength = 18,    // more rows in a call than the sequence holds tokens
     kErrKvPosition = 19,  // a position past the rotation table
-    kErrMaskRow = 20    // a mask row outside the masks
+    kErrMaskRow = 20,     // a mask row outside the masks
+    kErrAdapter = 21      // an adapter outside the pool, or a rank above the pool's
 };
 
 // ---------------------------------------------------------------------------

@@ -123,11 +123,11 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const __grid_constant__ 
         return ss;
     };
     float ss = squares(), eps = a.eps;
-    // squares outside fp32's range: the row once more times 2^-64 or 2^64 (beside an eps of 2^-60 or more the small ones
+    // squares outside fp32's range: the row once more times 2^-96 or 2^96 (beside an eps of 2^-66 or more the small ones
     // do not count); the norm takes the factor out again
-    const bool large = ss == INFINITY, small = ss < 0x1p-100f && eps < 0x1p-60f;
+    const bool large = ss == INFINITY, small = ss < 0x1p-100f && eps < 0x1p-66f;
     if (large || small) {
-        const float f = large ? 0x1p-64f : 0x1p64f;
+        const float f = large ? 0x1p-96f : 0x1p96f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll

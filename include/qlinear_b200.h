@@ -422,6 +422,34 @@ typedef struct ql_moe_route_rule {
 QL_API int ql_moe_route(const float *logits, int64_t logits_stride, int32_t *top_idx, float *top_w, int tokens,
                         int n_experts, int k, const ql_moe_route_rule *rule);
 
+/* ---- low-rank adapters beside a shared projection (no reference twin) ----------------------------------------------
+ * For rows x of many requests, each with its own adapter i of a pool, beside one to three projections of the same x
+ * whose outputs stand side by side in a row of y (q, k and v; gate and up):
+ *   h = scale[i] x A_i^T,   y = base + h B_i^T
+ * base is what the shared (quantised) projection gave; it may be y (same stride), or NULL for 0.  A row without an
+ * adapter gets y = base.  x and y must not overlap.
+ * The pool keeps n_adapters slots for each projection, of max_rank ranks; adapter i uses the first rank[i] of them
+ * (0: as none), what stands in the rest is not used.  type: QL_F16, QL_BF16 or QL_F32, of A and B.  in_dim: a
+ * multiple of 32; max_rank: a multiple of 8 up to 256; out_dim: any.  a and b start on 16 bytes; a pair that is NULL is
+ * a projection without adapters.  fp32 results: x, h and f32 weights enter the tensor cores as two tf32 limbs (22 bits),
+ * f16 and bf16 weights exactly, and sums are fp32. */
+typedef struct ql_lora_pool {
+    int32_t type, n_proj;
+    const void *a[3];    /* [n_adapters][max_rank][in_dim] */
+    const void *b[3];    /* [n_adapters][out_dim][max_rank] */
+    int32_t out_dim[3];  /* outputs of each projection; its first column of y is the sum of those before it */
+    int32_t in_dim, n_adapters, max_rank;
+    const int32_t *rank; /* device, [n_adapters]; NULL: max_rank */
+    const float *scale;  /* device, [n_adapters]; NULL: 1 */
+} ql_lora_pool;
+/* adapter: device, [n_seqs], the adapter of each sequence, < 0: none.  q_start == NULL: row s is the one row of sequence s
+ * (rows == n_seqs); otherwise sequence s has rows q_start[s] .. q_start[s + 1] - 1 (device, [n_seqs + 1], not falling; none is
+ * allowed), and rows before the first and behind the last sequence are left as they are.  Both are read on the device, so a
+ * captured CUDA graph follows them.  Rows of different sequences with one adapter share its weights.  An adapter outside the pool, or
+ * a rank outside 0 .. max_rank, counts as none and is reported by the next ql_check_device (QL_EDEVICE).  One launch. */
+QL_API int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, const float *base, int64_t base_stride,
+                       float *y, int64_t y_stride, const int32_t *adapter, int n_seqs, const int32_t *q_start, int rows);
+
 /* ---- opt-in int8 activation path, Q8_1 (reference kernel.cuh:47-52) -------------------
  * Changes numerics (activations rounded to int8 per 32), as in the reference, which keeps it off
  * by default (TensorTool.cpp:159-161).  Bytes of one Q8_1 row of in_dim activations (36 per 32). */

@@ -48,3 +48,32 @@ def test_route_rule(change):
 
 def test_route_of_no_tokens():
     Q.moe_route(None, 64, None, None, 0, 64, 4, Q.moe_route_rule(**RULE))
+
+
+LORA = dict(x=P, xs=64, base=P + 8192, bs=96, y=P + 65536, ys=96, ad=P, n=2, st=P, rows=5)
+POOL = dict(t=Q.F16, a=[P, None], b=[P, None], out_dims=[64, 32], in_dim=64, n_adapters=4, max_rank=16, rank=P, scale=P)
+
+
+@pytest.mark.parametrize("change", [dict(x=None), dict(y=None), dict(ad=None), dict(xs=63), dict(bs=95), dict(ys=95), dict(n=-1),
+                                    dict(rows=-1), dict(st=None), dict(x=P + 2), dict(y=P + 65537), dict(base=P + 2), dict(ad=P + 1),
+                                    dict(st=P + 2), dict(base=P + 65536, bs=97), dict(y=P)])
+def test_lora(change):
+    a = dict(LORA, **change)
+    _refused(Q.lora_add, Q.lora_pool(**POOL), *a.values())
+
+
+@pytest.mark.parametrize("change", [dict(t=Q.Q8_0), dict(t=5), dict(a=[], b=[], out_dims=[]), dict(a=[P, P]), dict(b=[P, P]),
+                                    dict(a=[P + 8, None]), dict(b=[P + 4, None]), dict(out_dims=[64, 0]), dict(out_dims=[-1, 97]),
+                                    dict(out_dims=[2 ** 31 - 1, 2 ** 31 - 1]), dict(in_dim=0), dict(in_dim=48), dict(in_dim=-32),
+                                    dict(n_adapters=-1), dict(max_rank=0), dict(max_rank=12), dict(max_rank=264), dict(rank=P + 2),
+                                    dict(scale=P + 1)])
+def test_lora_pool(change):
+    _refused(Q.lora_add, Q.lora_pool(**dict(POOL, **change)), *LORA.values())
+    with pytest.raises(ValueError):
+        Q.lora_pool(**dict(POOL, a=[P] * 4, b=[P] * 4, out_dims=[1] * 4))
+
+
+def test_lora_of_no_rows():
+    Q.lora_add(Q.lora_pool(**POOL), None, 64, None, 96, None, 96, None, 3, P, 0)
+    Q.lora_add(Q.lora_pool(**POOL), None, 64, None, 96, None, 96, None, 0, P, 7)
+    Q.lora_add(Q.lora_pool(**POOL), None, 64, None, 96, None, 96, None, 0, None, 0)
