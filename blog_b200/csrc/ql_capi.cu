@@ -1633,15 +1633,26 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
         a.n_seqs = n_seqs, a.rows = rows;
         a.x_vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_stride % 4 == 0;
         a.err = ws->err;
-        // Tiles: n rows of d adapters make at most (n + d (tm - 1)) / tm.
-        const int distinct = std::min(n_seqs, pool->n_adapters + 1), tm = lora_tile_rows(rows, distinct);
-        const int chunk = std::min(rows, kLoraChunk), chunks = (rows + kLoraChunk - 1) / kLoraChunk;
-        a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (tm - 1)) / tm);
-        const int64_t tiles = (int64_t)chunks * a.chunk_tiles;
-        a.cluster = 8;
-        while (a.cluster > 1 && tiles * a.n_proj * a.cluster > 4 * ws->sms) a.cluster /= 2;
-        if (tiles * a.cluster > INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
-        const cudaError_t e = lora_launch(a, pool->type == QL_F32 ? 0 : pool->type == QL_F16 ? 1 : 2, tm, g_stream);
+        const int type = pool->type == QL_F32 ? 0 : pool->type == QL_F16 ? 1 : 2;
+        const int distinct = std::min(n_seqs, pool->n_adapters + 1);
+        a.y_vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && y_stride % 4 == 0 &&
+                  (!base || (reinterpret_cast<uintptr_t>(base) % 16 == 0 && base_stride % 4 == 0));
+        for (int p = 0; p < a.n_proj; ++p) a.y_vec = a.y_vec && a.out[p] % 4 == 0;
+        cudaError_t e;
+        if (rows / distinct >= kLoraTileFrom && lora_tiles_plan(a, type, distinct, ws->sms)) {
+            if ((int64_t)rows * 8 > INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
+            e = lora_tiles_launch(a, type, g_stream);
+        } else {
+            // Tiles: n rows of d adapters make at most (n + d (tm - 1)) / tm.
+            const int tm = lora_tile_rows(rows, distinct);
+            const int chunk = std::min(rows, kLoraChunk), chunks = (rows + kLoraChunk - 1) / kLoraChunk;
+            a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (tm - 1)) / tm);
+            const int64_t tiles = (int64_t)chunks * a.chunk_tiles;
+            a.cluster = 8;
+            while (a.cluster > 1 && tiles * a.n_proj * a.cluster > 4 * ws->sms) a.cluster /= 2;
+            if (tiles * a.cluster > INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
+            e = lora_launch(a, type, tm, g_stream);
+        }
         ++t_launches;
         return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
     });

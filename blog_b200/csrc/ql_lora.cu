@@ -26,7 +26,6 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPass = 64;  // ranks that a warp sums at once
-enum { kW32, kW16, kWB16 };  // types of the weights
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -34,43 +33,6 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// v = hi + lo + less than 2^-22 |v|, both tf32.  (hi is cut off, so that it cannot overflow; the rest is exact.)
-__device__ __forceinline__ void limbs(float v, uint32_t &hi, uint32_t &lo) {
-    hi = __float_as_uint(v) & 0xFFFFE000u;
-    lo = (__float_as_uint(v - __uint_as_float(hi)) + 0x1000u) & 0xFFFFE000u;
-}
-
-template <int WT>
-struct Weight {
-    static constexpr int bytes = WT == kW32 ? 4 : 2;
-};
-// N consecutive weights as fp32 values (N = 2, 4, 8; the address a multiple of N elements).
-template <int WT, int N>
-__device__ __forceinline__ void load_weights(const void *p, int64_t at, uint32_t (&raw)[8]) {
-    const char *q = static_cast<const char *>(p) + at * Weight<WT>::bytes;
-    constexpr int words = N * Weight<WT>::bytes / 4;
-    if constexpr (words == 8) {
-        const uint4 u = reinterpret_cast<const uint4 *>(q)[0], v = reinterpret_cast<const uint4 *>(q)[1];
-        raw[0] = u.x, raw[1] = u.y, raw[2] = u.z, raw[3] = u.w, raw[4] = v.x, raw[5] = v.y, raw[6] = v.z, raw[7] = v.w;
-    } else if constexpr (words == 4) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(q);
-        raw[0] = u.x, raw[1] = u.y, raw[2] = u.z, raw[3] = u.w;
-    } else if constexpr (words == 2) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(q);
-        raw[0] = u.x, raw[1] = u.y;
-    } else {
-        raw[0] = *reinterpret_cast<const uint32_t *>(q);
-    }
-}
-// Weight i of them.
-template <int WT>
-__device__ __forceinline__ float weight(const uint32_t (&raw)[8], int i) {
-    if (WT == kW32) return __uint_as_float(raw[i]);
-    const uint32_t w = raw[i / 2];
-    if (WT == kWB16) return __uint_as_float(i % 2 ? w & 0xFFFF0000u : w << 16);
-    return half_bits_to_float(i % 2 ? w >> 16 : w);
-}
-
 // A fragment of 16 rows x 8: elements 2 j and 2 j + 1 of the rows g and g + 8, and their second limbs.
 template <int WT>
 __device__ __forceinline__ void fragment(const uint32_t (&r0)[8], const uint32_t (&r1)[8], int j, uint32_t (&hi)[4],
@@ -86,94 +48,9 @@ __device__ __forceinline__ void fragment(const uint32_t (&r0)[8], const uint32_t
     }
 }
 
-// The tile that a cluster works on.
-struct Tile {
-    int id, first, n;  // adapter (< 0: none), place of its first row among the adapter's, rows
-};
-
-// Finds tile `t` of the rows r0 .. r0 + n: rows of equal adapters in order, tm at a time, tiles in the order of their
-// first rows.  list receives the rows; every thread returns the same tile (n = 0: there are fewer).
-__device__ Tile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, int *ids, int *list, int *box) {
-    const int tid = threadIdx.x;
-    constexpr int kNone = -1, kOutside = -2;  // of no adapter; of no sequence: left as it is
-    constexpr int kPer = kLoraChunk / kThreads;
-    int id[kPer], place[kPer];
-#pragma unroll
-    for (int h = 0; h < kPer; ++h) {
-        const int i = h * kThreads + tid;
-        id[h] = kOutside;
-        if (i < n) {
-            int s = r0 + i;
-            if (a.q_start != nullptr) {  // the last sequence that starts at or before the row
-                int lo = 0, hi = a.n_seqs + 1;
-                while (lo < hi) {
-                    const int mid = (lo + hi) / 2;
-                    if (a.q_start[mid] <= r0 + i)
-                        lo = mid + 1;
-                    else
-                        hi = mid;
-                }
-                s = lo - 1;
-            }
-            if (s >= 0 && s < a.n_seqs) {
-                id[h] = a.adapter[s];
-                if (id[h] >= a.n_adapters) {
-                    atomicExch(a.err, kErrAdapter);
-                    id[h] = kNone;
-                }
-                id[h] = max(id[h], kNone);
-            }
-        }
-        ids[i] = id[h];
-    }
-    if (tid < tm) list[tid] = -1;
-    if (tid == 0) box[0] = 0, box[1] = 0, box[2] = 0;  // rows, adapter, place
-    __syncthreads();
-    __shared__ int leaders[kPer * kWarps];
-    unsigned before[kPer];
-    bool leads[kPer];
-#pragma unroll
-    for (int h = 0; h < kPer; ++h) {
-        const int i = h * kThreads + tid;
-        place[h] = 0;
-        if (id[h] > kOutside) {
-            for (int j = 0; j + 4 <= i; j += 4) {
-                const int4 v = *reinterpret_cast<const int4 *>(ids + j);
-                place[h] += (v.x == id[h]) + (v.y == id[h]) + (v.z == id[h]) + (v.w == id[h]);
-            }
-            for (int j = i & ~3; j < i; ++j) place[h] += ids[j] == id[h];
-        }
-        leads[h] = id[h] > kOutside && place[h] % tm == 0;
-        const unsigned m = __ballot_sync(0xffffffffu, leads[h]);
-        before[h] = __popc(m & ((1u << (tid % 32)) - 1));
-        if (tid % 32 == 0) leaders[h * kWarps + tid / 32] = __popc(m);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < kPer; ++h) {
-        int k = before[h];
-        for (int w = 0; w < h * kWarps + tid / 32; ++w) k += leaders[w];
-        if (leads[h] && k == t) box[0] = 1, box[1] = id[h], box[2] = place[h];
-    }
-    __syncthreads();
-    const Tile found{box[1], box[2], box[0]};
-    __syncthreads();
-    if (found.n == 0) return found;
-#pragma unroll
-    for (int h = 0; h < kPer; ++h) {
-        const int k = place[h] - found.first;
-        if (id[h] == found.id && k >= 0 && k < tm) {
-            list[k] = r0 + h * kThreads + tid;
-            atomicMax(box, k + 1);
-        }
-    }
-    __syncthreads();
-    return Tile{found.id, found.first, box[0]};
-}
-
 // KU: ranks per step of the second product (8, 16 or 32): a lane has KU / 4 consecutive ranks.
 template <int WT, int NT, int KU>
-__device__ __forceinline__ void expand(const LoraArgs &a, const Tile &tile, int proj, int rank, int part, int parts,
+__device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, int proj, int rank, int part, int parts,
                                        const int *list, const float *hi, const float *lo, int pitch) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int n_out = a.out[proj];
@@ -253,7 +130,7 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
     const int parts = a.cluster, part = blockIdx.x % parts, proj = blockIdx.y;
     const int tile_no = blockIdx.x / parts, r0 = tile_no / a.chunk_tiles * kLoraChunk;
-    const Tile tile = find_tile(a, tile_no % a.chunk_tiles, r0, min(kLoraChunk, a.rows - r0), TM, ids, list, box);
+    const LoraTile tile = find_tile<kThreads>(a, tile_no % a.chunk_tiles, r0, min(kLoraChunk, a.rows - r0), TM, ids, list, box);
     if (tile.n == 0) return;  // (every CTA of the cluster)
     int rank = 0;
     if (tile.id >= 0 && a.a[proj] != nullptr) {

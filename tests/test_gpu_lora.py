@@ -264,3 +264,23 @@ def test_replay_follows_the_device(lens):
     c.y.zero_()
     c.check()
     assert torch.equal(once, c.y) and Q.last_launch_count() == 1
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("n_in,outs,max_rank,lens", [
+    (32, (64,), 16, [128]), (64, (4,), 8, [130]), (96, (64, 64, 64), 64, [200, 70]), (896, (896, 128, 128), 64, [1000, 333]),
+    (3584, (512,), 128, [513]), (1024, (260, 68), 96, [600, 64]), (512, (260, 68), 104, [300]), (2048, (1024,), 192, [257]),
+    (8192, (8192, 1024, 1024), 64, [128]), (640, (128, 100, 36), 40, [90, 0, 51, 700, 128, 1]), (128, (64,), 256, [300]),
+    (4128, (192, 64), 16, [5000])])
+def test_long_prompts(type_, n_in, outs, max_rank, lens):
+    """Tiles of 128 rows, their clusters, ranks side by side, and those that go one projection at a time."""
+    adapter = [i % 2 for i in range(len(lens))]
+    far = Case(type_, n_in, outs, adapter, lens=lens, max_rank=max_rank, ranks=[max_rank, max(1, max_rank - 11)], n_adapters=2,
+               gap=5, seed=n_in).check()
+    assert far < 1e-6, far
+
+
+def test_long_prompts_some_without():
+    for base in ("other", "same", "none"):
+        for without in ((), (0,), (1,), (0, 2), (0, 1, 2)):
+            Case(Q.BF16, 256, (132, 64, 200), [0, -1, 1], lens=[200, 150, 90], base=base, without=without, ranks=[16, 0], gap=1).check()
