@@ -1585,6 +1585,21 @@ int ql_moe_route(const float *logits, int64_t logits_stride, int32_t *top_idx, f
 }
 
 // ---- low-rank adapters -----------------------------------------------------------------
+namespace {
+// Rows of `width` floats, `stride` apart, in boxes of 32 x 32 with the 128-byte swizzle.  (Encoded for the call: it is
+// the caller's address.)
+bool f32_rows_map(CUtensorMap *out, const float *base, int64_t width, int64_t rows, int64_t stride) {
+    auto enc = tensor_map_encoder();
+    if (enc == nullptr || stride >= (int64_t(1) << 38)) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)stride * 4};
+    const cuuint32_t box[2] = {32, 32}, estr[2] = {1, 1};
+    return enc(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float *>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+}  // namespace
+
 int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, const float *base, int64_t base_stride, float *y,
                 int64_t y_stride, const int32_t *adapter, int n_seqs, const int32_t *q_start, int rows) {
     return guarded([&] {
@@ -1639,9 +1654,11 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
                   (!base || (reinterpret_cast<uintptr_t>(base) % 16 == 0 && base_stride % 4 == 0));
         for (int p = 0; p < a.n_proj; ++p) a.y_vec = a.y_vec && a.out[p] % 4 == 0;
         cudaError_t e;
-        if (rows / distinct >= kLoraTileFrom && lora_tiles_plan(a, type, distinct, ws->sms)) {
-            if ((int64_t)rows * 8 > INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
-            e = lora_tiles_launch(a, type, g_stream);
+        LoraMaps maps;
+        if (rows / distinct >= kLoraTileFrom && rows <= INT32_MAX / 8 && lora_tiles_plan(a, type, distinct, ws->sms) &&
+            f32_rows_map(&maps.x, x, pool->in_dim, rows, x_stride) && f32_rows_map(&maps.y, y, width, rows, y_stride) &&
+            f32_rows_map(&maps.base, base ? base : y, width, rows, base ? base_stride : y_stride)) {
+            e = lora_tiles_launch(a, maps, type, g_stream);
         } else {
             // Tiles: n rows of d adapters make at most (n + d (tm - 1)) / tm.
             const int tm = lora_tile_rows(rows, distinct);

@@ -125,12 +125,12 @@ template <int WT, int NT>
 __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ LoraArgs a) {
     constexpr int TM = 8 * NT, MT = kPass / 16;
     extern __shared__ __align__(16) float smem[];
-    __shared__ __align__(16) int ids[kLoraChunk];
-    __shared__ int list[TM], box[3];
+    __shared__ LoraFind find;
+    __shared__ int list[TM];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
     const int parts = a.cluster, part = blockIdx.x % parts, proj = blockIdx.y;
     const int tile_no = blockIdx.x / parts, r0 = tile_no / a.chunk_tiles * kLoraChunk;
-    const LoraTile tile = find_tile<kThreads>(a, tile_no % a.chunk_tiles, r0, min(kLoraChunk, a.rows - r0), TM, ids, list, box);
+    const LoraTile tile = find_tile<kThreads>(a, tile_no % a.chunk_tiles, r0, min(kLoraChunk, a.rows - r0), TM, find, list);
     if (tile.n == 0) return;  // (every CTA of the cluster)
     int rank = 0;
     if (tile.id >= 0 && a.a[proj] != nullptr) {

@@ -1,5 +1,7 @@
 // Low-rank adapters beside a shared projection (ql_lora.cu): launch arguments.
 #pragma once
+#include <cuda.h>
+
 #include "ql_common.cuh"
 
 namespace ql {
@@ -26,8 +28,13 @@ struct LoraArgs {
     // tiles on tcgen05 only:
     bool y_vec;       // base, y and every projection's columns start on 16 bytes, whole groups of 4
     bool split;       // a projection per blockIdx.y, not all in one
-    int ring, ring_bytes;  // stages of widened weights
+    int ring, ring_bytes, raw_bytes;  // stages of widened weights, and of weights on their way
     int *err;
+};
+
+// x, base and y as rows of f32, in boxes of 32 columns and 32 rows (base: y's where there is none).
+struct LoraMaps {
+    CUtensorMap x, base, y;
 };
 
 enum { kW32, kW16, kWB16 };  // types of the weights
@@ -74,17 +81,36 @@ struct LoraTile {
     int id, first, n;  // adapter (< 0: none), place of its first row among the adapter's, rows
 };
 
+// What find_tile needs of shared memory.
+struct LoraFind {
+    int starts[kLoraChunk + 1], adapters[kLoraChunk];  // of the sequences, where there are no more
+    int2 kinds[kLoraChunk];                            // per warp: adapters and how many of its rows have them
+    int n_kinds[kLoraChunk / 32], leaders[kLoraChunk / 32];
+    int found[3];
+};
+
 // Finds tile t of the rows r0 .. r0 + n: rows of equal adapters in order, tm at a time, tiles in the order of their
 // first rows.  list receives the rows; every thread returns the same tile (n = 0: there are fewer).
 template <int THREADS>
-__device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, int *ids, int *list, int *box) {
-    const int tid = threadIdx.x;
+__device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, LoraFind &f, int *list) {
+    const int tid = threadIdx.x, lane = tid % 32;
     constexpr int kNone = -1, kOutside = -2;  // of no adapter; of no sequence: left as it is
-    constexpr int kPer = kLoraChunk / THREADS;
+    constexpr int kPer = kLoraChunk / THREADS, kWarps = THREADS / 32;
+    const bool staged = a.q_start != nullptr && a.n_seqs <= kLoraChunk;
+    if (staged)
+        for (int i = tid; i <= a.n_seqs; i += THREADS) {
+            f.starts[i] = a.q_start[i];
+            if (i < a.n_seqs) f.adapters[i] = a.adapter[i];
+        }
+    for (int i = tid; i < tm; i += THREADS) list[i] = -1;
+    if (tid < 3) f.found[tid] = 0;
+    __syncthreads();
     int id[kPer], place[kPer];
+    bool leads[kPer];
+    unsigned same[kPer];
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
-        const int i = h * THREADS + tid;
+        const int i = h * THREADS + tid, w = h * kWarps + tid / 32;
         id[h] = kOutside;
         if (i < n) {
             int s = r0 + i;
@@ -92,7 +118,7 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, i
                 int lo = 0, hi = a.n_seqs + 1;
                 while (lo < hi) {
                     const int mid = (lo + hi) / 2;
-                    if (a.q_start[mid] <= r0 + i)
+                    if ((staged ? f.starts[mid] : a.q_start[mid]) <= r0 + i)
                         lo = mid + 1;
                     else
                         hi = mid;
@@ -100,7 +126,7 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, i
                 s = lo - 1;
             }
             if (s >= 0 && s < a.n_seqs) {
-                id[h] = a.adapter[s];
+                id[h] = staged ? f.adapters[s] : a.adapter[s];
                 if (id[h] >= a.n_adapters) {
                     atomicExch(a.err, kErrAdapter);
                     id[h] = kNone;
@@ -108,39 +134,55 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, i
                 id[h] = max(id[h], kNone);
             }
         }
-        ids[i] = id[h];
+        // the warp's adapters, each with its rows: their lowest lanes write them down
+        same[h] = __match_any_sync(0xffffffffu, id[h]);
+        const unsigned firsts = __ballot_sync(0xffffffffu, __ffs(same[h]) - 1 == lane);
+        place[h] = __popc(same[h] & ((1u << lane) - 1));
+        if (__ffs(same[h]) - 1 == lane) f.kinds[w * 32 + __popc(firsts & ((1u << lane) - 1))] = make_int2(id[h], __popc(same[h]));
+        if (lane == 0) f.n_kinds[w] = __popc(firsts);
     }
-    if (tid < tm) list[tid] = -1;
-    if (tid == 0) box[0] = 0, box[1] = 0, box[2] = 0;  // rows, adapter, place
     __syncthreads();
-    __shared__ int leaders[kPer * (THREADS / 32)];
-    unsigned before[kPer];
-    bool leads[kPer];
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
-        const int i = h * THREADS + tid;
-        place[h] = 0;
-        if (id[h] > kOutside) {
-            for (int j = 0; j + 4 <= i; j += 4) {
-                const int4 v = *reinterpret_cast<const int4 *>(ids + j);
-                place[h] += (v.x == id[h]) + (v.y == id[h]) + (v.z == id[h]) + (v.w == id[h]);
+        const int w = h * kWarps + tid / 32, first = __ffs(same[h]) - 1;
+        int before = 0;  // rows of this adapter in the warps before
+        const unsigned firsts = __ballot_sync(0xffffffffu, first == lane && id[h] != kOutside);
+        if (__popc(firsts) <= 4) {  // few kinds: a lane looks through a warp's
+            for (unsigned left = firsts; left != 0; left &= left - 1) {
+                const int kind = __shfl_sync(0xffffffffu, id[h], __ffs(left) - 1);
+                int n_before = 0;
+                if (lane < w)
+                    for (int k = 0; k < f.n_kinds[lane]; ++k) {
+                        const int2 v = f.kinds[lane * 32 + k];
+                        if (v.x == kind) n_before = v.y;
+                    }
+                n_before = __reduce_add_sync(0xffffffffu, n_before);
+                if (id[h] == kind) before = n_before;
             }
-            for (int j = i & ~3; j < i; ++j) place[h] += ids[j] == id[h];
+        } else {  // the lowest lane of each looks through all
+            if (first == lane && id[h] != kOutside)
+                for (int v = 0; v < w; ++v)
+                    for (int k = 0; k < f.n_kinds[v]; ++k) {
+                        const int2 kind = f.kinds[v * 32 + k];
+                        if (kind.x == id[h]) before += kind.y;
+                    }
+            before = __shfl_sync(0xffffffffu, before, first);
         }
-        leads[h] = id[h] > kOutside && place[h] % tm == 0;
+        place[h] += before;
+        leads[h] = id[h] != kOutside && place[h] % tm == 0;
         const unsigned m = __ballot_sync(0xffffffffu, leads[h]);
-        before[h] = __popc(m & ((1u << (tid % 32)) - 1));
-        if (tid % 32 == 0) leaders[h * (THREADS / 32) + tid / 32] = __popc(m);
+        same[h] = __popc(m & ((1u << lane) - 1));  // (from here: leaders before this one in its warp)
+        if (lane == 0) f.leaders[w] = __popc(m);
     }
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
-        int k = before[h];
-        for (int w = 0; w < h * (THREADS / 32) + tid / 32; ++w) k += leaders[w];
-        if (leads[h] && k == t) box[0] = 1, box[1] = id[h], box[2] = place[h];
+        const int w = h * kWarps + tid / 32;
+        const int k = (int)same[h] + __reduce_add_sync(0xffffffffu, lane < w ? f.leaders[lane] : 0);
+        if (leads[h] && k == t) f.found[0] = 1, f.found[1] = id[h], f.found[2] = place[h];
     }
     __syncthreads();
-    const LoraTile found{box[1], box[2], box[0]};
+    const LoraTile found{f.found[1], f.found[2], f.found[0]};
     __syncthreads();
     if (found.n == 0) return found;
 #pragma unroll
@@ -148,11 +190,11 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, i
         const int k = place[h] - found.first;
         if (id[h] == found.id && k >= 0 && k < tm) {
             list[k] = r0 + h * THREADS + tid;
-            atomicMax(box, k + 1);
+            atomicMax(f.found, k + 1);
         }
     }
     __syncthreads();
-    return LoraTile{found.id, found.first, box[0]};
+    return LoraTile{found.id, found.first, f.found[0]};
 }
 
 // Rows of a tile, by the rows of the call.
@@ -160,6 +202,6 @@ int lora_tile_rows(int rows, int n_seqs);
 cudaError_t lora_launch(const LoraArgs &a, int type, int tile_rows, cudaStream_t s);
 // Tiles of 128 rows: fills in what the launch needs; false: not for these sizes or this alignment.
 bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms);
-cudaError_t lora_tiles_launch(const LoraArgs &a, int type, cudaStream_t s);
+cudaError_t lora_tiles_launch(const LoraArgs &a, const LoraMaps &maps, int type, cudaStream_t s);
 
 }  // namespace ql

@@ -29,16 +29,16 @@ namespace {
 
 constexpr int kThreads = 512, kRowWarps = 8;
 constexpr int kTile = kLoraTile, kDepth = 4;   // rows; blocks of a warp in flight and in use
-constexpr int kGroup = 2;                      // blocks of 32 columns between two sums in registers
 constexpr int kSlice = 64;                     // outputs of one product
 constexpr int kSlot = 32 * 128;                // bytes of a warp's block: 32 rows of 32 values
-constexpr int kMaxRing = 4;                    // stages of widened weights
+constexpr int kMaxRing = 4, kRaw = 4;          // stages of widened weights, and of weights on their way
 constexpr uint32_t kLimbs = 384;               // TMEM columns: h's two accumulators of up to 192, then x's limbs twice
 // Registers per thread of the roles; 16 warps launch with 128 each.
-constexpr int kRowRegs = 168, kOtherRegs = 88;
+constexpr int kRowRegs = 184, kOtherRegs = 72;
 static_assert(2 * kRowRegs + 2 * kOtherRegs == 4 * 128, "the block's registers at launch");
 
 struct Bars {
+    uint64_t land[kRowWarps][kDepth];          // a warp's blocks from memory
     uint64_t x_full[2], x_empty[2];            // x's limbs, by parity of the block
     uint64_t w_full[kMaxRing], w_empty[kMaxRing];
     uint64_t sum_full[2], sum_empty[2];        // h's accumulators
@@ -119,18 +119,23 @@ __device__ __forceinline__ void reg_inc() {
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_2d(const void *map, int c0, int c1, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(c0), "r"(c1), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
 template <int N>
-__device__ __forceinline__ void copies_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void stores_read() {  // all but the last N have read their shared memory
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float remote(uint32_t addr, uint32_t rank) {  // a word of another CTA's shared memory
+__device__ __forceinline__ float4 remote(uint32_t addr, uint32_t rank) {  // of another CTA's shared memory
     uint32_t r;
-    float v;
+    float4 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(r) : "memory");
     return v;
 }
 
@@ -149,15 +154,16 @@ __device__ __forceinline__ Slice slice_of(const LoraArgs &a, int p0, int np, int
 }
 
 template <int WT>
-__global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_constant__ LoraArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraMaps maps) {
     constexpr int LW = WT == kW32 ? 2 : 1;  // limbs of a weight
+    constexpr int kGroup = 4 / LW;          // blocks of 32 columns between two sums in registers
     extern __shared__ uint8_t sm_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t *ring = sm;                                              // [kRowWarps][kDepth][kSlot]
+    uint8_t *ring = sm;                                              // [kDepth][kRowWarps][kSlot]
     uint8_t *weights = sm + kRowWarps * kDepth * kSlot;              // [a.ring][a.ring_bytes]
-    float *shares = reinterpret_cast<float *>(sm);                   // [ranks][kTile], between the two products
+    float *shares = reinterpret_cast<float *>(sm);                   // [kTile][ranks], between the two products
     __shared__ Bars b;
-    __shared__ int list[kTile], box[3];
+    __shared__ int list[kTile];
     auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
     const int warp = uni(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int parts = a.cluster, part = blockIdx.x % parts;
@@ -165,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     const int chunks = (a.rows + kLoraChunk - 1) / kLoraChunk, tile_no = blockIdx.x / parts;
     const int r0 = tile_no % chunks * kLoraChunk;
     const LoraTile tile = find_tile<kThreads>(a, tile_no / chunks, r0, min(kLoraChunk, a.rows - r0), kTile,
-                                              reinterpret_cast<int *>(sm), list, box);
+                                              *reinterpret_cast<LoraFind *>(sm), list);
     if (tile.n == 0) return;  // (every CTA of the cluster)
     int rank = 0;
     if (tile.id >= 0) {
@@ -194,6 +200,11 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     const int bufs = 2 * R + 4 * kSlice <= 512 ? 2 : 1;
     auto out_at = [](int buf) { return 512u - 2 * kSlice * (buf + 1); };
 
+    // a row warp's rows: how many there are, and whether they lie together
+    const int q32 = (warp & 3) * 32, live = warp < kRowWarps ? max(0, min(32, tile.n - q32)) : 0;
+    const int row0 = live > 0 ? uni(list[q32]) : 0;
+    const bool together = live > 0 && uni(list[q32 + live - 1]) - row0 == live - 1;
+    if (live > 0 && lane < kDepth) mbar_init(&b.land[warp][lane], together ? 1 : 32);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b.x_full[i], 4), mbar_init(&b.x_empty[i], 1);
@@ -203,8 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         for (int i = 0; i < kMaxRing; ++i) mbar_init(&b.w_full[i], 4), mbar_init(&b.w_empty[i], 1);
         mbar_init(&b.h_full, kRowWarps);
         b.abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 12) tmem_alloc(&b.tmem, 512);
     tc_fence_before();
     __syncthreads();
@@ -230,29 +241,73 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         // ------------------------------------ rows: a thread per row and parity ------------------------------------
         reg_inc<kRowRegs>();
         const int q = warp & 3, wg = warp >> 2;
-        uint8_t *mine = ring + warp * kDepth * kSlot;
-        const uint32_t mine32 = smem_u32(mine);
+        uint8_t *mine = ring + warp * kSlot;  // (its slots kRowWarps * kSlot apart)
         const uint32_t lanes = (uint32_t)(32 * q) << 16;
-        int row_of[8];  // the rows that this lane copies: 8 lanes a row of 128 bytes
-#pragma unroll
-        for (int it = 0; it < 8; ++it) row_of[it] = 32 * q + 4 * it + lane / 8 < tile.n ? list[32 * q + 4 * it + lane / 8] : -1;
         auto place = [&](int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) * 16)); };
+        auto slot_of = [&](int m) { return mine + (m % kDepth) * (kRowWarps * kSlot); };
+        int issued = 0, used = 0;  // blocks asked for, and taken
+        // 32 columns of this warp's rows into the next slot: one tiled copy where the rows lie together (in rows that are
+        // another sequence's, too), 16 bytes per lane elsewhere
+        auto fetch = [&](const CUtensorMap &map, const float *from, int64_t stride, int col, int width) {
+            if (live > 0) {
+                uint64_t *bar = &b.land[warp][issued % kDepth];
+                const uint32_t dst = smem_u32(slot_of(issued));
+                if (together) {
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(bar, kSlot);
+                        tma_box2d(slot_of(issued), &map, col, row0, bar);
+                    }
+                } else {
+                    const int c = (lane & 7) * 4;
+#pragma unroll
+                    for (int it = 0; it < 8; ++it) {
+                        const int r = 4 * it + lane / 8;
+                        if (r < live && c < width) copy16(dst + place(r, lane & 7), from + list[32 * q + r] * stride + col + c);
+                    }
+                    cp_async_mbar_arrive(bar);
+                }
+            }
+            ++issued;
+        };
+        auto landed = [&](int m) {
+            return live == 0 || __all_sync(0xffffffffu, wait(&b.land[warp][m % kDepth], m / kDepth));
+        };
         bool ok = true;
+        // the first of 64 outputs, this warp's 32 of them, and whether there are any
+        auto outputs = [&](int j, Slice &s, int &col, int &width) {
+            s = slice_of(a, p0, np, j);
+            width = min(32, a.out[s.p] - s.o0 - 32 * wg);
+            col = a.col[s.p] + s.o0 + 32 * wg;
+            return width > 0;
+        };
+        int asked = j0;  // outputs whose base has been asked for
+        int taken = 0;   // slots that the shares of h stand in, until they are read by all (the cluster's second barrier)
+        auto free_slots = [&] {
+            if (taken == 0) return;
+            taken = 0;
+            cluster_wait();
+            fence_proxy_async_smem();
+        };
+        auto fetch_base = [&] {
+            Slice s;
+            int col, width;
+            if (asked < j1 && outputs(asked, s, col, width)) {
+                if (issued % kDepth < taken) free_slots();
+                if (a.base != nullptr)
+                    fetch(maps.base, a.base, a.base_stride, col, width);
+                else
+                    ++issued;
+            }
+            ++asked;
+        };
         if (R > 0) {
             float sum[6][16];
 #pragma unroll
             for (int c = 0; c < 6; ++c)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sum[c][e] = 0.f;
-            auto fetch = [&](int k) {  // block wg + 2 k into slot k
-                if (wg + 2 * k < n_blocks) {
-                    const uint32_t dst = mine32 + (k % kDepth) * kSlot;
-                    const float *src = a.x + (int64_t)(i0 + wg + 2 * k) * 32 + (lane & 7) * 4;
-#pragma unroll
-                    for (int it = 0; it < 8; ++it)
-                        if (row_of[it] >= 0) copy16(dst + place(4 * it + lane / 8, lane & 7), src + row_of[it] * a.x_stride);
-                }
-                copies_end();
+            auto fetch_x = [&](int k) {  // block wg + 2 k
+                if (wg + 2 * k < n_blocks) fetch(maps.x, a.x, a.x_stride, (i0 + wg + 2 * k) * 32, 32);
             };
             int settled = 0;
             auto settle = [&] {  // one more group of blocks
@@ -260,15 +315,19 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 if (!__all_sync(0xffffffffu, wait(&b.sum_full[buf], settled >> 1))) return false;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < 6; ++c) {
-                    const int col = (2 * c + wg) * 16;
-                    if (col < R) {
-                        uint32_t v[16];
-                        tmem_ld16(tmem + lanes + buf * (kLimbs / 2) + col, v);
-                        tmem_wait_ld();
+                for (int c = 0; c < 6; c += 2) {
+                    uint32_t v[2][16];
+                    const uint32_t at = tmem + lanes + buf * (kLimbs / 2) + (2 * c + wg) * 16;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) sum[c][e] += __uint_as_float(v[e]);
-                    }
+                    for (int i = 0; i < 2; ++i)
+                        if ((2 * (c + i) + wg) * 16 < R) tmem_ld16(at + 32 * i, v[i]);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if ((2 * (c + i) + wg) * 16 < R) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) sum[c + i][e] += __uint_as_float(v[i][e]);
+                        }
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -276,15 +335,13 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 ++settled;
                 return true;
             };
-            for (int k = 0; k < kDepth - 1; ++k) fetch(k);
+            for (int k = 0; k < kDepth - 1; ++k) fetch_x(k);
             const uint32_t limbs_at = tmem + lanes + kLimbs + wg * 64;
             for (int k = 0; wg + 2 * k < n_blocks && ok; ++k) {
-                copies_wait<kDepth - 2>();
-                __syncwarp();
-                if (k > 0) ok = __all_sync(0xffffffffu, wait(&b.x_empty[wg], k - 1));
+                ok = landed(k) && (k == 0 || __all_sync(0xffffffffu, wait(&b.x_empty[wg], k - 1)));
                 if (!ok) break;
                 tc_fence_after();
-                const uint8_t *slot = mine + (k % kDepth) * kSlot;
+                const uint8_t *slot = slot_of(k);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t hi[16], lo[16];
@@ -303,30 +360,34 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 tc_fence_before();
                 __syncwarp();  // (every lane has read its row: the slot before this one's may be filled)
                 if (lane == 0) mbar_arrive(&b.x_full[wg]);
-                fetch(k + kDepth - 1);
-                // the group before this block's
-                const int g = (wg + 2 * k) / kGroup;
-                while (ok && settled < g) ok = settle();
+                ++used;
+                fetch_x(k + kDepth - 1);
+                // the groups before this block's
+                while (ok && settled < (wg + 2 * k) / kGroup) ok = settle();
             }
-            copies_wait<0>();
             while (ok && settled < groups) ok = settle();
-            // the CTA's share of h, a rank's rows together; the slots of x are all read by now
+            // the CTA's share of h, by rows (4 ranks at a place that neighbours do not have a bank in common with); the
+            // slots of x are all read by now
+            const int spread = R % 32 == 0 ? 7 : 3;
+            auto share_at = [&](int col) { return (32 * q + lane) * R + ((col / 4) ^ (lane & spread)) * 4; };
             asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
             for (int c = 0; c < 6; ++c) {
                 const int col = (2 * c + wg) * 16;
                 if (col < R) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) shares[(col + e) * kTile + 32 * q + lane] = sum[c][e];
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<float4 *>(shares + share_at(col + e)) =
+                            make_float4(sum[c][e], sum[c][e + 1], sum[c][e + 2], sum[c][e + 3]);
                 }
             }
-            if (parts > 1) {
-                __syncwarp();
-                cluster_arrive();
-                cluster_wait();
-            } else {
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-            }
+            // meanwhile the base into slots that the shares leave free
+            taken = (R * kTile * 4 + kRowWarps * kSlot - 1) / (kRowWarps * kSlot);
+            if (ok)
+                for (int k = 0; k < kDepth - 1 && issued % kDepth >= taken; ++k) fetch_base();
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
             // h's limbs of the projections that this CTA's outputs need, 16 ranks at a time
             const float scale = a.scale != nullptr ? a.scale[tile.id] : 1.f;
             const int pa = j0 < j1 ? slice_of(a, p0, np, j0).p : 0, pb = j0 < j1 ? slice_of(a, p0, np, j1 - 1).p : -1;
@@ -338,15 +399,20 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 if (!need) continue;
                 uint32_t hi[16], lo[16];
                 float s[16];
-                const uint32_t at = smem_u32(shares + c * 16 * kTile + 32 * q + lane);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = 0.f;
-                for (int y = 0; y < parts; ++y) {
-                    float v[16];
+                for (int y = 0; y < parts; y += 4) {  // (four CTAs' loads in flight)
+                    float4 v[4][4];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = remote(at + e * kTile * 4, y);
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) s[e] += v[e];
+                        for (int e = 0; e < 4; ++e)
+                            v[i][e] = y + i < parts ? remote(smem_u32(shares + share_at(16 * c + 4 * e)), y + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[4 * e] += v[i][e].x, s[4 * e + 1] += v[i][e].y, s[4 * e + 2] += v[i][e].z, s[4 * e + 3] += v[i][e].w;
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) limbs(s[e] * scale, hi[e], lo[e]);
@@ -358,123 +424,96 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(&b.h_full);
             __syncwarp();
-            if (parts > 1) {  // the shares are read: what follows may take their place
-                cluster_arrive();
-                cluster_wait();
-            } else {
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-            }
+            cluster_arrive();  // the shares are read
         }
         // outputs: 64 at a time, this warp's 32 rows and half of the columns
-        auto fetch = [&](int j) {
-            if (j < j1 && a.base != nullptr) {
-                const Slice s = slice_of(a, p0, np, j);
-                const int o = s.o0 + 32 * wg + (lane & 7) * 4;
-                if (o < a.out[s.p]) {
-                    const uint32_t dst = mine32 + ((j - j0) % kDepth) * kSlot;
-                    const float *src = a.base + a.col[s.p] + o;
-#pragma unroll
-                    for (int it = 0; it < 8; ++it)
-                        if (row_of[it] >= 0) copy16(dst + place(4 * it + lane / 8, lane & 7), src + row_of[it] * a.base_stride);
-                }
-            }
-            copies_end();
-        };
-        for (int k = 0; k < kDepth - 1; ++k) fetch(j0 + k);
+        if (ok)
+            while (asked < j0 + kDepth - 1) fetch_base();
         int done = 0;  // products so far
         for (int j = j0; j < j1 && ok; ++j) {
-            copies_wait<kDepth - 2>();
-            __syncwarp();
-            const Slice s = slice_of(a, p0, np, j);
+            Slice s;
+            int col, width;
+            const bool any = outputs(j, s, col, width);
             bool has = false;
 #pragma unroll
             for (int p = 0; p < kLoraMaxProj; ++p) has |= p == s.p && first[p] >= 0;
-            uint8_t *slot = mine + ((j - j0) % kDepth) * kSlot;
+            uint8_t *slot = slot_of(used);
+            float4 w[8];
+            if (any && a.base != nullptr) {
+                ok = landed(used);
+                if (!ok) break;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) w[c] = *reinterpret_cast<const float4 *>(slot + place(lane, c));
+            } else {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) w[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
             if (has) {
                 const int buf = done % bufs;
                 ok = __all_sync(0xffffffffu, wait(&b.y_full[buf], done / bufs));
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t v[32], w[32];
+                uint32_t v[32], z[32];
                 const uint32_t at = tmem + lanes + out_at(buf) + 32 * wg;
                 tmem_ld16(at, v);
                 tmem_ld16(at + 16, v + 16);
-                tmem_ld16(at + kSlice, w);
-                tmem_ld16(at + kSlice + 16, w + 16);
+                tmem_ld16(at + kSlice, z);
+                tmem_ld16(at + kSlice + 16, z + 16);
                 tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + __uint_as_float(w[e]));
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&b.y_empty[buf]);
                 ++done;
+                auto sum = [&](int e) { return __uint_as_float(v[e]) + __uint_as_float(z[e]); };
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    float4 *at = reinterpret_cast<float4 *>(slot + place(lane, c));
-                    float4 w = a.base != nullptr ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
-                    w.x += __uint_as_float(v[4 * c]), w.y += __uint_as_float(v[4 * c + 1]);
-                    w.z += __uint_as_float(v[4 * c + 2]), w.w += __uint_as_float(v[4 * c + 3]);
-                    *at = w;
-                }
-                __syncwarp();
+                for (int c = 0; c < 8; ++c)
+                    w[c].x += sum(4 * c), w[c].y += sum(4 * c + 1), w[c].z += sum(4 * c + 2), w[c].w += sum(4 * c + 3);
             }
-            const int o = s.o0 + 32 * wg + (lane & 7) * 4;
-            if (o < a.out[s.p]) {
-                float *dst = a.y + a.col[s.p] + o;
+            if (any) {
+                if (has || a.base == nullptr) {  // (else the slot holds the result)
 #pragma unroll
-                for (int it = 0; it < 8; ++it) {
-                    if (row_of[it] < 0) continue;
-                    const float4 w = has || a.base != nullptr ? *reinterpret_cast<const float4 *>(slot + place(4 * it + lane / 8, lane & 7))
-                                                              : make_float4(0.f, 0.f, 0.f, 0.f);
-                    *reinterpret_cast<float4 *>(dst + row_of[it] * a.y_stride) = w;
+                    for (int c = 0; c < 8; ++c) *reinterpret_cast<float4 *>(slot + place(lane, c)) = w[c];
                 }
+                if (together && live == 32 && width == 32) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tma_store_2d(&maps.y, col, row0, smem_u32(slot));
+                } else {
+                    __syncwarp();
+                    const int c = (lane & 7) * 4;
+#pragma unroll
+                    for (int it = 0; it < 8; ++it) {
+                        const int r = 4 * it + lane / 8;
+                        if (r < live && c < width)
+                            *reinterpret_cast<float4 *>(a.y + list[32 * q + r] * a.y_stride + col + c) =
+                                *reinterpret_cast<const float4 *>(slot + place(r, lane & 7));
+                    }
+                }
+                ++used;
             }
-            __syncwarp();  // (the slot is read)
-            fetch(j + kDepth - 1);
+            if (lane == 0) stores_read<1>();
+            __syncwarp();  // (the slot before this one's is free)
+            fetch_base();
         }
-        copies_wait<0>();
+        free_slots();
+        // never leave with copies in flight
+        if (live > 0 && (a.base != nullptr || used < issued))
+            for (int m = used; m < issued; ++m) mbar_wait(&b.land[warp][m % kDepth], (uint32_t)(m / kDepth) & 1u, nullptr, 0);
+        if (lane == 0) stores_read<0>();
+        __syncwarp();
         reg_dec<128>();
     } else if (warp < 12) {
         // ------------------------------------ weights: widened to tf32 ------------------------------------
         reg_dec<kOtherRegs>();
-        const int wt = threadIdx.x - 32 * kRowWarps;
-        const int limb_bytes = a.ring_bytes / LW;
-        int entry = 0;
-        bool ok = true;
-        // chunks of 8 weights: chunk c of a row of 4 goes to two 16-byte places of its 128 bytes
-        auto put = [&](uint8_t *stage, int c, const uint32_t (&raw)[8]) {
-            const int row = c >> 2, ch = c & 3;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = weight<WT>(raw, 4 * h + e);
-                    if (WT == kW32)
-                        limbs(v, hi[e], lo[e]);
-                    else
-                        hi[e] = __float_as_uint(v);
-                }
-                uint8_t *at = stage + row * 128 + (((2 * ch + h) ^ (row & 7)) * 16);
-                *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                if (WT == kW32) *reinterpret_cast<uint4 *>(at + limb_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            }
-        };
-        auto take = [&] {  // the next stage, empty
-            const int st = entry % a.ring;
-            if (entry >= a.ring) ok = __all_sync(0xffffffffu, wait(&b.w_empty[st], entry / a.ring - 1));
-            return weights + st * a.ring_bytes;
-        };
-        auto give = [&] {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&b.w_full[entry % a.ring]);
-            ++entry;
-        };
         if (R > 0) {
-            constexpr int kMax = (WT == kW32 ? 96 : 192) / 32;  // chunks of a thread
-            uint32_t raw[kMax][8];
-            const int n_chunks = R * 4;
+            const int wt = threadIdx.x - 32 * kRowWarps;
+            const int limb_bytes = a.ring_bytes / LW;
+            // Stages: this CTA's blocks of A, then 64 rows of B and 32 ranks at a time.  A thread copies its chunks of 8
+            // weights kRaw stages ahead and widens them itself: chunk c = wt + 128 m is a quarter of row c / 4.
+            const int steps = (rank + 31) / 32, n_chunks = R * 4;
+            int n_stages = n_blocks;
+            for (int j = j0; j < j1; ++j) n_stages += a.a[slice_of(a, p0, np, j).p] != nullptr ? steps : 0;
+            constexpr int kMax = 6 / LW;
             const char *from[kMax];  // null: a row of zeros
 #pragma unroll
             for (int m = 0; m < kMax; ++m) {
@@ -487,67 +526,103 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                                   (((int64_t)tile.id * a.max_rank + r) * a.in_dim + i0 * 32 + (wt & 3) * 8) * Weight<WT>::bytes;
                 }
             }
-            auto fetch = [&](int i) {
+            uint8_t *raw = weights + a.ring * a.ring_bytes + wt * 16 * LW;
+            auto raw_at = [&](int e, int m) { return raw + (e % kRaw) * a.raw_bytes + m * (128 * 16 * LW); };
+            auto copy = [&](uint8_t *dst, const char *src) {
 #pragma unroll
-                for (int m = 0; m < kMax; ++m) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) raw[m][e] = 0;
-                    if (from[m] != nullptr && i < n_blocks) load_weights<WT, 8>(from[m], (int64_t)i * 32, raw[m]);
+                for (int h = 0; h < LW; ++h) copy16(smem_u32(dst) + 16 * h, src + 16 * h);
+            };
+            // the slice and step of the next stage of B, for the copies and for the widening
+            struct At {
+                int j, k;
+            };
+            auto next = [&](At &at) {
+                if (++at.k == steps) {
+                    at.k = 0;
+                    do ++at.j;
+                    while (at.j < j1 && a.a[slice_of(a, p0, np, at.j).p] == nullptr);
                 }
             };
-            fetch(0);
-            for (int i = 0; i < n_blocks && ok; ++i) {
-                uint8_t *stage = take();
-                if (!ok) break;
+            At ahead{j0 - 1, steps - 1}, here{j0 - 1, steps - 1};
+            next(ahead), next(here);
+            auto fetch = [&](int e) {
+                if (e < n_blocks) {
 #pragma unroll
-                for (int m = 0; m < kMax; ++m)
-                    if (wt + 128 * m < n_chunks) put(stage, wt + 128 * m, raw[m]);
-                fetch(i + 1);  // (under way while the stages are used up)
-                give();
-            }
-            if (parts > 1) {
-                __syncwarp();
-                cluster_arrive();
-                cluster_wait();
-                cluster_arrive();
-            }
-            // 64 rows of B, 32 ranks at a time
-            const int steps = (rank + 31) / 32;
-            for (int j = j0; j < j1 && ok; ++j) {
-                const Slice s = slice_of(a, p0, np, j);
-                if (a.a[s.p] == nullptr) continue;
-                for (int k = 0; k < steps; ++k) {
-                    uint32_t two[2][8];
+                    for (int m = 0; m < kMax; ++m)
+                        if (from[m] != nullptr) copy(raw_at(e, m), from[m] + (int64_t)e * 32 * Weight<WT>::bytes);
+                } else if (e < n_stages) {
+                    const Slice s = slice_of(a, p0, np, ahead.j);
+                    const int r = 32 * ahead.k + (wt & 3) * 8;
 #pragma unroll
                     for (int m = 0; m < 2; ++m) {
-                        const int c = wt + 128 * m, o = s.o0 + (c >> 2), r = 32 * k + (c & 3) * 8;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) two[m][e] = 0;
-                        if (o < a.out[s.p] && r < rank) {
-                            load_weights<WT, 8>(a.b[s.p], ((int64_t)tile.id * a.out[s.p] + o) * a.max_rank + r, two[m]);
-                            if (r + 8 > rank) {  // what stands behind the last rank is of no meaning
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    if (r + e >= rank) {
-                                        if (WT == kW32)
-                                            two[m][e] = 0;
-                                        else
-                                            two[m][e / 2] &= e % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-                                    }
-                            }
-                        }
+                        const int o = s.o0 + (wt >> 2) + 32 * m;
+                        if (o < a.out[s.p] && r < rank)
+                            copy(raw_at(e, m), static_cast<const char *>(a.b[s.p]) +
+                                                   (((int64_t)tile.id * a.out[s.p] + o) * a.max_rank + r) * Weight<WT>::bytes);
                     }
-                    uint8_t *stage = take();
-                    if (!ok) break;
-                    put(stage, wt, two[0]);
-                    put(stage, wt + 128, two[1]);
-                    give();
+                    next(ahead);
                 }
-            }
-            if (parts > 1) {
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            // a chunk of 8 weights, those from `valid` on zero, into two 16-byte places of its row of 128 bytes
+            auto put = [&](uint8_t *stage, int m, const uint8_t *src, int valid) {
+                uint32_t w[8];
+                load_weights<WT, 8>(src, 0, w);
+                const int row = (wt >> 2) + 32 * m, ch = wt & 3;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = 4 * h + e < valid ? weight<WT>(w, 4 * h + e) : 0.f;
+                        if (WT == kW32)
+                            limbs(v, hi[e], lo[e]);
+                        else
+                            hi[e] = __float_as_uint(v);
+                    }
+                    uint8_t *at = stage + row * 128 + (((2 * ch + h) ^ (row & 7)) * 16);
+                    *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if (WT == kW32) *reinterpret_cast<uint4 *>(at + limb_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+            };
+            for (int e = 0; e < kRaw - 1; ++e) fetch(e);
+            bool ok = true, passed = false;  // the cluster's barrier between the two products
+            auto pass = [&] {
+                if (!passed) {
+                    __syncwarp();
+                    cluster_arrive();
+                    cluster_wait();
+                    cluster_arrive();
+                }
+                passed = true;
+            };
+            for (int e = 0; e < n_stages && ok; ++e) {
+                if (e == n_blocks) pass();
+                const int st = e % a.ring;
+                if (e >= a.ring) ok = __all_sync(0xffffffffu, wait(&b.w_empty[st], e / a.ring - 1));
+                if (!ok) break;
+                asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 2) : "memory");
+                uint8_t *stage = weights + st * a.ring_bytes;
+                if (e < n_blocks) {
+#pragma unroll
+                    for (int m = 0; m < kMax; ++m)
+                        if (wt + 128 * m < n_chunks) put(stage, m, raw_at(e, m), from[m] != nullptr ? 8 : 0);
+                } else {
+                    const Slice s = slice_of(a, p0, np, here.j);
+                    const int valid = rank - 32 * here.k - (wt & 3) * 8;  // (what stands behind the last rank is of no meaning)
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) put(stage, m, raw_at(e, m), s.o0 + (wt >> 2) + 32 * m < a.out[s.p] ? valid : 0);
+                    next(here);
+                }
+                fence_proxy_async_smem();
                 __syncwarp();
-                cluster_wait();
+                if (lane == 0) mbar_arrive(&b.w_full[st]);
+                fetch(e + kRaw - 1);
             }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            pass();
+            __syncwarp();
+            cluster_wait();
         }
     } else {
         // ------------------------------------ products ------------------------------------
@@ -582,12 +657,10 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                     ++entry;
                 }
             }
-            if (parts > 1) {
-                __syncwarp();
-                cluster_arrive();
-                cluster_wait();
-                cluster_arrive();
-            }
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+            cluster_arrive();
             if (warp == 12 && ok) {
                 const uint32_t idesc = idesc_of(kSlice);
                 const int steps = (rank + 31) / 32;
@@ -626,10 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                     ++done;
                 }
             }
-            if (parts > 1) {
-                __syncwarp();
-                cluster_wait();
-            }
+            __syncwarp();
+            cluster_wait();
         }
     }
     tc_fence_before();
@@ -642,8 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
 }
 
 template <int WT>
-cudaError_t launch(const LoraArgs &a, cudaStream_t s) {
-    const int smem = 1024 + kRowWarps * kDepth * kSlot + a.ring * a.ring_bytes;
+cudaError_t launch(const LoraArgs &a, const LoraMaps &maps, cudaStream_t s) {
+    const int smem = 1024 + kRowWarps * kDepth * kSlot + a.ring * a.ring_bytes + kRaw * a.raw_bytes;
     cudaError_t e = cudaFuncSetAttribute(lora_tiles_kernel<WT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -657,7 +728,7 @@ cudaError_t launch(const LoraArgs &a, cudaStream_t s) {
     at[0].val.clusterDim = {(unsigned)a.cluster, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, lora_tiles_kernel<WT>, a);
+    return cudaLaunchKernelEx(&cfg, lora_tiles_kernel<WT>, a, maps);
 }
 }  // namespace
 
@@ -667,7 +738,8 @@ bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
     const int ranks = a.split ? r16 : r16 * a.n_proj;
     if (ranks > most || !a.x_vec || !a.y_vec) return false;
     a.ring_bytes = limbs * std::max(ranks, kSlice) * 128;
-    a.ring = std::min(kMaxRing, (224 * 1024 - kRowWarps * kDepth * kSlot) / a.ring_bytes);
+    a.raw_bytes = std::max((ranks * 4 + 127) / 128, 2) * 128 * 16 * limbs;
+    a.ring = std::min(kMaxRing, (224 * 1024 - kRowWarps * kDepth * kSlot - kRaw * a.raw_bytes) / a.ring_bytes);
     const int chunk = std::min(a.rows, kLoraChunk);
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (kTile - 1)) / kTile);
     // CTAs per tile: the fewest rounds of the SMs in all, counting what a CTA takes beside its share (as much as a
@@ -684,8 +756,8 @@ bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
     return true;
 }
 
-cudaError_t lora_tiles_launch(const LoraArgs &a, int type, cudaStream_t s) {
-    return type == 0 ? launch<kW32>(a, s) : type == 1 ? launch<kW16>(a, s) : launch<kWB16>(a, s);
+cudaError_t lora_tiles_launch(const LoraArgs &a, const LoraMaps &maps, int type, cudaStream_t s) {
+    return type == 0 ? launch<kW32>(a, maps, s) : type == 1 ? launch<kW16>(a, maps, s) : launch<kWB16>(a, maps, s);
 }
 
 }  // namespace ql
