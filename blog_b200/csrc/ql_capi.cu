@@ -1586,17 +1586,27 @@ int ql_moe_route(const float *logits, int64_t logits_stride, int32_t *top_idx, f
 
 // ---- low-rank adapters -----------------------------------------------------------------
 namespace {
-// Rows of `width` floats, `stride` apart, in boxes of 32 x 32 with the 128-byte swizzle.  (Encoded for the call: it is
-// the caller's address.)
-bool f32_rows_map(CUtensorMap *out, const float *base, int64_t width, int64_t rows, int64_t stride) {
+// Rows of `width` elements, `stride` apart, in boxes of 128 bytes and box_rows with the 128-byte swizzle.  (Encoded for
+// the call: it is the caller's address.)
+bool rows_map(CUtensorMap *out, bool bf16, const void *base, int64_t width, int64_t rows, int64_t stride, int box_rows) {
     auto enc = tensor_map_encoder();
+    const int el = bf16 ? 2 : 4;
     if (enc == nullptr || stride >= (int64_t(1) << 38)) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)stride * 4};
-    const cuuint32_t box[2] = {32, 32}, estr[2] = {1, 1};
-    return enc(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float *>(base), dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t strides[1] = {(cuuint64_t)stride * el};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / el), (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    return enc(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(base), dims,
+               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Those of a call in tiles of 128 rows.
+bool lora_maps(LoraMaps &m, const LoraArgs &a, int64_t width, bool bf16) {
+    if (!rows_map(&m.x, false, a.x, a.in_dim, a.rows, a.x_stride, 32) || !rows_map(&m.y, false, a.y, width, a.rows, a.y_stride, 32) ||
+        !rows_map(&m.base, false, a.base ? a.base : a.y, width, a.rows, a.base ? a.base_stride : a.y_stride, 32))
+        return false;
+    for (int p = 0; p < a.n_proj && bf16; ++p)
+        if (a.a[p] && !rows_map(&m.a[p], true, a.a[p], a.in_dim, (int64_t)a.n_adapters * a.max_rank, a.in_dim, 16)) return false;
+    return true;
 }
 }  // namespace
 
@@ -1655,9 +1665,8 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
         for (int p = 0; p < a.n_proj; ++p) a.y_vec = a.y_vec && a.out[p] % 4 == 0;
         cudaError_t e;
         LoraMaps maps;
-        if (rows / distinct >= kLoraTileFrom && rows <= INT32_MAX / 8 && lora_tiles_plan(a, type, distinct, ws->sms) &&
-            f32_rows_map(&maps.x, x, pool->in_dim, rows, x_stride) && f32_rows_map(&maps.y, y, width, rows, y_stride) &&
-            f32_rows_map(&maps.base, base ? base : y, width, rows, base ? base_stride : y_stride)) {
+        if (rows / distinct >= kLoraTileFrom && rows <= INT32_MAX / 8 && (int64_t)a.n_adapters * a.max_rank <= INT32_MAX &&
+            lora_tiles_plan(a, type, distinct, ws->sms) && lora_maps(maps, a, width, type == 2)) {
             e = lora_tiles_launch(a, maps, type, g_stream);
         } else {
             // Tiles: n rows of d adapters make at most (n + d (tm - 1)) / tm.

@@ -28,13 +28,15 @@ struct LoraArgs {
     // tiles on tcgen05 only:
     bool y_vec;       // base, y and every projection's columns start on 16 bytes, whole groups of 4
     bool split;       // a projection per blockIdx.y, not all in one
-    int ring, ring_bytes, raw_bytes;  // stages of widened weights, and of weights on their way
+    int ring, ring_bytes;      // stages of A in the products' layout
+    int raw_bytes, raw_total;  // a stage of weights on their way, and all of them
     int *err;
 };
 
-// x, base and y as rows of f32, in boxes of 32 columns and 32 rows (base: y's where there is none).
+// x, base and y as rows of f32, in boxes of 32 columns and 32 rows (base: y's where there is none); bf16 A as rows of
+// ranks, in boxes of 64 columns and 16 ranks.
 struct LoraMaps {
-    CUtensorMap x, base, y;
+    CUtensorMap x, base, y, a[kLoraMaxProj];
 };
 
 enum { kW32, kW16, kWB16 };  // types of the weights

@@ -5,18 +5,20 @@
 // product), adds the shares through distributed shared memory and takes its share of the outputs, 64 at a time.  x, the
 // base and y go through memory once.
 //
-//   h:  x arrives by cp.async in blocks of 32 columns, a warp its own 32 rows; a thread takes its row's 32 values apart
-//       into two tf32 limbs and writes them to tensor memory, the A operand.  A (f16, bf16: exact in tf32; f32: two
-//       limbs) is the B operand in shared memory.
-//   y:  h's limbs are the A operand in tensor memory, B's rows the B operand; a warp adds the product to the base, which
-//       arrives by cp.async as x did, and writes its rows' 128 bytes together.
+//   h:  a warp's 32 rows of x arrive in blocks of 32 columns; a thread takes its row's values apart into limbs and writes
+//       them to tensor memory, the A operand; A's ranks are the B operand in shared memory.
+//   y:  h's limbs are the A operand in tensor memory, B's rows the B operand; a warp adds the product to its rows of the
+//       base, which arrive as x did, and they leave as a tiled copy.
+// bf16 weights: kind::f16, x and h in three bf16 limbs (8 bits each, cut off: together every bit of the value); A goes from
+// memory to the operand's place by tiled copies.  f16 and f32 weights: kind::tf32, two limbs (22 bits) of x and h; 4 warps
+// widen the weights, f16 to one limb, f32 to two.
 //
 // The tensor cores cut off what they add up, so a sum over thousands of columns would lose bits in one direction: h's
-// accumulators start again every kGroup blocks, in two buffers, and are added up in registers with rounding; y's second
-// limbs have accumulators of their own.
+// accumulators start again every kGroup blocks, in two buffers, and are added up in registers with rounding; beyond 64
+// ranks y's lower limbs have accumulators of their own.
 //
 // Bound: memory, x once in and y once through.  Roles: 8 warps for rows (two per quarter of the tile, one for even and
-// one for odd blocks, then one for each half of 64 outputs), 4 that widen weights, one that issues the products.
+// one for odd blocks, then one for each half of 64 outputs), 4 for weights, one that issues the products.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -32,6 +34,8 @@ constexpr int kTile = kLoraTile, kDepth = 4;   // rows; blocks of a warp in flig
 constexpr int kSlice = 64;                     // outputs of one product
 constexpr int kSlot = 32 * 128;                // bytes of a warp's block: 32 rows of 32 values
 constexpr int kMaxRing = 4, kRaw = 4;          // stages of widened weights, and of weights on their way
+constexpr int kMaxOut = 8, kAhead = 4;         // stages of 64 rows of B, and how far ahead they are asked for
+static_assert(kAhead <= 4, "the waits for copies");
 constexpr uint32_t kLimbs = 384;               // TMEM columns: h's two accumulators of up to 192, then x's limbs twice
 // Registers per thread of the roles; 16 warps launch with 128 each.
 constexpr int kRowRegs = 184, kOtherRegs = 72;
@@ -40,7 +44,8 @@ static_assert(2 * kRowRegs + 2 * kOtherRegs == 4 * 128, "the block's registers a
 struct Bars {
     uint64_t land[kRowWarps][kDepth];          // a warp's blocks from memory
     uint64_t x_full[2], x_empty[2];            // x's limbs, by parity of the block
-    uint64_t w_full[kMaxRing], w_empty[kMaxRing];
+    uint64_t w_full[kMaxRing], w_empty[kMaxRing];  // stages of A
+    uint64_t v_free, v_full[kMaxOut], v_empty[kMaxOut];  // A's stages are all read: B's take their place
     uint64_t sum_full[2], sum_empty[2];        // h's accumulators
     uint64_t h_full;                           // h's limbs
     uint64_t y_full[2], y_empty[2];            // the products of 64 outputs
@@ -59,20 +64,32 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // D (+)= A B: A in tensor memory, B in shared memory (K-major rows of 128 bytes, 128-byte swizzle, 8 rows 1024 bytes).
+template <bool B16>
 __device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
     constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
-        "mov.b64 db, {%2, %5};\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(hi)
-        : "memory");
+    if constexpr (B16)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+            "mov.b64 db, {%2, %5};\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(hi)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+            "mov.b64 db, {%2, %5};\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(hi)
+            : "memory");
 }
 __device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | (1u << 16); }
-// f32 accumulator, tf32 operands, both K-major, M 128.
+// f32 accumulator, bf16 (1) or tf32 (2) operands, both K-major, M 128.
+template <bool B16>
 __device__ __forceinline__ uint32_t idesc_of(int n) {
-    return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+    constexpr uint32_t t = B16 ? 1 : 2;
+    return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -96,6 +113,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *v) {
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+// Two values in three bf16 limbs, cut off one after another (8 bits each: nothing is left), packed.
+__device__ __forceinline__ void limbs_b16(float x, float y, uint32_t &a, uint32_t &b, uint32_t &c) {
+    constexpr uint32_t m = 0xFFFF0000u;
+    a = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    const float x1 = x - __uint_as_float(__float_as_uint(x) & m), y1 = y - __uint_as_float(__float_as_uint(y) & m);
+    b = __byte_perm(__float_as_uint(x1), __float_as_uint(y1), 0x7632);
+    const float x2 = x1 - __uint_as_float(__float_as_uint(x1) & m), y2 = y1 - __uint_as_float(__float_as_uint(y1) & m);
+    c = __byte_perm(__float_as_uint(x2), __float_as_uint(y2), 0x7632);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -131,37 +162,45 @@ __device__ __forceinline__ void stores_read() {  // all but the last N have read
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float4 remote(uint32_t addr, uint32_t rank) {  // of another CTA's shared memory
+__device__ __forceinline__ float remote(uint32_t addr, uint32_t rank) {  // a word of another CTA's shared memory
     uint32_t r;
-    float4 v;
+    float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(r) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
     return v;
 }
 
-// Where outputs stand: slice j of the tile's projections p0 .. p0 + np, 64 columns of one projection.
+// Where outputs stand: 64 columns from o0 of projection p.
 struct Slice {
     int p, o0;
-};
-__device__ __forceinline__ Slice slice_of(const LoraArgs &a, int p0, int np, int j) {
-    int p = p0;
+    // the one after j others, of projections p0 .. p0 + np
+    __device__ __forceinline__ void seek(const LoraArgs &a, int p0, int np, int j) {
+        p = p0;
 #pragma unroll
-    for (int q = 0; q < kLoraMaxProj - 1; ++q) {
-        const int n = (a.out[p] + kSlice - 1) / kSlice;
-        if (p < p0 + np - 1 && j >= n) j -= n, ++p;
+        for (int q = 0; q < kLoraMaxProj - 1; ++q) {
+            const int n = (a.out[p] + kSlice - 1) / kSlice;
+            if (p < p0 + np - 1 && j >= n) j -= n, ++p;
+        }
+        o0 = j * kSlice;
     }
-    return {p, j * kSlice};
-}
+    __device__ __forceinline__ void step(const LoraArgs &a) {
+        o0 += kSlice;
+        if (o0 >= a.out[p]) o0 = 0, p = min(p + 1, kLoraMaxProj - 1);
+    }
+};
+__device__ __forceinline__ int pick(const int (&v)[kLoraMaxProj], int p) { return p == 0 ? v[0] : p == 1 ? v[1] : v[2]; }
 
 template <int WT>
 __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_constant__ LoraArgs a, const __grid_constant__ LoraMaps maps) {
+    constexpr bool B16 = WT == kWB16;
     constexpr int LW = WT == kW32 ? 2 : 1;  // limbs of a weight
     constexpr int kGroup = 4 / LW;          // blocks of 32 columns between two sums in registers
+    constexpr int kPer = B16 ? 64 : 32;     // columns of a stage of A, ranks of a stage of B: rows of 128 bytes
     extern __shared__ uint8_t sm_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *ring = sm;                                              // [kDepth][kRowWarps][kSlot]
     uint8_t *weights = sm + kRowWarps * kDepth * kSlot;              // [a.ring][a.ring_bytes]
-    float *shares = reinterpret_cast<float *>(sm);                   // [kTile][ranks], between the two products
+    float *shares = reinterpret_cast<float *>(sm);                   // [ranks][kTile], between the two products
     __shared__ Bars b;
     __shared__ int list[kTile];
     auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
@@ -196,9 +235,20 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     const int n_blocks = R > 0 ? (int)((int64_t)blocks * (part + 1) / parts) - i0 : 0;
     const int j0 = (int)((int64_t)slices * part / parts), j1 = (int)((int64_t)slices * (part + 1) / parts);
     const int groups = (n_blocks + kGroup - 1) / kGroup;
-    // the outputs' accumulators, of first and of second limbs: two pairs where h's limbs leave room, behind them
-    const int bufs = 2 * R + 4 * kSlice <= 512 ? 2 : 1;
-    auto out_at = [](int buf) { return 512u - 2 * kSlice * (buf + 1); };
+    // the ranks of h that this CTA's outputs need, and their limbs' columns of tensor memory: all first limbs, all second
+    Slice from, to;
+    from.seek(a, p0, np, min(j0, slices - 1)), to.seek(a, p0, np, max(j1 - 1, 0));
+    int need[kLoraMaxProj], n_need = 0;
+#pragma unroll
+    for (int p = 0; p < kLoraMaxProj; ++p) {
+        need[p] = -1;
+        if (j0 < j1 && p >= from.p && p <= to.p && first[p] >= 0) need[p] = n_need, n_need += r16;
+    }
+    const int limb_cols = B16 ? n_need / 2 : n_need, h_cols = (B16 ? 3 : 2) * limb_cols;
+    // the outputs' accumulators at the end of tensor memory, two where h's limbs leave room
+    const bool apart = rank > 64;
+    const int out_cols = apart ? 2 * kSlice : kSlice, bufs = h_cols + 2 * out_cols <= 512 ? 2 : 1;
+    auto out_at = [&](int buf) { return 512u - out_cols * (buf + 1); };
 
     // a row warp's rows: how many there are, and whether they lie together
     const int q32 = (warp & 3) * 32, live = warp < kRowWarps ? max(0, min(32, tile.n - q32)) : 0;
@@ -211,7 +261,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             mbar_init(&b.sum_full[i], 1), mbar_init(&b.sum_empty[i], kRowWarps);
             mbar_init(&b.y_full[i], 1), mbar_init(&b.y_empty[i], kRowWarps);
         }
-        for (int i = 0; i < kMaxRing; ++i) mbar_init(&b.w_full[i], 4), mbar_init(&b.w_empty[i], 1);
+        for (int i = 0; i < kMaxRing; ++i) mbar_init(&b.w_full[i], B16 ? 1 : 4), mbar_init(&b.w_empty[i], 1);
+        for (int i = 0; i < kMaxOut; ++i) mbar_init(&b.v_full[i], 4), mbar_init(&b.v_empty[i], 1);
+        mbar_init(&b.v_free, 1);
         mbar_init(&b.h_full, kRowWarps);
         b.abort = 0;
     }
@@ -273,13 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             return live == 0 || __all_sync(0xffffffffu, wait(&b.land[warp][m % kDepth], m / kDepth));
         };
         bool ok = true;
-        // the first of 64 outputs, this warp's 32 of them, and whether there are any
-        auto outputs = [&](int j, Slice &s, int &col, int &width) {
-            s = slice_of(a, p0, np, j);
-            width = min(32, a.out[s.p] - s.o0 - 32 * wg);
-            col = a.col[s.p] + s.o0 + 32 * wg;
-            return width > 0;
-        };
+        // this warp's 32 of a slice's 64 outputs: the first column of y, and how many there are
+        auto col_of = [&](const Slice &s) { return a.col[s.p] + s.o0 + 32 * wg; };
+        auto width_of = [&](const Slice &s) { return min(32, a.out[s.p] - s.o0 - 32 * wg); };
         int asked = j0;  // outputs whose base has been asked for
         int taken = 0;   // slots that the shares of h stand in, until they are read by all (the cluster's second barrier)
         auto free_slots = [&] {
@@ -288,15 +336,18 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             cluster_wait();
             fence_proxy_async_smem();
         };
+        Slice next = from;
         auto fetch_base = [&] {
-            Slice s;
-            int col, width;
-            if (asked < j1 && outputs(asked, s, col, width)) {
-                if (issued % kDepth < taken) free_slots();
-                if (a.base != nullptr)
-                    fetch(maps.base, a.base, a.base_stride, col, width);
-                else
-                    ++issued;
+            if (asked < j1) {
+                const int width = width_of(next);
+                if (width > 0) {
+                    if (issued % kDepth < taken) free_slots();
+                    if (a.base != nullptr)
+                        fetch(maps.base, a.base, a.base_stride, col_of(next), width);
+                    else
+                        ++issued;
+                }
+                next.step(a);
             }
             ++asked;
         };
@@ -342,19 +393,31 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 if (!ok) break;
                 tc_fence_after();
                 const uint8_t *slot = slot_of(k);
+                if constexpr (B16) {
+                    uint32_t l[3][16];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float4 v = *reinterpret_cast<const float4 *>(slot + place(lane, 4 * h + c));
-                        limbs(v.x, hi[4 * c], lo[4 * c]);
-                        limbs(v.y, hi[4 * c + 1], lo[4 * c + 1]);
-                        limbs(v.z, hi[4 * c + 2], lo[4 * c + 2]);
-                        limbs(v.w, hi[4 * c + 3], lo[4 * c + 3]);
+                    for (int c = 0; c < 8; ++c) {
+                        const float4 v = *reinterpret_cast<const float4 *>(slot + place(lane, c));
+                        limbs_b16(v.x, v.y, l[0][2 * c], l[1][2 * c], l[2][2 * c]);
+                        limbs_b16(v.z, v.w, l[0][2 * c + 1], l[1][2 * c + 1], l[2][2 * c + 1]);
                     }
-                    tmem_st16(limbs_at + 16 * h, hi);
-                    tmem_st16(limbs_at + 32 + 16 * h, lo);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) tmem_st16(limbs_at + 16 * i, l[i]);
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float4 v = *reinterpret_cast<const float4 *>(slot + place(lane, 4 * h + c));
+                            limbs(v.x, hi[4 * c], lo[4 * c]);
+                            limbs(v.y, hi[4 * c + 1], lo[4 * c + 1]);
+                            limbs(v.z, hi[4 * c + 2], lo[4 * c + 2]);
+                            limbs(v.w, hi[4 * c + 3], lo[4 * c + 3]);
+                        }
+                        tmem_st16(limbs_at + 16 * h, hi);
+                        tmem_st16(limbs_at + 32 + 16 * h, lo);
+                    }
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -366,19 +429,14 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 while (ok && settled < (wg + 2 * k) / kGroup) ok = settle();
             }
             while (ok && settled < groups) ok = settle();
-            // the CTA's share of h, by rows (4 ranks at a place that neighbours do not have a bank in common with); the
-            // slots of x are all read by now
-            const int spread = R % 32 == 0 ? 7 : 3;
-            auto share_at = [&](int col) { return (32 * q + lane) * R + ((col / 4) ^ (lane & spread)) * 4; };
+            // the CTA's share of h, a rank's rows together; the slots of x are all read by now
             asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
             for (int c = 0; c < 6; ++c) {
                 const int col = (2 * c + wg) * 16;
                 if (col < R) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<float4 *>(shares + share_at(col + e)) =
-                            make_float4(sum[c][e], sum[c][e + 1], sum[c][e + 2], sum[c][e + 3]);
+                    for (int e = 0; e < 16; ++e) shares[(col + e) * kTile + 32 * q + lane] = sum[c][e];
                 }
             }
             // meanwhile the base into slots that the shares leave free
@@ -388,36 +446,44 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             __syncwarp();
             cluster_arrive();
             cluster_wait();
-            // h's limbs of the projections that this CTA's outputs need, 16 ranks at a time
+            // h's limbs, 16 ranks at a time
             const float scale = a.scale != nullptr ? a.scale[tile.id] : 1.f;
-            const int pa = j0 < j1 ? slice_of(a, p0, np, j0).p : 0, pb = j0 < j1 ? slice_of(a, p0, np, j1 - 1).p : -1;
-            for (int c = wg; c * 16 < R; c += 2) {
-                bool need = false;
+            for (int c = wg; c * 16 < n_need; c += 2) {
+                int col = 0, left = 0;  // where the 16 stand among all ranks, and how many of them are in use
 #pragma unroll
                 for (int p = 0; p < kLoraMaxProj; ++p)
-                    need |= first[p] >= 0 && p >= pa && p <= pb && c * 16 >= first[p] && c * 16 < first[p] + r16;
-                if (!need) continue;
-                uint32_t hi[16], lo[16];
+                    if (need[p] >= 0 && c * 16 >= need[p] && c * 16 < need[p] + r16)
+                        col = first[p] + c * 16 - need[p], left = rank - (c * 16 - need[p]);
+                const uint32_t at = smem_u32(shares + col * kTile + 32 * q + lane);
                 float s[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = 0.f;
                 for (int y = 0; y < parts; y += 4) {  // (four CTAs' loads in flight)
-                    float4 v[4][4];
+                    float v[4][16];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[i][e] = y + i < parts ? remote(smem_u32(shares + share_at(16 * c + 4 * e)), y + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        for (int e = 0; e < 16; ++e) v[i][e] = y + i < parts ? remote(at + e * kTile * 4, y + i) : 0.f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s[4 * e] += v[i][e].x, s[4 * e + 1] += v[i][e].y, s[4 * e + 2] += v[i][e].z, s[4 * e + 3] += v[i][e].w;
+                        for (int e = 0; e < 16; ++e) s[e] += v[i][e];
                 }
+                // (what stands behind the last rank is of no meaning)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) limbs(s[e] * scale, hi[e], lo[e]);
-                tmem_st16(tmem + lanes + c * 16, hi);
-                tmem_st16(tmem + lanes + R + c * 16, lo);
+                for (int e = 0; e < 16; ++e) s[e] = e < left ? s[e] * scale : 0.f;
+                uint32_t l[3][16];
+                if constexpr (B16) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) limbs_b16(s[2 * e], s[2 * e + 1], l[0][e], l[1][e], l[2][e]);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) tmem_st8(tmem + lanes + i * limb_cols + c * 8, l[i]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) limbs(s[e], l[0][e], l[1][e]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) tmem_st16(tmem + lanes + i * limb_cols + c * 16, l[i]);
+                }
             }
             tmem_wait_st();
             tc_fence_before();
@@ -430,13 +496,10 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         if (ok)
             while (asked < j0 + kDepth - 1) fetch_base();
         int done = 0;  // products so far
-        for (int j = j0; j < j1 && ok; ++j) {
-            Slice s;
-            int col, width;
-            const bool any = outputs(j, s, col, width);
-            bool has = false;
-#pragma unroll
-            for (int p = 0; p < kLoraMaxProj; ++p) has |= p == s.p && first[p] >= 0;
+        Slice s = from;
+        for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
+            const int col = col_of(s), width = width_of(s);
+            const bool any = width > 0, has = pick(need, s.p) >= 0;
             uint8_t *slot = slot_of(used);
             float4 w[8];
             if (any && a.base != nullptr) {
@@ -453,21 +516,29 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 ok = __all_sync(0xffffffffu, wait(&b.y_full[buf], done / bufs));
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t v[32], z[32];
+                uint32_t v[32];
                 const uint32_t at = tmem + lanes + out_at(buf) + 32 * wg;
                 tmem_ld16(at, v);
                 tmem_ld16(at + 16, v + 16);
-                tmem_ld16(at + kSlice, z);
-                tmem_ld16(at + kSlice + 16, z + 16);
-                tmem_wait_ld();
+                if (apart) {
+                    uint32_t z[32];
+                    tmem_ld16(at + kSlice, z);
+                    tmem_ld16(at + kSlice + 16, z + 16);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + __uint_as_float(z[e]));
+                } else {
+                    tmem_wait_ld();
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&b.y_empty[buf]);
                 ++done;
-                auto sum = [&](int e) { return __uint_as_float(v[e]) + __uint_as_float(z[e]); };
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    w[c].x += sum(4 * c), w[c].y += sum(4 * c + 1), w[c].z += sum(4 * c + 2), w[c].w += sum(4 * c + 3);
+                for (int c = 0; c < 8; ++c) {
+                    w[c].x += __uint_as_float(v[4 * c]), w[c].y += __uint_as_float(v[4 * c + 1]);
+                    w[c].z += __uint_as_float(v[4 * c + 2]), w[c].w += __uint_as_float(v[4 * c + 3]);
+                }
             }
             if (any) {
                 if (has || a.base == nullptr) {  // (else the slot holds the result)
@@ -503,72 +574,13 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         __syncwarp();
         reg_dec<128>();
     } else if (warp < 12) {
-        // ------------------------------------ weights: widened to tf32 ------------------------------------
+        // ------------------------------------ weights ------------------------------------
         reg_dec<kOtherRegs>();
         if (R > 0) {
             const int wt = threadIdx.x - 32 * kRowWarps;
-            const int limb_bytes = a.ring_bytes / LW;
-            // Stages: this CTA's blocks of A, then 64 rows of B and 32 ranks at a time.  A thread copies its chunks of 8
-            // weights kRaw stages ahead and widens them itself: chunk c = wt + 128 m is a quarter of row c / 4.
-            const int steps = (rank + 31) / 32, n_chunks = R * 4;
-            int n_stages = n_blocks;
-            for (int j = j0; j < j1; ++j) n_stages += a.a[slice_of(a, p0, np, j).p] != nullptr ? steps : 0;
-            constexpr int kMax = 6 / LW;
-            const char *from[kMax];  // null: a row of zeros
-#pragma unroll
-            for (int m = 0; m < kMax; ++m) {
-                from[m] = nullptr;
-#pragma unroll
-                for (int p = 0; p < kLoraMaxProj; ++p) {
-                    const int r = ((wt + 128 * m) >> 2) - first[p];
-                    if (first[p] >= 0 && r >= 0 && r < rank)
-                        from[m] = static_cast<const char *>(a.a[p]) +
-                                  (((int64_t)tile.id * a.max_rank + r) * a.in_dim + i0 * 32 + (wt & 3) * 8) * Weight<WT>::bytes;
-                }
-            }
-            uint8_t *raw = weights + a.ring * a.ring_bytes + wt * 16 * LW;
-            auto raw_at = [&](int e, int m) { return raw + (e % kRaw) * a.raw_bytes + m * (128 * 16 * LW); };
-            auto copy = [&](uint8_t *dst, const char *src) {
-#pragma unroll
-                for (int h = 0; h < LW; ++h) copy16(smem_u32(dst) + 16 * h, src + 16 * h);
-            };
-            // the slice and step of the next stage of B, for the copies and for the widening
-            struct At {
-                int j, k;
-            };
-            auto next = [&](At &at) {
-                if (++at.k == steps) {
-                    at.k = 0;
-                    do ++at.j;
-                    while (at.j < j1 && a.a[slice_of(a, p0, np, at.j).p] == nullptr);
-                }
-            };
-            At ahead{j0 - 1, steps - 1}, here{j0 - 1, steps - 1};
-            next(ahead), next(here);
-            auto fetch = [&](int e) {
-                if (e < n_blocks) {
-#pragma unroll
-                    for (int m = 0; m < kMax; ++m)
-                        if (from[m] != nullptr) copy(raw_at(e, m), from[m] + (int64_t)e * 32 * Weight<WT>::bytes);
-                } else if (e < n_stages) {
-                    const Slice s = slice_of(a, p0, np, ahead.j);
-                    const int r = 32 * ahead.k + (wt & 3) * 8;
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        const int o = s.o0 + (wt >> 2) + 32 * m;
-                        if (o < a.out[s.p] && r < rank)
-                            copy(raw_at(e, m), static_cast<const char *>(a.b[s.p]) +
-                                                   (((int64_t)tile.id * a.out[s.p] + o) * a.max_rank + r) * Weight<WT>::bytes);
-                    }
-                    next(ahead);
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            // a chunk of 8 weights, those from `valid` on zero, into two 16-byte places of its row of 128 bytes
-            auto put = [&](uint8_t *stage, int m, const uint8_t *src, int valid) {
-                uint32_t w[8];
-                load_weights<WT, 8>(src, 0, w);
-                const int row = (wt >> 2) + 32 * m, ch = wt & 3;
+            bool ok = true;
+            // A chunk of 8 weights (those from `valid` on zero) widened into two 16-byte places of its row of 128 bytes.
+            auto put = [&](uint8_t *at_row, int row, int ch, const uint32_t (&w)[8], int valid, int limb) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t hi[4], lo[4];
@@ -580,47 +592,177 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                         else
                             hi[e] = __float_as_uint(v);
                     }
-                    uint8_t *at = stage + row * 128 + (((2 * ch + h) ^ (row & 7)) * 16);
+                    uint8_t *at = at_row + row * 128 + (((2 * ch + h) ^ (row & 7)) * 16);
                     *reinterpret_cast<uint4 *>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if (WT == kW32) *reinterpret_cast<uint4 *>(at + limb_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    if (WT == kW32) *reinterpret_cast<uint4 *>(at + limb) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
             };
-            for (int e = 0; e < kRaw - 1; ++e) fetch(e);
-            bool ok = true, passed = false;  // the cluster's barrier between the two products
-            auto pass = [&] {
-                if (!passed) {
-                    __syncwarp();
-                    cluster_arrive();
-                    cluster_wait();
-                    cluster_arrive();
+            if constexpr (B16) {
+                // A as it stands, 64 columns of 16 ranks in a copy (ranks not in use among them: their sums are left out)
+                if (wt == 0) {
+                    const int n = (n_blocks + 1) / 2;
+                    int e = 0;
+                    for (; e < n; ++e) {
+                        const int st = e % a.ring;
+                        if (e >= a.ring && !wait(&b.w_empty[st], e / a.ring - 1)) break;
+                        mbar_arrive_expect_tx(&b.w_full[st], R * 128);
+                        uint8_t *stage = weights + st * a.ring_bytes;
+#pragma unroll
+                        for (int p = 0; p < kLoraMaxProj; ++p)
+                            if (first[p] >= 0)
+                                for (int r = 0; r < r16; r += 16)
+                                    tma_box2d(stage + (first[p] + r) * 128, &maps.a[p], (i0 + 2 * e) * 32, tile.id * a.max_rank + r,
+                                              &b.w_full[st]);
+                    }
+                    // never leave with copies in flight
+                    for (int m = max(0, e - a.ring); m < e; ++m)
+                        mbar_wait(&b.w_full[m % a.ring], (uint32_t)(m / a.ring) & 1u, nullptr, 0);
                 }
-                passed = true;
-            };
-            for (int e = 0; e < n_stages && ok; ++e) {
-                if (e == n_blocks) pass();
-                const int st = e % a.ring;
-                if (e >= a.ring) ok = __all_sync(0xffffffffu, wait(&b.w_empty[st], e / a.ring - 1));
-                if (!ok) break;
-                asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 2) : "memory");
-                uint8_t *stage = weights + st * a.ring_bytes;
-                if (e < n_blocks) {
+                __syncwarp();
+            } else {
+                // A thread copies its chunks of 8 weights kRaw stages ahead and widens them itself: chunk wt + 128 m is a
+                // quarter of row (wt + 128 m) / 4.
+                constexpr int kMax = 6 / LW;
+                const char *src[kMax];  // null: a row of zeros
+#pragma unroll
+                for (int m = 0; m < kMax; ++m) {
+                    src[m] = nullptr;
+#pragma unroll
+                    for (int p = 0; p < kLoraMaxProj; ++p) {
+                        const int r = ((wt + 128 * m) >> 2) - first[p];
+                        if (first[p] >= 0 && r >= 0 && r < rank)
+                            src[m] = static_cast<const char *>(a.a[p]) +
+                                     (((int64_t)tile.id * a.max_rank + r) * a.in_dim + i0 * 32 + (wt & 3) * 8) * Weight<WT>::bytes;
+                    }
+                }
+                uint8_t *raw = weights + a.ring * a.ring_bytes + wt * 16 * LW;
+                auto raw_at = [&](int e, int m) { return raw + (e % kRaw) * a.raw_bytes + m * (128 * 16 * LW); };
+                auto fetch = [&](int e) {
+                    if (e < n_blocks) {
+#pragma unroll
+                        for (int m = 0; m < kMax; ++m)
+                            if (src[m] != nullptr)
+#pragma unroll
+                                for (int h = 0; h < LW; ++h)
+                                    copy16(smem_u32(raw_at(e, m)) + 16 * h, src[m] + (int64_t)e * 32 * Weight<WT>::bytes + 16 * h);
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                };
+                for (int e = 0; e < kRaw - 1; ++e) fetch(e);
+                for (int e = 0; e < n_blocks; ++e) {
+                    const int st = e % a.ring;
+                    if (e >= a.ring) ok = __all_sync(0xffffffffu, wait(&b.w_empty[st], e / a.ring - 1));
+                    if (!ok) break;
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 2) : "memory");
+                    uint8_t *stage = weights + st * a.ring_bytes;
+                    uint32_t w[kMax][8];
 #pragma unroll
                     for (int m = 0; m < kMax; ++m)
-                        if (wt + 128 * m < n_chunks) put(stage, m, raw_at(e, m), from[m] != nullptr ? 8 : 0);
-                } else {
-                    const Slice s = slice_of(a, p0, np, here.j);
-                    const int valid = rank - 32 * here.k - (wt & 3) * 8;  // (what stands behind the last rank is of no meaning)
+                        if (wt + 128 * m < 4 * R) load_weights<WT, 8>(raw_at(e, m), 0, w[m]);
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) put(stage, m, raw_at(e, m), s.o0 + (wt >> 2) + 32 * m < a.out[s.p] ? valid : 0);
-                    next(here);
+                    for (int m = 0; m < kMax; ++m)
+                        if (wt + 128 * m < 4 * R) put(stage, (wt >> 2) + 32 * m, wt & 3, w[m], src[m] != nullptr ? 8 : 0, a.ring_bytes / 2);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&b.w_full[st]);
+                    fetch(e + kRaw - 1);
+                }
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+            cluster_arrive();
+            // B: 64 rows and kPer ranks at a time, kAhead stages ahead, in the place of A's stages
+            ok = ok && __all_sync(0xffffffffu, wait(&b.v_free, 0));
+            constexpr int kBytes = kSlice * 128 * LW, kChunks = B16 ? 4 : 2;  // of a stage; chunks of a thread
+            const int n_out = min(kMaxOut, a.ring * a.ring_bytes / kBytes), steps = (rank + kPer - 1) / kPer;
+            const int n_ahead = min(kAhead, n_out - 1);
+            struct At {  // a stage: its outputs and its step of ranks
+                Slice s;
+                int j, k;
+            };
+            At ahead{from, j0, 0};
+            while (ahead.j < j1 && pick(need, ahead.s.p) < 0) ahead.s.step(a), ++ahead.j;
+            At here = ahead;
+            auto step = [&](At &at) {
+                if (++at.k < steps) return;
+                at.k = 0;
+                do at.s.step(a), ++at.j;
+                while (at.j < j1 && pick(need, at.s.p) < 0);
+            };
+            // this thread's chunk m of 8 ranks: its row and first rank, null where there is none
+            auto chunk = [&](const At &at, int m, int &row, int &ch, int &valid) {
+                row = B16 ? (wt >> 3) + 16 * m : (wt >> 2) + 32 * m;
+                ch = B16 ? wt & 7 : wt & 3;
+                const int o = at.s.o0 + row, r = at.k * kPer + 8 * ch;
+                valid = o < a.out[at.s.p] ? rank - r : 0;
+                return static_cast<const char *>(a.b[at.s.p]) + (((int64_t)tile.id * a.out[at.s.p] + o) * a.max_rank + r) * Weight<WT>::bytes;
+            };
+            int asked = 0, e = 0;
+            uint8_t *raw = weights + a.ring * a.ring_bytes + wt * 16 * LW;
+            auto fetch = [&] {
+                if (ahead.j < j1) {
+                    const int st = asked % n_out;
+                    if (asked >= n_out) ok = __all_sync(0xffffffffu, wait(&b.v_empty[st], asked / n_out - 1));
+                    if (ok) {
+#pragma unroll
+                        for (int m = 0; m < kChunks; ++m) {
+                            int row, ch, valid;
+                            const char *p = chunk(ahead, m, row, ch, valid);
+                            if (B16) {  // straight to its place
+                                uint8_t *at = weights + st * kBytes + row * 128 + ((ch ^ (row & 7)) * 16);
+                                if (valid >= 8) {
+                                    copy16(smem_u32(at), p);
+                                } else if (ahead.k * kPer + 8 * ch < r16) {  // (what stands behind the last rank is of no meaning)
+                                    uint4 w = valid > 0 ? *reinterpret_cast<const uint4 *>(p) : make_uint4(0, 0, 0, 0);
+                                    uint32_t *v = &w.x;
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        v[i] = 2 * i + 1 < valid ? v[i] : 2 * i < valid ? v[i] & 0xFFFFu : 0u;
+                                    *reinterpret_cast<uint4 *>(at) = w;
+                                }
+                            } else if (valid > 0) {
+#pragma unroll
+                                for (int h = 0; h < LW; ++h)
+                                    copy16(smem_u32(raw + (asked % (kAhead + 1)) * (kChunks * 128 * 16 * LW) + m * (128 * 16 * LW)) + 16 * h, p + 16 * h);
+                            }
+                        }
+                    }
+                    step(ahead);
+                    ++asked;
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            if (ok)
+                for (int i = 0; i < n_ahead; ++i) fetch();
+            while (ok && here.j < j1) {
+                const int st = e % n_out;
+                switch (n_ahead) {  // the oldest of them
+                case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+                case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+                case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+                default: asm volatile("cp.async.wait_group 0;" ::: "memory");
+                }
+                if constexpr (!B16) {
+                    uint32_t w[kChunks][8];
+                    int row[kChunks], ch[kChunks], valid[kChunks];
+#pragma unroll
+                    for (int m = 0; m < kChunks; ++m) {
+                        chunk(here, m, row[m], ch[m], valid[m]);
+                        load_weights<WT, 8>(raw + (e % (kAhead + 1)) * (kChunks * 128 * 16 * LW) + m * (128 * 16 * LW), 0, w[m]);
+                    }
+#pragma unroll
+                    for (int m = 0; m < kChunks; ++m) put(weights + st * kBytes, row[m], ch[m], w[m], valid[m], kBytes / 2);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&b.w_full[st]);
-                fetch(e + kRaw - 1);
+                if (lane == 0) mbar_arrive(&b.v_full[st]);
+                ++e;
+                step(here);
+                fetch();
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            pass();
             __syncwarp();
             cluster_wait();
         }
@@ -628,33 +770,39 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         // ------------------------------------ products ------------------------------------
         reg_dec<kOtherRegs>();
         if (R > 0) {
-            const int limb = a.ring_bytes / LW / 16;
-            int entry = 0;
             bool ok = true;
             if (warp == 12) {
-                const uint32_t idesc = idesc_of(R);
+                const uint32_t idesc = idesc_of<B16>(R);
                 for (int i = 0; i < n_blocks && ok; ++i) {
-                    const int wg = i & 1, g = i / kGroup, buf = g & 1, st = entry % a.ring;
+                    const int wg = i & 1, g = i / kGroup, buf = g & 1, e = B16 ? i >> 1 : i, st = e % a.ring;
                     if (i % kGroup == 0 && g >= 2) ok = wait(&b.sum_empty[buf], g / 2 - 1);
-                    ok = ok && wait(&b.x_full[wg], i >> 1) && wait(&b.w_full[st], entry / a.ring);
+                    ok = ok && wait(&b.x_full[wg], i >> 1) && wait(&b.w_full[st], e / a.ring);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint32_t d = tmem + buf * (kLimbs / 2), x = tmem + kLimbs + wg * 64;
                         const uint32_t w = desc_lo(smem_u32(weights + st * a.ring_bytes));
+                        if constexpr (B16) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            mma(d, x + 32 + 8 * k, w + 2 * k, idesc, i % kGroup != 0 || k != 0);
-                            if (WT == kW32) mma(d, x + 8 * k, w + limb + 2 * k, idesc, 1);
-                            mma(d, x + 8 * k, w + 2 * k, idesc, 1);
+                            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                                for (int l = 2; l >= 0; --l)
+                                    mma<true>(d, x + 16 * l + 8 * k, w + 4 * wg + 2 * k, idesc, i % kGroup != 0 || k != 0 || l != 2);
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                mma<false>(d, x + 32 + 8 * k, w + 2 * k, idesc, i % kGroup != 0 || k != 0);
+                                if (WT == kW32) mma<false>(d, x + 8 * k, w + a.ring_bytes / 32 + 2 * k, idesc, 1);
+                                mma<false>(d, x + 8 * k, w + 2 * k, idesc, 1);
+                            }
                         }
                         mma_commit(&b.x_empty[wg]);
-                        mma_commit(&b.w_empty[st]);
+                        if (!B16 || wg == 1 || i == n_blocks - 1) mma_commit(&b.w_empty[st]);
                         if (i % kGroup == kGroup - 1 || i == n_blocks - 1) mma_commit(&b.sum_full[buf]);
+                        if (i == n_blocks - 1) mma_commit(&b.v_free);
                     }
                     __syncwarp();
-                    ++entry;
                 }
             }
             __syncwarp();
@@ -662,39 +810,51 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             cluster_wait();
             cluster_arrive();
             if (warp == 12 && ok) {
-                const uint32_t idesc = idesc_of(kSlice);
-                const int steps = (rank + 31) / 32;
-                int done = 0;
+                constexpr int kBytes = kSlice * 128 * LW;
+                const uint32_t idesc = idesc_of<B16>(kSlice);
+                const int n_out = min(kMaxOut, a.ring * a.ring_bytes / kBytes), steps = (rank + kPer - 1) / kPer;
+                const uint32_t second = apart ? kSlice : 0;  // the lower limbs' accumulators
+                int done = 0, e = 0;
+                Slice s = from;
                 ok = __all_sync(0xffffffffu, wait(&b.h_full, 0));
-                for (int j = j0; j < j1 && ok; ++j) {
-                    const Slice s = slice_of(a, p0, np, j);
-                    int h0 = -1;
-#pragma unroll
-                    for (int p = 0; p < kLoraMaxProj; ++p)
-                        if (p == s.p) h0 = first[p];
+                for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
+                    const int h0 = pick(need, s.p);
                     if (h0 < 0) continue;
                     const int buf = done % bufs;
                     if (done >= bufs) ok = __all_sync(0xffffffffu, wait(&b.y_empty[buf], done / bufs - 1));
                     for (int k = 0; k < steps && ok; ++k) {
-                        const int st = entry % a.ring;
-                        ok = __all_sync(0xffffffffu, wait(&b.w_full[st], entry / a.ring));
+                        const int st = e % n_out;
+                        ok = __all_sync(0xffffffffu, wait(&b.v_full[st], e / n_out));
                         if (!ok) break;
                         tc_fence_after();
                         if (elect_one()) {
-                            const uint32_t d = tmem + out_at(buf), h = tmem + h0 + 32 * k;
-                            const uint32_t w = desc_lo(smem_u32(weights + st * a.ring_bytes));
+                            const uint32_t d = tmem + out_at(buf);
+                            const uint32_t w = desc_lo(smem_u32(weights + st * kBytes));
+                            if constexpr (B16) {
+                                const uint32_t h = tmem + (h0 + 64 * k) / 2;
 #pragma unroll
-                            for (int m = 0; m < 4; ++m) {
-                                if (32 * k + 8 * m >= r16) break;
-                                mma(d + kSlice, h + R + 8 * m, w + 2 * m, idesc, k + m != 0);
-                                if (WT == kW32) mma(d + kSlice, h + 8 * m, w + limb + 2 * m, idesc, 1);
-                                mma(d, h + 8 * m, w + 2 * m, idesc, k + m != 0);
+                                for (int m = 0; m < 4; ++m) {
+                                    if (64 * k + 16 * m >= r16) break;
+#pragma unroll
+                                    for (int l = 2; l >= 0; --l)
+                                        mma<true>(d + (l > 0 ? second : 0), h + l * limb_cols + 8 * m, w + 2 * m, idesc,
+                                                  k != 0 || m != 0 || (l != 2 && (l != 0 || !apart)));
+                                }
+                            } else {
+                                const uint32_t h = tmem + h0 + 32 * k;
+#pragma unroll
+                                for (int m = 0; m < 4; ++m) {
+                                    if (32 * k + 8 * m >= r16) break;
+                                    mma<false>(d + second, h + limb_cols + 8 * m, w + 2 * m, idesc, k + m != 0);
+                                    if (WT == kW32) mma<false>(d + second, h + 8 * m, w + kBytes / 32 + 2 * m, idesc, 1);
+                                    mma<false>(d, h + 8 * m, w + 2 * m, idesc, k + m != 0 || !apart);
+                                }
                             }
-                            mma_commit(&b.w_empty[st]);
+                            mma_commit(&b.v_empty[st]);
                             if (k == steps - 1) mma_commit(&b.y_full[buf]);
                         }
                         __syncwarp();
-                        ++entry;
+                        ++e;
                     }
                     ++done;
                 }
@@ -714,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
 
 template <int WT>
 cudaError_t launch(const LoraArgs &a, const LoraMaps &maps, cudaStream_t s) {
-    const int smem = 1024 + kRowWarps * kDepth * kSlot + a.ring * a.ring_bytes + kRaw * a.raw_bytes;
+    const int smem = 1024 + kRowWarps * kDepth * kSlot + a.ring * a.ring_bytes + a.raw_total;
     cudaError_t e = cudaFuncSetAttribute(lora_tiles_kernel<WT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -738,8 +898,11 @@ bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
     const int ranks = a.split ? r16 : r16 * a.n_proj;
     if (ranks > most || !a.x_vec || !a.y_vec) return false;
     a.ring_bytes = limbs * std::max(ranks, kSlice) * 128;
-    a.raw_bytes = std::max((ranks * 4 + 127) / 128, 2) * 128 * 16 * limbs;
-    a.ring = std::min(kMaxRing, (224 * 1024 - kRowWarps * kDepth * kSlot - kRaw * a.raw_bytes) / a.ring_bytes);
+    a.raw_bytes = (ranks * 4 + 127) / 128 * 128 * 16 * limbs;
+    // (bf16: none on the way; others: four stages of A, five of B)
+    a.raw_total = type == 2 ? 0 : std::max(kRaw * a.raw_bytes, (kAhead + 1) * 2 * 128 * 16 * limbs);
+    a.ring = std::min(kMaxRing, (224 * 1024 - kRowWarps * kDepth * kSlot - a.raw_total) / a.ring_bytes);
+    if (a.ring < 2) return false;
     const int chunk = std::min(a.rows, kLoraChunk);
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (kTile - 1)) / kTile);
     // CTAs per tile: the fewest rounds of the SMs in all, counting what a CTA takes beside its share (as much as a
