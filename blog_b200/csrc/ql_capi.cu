@@ -1601,8 +1601,8 @@ bool rows_map(CUtensorMap *out, bool bf16, const void *base, int64_t width, int6
 }
 // Those of a call in tiles of 128 rows.
 bool lora_maps(LoraMaps &m, const LoraArgs &a, int64_t width, bool bf16) {
-    if (!rows_map(&m.x, false, a.x, a.in_dim, a.rows, a.x_stride, 32) || !rows_map(&m.y, false, a.y, width, a.rows, a.y_stride, 32) ||
-        !rows_map(&m.base, false, a.base ? a.base : a.y, width, a.rows, a.base ? a.base_stride : a.y_stride, 32))
+    if (!rows_map(&m.x, false, a.x, a.in_dim, a.rows, a.x_stride, kLoraTile) || !rows_map(&m.y, false, a.y, width, a.rows, a.y_stride, kLoraTile) ||
+        !rows_map(&m.base, false, a.base ? a.base : a.y, width, a.rows, a.base ? a.base_stride : a.y_stride, kLoraTile))
         return false;
     for (int p = 0; p < a.n_proj && bf16; ++p)
         if (a.a[p] && !rows_map(&m.a[p], true, a.a[p], a.in_dim, (int64_t)a.n_adapters * a.max_rank, a.in_dim, 16)) return false;

@@ -33,7 +33,7 @@ struct LoraArgs {
     int *err;
 };
 
-// x, base and y as rows of f32, in boxes of 32 columns and 32 rows (base: y's where there is none); bf16 A as rows of
+// x, base and y as rows of f32, in boxes of 32 columns and a tile's rows (base: y's where there is none); bf16 A as rows of
 // ranks, in boxes of 64 columns and 16 ranks.
 struct LoraMaps {
     CUtensorMap x, base, y, a[kLoraMaxProj];

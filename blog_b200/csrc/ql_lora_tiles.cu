@@ -32,7 +32,7 @@ namespace {
 constexpr int kThreads = 512, kRowWarps = 8;
 constexpr int kTile = kLoraTile, kDepth = 4;   // rows; blocks of a warp in flight and in use
 constexpr int kSlice = 64;                     // outputs of one product
-constexpr int kSlot = 32 * 128;                // bytes of a warp's block: 32 rows of 32 values
+constexpr int kSlot = 32 * 128;                // bytes of a warp's block: 32 rows of 32 values; four lie together
 constexpr int kMaxRing = 4, kRaw = 4;          // stages of widened weights, and of weights on their way
 constexpr int kMaxOut = 8, kAhead = 4;         // stages of 64 rows of B, and how far ahead they are asked for
 static_assert(kAhead <= 4, "the waits for copies");
@@ -42,7 +42,7 @@ constexpr int kRowRegs = 184, kOtherRegs = 72;
 static_assert(2 * kRowRegs + 2 * kOtherRegs == 4 * 128, "the block's registers at launch");
 
 struct Bars {
-    uint64_t land[kRowWarps][kDepth];          // a warp's blocks from memory
+    uint64_t land[2][kDepth], free[2][kDepth];  // blocks of x, then of the base, by half of the row warps
     uint64_t x_full[2], x_empty[2];            // x's limbs, by parity of the block
     uint64_t w_full[kMaxRing], w_empty[kMaxRing];  // stages of A
     uint64_t v_free, v_full[kMaxOut], v_empty[kMaxOut];  // A's stages are all read: B's take their place
@@ -154,7 +154,6 @@ __device__ __forceinline__ void tma_store_2d(const void *map, int c0, int c1, ui
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(reinterpret_cast<uint64_t>(map)),
                  "r"(c0), "r"(c1), "r"(src)
                  : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 template <int N>
 __device__ __forceinline__ void stores_read() {  // all but the last N have read their shared memory
@@ -195,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     constexpr bool B16 = WT == kWB16;
     constexpr int LW = WT == kW32 ? 2 : 1;  // limbs of a weight
     constexpr int kGroup = 4 / LW;          // blocks of 32 columns between two sums in registers
+    constexpr int NC = 6 / LW;              // groups of 16 ranks that a row warp sums, at most
     constexpr int kPer = B16 ? 64 : 32;     // columns of a stage of A, ranks of a stage of B: rows of 128 bytes
     extern __shared__ uint8_t sm_raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~uintptr_t(1023));
@@ -250,11 +250,10 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     const int out_cols = apart ? 2 * kSlice : kSlice, bufs = h_cols + 2 * out_cols <= 512 ? 2 : 1;
     auto out_at = [&](int buf) { return 512u - out_cols * (buf + 1); };
 
-    // a row warp's rows: how many there are, and whether they lie together
-    const int q32 = (warp & 3) * 32, live = warp < kRowWarps ? max(0, min(32, tile.n - q32)) : 0;
-    const int row0 = live > 0 ? uni(list[q32]) : 0;
-    const bool together = live > 0 && uni(list[q32 + live - 1]) - row0 == live - 1;
-    if (live > 0 && lane < kDepth) mbar_init(&b.land[warp][lane], together ? 1 : 32);
+    // Whether the tile's rows lie together: then one warp asks for them in tiled copies of 128 rows (of another sequence's
+    // among them where the tile has fewer), and sends y off; else the row warps copy theirs 16 bytes at a time.
+    const int row0 = uni(list[0]);
+    const bool joint = uni(list[tile.n - 1]) - row0 == tile.n - 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b.x_full[i], 4), mbar_init(&b.x_empty[i], 1);
@@ -264,10 +263,15 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         for (int i = 0; i < kMaxRing; ++i) mbar_init(&b.w_full[i], B16 ? 1 : 4), mbar_init(&b.w_empty[i], 1);
         for (int i = 0; i < kMaxOut; ++i) mbar_init(&b.v_full[i], 4), mbar_init(&b.v_empty[i], 1);
         mbar_init(&b.v_free, 1);
+        for (int i = 0; i < 2; ++i)
+            for (int k = 0; k < kDepth; ++k) {
+                mbar_init(&b.land[i][k], joint ? 1 : (tile.n + 31) / 32 * 32);
+                mbar_init(&b.free[i][k], 4);
+            }
         mbar_init(&b.h_full, kRowWarps);
         b.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (warp == 12) tmem_alloc(&b.tmem, 512);
     tc_fence_before();
     __syncthreads();
@@ -289,96 +293,66 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         return true;
     };
 
+    // a half's 32 of a slice's 64 outputs: the first column of y, and how many there are
+    auto col_of = [&](const Slice &s, int half) { return a.col[s.p] + s.o0 + 32 * half; };
+    auto width_of = [&](const Slice &s, int half) { return min(32, a.out[s.p] - s.o0 - 32 * half); };
+    // slots of the ring that the shares of h take, until the cluster's second barrier
+    const int taken = (R * kTile * 4 + kRowWarps * kSlot - 1) / (kRowWarps * kSlot);
+
     if (warp < kRowWarps) {
         // ------------------------------------ rows: a thread per row and parity ------------------------------------
         reg_inc<kRowRegs>();
         const int q = warp & 3, wg = warp >> 2;
+        const int live = max(0, min(32, tile.n - 32 * q));
         uint8_t *mine = ring + warp * kSlot;  // (its slots kRowWarps * kSlot apart)
         const uint32_t lanes = (uint32_t)(32 * q) << 16;
         auto place = [&](int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) * 16)); };
         auto slot_of = [&](int m) { return mine + (m % kDepth) * (kRowWarps * kSlot); };
-        int issued = 0, used = 0;  // blocks asked for, and taken
-        // 32 columns of this warp's rows into the next slot: one tiled copy where the rows lie together (in rows that are
-        // another sequence's, too), 16 bytes per lane elsewhere
-        auto fetch = [&](const CUtensorMap &map, const float *from, int64_t stride, int col, int width) {
+        int issued = 0, used = 0;  // blocks asked for (by this warp), and taken
+        // 32 columns of this warp's rows into the next slot, where the tile's rows do not lie together
+        auto fetch = [&](const float *from, int64_t stride, int col, int width) {
             if (live > 0) {
-                uint64_t *bar = &b.land[warp][issued % kDepth];
                 const uint32_t dst = smem_u32(slot_of(issued));
-                if (together) {
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(bar, kSlot);
-                        tma_box2d(slot_of(issued), &map, col, row0, bar);
-                    }
-                } else {
-                    const int c = (lane & 7) * 4;
+                const int c = (lane & 7) * 4;
 #pragma unroll
-                    for (int it = 0; it < 8; ++it) {
-                        const int r = 4 * it + lane / 8;
-                        if (r < live && c < width) copy16(dst + place(r, lane & 7), from + list[32 * q + r] * stride + col + c);
-                    }
-                    cp_async_mbar_arrive(bar);
+                for (int it = 0; it < 8; ++it) {
+                    const int r = 4 * it + lane / 8;
+                    if (r < live && c < width) copy16(dst + place(r, lane & 7), from + list[32 * q + r] * stride + col + c);
                 }
+                cp_async_mbar_arrive(&b.land[wg][issued % kDepth]);
             }
             ++issued;
         };
-        auto landed = [&](int m) {
-            return live == 0 || __all_sync(0xffffffffu, wait(&b.land[warp][m % kDepth], m / kDepth));
+        auto landed = [&] {
+            return (!joint && live == 0) || __all_sync(0xffffffffu, wait(&b.land[wg][used % kDepth], used / kDepth));
+        };
+        auto give_back = [&] {  // the slot in use
+            __syncwarp();
+            if (joint && lane == 0) mbar_arrive(&b.free[wg][used % kDepth]);
+            ++used;
         };
         bool ok = true;
-        // this warp's 32 of a slice's 64 outputs: the first column of y, and how many there are
-        auto col_of = [&](const Slice &s) { return a.col[s.p] + s.o0 + 32 * wg; };
-        auto width_of = [&](const Slice &s) { return min(32, a.out[s.p] - s.o0 - 32 * wg); };
-        int asked = j0;  // outputs whose base has been asked for
-        int taken = 0;   // slots that the shares of h stand in, until they are read by all (the cluster's second barrier)
-        auto free_slots = [&] {
-            if (taken == 0) return;
-            taken = 0;
-            cluster_wait();
-            fence_proxy_async_smem();
-        };
-        Slice next = from;
-        auto fetch_base = [&] {
-            if (asked < j1) {
-                const int width = width_of(next);
-                if (width > 0) {
-                    if (issued % kDepth < taken) free_slots();
-                    if (a.base != nullptr)
-                        fetch(maps.base, a.base, a.base_stride, col_of(next), width);
-                    else
-                        ++issued;
-                }
-                next.step(a);
-            }
-            ++asked;
-        };
         if (R > 0) {
-            float sum[6][16];
+            float sum[NC][16];
 #pragma unroll
-            for (int c = 0; c < 6; ++c)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sum[c][e] = 0.f;
-            auto fetch_x = [&](int k) {  // block wg + 2 k
-                if (wg + 2 * k < n_blocks) fetch(maps.x, a.x, a.x_stride, (i0 + wg + 2 * k) * 32, 32);
-            };
             int settled = 0;
             auto settle = [&] {  // one more group of blocks
                 const int buf = settled & 1;
                 if (!__all_sync(0xffffffffu, wait(&b.sum_full[buf], settled >> 1))) return false;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < 6; c += 2) {
-                    uint32_t v[2][16];
-                    const uint32_t at = tmem + lanes + buf * (kLimbs / 2) + (2 * c + wg) * 16;
+                for (int c = 0; c < NC; ++c) {
+                    const int col = (2 * c + wg) * 16;
+                    if (col < R) {
+                        uint32_t v[16];
+                        tmem_ld16(tmem + lanes + buf * (kLimbs / 2) + col, v);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if ((2 * (c + i) + wg) * 16 < R) tmem_ld16(at + 32 * i, v[i]);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if ((2 * (c + i) + wg) * 16 < R) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) sum[c + i][e] += __uint_as_float(v[i][e]);
-                        }
+                        for (int e = 0; e < 16; ++e) sum[c][e] += __uint_as_float(v[e]);
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -386,34 +360,49 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 ++settled;
                 return true;
             };
-            for (int k = 0; k < kDepth - 1; ++k) fetch_x(k);
+            int asked = wg;  // the next block to ask for
+            auto fetch_x = [&] {
+                if (!joint && asked < n_blocks) fetch(a.x, a.x_stride, (i0 + asked) * 32, 32);
+                asked += 2;
+            };
+            for (int k = 0; k < kDepth; ++k) fetch_x();
+            float4 v[8];  // this row's part of a block
+            auto take = [&] {
+                if (!landed()) return false;
+                const uint8_t *slot = slot_of(used);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const float4 *>(slot + place(lane, c));
+                give_back();
+                fetch_x();
+                return true;
+            };
+            if (wg < n_blocks) ok = take();
             const uint32_t limbs_at = tmem + lanes + kLimbs + wg * 64;
-            for (int k = 0; wg + 2 * k < n_blocks && ok; ++k) {
-                ok = landed(k) && (k == 0 || __all_sync(0xffffffffu, wait(&b.x_empty[wg], k - 1)));
+            for (int i = wg; i < n_blocks && ok; i += 2) {
+                if (i >= 2) ok = __all_sync(0xffffffffu, wait(&b.x_empty[wg], (i >> 1) - 1));
                 if (!ok) break;
                 tc_fence_after();
-                const uint8_t *slot = slot_of(k);
-                if constexpr (B16) {
-                    uint32_t l[3][16];
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const float4 v = *reinterpret_cast<const float4 *>(slot + place(lane, c));
-                        limbs_b16(v.x, v.y, l[0][2 * c], l[1][2 * c], l[2][2 * c]);
-                        limbs_b16(v.z, v.w, l[0][2 * c + 1], l[1][2 * c + 1], l[2][2 * c + 1]);
-                    }
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (B16) {
+                        uint32_t l[3][8];
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) tmem_st16(limbs_at + 16 * i, l[i]);
-                } else {
+                        for (int c = 0; c < 4; ++c) {
+                            const float4 w = v[4 * h + c];
+                            limbs_b16(w.x, w.y, l[0][2 * c], l[1][2 * c], l[2][2 * c]);
+                            limbs_b16(w.z, w.w, l[0][2 * c + 1], l[1][2 * c + 1], l[2][2 * c + 1]);
+                        }
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                        for (int n = 0; n < 3; ++n) tmem_st8(limbs_at + 16 * n + 8 * h, l[n]);
+                    } else {
                         uint32_t hi[16], lo[16];
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            const float4 v = *reinterpret_cast<const float4 *>(slot + place(lane, 4 * h + c));
-                            limbs(v.x, hi[4 * c], lo[4 * c]);
-                            limbs(v.y, hi[4 * c + 1], lo[4 * c + 1]);
-                            limbs(v.z, hi[4 * c + 2], lo[4 * c + 2]);
-                            limbs(v.w, hi[4 * c + 3], lo[4 * c + 3]);
+                            const float4 w = v[4 * h + c];
+                            limbs(w.x, hi[4 * c], lo[4 * c]);
+                            limbs(w.y, hi[4 * c + 1], lo[4 * c + 1]);
+                            limbs(w.z, hi[4 * c + 2], lo[4 * c + 2]);
+                            limbs(w.w, hi[4 * c + 3], lo[4 * c + 3]);
                         }
                         tmem_st16(limbs_at + 16 * h, hi);
                         tmem_st16(limbs_at + 32 + 16 * h, lo);
@@ -421,28 +410,24 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                __syncwarp();  // (every lane has read its row: the slot before this one's may be filled)
+                __syncwarp();
                 if (lane == 0) mbar_arrive(&b.x_full[wg]);
-                ++used;
-                fetch_x(k + kDepth - 1);
+                __syncwarp();
+                if (i + 2 < n_blocks) ok = take();
                 // the groups before this block's
-                while (ok && settled < (wg + 2 * k) / kGroup) ok = settle();
+                while (ok && settled < i / kGroup) ok = settle();
             }
             while (ok && settled < groups) ok = settle();
             // the CTA's share of h, a rank's rows together; the slots of x are all read by now
             asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
-            for (int c = 0; c < 6; ++c) {
+            for (int c = 0; c < NC; ++c) {
                 const int col = (2 * c + wg) * 16;
                 if (col < R) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) shares[(col + e) * kTile + 32 * q + lane] = sum[c][e];
                 }
             }
-            // meanwhile the base into slots that the shares leave free
-            taken = (R * kTile * 4 + kRowWarps * kSlot - 1) / (kRowWarps * kSlot);
-            if (ok)
-                for (int k = 0; k < kDepth - 1 && issued % kDepth >= taken; ++k) fetch_base();
             __syncwarp();
             cluster_arrive();
             cluster_wait();
@@ -491,20 +476,36 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             if (lane == 0) mbar_arrive(&b.h_full);
             __syncwarp();
             cluster_arrive();  // the shares are read
+            cluster_wait();
         }
         // outputs: 64 at a time, this warp's 32 rows and half of the columns
+        Slice next = from;
+        int asked = j0;
+        auto fetch_base = [&] {  // the next base to ask for
+            for (; asked < j1 && !joint && a.base != nullptr; ++asked) {
+                const int width = width_of(next, wg), col = col_of(next, wg);
+                next.step(a);
+                if (width > 0) {
+                    fetch(a.base, a.base_stride, col, width);
+                    ++asked;
+                    return;
+                }
+            }
+        };
         if (ok)
-            while (asked < j0 + kDepth - 1) fetch_base();
+            for (int k = 0; k < kDepth; ++k) fetch_base();
         int done = 0;  // products so far
         Slice s = from;
         for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
-            const int col = col_of(s), width = width_of(s);
+            const int col = col_of(s, wg), width = width_of(s, wg);
             const bool any = width > 0, has = pick(need, s.p) >= 0;
             uint8_t *slot = slot_of(used);
             float4 w[8];
-            if (any && a.base != nullptr) {
-                ok = landed(used);
+            if (any && (joint || a.base != nullptr)) {
+                ok = landed();
                 if (!ok) break;
+            }
+            if (any && a.base != nullptr) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) w[c] = *reinterpret_cast<const float4 *>(slot + place(lane, c));
             } else {
@@ -545,10 +546,8 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
 #pragma unroll
                     for (int c = 0; c < 8; ++c) *reinterpret_cast<float4 *>(slot + place(lane, c)) = w[c];
                 }
-                if (together && live == 32 && width == 32) {
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) tma_store_2d(&maps.y, col, row0, smem_u32(slot));
+                if (joint && tile.n == kTile && width == 32) {
+                    fence_proxy_async_smem();  // (it is sent off when all four warps have written theirs)
                 } else {
                     __syncwarp();
                     const int c = (lane & 7) * 4;
@@ -560,17 +559,11 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                                 *reinterpret_cast<const float4 *>(slot + place(r, lane & 7));
                     }
                 }
-                ++used;
+                give_back();
+                fetch_base();
             }
-            if (lane == 0) stores_read<1>();
-            __syncwarp();  // (the slot before this one's is free)
-            fetch_base();
         }
-        free_slots();
-        // never leave with copies in flight
-        if (live > 0 && (a.base != nullptr || used < issued))
-            for (int m = used; m < issued; ++m) mbar_wait(&b.land[warp][m % kDepth], (uint32_t)(m / kDepth) & 1u, nullptr, 0);
-        if (lane == 0) stores_read<0>();
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
         reg_dec<128>();
     } else if (warp < 12) {
@@ -766,6 +759,86 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             __syncwarp();
             cluster_wait();
         }
+    } else if (warp == 13) {
+        // ------------------------------------ rows that lie together, to and from memory ------------------------------------
+        reg_dec<kOtherRegs>();
+        int issued[2] = {0, 0};
+        bool ok = true;
+        auto load = [&](int half, const CUtensorMap *map, int col) {  // null: the slot only
+            const int m = issued[half], st = m % kDepth;
+            if (m >= kDepth && !wait(&b.free[half][st], m / kDepth - 1)) return false;
+            if (map != nullptr) {
+                mbar_arrive_expect_tx(&b.land[half][st], 4 * kSlot);
+                tma_box2d(ring + (st * kRowWarps + 4 * half) * kSlot, map, col, row0, &b.land[half][st]);
+            } else {
+                mbar_arrive(&b.land[half][st]);
+            }
+            ++issued[half];
+            return true;
+        };
+        Slice next[2] = {from, from};
+        int asked[2] = {j0, j0};
+        // the next base of a half, unless its slot is one of those below `from_slot`
+        auto load_base = [&](int half, int from_slot) {
+            while (asked[half] < j1 && width_of(next[half], half) <= 0) next[half].step(a), ++asked[half];
+            if (asked[half] >= j1 || issued[half] % kDepth < from_slot) return false;
+            ok = ok && load(half, a.base != nullptr ? &maps.base : nullptr, col_of(next[half], half));
+            next[half].step(a), ++asked[half];
+            return ok;
+        };
+        int ahead[2] = {0, 0};
+        if (joint && lane == 0) {
+            for (int i = 0; i < n_blocks && ok; ++i) {
+                if (i & 1)
+                    ok = load(1, &maps.x, (i0 + i) * 32);
+                else
+                    ok = load(0, &maps.x, (i0 + i) * 32);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                while (ok && ahead[h] < kDepth && load_base(h, taken)) ++ahead[h];
+        }
+        __syncwarp();
+        if (R > 0) {
+            cluster_arrive();
+            cluster_wait();
+            cluster_arrive();
+            cluster_wait();
+            fence_proxy_async_smem();
+        }
+        if (joint && lane == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                while (ok && ahead[h] < kDepth && load_base(h, 0)) ++ahead[h];
+            int used[2] = {(n_blocks + 1) / 2, n_blocks / 2}, before = -1;
+            Slice s = from;
+            for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int width = width_of(s, h);
+                    if (width <= 0 || !ok) continue;
+                    const int st = used[h] % kDepth;
+                    ok = wait(&b.free[h][st], used[h] / kDepth);
+                    if (!ok) break;
+                    ++used[h];
+                    if (tile.n == kTile && width == 32)
+                        tma_store_2d(&maps.y, col_of(s, h), row0, smem_u32(ring + (st * kRowWarps + 4 * h) * kSlot));
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    // the slot before this one may be filled once it has been read
+                    stores_read<1>();
+                    if (before == 0) load_base(0, 0);
+                    if (before == 1) load_base(1, 0);
+                    before = h;
+                }
+            }
+            // never leave with copies in flight
+            stores_read<0>();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                for (int m = max(0, issued[h] - kDepth); m < issued[h]; ++m)
+                    mbar_wait(&b.land[h][m % kDepth], (uint32_t)(m / kDepth) & 1u, nullptr, 0);
+        }
+        __syncwarp();
     } else {
         // ------------------------------------ products ------------------------------------
         reg_dec<kOtherRegs>();
