@@ -1605,7 +1605,9 @@ bool lora_maps(LoraMaps &m, const LoraArgs &a, int64_t width, bool bf16) {
         !rows_map(&m.base, false, a.base ? a.base : a.y, width, a.rows, a.base ? a.base_stride : a.y_stride, kLoraTile))
         return false;
     for (int p = 0; p < a.n_proj && bf16; ++p)
-        if (a.a[p] && !rows_map(&m.a[p], true, a.a[p], a.in_dim, (int64_t)a.n_adapters * a.max_rank, a.in_dim, 16)) return false;
+        if (a.a[p] && (!rows_map(&m.a16[p], true, a.a[p], a.in_dim, (int64_t)a.n_adapters * a.max_rank, a.in_dim, 16) ||
+                       !rows_map(&m.a64[p], true, a.a[p], a.in_dim, (int64_t)a.n_adapters * a.max_rank, a.in_dim, 64)))
+            return false;
     return true;
 }
 }  // namespace

@@ -34,9 +34,9 @@ struct LoraArgs {
 };
 
 // x, base and y as rows of f32, in boxes of 32 columns and a tile's rows (base: y's where there is none); bf16 A as rows of
-// ranks, in boxes of 64 columns and 16 ranks.
+// ranks, in boxes of 64 columns and 16 or 64 ranks.
 struct LoraMaps {
-    CUtensorMap x, base, y, a[kLoraMaxProj];
+    CUtensorMap x, base, y, a16[kLoraMaxProj], a64[kLoraMaxProj];
 };
 
 enum { kW32, kW16, kWB16 };  // types of the weights
@@ -86,8 +86,8 @@ struct LoraTile {
 // What find_tile needs of shared memory.
 struct LoraFind {
     int starts[kLoraChunk + 1], adapters[kLoraChunk];  // of the sequences, where there are no more
-    int2 kinds[kLoraChunk];                            // per warp: adapters and how many of its rows have them
-    int n_kinds[kLoraChunk / 32], leaders[kLoraChunk / 32];
+    int2 kinds[24 * 32];                               // per warp (24 at most): adapters and how many of its rows have them
+    int n_kinds[24], leaders[24];
     int found[3];
 };
 
@@ -97,7 +97,7 @@ template <int THREADS>
 __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, LoraFind &f, int *list) {
     const int tid = threadIdx.x, lane = tid % 32;
     constexpr int kNone = -1, kOutside = -2;  // of no adapter; of no sequence: left as it is
-    constexpr int kPer = kLoraChunk / THREADS, kWarps = THREADS / 32;
+    constexpr int kPer = (kLoraChunk + THREADS - 1) / THREADS, kWarps = THREADS / 32;
     const bool staged = a.q_start != nullptr && a.n_seqs <= kLoraChunk;
     if (staged)
         for (int i = tid; i <= a.n_seqs; i += THREADS) {

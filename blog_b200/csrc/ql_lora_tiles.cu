@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 }
             };
             if constexpr (B16) {
-                // A as it stands, 64 columns of 16 ranks in a copy (ranks not in use among them: their sums are left out)
+                // A as it stands, 64 columns of 64 or 16 ranks in a copy (ranks not in use among them: their sums are left out)
                 if (wt == 0) {
                     const int n = (n_blocks + 1) / 2;
                     int e = 0;
@@ -603,9 +603,12 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
 #pragma unroll
                         for (int p = 0; p < kLoraMaxProj; ++p)
                             if (first[p] >= 0)
-                                for (int r = 0; r < r16; r += 16)
-                                    tma_box2d(stage + (first[p] + r) * 128, &maps.a[p], (i0 + 2 * e) * 32, tile.id * a.max_rank + r,
-                                              &b.w_full[st]);
+                                for (int r = 0; r < r16;) {
+                                    const bool many = r16 - r >= 64;
+                                    tma_box2d(stage + (first[p] + r) * 128, many ? &maps.a64[p] : &maps.a16[p], (i0 + 2 * e) * 32,
+                                              tile.id * a.max_rank + r, &b.w_full[st]);
+                                    r += many ? 64 : 16;
+                                }
                     }
                     // never leave with copies in flight
                     for (int m = max(0, e - a.ring); m < e; ++m)
@@ -810,7 +813,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 while (ok && ahead[h] < kDepth && load_base(h, 0)) ++ahead[h];
-            int used[2] = {(n_blocks + 1) / 2, n_blocks / 2}, before = -1;
+            // A slot is filled again when its store has read it, three stores later.
+            int used[2] = {(n_blocks + 1) / 2, n_blocks / 2}, stored = 0;
+            unsigned order = 0;  // the halves of the last stores, the latest in bit 0
             Slice s = from;
             for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
 #pragma unroll
@@ -820,15 +825,17 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                     const int st = used[h] % kDepth;
                     ok = wait(&b.free[h][st], used[h] / kDepth);
                     if (!ok) break;
-                    ++used[h];
+                    ++used[h], ++stored, order = order << 1 | h;
                     if (tile.n == kTile && width == 32)
                         tma_store_2d(&maps.y, col_of(s, h), row0, smem_u32(ring + (st * kRowWarps + 4 * h) * kSlot));
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    // the slot before this one may be filled once it has been read
-                    stores_read<1>();
-                    if (before == 0) load_base(0, 0);
-                    if (before == 1) load_base(1, 0);
-                    before = h;
+                    if (stored > 3) {
+                        stores_read<3>();
+                        if (order >> 3 & 1)
+                            load_base(1, 0);
+                        else
+                            load_base(0, 0);
+                    }
                 }
             }
             // never leave with copies in flight
@@ -965,6 +972,32 @@ cudaError_t launch(const LoraArgs &a, const LoraMaps &maps, cudaStream_t s) {
 }
 }  // namespace
 
+namespace {
+// How many clusters of c CTAs the device runs at once (one CTA takes an SM's shared memory; an odd GPC holds fewer).
+int clusters_at_once(int c, int sms) {
+    static std::atomic<int> known[64][9];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return std::max(1, sms / c);
+    int n = known[dev][c].load();
+    if (n == 0) {
+        constexpr int smem = 224 * 1024;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim = {(unsigned)c, 1, 1};
+        cfg.attrs = at, cfg.numAttrs = 1;
+        if (cudaFuncSetAttribute(lora_tiles_kernel<kWB16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, lora_tiles_kernel<kWB16>, &cfg) != cudaSuccess || n <= 0) {
+            (void)cudaGetLastError();
+            n = std::max(1, sms / c);
+        }
+        known[dev][c].store(n);
+    }
+    return n;
+}
+}  // namespace
+
 bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
     const int limbs = type == 0 ? 2 : 1, most = 192 / limbs, r16 = (a.max_rank + 15) / 16 * 16;
     a.split = r16 * a.n_proj > most;
@@ -978,15 +1011,16 @@ bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
     if (a.ring < 2) return false;
     const int chunk = std::min(a.rows, kLoraChunk);
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (kTile - 1)) / kTile);
-    // CTAs per tile: the fewest rounds of the SMs in all, counting what a CTA takes beside its share (as much as a
-    // share of one eighth of 8192 inputs and as many outputs)
-    const int64_t tiles = ((int64_t)a.rows + kTile - 1) / kTile * (a.split ? a.n_proj : 1);
+    // CTAs per tile: what the rounds of the GPU take in all, by the bytes of a CTA's share and what it takes beside it
+    // (as much as 4000 columns).
+    const int64_t tiles = (((int64_t)a.rows + kTile - 1) / kTile + a.n_seqs - 1) * (a.split ? a.n_proj : 1);
+    int64_t width = a.in_dim;
+    for (int p = 0; p < a.n_proj; ++p) width += 2 * a.out[p];
     double best = 0;
     a.cluster = 1;
     for (int c = 1; c <= std::min(8, a.in_dim / 32); ++c) {
-        int64_t width = a.in_dim;
-        for (int p = 0; p < a.n_proj; ++p) width += 2 * a.out[p];
-        const double time = (double)((tiles * c + sms - 1) / sms) * ((double)width / c + 3000.0);
+        const int at_once = clusters_at_once(c, sms);
+        const double time = (double)((tiles + at_once - 1) / at_once) * ((double)width / c + 4000.0);
         if (best == 0 || time < best) best = time, a.cluster = c;
     }
     return true;
