@@ -100,10 +100,12 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
     constexpr int kPer = (kLoraChunk + THREADS - 1) / THREADS, kWarps = THREADS / 32;
     const bool staged = a.q_start != nullptr && a.n_seqs <= kLoraChunk;
     if (staged)
+#pragma unroll 1
         for (int i = tid; i <= a.n_seqs; i += THREADS) {
             f.starts[i] = a.q_start[i];
             if (i < a.n_seqs) f.adapters[i] = a.adapter[i];
         }
+#pragma unroll 1
     for (int i = tid; i < tm; i += THREADS) list[i] = -1;
     if (tid < 3) f.found[tid] = 0;
     __syncthreads();
@@ -118,6 +120,7 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
             int s = r0 + i;
             if (a.q_start != nullptr) {  // the last sequence that starts at or before the row
                 int lo = 0, hi = a.n_seqs + 1;
+#pragma unroll 1
                 while (lo < hi) {
                     const int mid = (lo + hi) / 2;
                     if ((staged ? f.starts[mid] : a.q_start[mid]) <= r0 + i)
@@ -150,10 +153,12 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
         int before = 0;  // rows of this adapter in the warps before
         const unsigned firsts = __ballot_sync(0xffffffffu, first == lane && id[h] != kOutside);
         if (__popc(firsts) <= 4) {  // few kinds: a lane looks through a warp's
+#pragma unroll 1
             for (unsigned left = firsts; left != 0; left &= left - 1) {
                 const int kind = __shfl_sync(0xffffffffu, id[h], __ffs(left) - 1);
                 int n_before = 0;
                 if (lane < w)
+#pragma unroll 1
                     for (int k = 0; k < f.n_kinds[lane]; ++k) {
                         const int2 v = f.kinds[lane * 32 + k];
                         if (v.x == kind) n_before = v.y;
@@ -163,7 +168,9 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
             }
         } else {  // the lowest lane of each looks through all
             if (first == lane && id[h] != kOutside)
+#pragma unroll 1
                 for (int v = 0; v < w; ++v)
+#pragma unroll 1
                     for (int k = 0; k < f.n_kinds[v]; ++k) {
                         const int2 kind = f.kinds[v * 32 + k];
                         if (kind.x == id[h]) before += kind.y;

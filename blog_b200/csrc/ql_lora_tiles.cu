@@ -36,6 +36,7 @@ constexpr int kSlot = 32 * 128;                // bytes of a warp's block: 32 ro
 constexpr int kMaxRing = 4, kRaw = 4;          // stages of widened weights, and of weights on their way
 constexpr int kMaxOut = 8, kAhead = 4;         // stages of 64 rows of B, and how far ahead they are asked for
 static_assert(kAhead <= 4, "the waits for copies");
+constexpr uint32_t kTries = 1u << 27;          // of a wait, each of 20 cycles or more
 constexpr uint32_t kLimbs = 384;               // TMEM columns: h's two accumulators of up to 192, then x's limbs twice
 // Registers per thread of the roles; 16 warps launch with 128 each.
 constexpr int kRowRegs = 184, kOtherRegs = 72;
@@ -169,6 +170,15 @@ __device__ __forceinline__ float remote(uint32_t addr, uint32_t rank) {  // a wo
     return v;
 }
 
+// A place in a ring of n and the round that it is in.
+struct Turn {
+    int at = 0;
+    uint32_t round = 0;
+    __device__ __forceinline__ void next(int n) {
+        if (++at == n) at = 0, ++round;
+    }
+};
+
 // Where outputs stand: 64 columns from o0 of projection p.
 struct Slice {
     int p, o0;
@@ -223,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     if (rank == 0 && a.y == a.base) return;
     const int p0 = a.split ? blockIdx.y : 0, np = a.split ? 1 : a.n_proj;
     const int r16 = (rank + 15) / 16 * 16;
+    auto part_of = [&](int n, int k) { return (int)((uint32_t)n * (uint32_t)k / (uint32_t)parts); };  // (n is below 2^28)
     int first[kLoraMaxProj], R = 0, slices = 0;  // first rank of each projection, all ranks
 #pragma unroll
     for (int p = 0; p < kLoraMaxProj; ++p) {
@@ -231,9 +242,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         slices += (a.out[p] + kSlice - 1) / kSlice;
         if (rank > 0 && a.a[p] != nullptr) first[p] = R, R += r16;
     }
-    const int blocks = a.in_dim / 32, i0 = (int)((int64_t)blocks * part / parts);
-    const int n_blocks = R > 0 ? (int)((int64_t)blocks * (part + 1) / parts) - i0 : 0;
-    const int j0 = (int)((int64_t)slices * part / parts), j1 = (int)((int64_t)slices * (part + 1) / parts);
+    const int blocks = a.in_dim / 32, i0 = part_of(blocks, part);
+    const int n_blocks = R > 0 ? part_of(blocks, part + 1) - i0 : 0;
+    const int j0 = part_of(slices, part), j1 = part_of(slices, part + 1);
     const int groups = (n_blocks + kGroup - 1) / kGroup;
     // the ranks of h that this CTA's outputs need, and their limbs' columns of tensor memory: all first limbs, all second
     Slice from, to;
@@ -255,15 +266,20 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     const int row0 = uni(list[0]);
     const bool joint = uni(list[tile.n - 1]) - row0 == tile.n - 1;
     if (threadIdx.x == 0) {
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
             mbar_init(&b.x_full[i], 4), mbar_init(&b.x_empty[i], 1);
             mbar_init(&b.sum_full[i], 1), mbar_init(&b.sum_empty[i], kRowWarps);
             mbar_init(&b.y_full[i], 1), mbar_init(&b.y_empty[i], kRowWarps);
         }
+#pragma unroll 1
         for (int i = 0; i < kMaxRing; ++i) mbar_init(&b.w_full[i], B16 ? 1 : 4), mbar_init(&b.w_empty[i], 1);
+#pragma unroll 1
         for (int i = 0; i < kMaxOut; ++i) mbar_init(&b.v_full[i], 4), mbar_init(&b.v_empty[i], 1);
         mbar_init(&b.v_free, 1);
+#pragma unroll 1
         for (int i = 0; i < 2; ++i)
+#pragma unroll 1
             for (int k = 0; k < kDepth; ++k) {
                 mbar_init(&b.land[i][k], joint ? 1 : (tile.n + 31) / 32 * 32);
                 mbar_init(&b.free[i][k], 4);
@@ -278,18 +294,16 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     tc_fence_after();
     const uint32_t tmem = uni(b.tmem);
     volatile int *abort_flag = &b.abort;
-    // Bounded wait (about 2 s): false, and everybody told, when it ran out or another role gave up.
-    auto wait = [&](uint64_t *bar, int phase) {
-        if (mbar_try_wait(bar, (uint32_t)phase & 1u)) return true;
-        const long long t0 = clock64();
-        while (!mbar_try_wait(bar, (uint32_t)phase & 1u)) {
-            if (*abort_flag) return false;
-            if (clock64() - t0 > 4000000000ll) {
+    // Bounded wait: false, and everybody told, when it ran out (seconds) or another role gave up.  (Few instructions: there
+    // are many of these, and the roles' code has to stay in the instruction cache.)
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+#pragma unroll 1
+        for (uint32_t n = 0; !mbar_try_wait(bar, parity & 1u); ++n)
+            if (n >= kTries || *abort_flag) {
                 atomicExch(a.err, kErrWaitFull);
                 *abort_flag = 1;
                 return false;
             }
-        }
         return true;
     };
 
@@ -365,6 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 if (!joint && asked < n_blocks) fetch(a.x, a.x_stride, (i0 + asked) * 32, 32);
                 asked += 2;
             };
+#pragma unroll 1
             for (int k = 0; k < kDepth; ++k) fetch_x();
             float4 v[8];  // this row's part of a block
             auto take = [&] {
@@ -378,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             };
             if (wg < n_blocks) ok = take();
             const uint32_t limbs_at = tmem + lanes + kLimbs + wg * 64;
+#pragma unroll 1
             for (int i = wg; i < n_blocks && ok; i += 2) {
                 if (i >= 2) ok = __all_sync(0xffffffffu, wait(&b.x_empty[wg], (i >> 1) - 1));
                 if (!ok) break;
@@ -415,8 +431,10 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 __syncwarp();
                 if (i + 2 < n_blocks) ok = take();
                 // the groups before this block's
+#pragma unroll 1
                 while (ok && settled < i / kGroup) ok = settle();
             }
+#pragma unroll 1
             while (ok && settled < groups) ok = settle();
             // the CTA's share of h, a rank's rows together; the slots of x are all read by now
             asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -433,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             cluster_wait();
             // h's limbs, 16 ranks at a time
             const float scale = a.scale != nullptr ? a.scale[tile.id] : 1.f;
+#pragma unroll 1
             for (int c = wg; c * 16 < n_need; c += 2) {
                 int col = 0, left = 0;  // where the 16 stand among all ranks, and how many of them are in use
 #pragma unroll
@@ -443,6 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 float s[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll 1
                 for (int y = 0; y < parts; y += 4) {  // (four CTAs' loads in flight)
                     float v[4][16];
 #pragma unroll
@@ -482,6 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         Slice next = from;
         int asked = j0;
         auto fetch_base = [&] {  // the next base to ask for
+#pragma unroll 1
             for (; asked < j1 && !joint && a.base != nullptr; ++asked) {
                 const int width = width_of(next, wg), col = col_of(next, wg);
                 next.step(a);
@@ -493,9 +514,11 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             }
         };
         if (ok)
+#pragma unroll 1
             for (int k = 0; k < kDepth; ++k) fetch_base();
-        int done = 0;  // products so far
+        Turn out;  // of the accumulators
         Slice s = from;
+#pragma unroll 1
         for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
             const int col = col_of(s, wg), width = width_of(s, wg);
             const bool any = width > 0, has = pick(need, s.p) >= 0;
@@ -513,8 +536,8 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 for (int c = 0; c < 8; ++c) w[c] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
             if (has) {
-                const int buf = done % bufs;
-                ok = __all_sync(0xffffffffu, wait(&b.y_full[buf], done / bufs));
+                const int buf = out.at;
+                ok = __all_sync(0xffffffffu, wait(&b.y_full[buf], out.round));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t v[32];
@@ -534,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&b.y_empty[buf]);
-                ++done;
+                out.next(bufs);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     w[c].x += __uint_as_float(v[4 * c]), w[c].y += __uint_as_float(v[4 * c + 1]);
@@ -595,14 +618,17 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 if (wt == 0) {
                     const int n = (n_blocks + 1) / 2;
                     int e = 0;
-                    for (; e < n; ++e) {
-                        const int st = e % a.ring;
-                        if (e >= a.ring && !wait(&b.w_empty[st], e / a.ring - 1)) break;
+                    Turn w;
+#pragma unroll 1
+                    for (; e < n; ++e, w.next(a.ring)) {
+                        const int st = w.at;
+                        if (w.round > 0 && !wait(&b.w_empty[st], w.round - 1)) break;
                         mbar_arrive_expect_tx(&b.w_full[st], R * 128);
                         uint8_t *stage = weights + st * a.ring_bytes;
 #pragma unroll
                         for (int p = 0; p < kLoraMaxProj; ++p)
                             if (first[p] >= 0)
+#pragma unroll 1
                                 for (int r = 0; r < r16;) {
                                     const bool many = r16 - r >= 64;
                                     tma_box2d(stage + (first[p] + r) * 128, many ? &maps.a64[p] : &maps.a16[p], (i0 + 2 * e) * 32,
@@ -611,6 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                                 }
                     }
                     // never leave with copies in flight
+#pragma unroll 1
                     for (int m = max(0, e - a.ring); m < e; ++m)
                         mbar_wait(&b.w_full[m % a.ring], (uint32_t)(m / a.ring) & 1u, nullptr, 0);
                 }
@@ -644,10 +671,13 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                     }
                     asm volatile("cp.async.commit_group;" ::: "memory");
                 };
+#pragma unroll 1
                 for (int e = 0; e < kRaw - 1; ++e) fetch(e);
-                for (int e = 0; e < n_blocks; ++e) {
-                    const int st = e % a.ring;
-                    if (e >= a.ring) ok = __all_sync(0xffffffffu, wait(&b.w_empty[st], e / a.ring - 1));
+                Turn t;
+#pragma unroll 1
+                for (int e = 0; e < n_blocks; ++e, t.next(a.ring)) {
+                    const int st = t.at;
+                    if (t.round > 0) ok = __all_sync(0xffffffffu, wait(&b.w_empty[st], t.round - 1));
                     if (!ok) break;
                     asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 2) : "memory");
                     uint8_t *stage = weights + st * a.ring_bytes;
@@ -679,12 +709,14 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 int j, k;
             };
             At ahead{from, j0, 0};
+#pragma unroll 1
             while (ahead.j < j1 && pick(need, ahead.s.p) < 0) ahead.s.step(a), ++ahead.j;
             At here = ahead;
             auto step = [&](At &at) {
                 if (++at.k < steps) return;
                 at.k = 0;
                 do at.s.step(a), ++at.j;
+#pragma unroll 1
                 while (at.j < j1 && pick(need, at.s.p) < 0);
             };
             // this thread's chunk m of 8 ranks: its row and first rank, null where there is none
@@ -696,11 +728,12 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 return static_cast<const char *>(a.b[at.s.p]) + (((int64_t)tile.id * a.out[at.s.p] + o) * a.max_rank + r) * Weight<WT>::bytes;
             };
             int asked = 0, e = 0;
+            Turn to, in;  // of the stages asked for, and given
             uint8_t *raw = weights + a.ring * a.ring_bytes + wt * 16 * LW;
             auto fetch = [&] {
                 if (ahead.j < j1) {
-                    const int st = asked % n_out;
-                    if (asked >= n_out) ok = __all_sync(0xffffffffu, wait(&b.v_empty[st], asked / n_out - 1));
+                    const int st = to.at;
+                    if (to.round > 0) ok = __all_sync(0xffffffffu, wait(&b.v_empty[st], to.round - 1));
                     if (ok) {
 #pragma unroll
                         for (int m = 0; m < kChunks; ++m) {
@@ -725,15 +758,17 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                             }
                         }
                     }
-                    step(ahead);
+                    step(ahead), to.next(n_out);
                     ++asked;
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
             if (ok)
+#pragma unroll 1
                 for (int i = 0; i < n_ahead; ++i) fetch();
+#pragma unroll 1
             while (ok && here.j < j1) {
-                const int st = e % n_out;
+                const int st = in.at;
                 switch (n_ahead) {  // the oldest of them
                 case 4: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
                 case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
@@ -755,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&b.v_full[st]);
                 ++e;
-                step(here);
+                step(here), in.next(n_out);
                 fetch();
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -783,6 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         int asked[2] = {j0, j0};
         // the next base of a half, unless its slot is one of those below `from_slot`
         auto load_base = [&](int half, int from_slot) {
+#pragma unroll 1
             while (asked[half] < j1 && width_of(next[half], half) <= 0) next[half].step(a), ++asked[half];
             if (asked[half] >= j1 || issued[half] % kDepth < from_slot) return false;
             ok = ok && load(half, a.base != nullptr ? &maps.base : nullptr, col_of(next[half], half));
@@ -791,6 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         };
         int ahead[2] = {0, 0};
         if (joint && lane == 0) {
+#pragma unroll 1
             for (int i = 0; i < n_blocks && ok; ++i) {
                 if (i & 1)
                     ok = load(1, &maps.x, (i0 + i) * 32);
@@ -799,6 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
+#pragma unroll 1
                 while (ok && ahead[h] < kDepth && load_base(h, taken)) ++ahead[h];
         }
         __syncwarp();
@@ -812,11 +850,13 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         if (joint && lane == 0) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
+#pragma unroll 1
                 while (ok && ahead[h] < kDepth && load_base(h, 0)) ++ahead[h];
             // A slot is filled again when its store has read it, three stores later.
             int used[2] = {(n_blocks + 1) / 2, n_blocks / 2}, stored = 0;
             unsigned order = 0;  // the halves of the last stores, the latest in bit 0
             Slice s = from;
+#pragma unroll 1
             for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -842,6 +882,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             stores_read<0>();
 #pragma unroll
             for (int h = 0; h < 2; ++h)
+#pragma unroll 1
                 for (int m = max(0, issued[h] - kDepth); m < issued[h]; ++m)
                     mbar_wait(&b.land[h][m % kDepth], (uint32_t)(m / kDepth) & 1u, nullptr, 0);
         }
@@ -853,10 +894,12 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             bool ok = true;
             if (warp == 12) {
                 const uint32_t idesc = idesc_of<B16>(R);
+                Turn w_at;
+#pragma unroll 1
                 for (int i = 0; i < n_blocks && ok; ++i) {
-                    const int wg = i & 1, g = i / kGroup, buf = g & 1, e = B16 ? i >> 1 : i, st = e % a.ring;
+                    const int wg = i & 1, g = i / kGroup, buf = g & 1, st = w_at.at;
                     if (i % kGroup == 0 && g >= 2) ok = wait(&b.sum_empty[buf], g / 2 - 1);
-                    ok = ok && wait(&b.x_full[wg], i >> 1) && wait(&b.w_full[st], e / a.ring);
+                    ok = ok && wait(&b.x_full[wg], i >> 1) && wait(&b.w_full[st], w_at.round);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
@@ -883,6 +926,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                         if (i == n_blocks - 1) mma_commit(&b.v_free);
                     }
                     __syncwarp();
+                    if (!B16 || wg == 1) w_at.next(a.ring);
                 }
             }
             __syncwarp();
@@ -894,17 +938,19 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                 const uint32_t idesc = idesc_of<B16>(kSlice);
                 const int n_out = min(kMaxOut, a.ring * a.ring_bytes / kBytes), steps = (rank + kPer - 1) / kPer;
                 const uint32_t second = apart ? kSlice : 0;  // the lower limbs' accumulators
-                int done = 0, e = 0;
+                Turn in, out;  // the stages of B, and the accumulators
                 Slice s = from;
                 ok = __all_sync(0xffffffffu, wait(&b.h_full, 0));
+#pragma unroll 1
                 for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
                     const int h0 = pick(need, s.p);
                     if (h0 < 0) continue;
-                    const int buf = done % bufs;
-                    if (done >= bufs) ok = __all_sync(0xffffffffu, wait(&b.y_empty[buf], done / bufs - 1));
+                    const int buf = out.at;
+                    if (out.round > 0) ok = __all_sync(0xffffffffu, wait(&b.y_empty[buf], out.round - 1));
+#pragma unroll 1
                     for (int k = 0; k < steps && ok; ++k) {
-                        const int st = e % n_out;
-                        ok = __all_sync(0xffffffffu, wait(&b.v_full[st], e / n_out));
+                        const int st = in.at;
+                        ok = __all_sync(0xffffffffu, wait(&b.v_full[st], in.round));
                         if (!ok) break;
                         tc_fence_after();
                         if (elect_one()) {
@@ -934,9 +980,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                             if (k == steps - 1) mma_commit(&b.y_full[buf]);
                         }
                         __syncwarp();
-                        ++e;
+                        in.next(n_out);
                     }
-                    ++done;
+                    out.next(bufs);
                 }
             }
             __syncwarp();
