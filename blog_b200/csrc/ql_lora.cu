@@ -7,15 +7,19 @@
 // through distributed shared memory in rank order, and each takes its share of the outputs.  So nothing but y is
 // written to memory, and the result does not depend on the order in which CTAs run.
 //
-// Both products run on the tensor cores as mma.sync m16n8k8 with the weights as the 16 rows (tf32 holds f16 and bf16
-// weights exactly) and the tile's rows as the 8 columns, x and h as two tf32 limbs (22 bits), weights of 32 bits as two.
-// A warp reads x and A from memory straight into the registers of its fragments: it has columns of its own, so nothing
-// is shared before the warps' sums.  The tensor cores cut what they add up off towards zero, so their sums are added to
-// others with rounding every 64 columns or 32 ranks.
+// Both products run on the tensor cores (mma.sync) with the weights as the 16 rows and the tile's rows as the 8 columns, so
+// that weights go from memory straight into fragments, which hold them exactly; the fp32 operand is taken apart:
+//   bf16 weights  m16n8k16 bf16, x and h in three bf16 limbs (all of their bits)
+//   f16 weights   x: m16n8k8 tf32, two limbs (22 bits); h: m16n8k16 f16, two limbs of h times a power of two per row (22 bits
+//                 of the row's largest)
+//   f32 weights   m16n8k8 tf32, two limbs on both sides
+// A warp has columns of its own, so nothing is shared before the warps' sums.  The tensor cores cut what they add up off
+// towards zero, so their sums are added to others with rounding every 64 columns or 32 ranks.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ql_lora.cuh"
 
@@ -33,6 +37,17 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+template <bool BF16>
+__device__ __forceinline__ void mma_16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 // A fragment of 16 rows x 8: elements 2 j and 2 j + 1 of the rows g and g + 8, and their second limbs.
 template <int WT>
 __device__ __forceinline__ void fragment(const uint32_t (&r0)[8], const uint32_t (&r1)[8], int j, uint32_t (&hi)[4],
@@ -48,81 +63,146 @@ __device__ __forceinline__ void fragment(const uint32_t (&r0)[8], const uint32_t
     }
 }
 
-// KU: ranks per step of the second product (8, 16 or 32): a lane has KU / 4 consecutive ranks.
-template <int WT, int NT, int KU>
-__device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, int proj, int rank, int part, int parts,
-                                       const int *list, const float *hi, const float *lo, int pitch) {
+// KU: ranks per step of the second product (16 or 32): a lane has KU / 4 consecutive ranks.  OT: tiles of 16 outputs
+// whose loads are under way together.  o_begin .. o_end: this CTA's tiles.
+template <int WT, int NT, int KU, int OT>
+__device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, int proj, int rank, int o_begin, int o_end,
+                                       const int *list, const float *limb, int pitch, const float *unit) {
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int n_out = a.out[proj];
     const int64_t w0 = (int64_t)max(tile.id, 0) * n_out * a.max_rank;
-    for (int o0 = (part * kWarps + warp) * 16; o0 < n_out; o0 += parts * kWarps * 16) {
-        float base[NT][4], acc[NT][4], total[NT][4];
+    int row[NT][2];  // of the two rows that a lane has results of: the outputs of a row lie together
+    bool there[NT][2];
+    float scale[NT][2];  // (f16 limbs: of h's row)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int tok = nt * 8 + 2 * t + q % 2, o = o0 + g + 8 * (q / 2);
-                acc[nt][q] = total[nt][q] = 0.f;
-                base[nt][q] = a.base != nullptr && tok < tile.n && o < n_out
-                                  ? a.base[(int64_t)list[tok] * a.base_stride + a.col[proj] + o]
-                                  : 0.f;
-            }
-        for (int k0 = 0; k0 < rank; k0 += KU) {
-            uint32_t raw[2][8];
-            const int k = k0 + t * (KU / 4);
+        for (int q = 0; q < 2; ++q) {
+            there[nt][q] = nt * 8 + 2 * t + q < tile.n;
+            row[nt][q] = there[nt][q] ? list[nt * 8 + 2 * t + q] : 0;
+            scale[nt][q] = WT == kW16 && rank > 0 ? unit[nt * 8 + 2 * t + q] : 0.f;
+        }
+#pragma unroll 1
+    for (int tile0 = o_begin + warp * OT; tile0 < o_end; tile0 += kWarps * OT) {
+        float base[OT][NT][4], total[OT][NT][4];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) raw[r][i] = 0;
-                const int o = o0 + g + 8 * r;
-                if (o < n_out && k < rank) {
-                    load_weights<WT, KU / 4>(a.b[proj], w0 + (int64_t)o * a.max_rank + k, raw[r]);
-                    if (k + KU / 4 > rank) {  // what stands behind the last rank is of no meaning
-#pragma unroll
-                        for (int i = 0; i < KU / 4; ++i)
-                            if (k + i >= rank) {
-                                if (WT == kW32)
-                                    raw[r][i] = 0;
-                                else
-                                    raw[r][i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
-                            }
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < KU / 8; ++j) {
-                uint32_t wh[4], wl[4];
-                fragment<WT>(raw[0], raw[1], j, wh, wl);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float2 h = *reinterpret_cast<const float2 *>(hi + (nt * 8 + g) * pitch + k + 2 * j);
-                    const float2 l = *reinterpret_cast<const float2 *>(lo + (nt * 8 + g) * pitch + k + 2 * j);
-                    mma_tf32(acc[nt], wh, __float_as_uint(l.x), __float_as_uint(l.y));
-                    if (WT == kW32) mma_tf32(acc[nt], wl, __float_as_uint(h.x), __float_as_uint(h.y));
-                    mma_tf32(acc[nt], wh, __float_as_uint(h.x), __float_as_uint(h.y));
-                }
-            }
+        for (int u = 0; u < OT; ++u)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    total[nt][q] += acc[nt][q];
-                    acc[nt][q] = 0.f;
+                    const int o = (tile0 + u) * 16 + g + 8 * (q / 2);
+                    total[u][nt][q] = 0.f;
+                    base[u][nt][q] = a.base != nullptr && there[nt][q % 2] && tile0 + u < o_end && o < n_out
+                                         ? a.base[(int64_t)row[nt][q % 2] * a.base_stride + a.col[proj] + o]
+                                         : 0.f;
                 }
+#pragma unroll 1
+        for (int k0 = 0; k0 < rank; k0 += KU) {
+            uint32_t raw[OT][2][8];
+            const int k = k0 + t * (KU / 4);
+#pragma unroll
+            for (int u = 0; u < OT; ++u)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) raw[u][r][i] = 0;
+                    const int o = (tile0 + u) * 16 + g + 8 * r;
+                    if (tile0 + u < o_end && o < n_out && k < rank)
+                        load_weights<WT, KU / 4>(a.b[proj], w0 + (int64_t)o * a.max_rank + k, raw[u][r]);
+                }
+            if (k + KU / 4 > rank) {  // what stands behind the last rank is of no meaning
+#pragma unroll
+                for (int u = 0; u < OT; ++u)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int i = 0; i < KU / 4; ++i)
+                            if (k + i >= rank) {
+                                if (WT == kW32)
+                                    raw[u][r][i] = 0;
+                                else
+                                    raw[u][r][i / 2] &= i % 2 ? 0x0000FFFFu : 0xFFFF0000u;
+                            }
+            }
+            float acc[OT][NT][4];
+#pragma unroll
+            for (int u = 0; u < OT; ++u)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[u][nt][q] = 0.f;
+            if constexpr (WT != kW32) {  // 16-bit limbs: those of a lane's ranks lie together
+                constexpr int L = WT == kWB16 ? 3 : 2;
+                const uint16_t *l16 = reinterpret_cast<const uint16_t *>(limb);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int l = L - 1; l >= 0; --l) {
+                        uint32_t h[4] = {0, 0, 0, 0};
+                        const uint16_t *p = l16 + (l * 8 * NT + nt * 8 + g) * pitch + k;
+                        if (KU == 32) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(p);
+                            h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(p);
+                            h[0] = v.x, h[1] = v.y;
+                        }
+#pragma unroll
+                        for (int j = 0; j < KU / 16; ++j)
+#pragma unroll
+                            for (int u = 0; u < OT; ++u)
+                                mma_16<WT == kWB16>(acc[u][nt], raw[u][0][2 * j], raw[u][1][2 * j], raw[u][0][2 * j + 1],
+                                                    raw[u][1][2 * j + 1], h[2 * j], h[2 * j + 1]);
+                    }
+            } else {
+                const float *hi = limb, *lo = limb + 8 * NT * pitch;
+#pragma unroll
+                for (int j = 0; j < KU / 8; ++j) {
+                    float2 h[NT], l[NT];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        h[nt] = *reinterpret_cast<const float2 *>(hi + (nt * 8 + g) * pitch + k + 2 * j);
+                        l[nt] = *reinterpret_cast<const float2 *>(lo + (nt * 8 + g) * pitch + k + 2 * j);
+                    }
+#pragma unroll
+                    for (int u = 0; u < OT; ++u) {
+                        uint32_t wh[4], wl[4];
+                        fragment<WT>(raw[u][0], raw[u][1], j, wh, wl);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_tf32(acc[u][nt], wh, __float_as_uint(l[nt].x), __float_as_uint(l[nt].y));
+                            mma_tf32(acc[u][nt], wl, __float_as_uint(h[nt].x), __float_as_uint(h[nt].y));
+                            mma_tf32(acc[u][nt], wh, __float_as_uint(h[nt].x), __float_as_uint(h[nt].y));
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < OT; ++u)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) total[u][nt][q] += acc[u][nt][q];
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int u = 0; u < OT; ++u)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int tok = nt * 8 + 2 * t + q % 2, o = o0 + g + 8 * (q / 2);
-                if (tok < tile.n && o < n_out)
-                    a.y[(int64_t)list[tok] * a.y_stride + a.col[proj] + o] = base[nt][q] + total[nt][q];
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int o = (tile0 + u) * 16 + g + 8 * (q / 2);
+                    if (there[nt][q % 2] && tile0 + u < o_end && o < n_out)
+                        a.y[(int64_t)row[nt][q % 2] * a.y_stride + a.col[proj] + o] =
+                            WT == kW16 ? __fmaf_rn(total[u][nt][q], scale[nt][q % 2], base[u][nt][q]) : base[u][nt][q] + total[u][nt][q];
+                }
     }
 }
 
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 template <int WT, int NT>
-__global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ LoraArgs a) {
+__global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const __grid_constant__ LoraArgs a) {
     constexpr int TM = 8 * NT, MT = kPass / 16;
     extern __shared__ __align__(16) float smem[];
     __shared__ LoraFind find;
@@ -141,11 +221,30 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
         }
     }
     if (rank == 0 && a.y == a.base) return;
-    const int padded = (a.max_rank + 31) / 32 * 32, pitch = padded + 4;
+    // this CTA's outputs, and what they need asked for while h is computed
+    const int n16 = (a.out[proj] + 15) / 16;
+    const int o_begin = (int)((uint32_t)n16 * part / parts), o_end = (int)((uint32_t)n16 * (part + 1) / parts);
+    if (rank > 0 && o_begin < o_end) {
+        constexpr int el = Weight<WT>::bytes;
+        const int64_t first = (int64_t)tile.id * a.out[proj] + o_begin * 16, rows = min(o_end * 16, a.out[proj]) - o_begin * 16;
+        const char *w = static_cast<const char *>(a.b[proj]) + first * a.max_rank * el;
+        if (2 * rank > a.max_rank) {
+            for (int64_t at = (int64_t)tid * 128; at < rows * a.max_rank * el; at += kThreads * 128) prefetch_l2(w + at);
+        } else {  // (rows with long gaps)
+            for (int r = tid; r < rows; r += kThreads)
+                for (int at = 0; at < rank * el; at += 128) prefetch_l2(w + (int64_t)r * a.max_rank * el + at);
+        }
+    }
+    if (a.base != nullptr)
+        for (int r = warp; r < tile.n; r += kWarps) {
+            const float *p = a.base + (int64_t)list[r] * a.base_stride + a.col[proj];
+            for (int o = o_begin * 16 + lane * 32; o < min(o_end * 16, a.out[proj]); o += 32 * 32) prefetch_l2(p + o);
+        }
+    const int padded = (a.max_rank + 31) / 32 * 32, pitch = padded + (WT == kW32 ? 4 : 8);
     float *h = smem;                    // [padded][TM], this CTA's share; read by its cluster
-    float *hi = smem + padded * TM;     // [TM][pitch] twice: h in two limbs; before that the warps' sums
-    float *lo = hi + TM * pitch;
-    float *sums = hi;                   // [kWarps][kPass][TM]
+    float *limb = smem + padded * TM;   // [limbs][TM][pitch] of h, 16 bits each or 32; before that the warps' sums
+    float *sums = limb;                 // [kWarps][kPass][TM]
+    __shared__ float unit[TM];          // f16 limbs: what a row of them stands for
     cg::cluster_group cl = cg::this_cluster();
     if (rank > 0) {
         const int units = a.in_dim / 32;
@@ -207,19 +306,35 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[i] = p[i];
                     }
+                    if constexpr (WT == kWB16) {
+                        uint32_t l[3][4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t h0, h1, l0, l1;
-                        limbs(v[2 * j], h0, l0);
-                        limbs(v[2 * j + 1], h1, l1);
+                        for (int i = 0; i < 4; ++i) limbs_b16(v[2 * i], v[2 * i + 1], l[0][i], l[1][i], l[2][i]);
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             if (mt >= mts) break;
-                            uint32_t wh[4], wl[4];
-                            fragment<WT>(raw[mt][0], raw[mt][1], j, wh, wl);
-                            mma_tf32(acc[mt][nt], wh, l0, l1);
-                            if (WT == kW32) mma_tf32(acc[mt][nt], wl, h0, h1);
-                            mma_tf32(acc[mt][nt], wh, h0, h1);
+#pragma unroll
+                            for (int n = 2; n >= 0; --n)
+#pragma unroll
+                                for (int j = 0; j < 2; ++j)
+                                    mma_16<true>(acc[mt][nt], raw[mt][0][2 * j], raw[mt][1][2 * j], raw[mt][0][2 * j + 1],
+                                                 raw[mt][1][2 * j + 1], l[n][2 * j], l[n][2 * j + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t h0, h1, l0, l1;
+                            limbs(v[2 * j], h0, l0);
+                            limbs(v[2 * j + 1], h1, l1);
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                if (mt >= mts) break;
+                                uint32_t wh[4], wl[4];
+                                fragment<WT>(raw[mt][0], raw[mt][1], j, wh, wl);
+                                mma_tf32(acc[mt][nt], wh, l0, l1);
+                                if (WT == kW32) mma_tf32(acc[mt][nt], wl, h0, h1);
+                                mma_tf32(acc[mt][nt], wh, h0, h1);
+                            }
                         }
                     }
                 }
@@ -248,7 +363,8 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
         }
         if (parts > 1) cl.sync();
         const float scale = a.scale != nullptr ? a.scale[tile.id] : 1.f;
-        const int upto = rank <= 8 ? 8 : rank <= 16 ? 16 : (rank + 31) / 32 * 32;
+        const int upto = rank <= 16 ? 16 : (rank + 31) / 32 * 32;
+        uint16_t *l16 = reinterpret_cast<uint16_t *>(limb);
         for (int e = tid; e < upto * TM; e += kThreads) {
             const int r = e / TM, tok = e % TM;
             float s = 0.f;
@@ -258,20 +374,58 @@ __global__ void __launch_bounds__(kThreads) lora_kernel(const __grid_constant__ 
                 else
                     s = h[e];
             }
-            uint32_t v0, v1;
-            limbs(s * scale, v0, v1);
-            hi[tok * pitch + r] = __uint_as_float(v0);
-            lo[tok * pitch + r] = __uint_as_float(v1);
+            s *= scale;
+            if constexpr (WT == kWB16) {
+                uint32_t l[3];
+                limbs_b16(s, 0.f, l[0], l[1], l[2]);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) l16[(i * TM + tok) * pitch + r] = (uint16_t)l[i];
+            } else if constexpr (WT == kW16) {
+                limb[tok * pitch + r] = s;  // (taken apart below, when the row's largest is known)
+            } else {
+                uint32_t v0, v1;
+                limbs(s, v0, v1);
+                limb[tok * pitch + r] = __uint_as_float(v0);
+                limb[(TM + tok) * pitch + r] = __uint_as_float(v1);
+            }
+        }
+        if constexpr (WT == kW16) {
+            __syncthreads();
+            uint16_t *to = reinterpret_cast<uint16_t *>(limb + TM * pitch);
+            for (int tok = warp; tok < TM; tok += kWarps) {
+                uint32_t top = 0;  // (magnitudes order like their bits)
+                for (int r = lane; r < rank; r += 32) top = max(top, __float_as_uint(limb[tok * pitch + r]) & 0x7FFFFFFFu);
+                top = __reduce_max_sync(0xffffffffu, top);
+                // 2^f with the largest in [2^10, 2^11), within the normal range
+                const int f = min(max(264 - (int)(top >> 23), 1), 253);
+                const float up = __uint_as_float((uint32_t)f << 23);
+                if (lane == 0) unit[tok] = __uint_as_float((uint32_t)(254 - f) << 23);
+                for (int r = lane; r < upto; r += 32) {
+                    const float v = limb[tok * pitch + r] * up;
+                    const __half a0 = __float2half_rn(v);
+                    to[tok * pitch + r] = __half_as_ushort(a0);
+                    to[(TM + tok) * pitch + r] = __half_as_ushort(__float2half_rn(v - __half2float(a0)));
+                }
+            }
         }
         __syncthreads();
         if (parts > 1) cl.barrier_arrive();  // (its share is read until all have arrived)
     }
-    if (rank <= 8)
-        expand<WT, NT, 8>(a, tile, proj, rank, part, parts, list, hi, lo, pitch);
-    else if (rank <= 16)
-        expand<WT, NT, 16>(a, tile, proj, rank, part, parts, list, hi, lo, pitch);
+    // (several tiles of outputs at a time where every warp has as many)
+    constexpr int OT = NT == 1 ? (WT == kW32 ? 2 : 4) : NT == 2 ? 2 : 1;
+    const bool many = OT > 1 && o_end - o_begin >= kWarps * OT;
+    const float *from = limb + (WT == kW16 ? TM * pitch : 0);
+    auto go = [&](auto ku) {
+        constexpr int KU = decltype(ku)::value;
+        if (many)
+            expand<WT, NT, KU, OT>(a, tile, proj, rank, o_begin, o_end, list, from, pitch, unit);
+        else
+            expand<WT, NT, KU, 1>(a, tile, proj, rank, o_begin, o_end, list, from, pitch, unit);
+    };
+    if (rank <= 16)
+        go(std::integral_constant<int, 16>());
     else
-        expand<WT, NT, 32>(a, tile, proj, rank, part, parts, list, hi, lo, pitch);
+        go(std::integral_constant<int, 32>());
     if (rank > 0 && parts > 1) cl.barrier_wait();
 }
 
@@ -279,7 +433,8 @@ template <int WT, int NT>
 cudaError_t launch(const LoraArgs &a, cudaStream_t s) {
     constexpr int TM = 8 * NT;
     const int padded = (a.max_rank + 31) / 32 * 32;
-    const size_t smem = sizeof(float) * (padded * TM + std::max(2 * TM * (padded + 4), kWarps * kPass * TM));
+    // h, and the larger of its limbs (f16: with h once more before them) and the warps' sums
+    const size_t smem = sizeof(float) * (padded * TM + std::max(2 * TM * (padded + 8), kWarps * kPass * TM));
     cudaError_t e = cudaFuncSetAttribute(lora_kernel<WT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};

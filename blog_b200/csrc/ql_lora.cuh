@@ -47,6 +47,16 @@ __device__ __forceinline__ void limbs(float v, uint32_t &hi, uint32_t &lo) {
     lo = (__float_as_uint(v - __uint_as_float(hi)) + 0x1000u) & 0xFFFFE000u;
 }
 
+// Two values in three bf16 limbs, cut off one after another (8 bits each: nothing is left), packed.
+__device__ __forceinline__ void limbs_b16(float x, float y, uint32_t &a, uint32_t &b, uint32_t &c) {
+    constexpr uint32_t m = 0xFFFF0000u;
+    a = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    const float x1 = x - __uint_as_float(__float_as_uint(x) & m), y1 = y - __uint_as_float(__float_as_uint(y) & m);
+    b = __byte_perm(__float_as_uint(x1), __float_as_uint(y1), 0x7632);
+    const float x2 = x1 - __uint_as_float(__float_as_uint(x1) & m), y2 = y1 - __uint_as_float(__float_as_uint(y1) & m);
+    c = __byte_perm(__float_as_uint(x2), __float_as_uint(y2), 0x7632);
+}
+
 template <int WT>
 struct Weight {
     static constexpr int bytes = WT == kW32 ? 4 : 2;
@@ -98,6 +108,28 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
     const int tid = threadIdx.x, lane = tid % 32;
     constexpr int kNone = -1, kOutside = -2;  // of no adapter; of no sequence: left as it is
     constexpr int kPer = (kLoraChunk + THREADS - 1) / THREADS, kWarps = THREADS / 32;
+    if (a.q_start == nullptr && n <= 32) {  // a few single tokens: every warp finds the tile by itself
+        int id = kOutside;
+        if (lane < n) {
+            id = a.adapter[r0 + lane];
+            if (id >= a.n_adapters) {
+                atomicExch(a.err, kErrAdapter);
+                id = kNone;
+            }
+            id = max(id, kNone);
+        }
+        const unsigned same = __match_any_sync(0xffffffffu, id);
+        const int place = __popc(same & ((1u << lane) - 1));
+        unsigned leaders = __ballot_sync(0xffffffffu, id != kOutside && place % tm == 0);
+        for (int k = 0; k < t && leaders != 0; ++k) leaders &= leaders - 1;
+        if (leaders == 0) return LoraTile{0, 0, 0};
+        const int at = __ffs(leaders) - 1;
+        const LoraTile found{__shfl_sync(0xffffffffu, id, at), __shfl_sync(0xffffffffu, place, at),
+                             min(tm, __popc(__shfl_sync(0xffffffffu, same, at)) - __shfl_sync(0xffffffffu, place, at))};
+        if (tid < 32 && id == found.id && place >= found.first && place < found.first + tm) list[place - found.first] = r0 + lane;
+        __syncthreads();
+        return found;
+    }
     const bool staged = a.q_start != nullptr && a.n_seqs <= kLoraChunk;
     if (staged)
 #pragma unroll 1

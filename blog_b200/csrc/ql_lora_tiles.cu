@@ -120,15 +120,6 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t *v) {
                  "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
-// Two values in three bf16 limbs, cut off one after another (8 bits each: nothing is left), packed.
-__device__ __forceinline__ void limbs_b16(float x, float y, uint32_t &a, uint32_t &b, uint32_t &c) {
-    constexpr uint32_t m = 0xFFFF0000u;
-    a = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-    const float x1 = x - __uint_as_float(__float_as_uint(x) & m), y1 = y - __uint_as_float(__float_as_uint(y) & m);
-    b = __byte_perm(__float_as_uint(x1), __float_as_uint(y1), 0x7632);
-    const float x2 = x1 - __uint_as_float(__float_as_uint(x1) & m), y2 = y1 - __uint_as_float(__float_as_uint(y1) & m);
-    c = __byte_perm(__float_as_uint(x2), __float_as_uint(y2), 0x7632);
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ bool elect_one() {
@@ -1059,7 +1050,7 @@ bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (kTile - 1)) / kTile);
     // CTAs per tile: what the rounds of the GPU take in all, by the bytes of a CTA's share and what it takes beside it
     // (as much as 4000 columns).
-    const int64_t tiles = (((int64_t)a.rows + kTile - 1) / kTile + a.n_seqs - 1) * (a.split ? a.n_proj : 1);
+    const int64_t tiles = (((int64_t)a.rows + kTile - 1) / kTile + distinct - 1) * (a.split ? a.n_proj : 1);
     int64_t width = a.in_dim;
     for (int p = 0; p < a.n_proj; ++p) width += 2 * a.out[p];
     double best = 0;
