@@ -64,7 +64,9 @@ __device__ __forceinline__ void fragment(const uint32_t (&r0)[8], const uint32_t
 }
 
 // KU: ranks per step of the second product (16 or 32): a lane has KU / 4 consecutive ranks.  OT: tiles of 16 outputs
-// whose loads are under way together.  o_begin .. o_end: this CTA's tiles.
+// whose loads are under way together (2 or 4).  A lane's outputs lie side by side, so that its rows of base and y are read
+// and written 16 bytes at a time: row g + 8 r of tile u is output 32 (u / 2) + 4 g + 2 (u % 2) + r.  o_begin .. o_end: this
+// CTA's groups of 32 outputs.
 template <int WT, int NT, int KU, int OT>
 __device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, int proj, int rank, int o_begin, int o_end,
                                        const int *list, const float *limb, int pitch, const float *unit) {
@@ -83,20 +85,37 @@ __device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, 
             scale[nt][q] = WT == kW16 && rank > 0 ? unit[nt * 8 + 2 * t + q] : 0.f;
         }
 #pragma unroll 1
-    for (int tile0 = o_begin + warp * OT; tile0 < o_end; tile0 += kWarps * OT) {
-        float base[OT][NT][4], total[OT][NT][4];
+    for (int group = o_begin + warp * (OT / 2); group < o_end; group += kWarps * (OT / 2)) {
+        const int o_end1 = min(n_out, o_end * 32);
+        auto out_of = [&](int u, int r) { return (group + u / 2) * 32 + 4 * g + 2 * (u % 2) + r; };
+        // base and result: [pair of tiles][token][4 outputs]
+        float total[OT][NT][4];
+        float4 base[OT / 2][NT][2];
+#pragma unroll
+        for (int v = 0; v < OT / 2; ++v)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int o = out_of(2 * v, 0);
+                    base[v][nt][q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (a.base == nullptr || !there[nt][q]) continue;
+                    const float *p = a.base + (int64_t)row[nt][q] * a.base_stride + a.col[proj] + o;
+                    if (a.y_vec && o + 3 < o_end1) {
+                        base[v][nt][q] = *reinterpret_cast<const float4 *>(p);
+                    } else {
+                        if (o < o_end1) base[v][nt][q].x = p[0];
+                        if (o + 1 < o_end1) base[v][nt][q].y = p[1];
+                        if (o + 2 < o_end1) base[v][nt][q].z = p[2];
+                        if (o + 3 < o_end1) base[v][nt][q].w = p[3];
+                    }
+                }
 #pragma unroll
         for (int u = 0; u < OT; ++u)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int o = (tile0 + u) * 16 + g + 8 * (q / 2);
-                    total[u][nt][q] = 0.f;
-                    base[u][nt][q] = a.base != nullptr && there[nt][q % 2] && tile0 + u < o_end && o < n_out
-                                         ? a.base[(int64_t)row[nt][q % 2] * a.base_stride + a.col[proj] + o]
-                                         : 0.f;
-                }
+                for (int q = 0; q < 4; ++q) total[u][nt][q] = 0.f;
 #pragma unroll 1
         for (int k0 = 0; k0 < rank; k0 += KU) {
             uint32_t raw[OT][2][8];
@@ -107,8 +126,8 @@ __device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, 
                 for (int r = 0; r < 2; ++r) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) raw[u][r][i] = 0;
-                    const int o = (tile0 + u) * 16 + g + 8 * r;
-                    if (tile0 + u < o_end && o < n_out && k < rank)
+                    const int o = out_of(u, r);
+                    if (o < o_end1 && k < rank)
                         load_weights<WT, KU / 4>(a.b[proj], w0 + (int64_t)o * a.max_rank + k, raw[u][r]);
                 }
             if (k + KU / 4 > rank) {  // what stands behind the last rank is of no meaning
@@ -186,24 +205,40 @@ __device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, 
                     for (int q = 0; q < 4; ++q) total[u][nt][q] += acc[u][nt][q];
         }
 #pragma unroll
-        for (int u = 0; u < OT; ++u)
+        for (int v = 0; v < OT / 2; ++v)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int o = (tile0 + u) * 16 + g + 8 * (q / 2);
-                    if (there[nt][q % 2] && tile0 + u < o_end && o < n_out)
-                        a.y[(int64_t)row[nt][q % 2] * a.y_stride + a.col[proj] + o] =
-                            WT == kW16 ? __fmaf_rn(total[u][nt][q], scale[nt][q % 2], base[u][nt][q]) : base[u][nt][q] + total[u][nt][q];
+                for (int q = 0; q < 2; ++q) {
+                    const int o = out_of(2 * v, 0);
+                    auto sum = [&](float b, int u, int r) {
+                        const float d = total[u][nt][2 * r + q];
+                        return WT == kW16 ? __fmaf_rn(d, scale[nt][q], b) : b + d;
+                    };
+                    const float4 z = base[v][nt][q];
+                    const float4 w = make_float4(sum(z.x, 2 * v, 0), sum(z.y, 2 * v, 1), sum(z.z, 2 * v + 1, 0), sum(z.w, 2 * v + 1, 1));
+                    if (!there[nt][q]) continue;
+                    float *p = a.y + (int64_t)row[nt][q] * a.y_stride + a.col[proj] + o;
+                    if (a.y_vec && o + 3 < o_end1) {
+                        *reinterpret_cast<float4 *>(p) = w;
+                    } else {
+                        if (o < o_end1) p[0] = w.x;
+                        if (o + 1 < o_end1) p[1] = w.y;
+                        if (o + 2 < o_end1) p[2] = w.z;
+                        if (o + 3 < o_end1) p[3] = w.w;
+                    }
                 }
     }
 }
 
+__device__ __forceinline__ void prefetch_l2_bulk(const void *p, uint32_t bytes) {  // both multiples of 16
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 template <int WT, int NT>
 __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const __grid_constant__ LoraArgs a) {
-    constexpr int TM = 8 * NT, MT = kPass / 16;
+    constexpr int TM = 8 * NT;
     extern __shared__ __align__(16) float smem[];
     __shared__ LoraFind find;
     __shared__ int list[TM];
@@ -222,24 +257,23 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
     }
     if (rank == 0 && a.y == a.base) return;
     // this CTA's outputs, and what they need asked for while h is computed
-    const int n16 = (a.out[proj] + 15) / 16;
-    const int o_begin = (int)((uint32_t)n16 * part / parts), o_end = (int)((uint32_t)n16 * (part + 1) / parts);
-    if (rank > 0 && o_begin < o_end) {
+    const int n32 = (a.out[proj] + 31) / 32;
+    const int o_begin = (int)((uint32_t)n32 * part / parts), o_end = (int)((uint32_t)n32 * (part + 1) / parts);
+    const int n_mine = min(o_end * 32, a.out[proj]) - o_begin * 32;
+    if (rank > 0 && n_mine > 0) {
         constexpr int el = Weight<WT>::bytes;
-        const int64_t first = (int64_t)tile.id * a.out[proj] + o_begin * 16, rows = min(o_end * 16, a.out[proj]) - o_begin * 16;
-        const char *w = static_cast<const char *>(a.b[proj]) + first * a.max_rank * el;
+        const char *w = static_cast<const char *>(a.b[proj]) + ((int64_t)tile.id * a.out[proj] + o_begin * 32) * a.max_rank * el;
         if (2 * rank > a.max_rank) {
-            for (int64_t at = (int64_t)tid * 128; at < rows * a.max_rank * el; at += kThreads * 128) prefetch_l2(w + at);
+            if (tid == 0) prefetch_l2_bulk(w, (uint32_t)n_mine * a.max_rank * el);
         } else {  // (rows with long gaps)
-            for (int r = tid; r < rows; r += kThreads)
+#pragma unroll 1
+            for (int r = tid; r < n_mine; r += kThreads)
+#pragma unroll 1
                 for (int at = 0; at < rank * el; at += 128) prefetch_l2(w + (int64_t)r * a.max_rank * el + at);
         }
     }
-    if (a.base != nullptr)
-        for (int r = warp; r < tile.n; r += kWarps) {
-            const float *p = a.base + (int64_t)list[r] * a.base_stride + a.col[proj];
-            for (int o = o_begin * 16 + lane * 32; o < min(o_end * 16, a.out[proj]); o += 32 * 32) prefetch_l2(p + o);
-        }
+    if (a.base != nullptr && a.y_vec && n_mine > 0 && warp == 1 && lane < tile.n)
+        prefetch_l2_bulk(a.base + (int64_t)list[lane] * a.base_stride + a.col[proj] + o_begin * 32, (uint32_t)n_mine / 4 * 16);
     const int padded = (a.max_rank + 31) / 32 * 32, pitch = padded + (WT == kW32 ? 4 : 8);
     float *h = smem;                    // [padded][TM], this CTA's share; read by its cluster
     float *limb = smem + padded * TM;   // [limbs][TM][pitch] of h, 16 bits each or 32; before that the warps' sums
@@ -255,7 +289,9 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
             there[nt] = nt * 8 + g < tile.n;
             xr[nt] = a.x + (int64_t)(there[nt] ? list[nt * 8 + g] : 0) * a.x_stride + 8 * t;
         }
-        for (int p0 = 0; p0 < rank; p0 += kPass) {
+        // MT tiles of 16 ranks at a time, the loads of UN units of 32 columns under way together
+        auto pass = [&](auto mt_, auto un_, int p0) {
+            constexpr int MT = decltype(mt_)::value, UN = decltype(un_)::value;
             const int mts = min(MT, (rank - p0 + 15) / 16);
             const int64_t w0 = ((int64_t)tile.id * a.max_rank + p0) * a.in_dim + 8 * t;
             float total[MT][NT][4], acc[MT][NT][4];
@@ -265,85 +301,97 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) total[mt][nt][q] = acc[mt][nt][q] = 0.f;
-            auto settle = [&] {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            total[mt][nt][q] += acc[mt][nt][q];
-                            acc[mt][nt][q] = 0.f;
-                        }
-            };
             int since = 0;
-#pragma unroll 2
-            for (int u = part * kWarps + warp; u < units; u += parts * kWarps) {
-                uint32_t raw[MT][2][8];
+            const int step = parts * kWarps;
+#pragma unroll 1
+            for (int u0 = part * kWarps + warp; u0 < units; u0 += UN * step) {
+                uint32_t raw[UN][MT][2][8];
+                float4 x[UN][NT][2];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int n = 0; n < UN; ++n) {
+                    const int u = u0 + n * step;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const int row = mt * 16 + g + 8 * r;
-                        if (p0 + row < rank) {
-                            load_weights<WT, 8>(a.a[proj], w0 + (int64_t)row * a.in_dim + u * 32, raw[mt][r]);
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const int row = mt * 16 + g + 8 * r;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) raw[n][mt][r][i] = 0;
+                            if (u < units && p0 + row < rank)
+                                load_weights<WT, 8>(a.a[proj], w0 + (int64_t)row * a.in_dim + u * 32, raw[n][mt][r]);
+                        }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float *p = xr[nt] + u * 32;
+                        x[n][nt][0] = x[n][nt][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (u >= units || !there[nt]) continue;
+                        if (a.x_vec) {
+                            x[n][nt][0] = reinterpret_cast<const float4 *>(p)[0], x[n][nt][1] = reinterpret_cast<const float4 *>(p)[1];
                         } else {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) raw[mt][r][i] = 0;
+                            x[n][nt][0] = make_float4(p[0], p[1], p[2], p[3]), x[n][nt][1] = make_float4(p[4], p[5], p[6], p[7]);
                         }
                     }
+                }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float v[8];
-                    const float *p = xr[nt] + u * 32;
-                    if (!there[nt]) {
+                for (int n = 0; n < UN; ++n) {
+                    if (u0 + n * step >= units) break;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-                    } else if (a.x_vec) {
-                        const float4 c = reinterpret_cast<const float4 *>(p)[0], d = reinterpret_cast<const float4 *>(p)[1];
-                        v[0] = c.x, v[1] = c.y, v[2] = c.z, v[3] = c.w, v[4] = d.x, v[5] = d.y, v[6] = d.z, v[7] = d.w;
-                    } else {
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float4 c = x[n][nt][0], d = x[n][nt][1];
+                        const float v[8] = {c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w};
+                        if constexpr (WT == kWB16) {
+                            uint32_t l[3][4];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = p[i];
-                    }
-                    if constexpr (WT == kWB16) {
-                        uint32_t l[3][4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) limbs_b16(v[2 * i], v[2 * i + 1], l[0][i], l[1][i], l[2][i]);
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            if (mt >= mts) break;
-#pragma unroll
-                            for (int n = 2; n >= 0; --n)
-#pragma unroll
-                                for (int j = 0; j < 2; ++j)
-                                    mma_16<true>(acc[mt][nt], raw[mt][0][2 * j], raw[mt][1][2 * j], raw[mt][0][2 * j + 1],
-                                                 raw[mt][1][2 * j + 1], l[n][2 * j], l[n][2 * j + 1]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t h0, h1, l0, l1;
-                            limbs(v[2 * j], h0, l0);
-                            limbs(v[2 * j + 1], h1, l1);
+                            for (int i = 0; i < 4; ++i) limbs_b16(v[2 * i], v[2 * i + 1], l[0][i], l[1][i], l[2][i]);
 #pragma unroll
                             for (int mt = 0; mt < MT; ++mt) {
                                 if (mt >= mts) break;
-                                uint32_t wh[4], wl[4];
-                                fragment<WT>(raw[mt][0], raw[mt][1], j, wh, wl);
-                                mma_tf32(acc[mt][nt], wh, l0, l1);
-                                if (WT == kW32) mma_tf32(acc[mt][nt], wl, h0, h1);
-                                mma_tf32(acc[mt][nt], wh, h0, h1);
+#pragma unroll
+                                for (int m = 2; m >= 0; --m)
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j)
+                                        mma_16<true>(acc[mt][nt], raw[n][mt][0][2 * j], raw[n][mt][1][2 * j], raw[n][mt][0][2 * j + 1],
+                                                     raw[n][mt][1][2 * j + 1], l[m][2 * j], l[m][2 * j + 1]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t h0, h1, l0, l1;
+                                limbs(v[2 * j], h0, l0);
+                                limbs(v[2 * j + 1], h1, l1);
+#pragma unroll
+                                for (int mt = 0; mt < MT; ++mt) {
+                                    if (mt >= mts) break;
+                                    uint32_t wh[4], wl[4];
+                                    fragment<WT>(raw[n][mt][0], raw[n][mt][1], j, wh, wl);
+                                    mma_tf32(acc[mt][nt], wh, l0, l1);
+                                    if (WT == kW32) mma_tf32(acc[mt][nt], wl, h0, h1);
+                                    mma_tf32(acc[mt][nt], wh, h0, h1);
+                                }
                             }
                         }
                     }
+                    if (++since == 2 || n == UN - 1) {
+                        since = 0;
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    total[mt][nt][q] += acc[mt][nt][q];
+                                    acc[mt][nt][q] = 0.f;
+                                }
+                    }
                 }
-                if (++since == 2) {
-                    settle();
-                    since = 0;
-                }
+                since = 0;
             }
-            settle();
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) total[mt][nt][q] += acc[mt][nt][q];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -353,6 +401,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
                         *reinterpret_cast<float2 *>(sums + (warp * kPass + mt * 16 + g + 8 * r) * TM + nt * 8 + 2 * t) =
                             make_float2(total[mt][nt][2 * r], total[mt][nt][2 * r + 1]);
             __syncthreads();
+#pragma unroll 1
             for (int e = tid; e < mts * 16 * TM; e += kThreads) {
                 float s = 0.f;
 #pragma unroll
@@ -360,11 +409,19 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
                 h[p0 * TM + e] = s;
             }
             __syncthreads();
-        }
+        };
+        using std::integral_constant;
+        if (rank <= 16)
+            pass(integral_constant<int, 1>(), integral_constant<int, NT == 1 ? 4 : NT == 2 ? 2 : 1>(), 0);
+        else
+#pragma unroll 1
+            for (int p0 = 0; p0 < rank; p0 += kPass)
+                pass(integral_constant<int, kPass / 16>(), integral_constant<int, NT == 1 && WT != kW32 ? 2 : 1>(), p0);
         if (parts > 1) cl.sync();
         const float scale = a.scale != nullptr ? a.scale[tile.id] : 1.f;
         const int upto = rank <= 16 ? 16 : (rank + 31) / 32 * 32;
         uint16_t *l16 = reinterpret_cast<uint16_t *>(limb);
+#pragma unroll 1
         for (int e = tid; e < upto * TM; e += kThreads) {
             const int r = e / TM, tok = e % TM;
             float s = 0.f;
@@ -412,15 +469,15 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
         if (parts > 1) cl.barrier_arrive();  // (its share is read until all have arrived)
     }
     // (several tiles of outputs at a time where every warp has as many)
-    constexpr int OT = NT == 1 ? (WT == kW32 ? 2 : 4) : NT == 2 ? 2 : 1;
-    const bool many = OT > 1 && o_end - o_begin >= kWarps * OT;
+    constexpr int OT = NT == 1 && WT != kW32 ? 4 : 2;
+    const bool many = OT > 2 && o_end - o_begin >= kWarps * (OT / 2);
     const float *from = limb + (WT == kW16 ? TM * pitch : 0);
     auto go = [&](auto ku) {
         constexpr int KU = decltype(ku)::value;
         if (many)
             expand<WT, NT, KU, OT>(a, tile, proj, rank, o_begin, o_end, list, from, pitch, unit);
         else
-            expand<WT, NT, KU, 1>(a, tile, proj, rank, o_begin, o_end, list, from, pitch, unit);
+            expand<WT, NT, KU, 2>(a, tile, proj, rank, o_begin, o_end, list, from, pitch, unit);
     };
     if (rank <= 16)
         go(std::integral_constant<int, 16>());
