@@ -1667,18 +1667,13 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
         for (int p = 0; p < a.n_proj; ++p) a.y_vec = a.y_vec && a.out[p] % 4 == 0;
         cudaError_t e;
         LoraMaps maps;
-        if (rows / distinct >= kLoraTileFrom && rows <= INT32_MAX / 8 && (int64_t)a.n_adapters * a.max_rank <= INT32_MAX &&
+        if (rows >= kLoraTileRows && rows / distinct >= kLoraTileFrom && rows <= INT32_MAX / 8 && (int64_t)a.n_adapters * a.max_rank <= INT32_MAX &&
             lora_tiles_plan(a, type, distinct, ws->sms) && lora_maps(maps, a, width, type == 2)) {
             e = lora_tiles_launch(a, maps, type, g_stream);
         } else {
-            // Tiles: n rows of d adapters make at most (n + d (tm - 1)) / tm.
-            const int tm = lora_tile_rows(rows, distinct);
-            const int chunk = std::min(rows, kLoraChunk), chunks = (rows + kLoraChunk - 1) / kLoraChunk;
-            a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (tm - 1)) / tm);
-            const int64_t tiles = (int64_t)chunks * a.chunk_tiles;
-            a.cluster = 8;
-            while (a.cluster > 1 && tiles * a.n_proj * a.cluster > 4 * ws->sms) a.cluster /= 2;
-            if (tiles * a.cluster > INT32_MAX) return fail(QL_EINVAL, what + ": too many rows for one call");
+            const int tm = lora_plan(a, type, distinct, ws->sms);
+            if (((int64_t)rows + kLoraChunk - 1) / kLoraChunk * a.chunk_tiles * a.cluster > INT32_MAX)
+                return fail(QL_EINVAL, what + ": too many rows for one call");
             e = lora_launch(a, type, tm, g_stream);
         }
         ++t_launches;

@@ -19,6 +19,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "ql_lora.cuh"
@@ -486,12 +487,15 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
     if (rank > 0 && parts > 1) cl.barrier_wait();
 }
 
+// h, and the larger of its limbs (f16: with h once more before them) and the warps' sums
+size_t smem_bytes(int max_rank, int TM) {
+    const int padded = (max_rank + 31) / 32 * 32;
+    return sizeof(float) * (padded * TM + std::max(2 * TM * (padded + 8), kWarps * kPass * TM));
+}
+
 template <int WT, int NT>
 cudaError_t launch(const LoraArgs &a, cudaStream_t s) {
-    constexpr int TM = 8 * NT;
-    const int padded = (a.max_rank + 31) / 32 * 32;
-    // h, and the larger of its limbs (f16: with h once more before them) and the warps' sums
-    const size_t smem = sizeof(float) * (padded * TM + std::max(2 * TM * (padded + 8), kWarps * kPass * TM));
+    const size_t smem = smem_bytes(a.max_rank, 8 * NT);
     cudaError_t e = cudaFuncSetAttribute(lora_kernel<WT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -513,9 +517,53 @@ cudaError_t launch(const LoraArgs &a, int tile_rows, cudaStream_t s) {
 }
 }  // namespace
 
-int lora_tile_rows(int rows, int n_seqs) {
-    const int each = rows / std::max(1, n_seqs);
-    return each <= 8 ? 8 : each <= 16 ? 16 : 32;
+namespace {
+// How many clusters of c CTAs run at once, by the rows of a tile (8, 16, 32: two CTAs of an SM, two, one).
+int clusters_at_once(int nt, int c, int sms) {
+    static std::atomic<int> known[64][3][9];
+    const int k = nt == 1 ? 0 : nt == 2 ? 1 : 2;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return std::max(1, sms / c);
+    int n = known[dev][k][c].load();
+    if (n == 0) {
+        const void *f = k == 0 ? (const void *)lora_kernel<kWB16, 1> : k == 1 ? (const void *)lora_kernel<kWB16, 2> : (const void *)lora_kernel<kWB16, 4>;
+        const int smem = (int)smem_bytes(64, 8 * nt);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim = {(unsigned)c, 1, 1};
+        cfg.attrs = at, cfg.numAttrs = 1;
+        if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, f, &cfg) != cudaSuccess || n <= 0) {
+            (void)cudaGetLastError();
+            n = std::max(1, sms / c);
+        }
+        known[dev][k][c].store(n);
+    }
+    return n;
+}
+}  // namespace
+
+int lora_plan(LoraArgs &a, int type, int distinct, int sms) {
+    (void)type;
+    const int each = a.rows / distinct, tm = each <= 8 ? 8 : each <= 16 ? 16 : 32;
+    const int chunk = std::min(a.rows, kLoraChunk);
+    // n rows of d adapters make at most (n + d (tm - 1)) / tm tiles, and about half of those that are not full
+    a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (tm - 1)) / tm);
+    const int kinds = std::max(1, std::min(a.n_seqs, a.n_adapters));
+    const double tiles = std::max<double>(std::min(kinds, a.rows), (double)a.rows / tm + kinds / 2) * a.n_proj;
+    // CTAs per tile: what the rounds of the GPU take in all (parts of rounds count, tiles of low rank end early); beside its share a CTA takes as long as 2400 columns (one
+    // 64-row call of 7B q/k/v, rank 16: 41, 25, 17, 12 us with 1, 2, 4, 8)
+    int widest = 0;
+    for (int p = 0; p < a.n_proj; ++p) widest = std::max(widest, a.out[p]);
+    double best = 0;
+    for (int c = 1; c <= 8; c *= 2) {
+        const int at_once = clusters_at_once(tm / 8, c, sms);
+        const double time = std::max(1.0, tiles / at_once) * ((a.in_dim + 2.0 * widest) / c + 2400.0);
+        if (best == 0 || time < best) best = time, a.cluster = c;
+    }
+    return tm;
 }
 
 cudaError_t lora_launch(const LoraArgs &a, int type, int tile_rows, cudaStream_t s) {

@@ -8,8 +8,8 @@ namespace ql {
 
 constexpr int kLoraMaxRank = 256, kLoraMaxProj = 3;
 constexpr int kLoraChunk = 512;  // rows among which those of one adapter are brought together
-constexpr int kLoraTile = 128;   // rows of a tile on tcgen05, where an adapter has at least
-constexpr int kLoraTileFrom = 48;  // so many on average
+constexpr int kLoraTile = 128;   // rows of a tile on tcgen05, for calls of at least so many rows, and so many of each
+constexpr int kLoraTileRows = 400, kLoraTileFrom = 48;  // adapter on average
 
 struct LoraArgs {
     const void *a[kLoraMaxProj], *b[kLoraMaxProj];  // null: this projection has no adapters
@@ -238,8 +238,8 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
     return LoraTile{found.id, found.first, f.found[0]};
 }
 
-// Rows of a tile, by the rows of the call.
-int lora_tile_rows(int rows, int n_seqs);
+// Fills in what the launch needs; returns the rows of a tile.
+int lora_plan(LoraArgs &a, int type, int distinct, int sms);
 cudaError_t lora_launch(const LoraArgs &a, int type, int tile_rows, cudaStream_t s);
 // Tiles of 128 rows: fills in what the launch needs; false: not for these sizes or this alignment.
 bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms);
