@@ -4,215 +4,169 @@
 //   the k experts of largest c in them, the lowest id among equals, by descending c
 //   w_e = s_e [/ sum of the chosen s] * scale
 // Without a bias experts stand by their logits, which no rounding touches.  Otherwise the order is that of 64-bit scores:
-// the kernel first goes by scores in fp32, each within kNear of its value, and where two that stand next to each other
-// in the order, or at the border of the groups, are nearer than that (one token in a thousand of 256 experts), the
-// token is done again in 64 bits.  So neighbours 1e-7 apart come out as the definition says at the cost of fp32.
+// the kernel first goes by scores in fp32, whose errors have a bound, and where two that stand next to each other in the
+// order, or at the border of the groups, are nearer than that, the token is done again in 64 bits.  So neighbours 1e-7
+// apart come out as the definition says at the cost of fp32 (64-bit exponentials for every score would take 2 us per
+// million of them on their own).
 //
 // Bound: the launch and a warp's chain of loads, scores and k rounds of a maximum; a round is one warp reduction of an
-// order-preserving 32-bit key and one ballot.  Lane l has the NPL consecutive experts from l * NPL.
+// order-preserving key and one ballot.  Lane l has the NPL consecutive experts from l * NPL.
 #include "ql_route.cuh"
 
 namespace ql {
 namespace {
 
 constexpr int kWarps = 4;
-// How far an fp32 score is from its value, at most, in parts of the largest score ("unit") and of the sums that it goes
-// into: expf 2 units of 2^-24, the rounded exponent 0.4, the quotient 2, a sum of 1024 exponentials 37, the sums with
-// biases and in groups 1 each.  2^-18 holds 64.
-constexpr float kNear = 3.8146973e-6f;
 constexpr float kTiny = 1e-30f;  // chosen scores whose sum is below this are taken in 64 bits, too
 constexpr unsigned kAll = 0xffffffffu;
 
-// Larger key, larger value; 0 for what cannot be chosen (-inf, NaN).
+// Order-preserving keys: larger key, larger value; 0 for what cannot be chosen (-inf, NaN).
 __device__ __forceinline__ uint32_t order(float v) {
     if (!(v > -INFINITY)) return 0u;
     const uint32_t u = __float_as_uint(v == 0.f ? 0.f : v);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+__device__ __forceinline__ uint64_t order(double v) {
+    if (!(v > -INFINITY)) return 0ull;
+    const uint64_t u = (uint64_t)__double_as_longlong(v == 0.0 ? 0.0 : v);
+    return (u >> 63) ? ~u : (u | 1ull << 63);
+}
 __device__ __forceinline__ float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ double value(uint64_t k) { return __longlong_as_double((long long)(k >> 63 ? k ^ (1ull << 63) : ~k)); }
+__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(kAll, k); }
+__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
+    const uint32_t hi = __reduce_max_sync(kAll, (uint32_t)(k >> 32));
+    return (uint64_t)hi << 32 | __reduce_max_sync(kAll, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+}
+// In (0, 1]: no overflow on either side of the sigmoid.
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }
+__device__ __forceinline__ double quotient(double a, double b) { return a / b; }
 
-// The definition in 64 bits, one token by one warp.  c, s: n_experts values each in shared memory.
-__device__ __noinline__ void route_exact(const RouteArgs &a, int token, double *s, double *c) {
-    const int lane = threadIdx.x % 32, E = a.n_experts, per = E / a.n_groups;
-    const float *x = a.logits + (int64_t)token * a.logits_stride;
-    double mx = -INFINITY, total = 0.0;
-    if (!a.sigmoid) {
-        for (int e = lane; e < E; e += 32)
-            if (isfinite(x[e])) mx = fmax(mx, (double)x[e]);
-        for (int o = 16; o > 0; o >>= 1) mx = fmax(mx, __shfl_xor_sync(kAll, mx, o));
-        for (int e = lane; e < E; e += 32)
-            if (isfinite(x[e])) total += exp((double)x[e] - mx);
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
-    }
-    for (int e = lane; e < E; e += 32) {
-        const bool ok = isfinite(x[e]);
-        double v = 0.0;
-        if (ok) v = a.sigmoid ? 1.0 / (1.0 + exp(-(double)x[e])) : exp((double)x[e] - mx) / total;
-        double w = v;
-        if (a.bias != nullptr) w += (double)a.bias[e];
-        s[e] = v;
-        c[e] = ok && w > -INFINITY ? w : -INFINITY;  // (a bias of NaN or -inf: never chosen)
-    }
-    __syncwarp();
-    unsigned open = kAll;
-    if (a.n_groups > 1) {
-        double g = -INFINITY;  // lane g: its group's score
-        if (lane < a.n_groups) {
-            double b0 = -INFINITY, b1 = -INFINITY;
-            for (int e = lane * per; e < (lane + 1) * per; ++e) {
-                const double v = c[e];
-                if (v > b0)
-                    b1 = b0, b0 = v;
-                else if (v > b1)
-                    b1 = v;
-            }
-            g = b0;
-            if (a.group_best > 1 && b1 > -INFINITY) g += b1;
-        }
-        int better = 0;
-        for (int o = 0; o < a.n_groups; ++o) {
-            const double v = __shfl_sync(kAll, g, o);
-            better += v > g || (v == g && o < lane);
-        }
-        open = __ballot_sync(kAll, g > -INFINITY && better < a.top_groups);
-    }
-    double sum = 0.0, mine = 0.0;
-    int mine_e = -1;
-    for (int r = 0; r < a.k; ++r) {
-        double best = -INFINITY;
-        int at = E;
-        // without a bias the logits decide (two scores may round to the same 64 bits)
-        for (int e = lane; e < E; e += 32) {
-            if (!(c[e] > -INFINITY) || (a.n_groups > 1 && !(open >> (e / per) & 1u))) continue;
-            const double v = a.bias != nullptr ? c[e] : (double)x[e];
-            if (at == E || v > best) best = v, at = e;
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            const double v = __shfl_xor_sync(kAll, best, o);
-            const int e = __shfl_xor_sync(kAll, at, o);
-            if (e < E && (at == E || v > best || (v == best && e < at))) best = v, at = e;
-        }
-        if (at < E) {
-            const double p = s[at];
-            sum += p;
-            if (lane == r) mine = p, mine_e = at;
-            __syncwarp();
-            if (at % 32 == lane) c[at] = -INFINITY;
-        }
-        __syncwarp();
-    }
-    if (lane < a.k) {
-        const double w = a.renorm ? (sum > 0.0 ? mine / sum : 0.0) : mine;
-        a.top_idx[(int64_t)token * a.k + lane] = mine_e;
-        a.top_w[(int64_t)token * a.k + lane] = (float)(w * (double)a.scale);
-    }
-    __syncwarp();
+template <typename T>
+struct Key;
+template <>
+struct Key<float> {
+    using type = uint32_t;
+};
+template <>
+struct Key<double> {
+    using type = uint64_t;
+};
+
+// The score of a logit that may be chosen; mx and inv: the softmax's largest logit and the inverse of its sum.
+template <typename T>
+__device__ __forceinline__ T score_of(bool sigmoid, float l, float mx, T inv) {
+    if (!sigmoid) return exp_of((T)l - (T)mx) * inv;
+    const T z = exp_of(-fabs((T)l));
+    return quotient(l < 0.f ? z : (T)1, (T)1 + z);
 }
 
-template <int NPL>
-__global__ void __launch_bounds__(32 * kWarps) route_kernel(const __grid_constant__ RouteArgs a) {
-    extern __shared__ double smem[];  // per warp 2 n_experts; the fp32 pass takes n_experts floats of it
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, E = a.n_experts;
-    const int token = blockIdx.x * kWarps + warp;
-    if (token >= a.tokens) return;
+// One token by one warp, in fp32 or in 64 bits.  c: n_experts values in shared memory where there are groups.  false: two
+// scores are too near for fp32, nothing is written.
+template <typename T, int NPL>
+__device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
+    using K = typename Key<T>::type;
+    constexpr bool fast = sizeof(T) == 4;
+    const int lane = threadIdx.x % 32, E = a.n_experts, e0 = lane * NPL;
     const float *x = a.logits + (int64_t)token * a.logits_stride;
-    const int e0 = lane * NPL;
-    float l[NPL], s[NPL];
-    const bool vec = NPL % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    K key[NPL];
+    float mx = 0.f;
+    T inv = 1, unit = 1;  // unit: no score is above it
+    {
+        float l[NPL];
+        const bool vec = NPL % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
 #pragma unroll
-    for (int i = 0; i < NPL; i += NPL % 4 == 0 ? 4 : 1) {
-        if (NPL % 4 == 0 && vec && e0 + i + 3 < E) {
-            const float4 w = *reinterpret_cast<const float4 *>(x + e0 + i);
-            l[i] = w.x, l[(i + 1) % NPL] = w.y, l[(i + 2) % NPL] = w.z, l[(i + 3) % NPL] = w.w;
-        } else {
+        for (int i = 0; i < NPL; i += NPL % 4 == 0 ? 4 : 1) {
+            if (NPL % 4 == 0 && vec && e0 + i + 3 < E) {
+                const float4 w = *reinterpret_cast<const float4 *>(x + e0 + i);
+                l[i] = w.x, l[(i + 1) % NPL] = w.y, l[(i + 2) % NPL] = w.z, l[(i + 3) % NPL] = w.w;
+            } else {
 #pragma unroll
-            for (int j = 0; j < (NPL % 4 == 0 ? 4 : 1); ++j) l[(i + j) % NPL] = e0 + i + j < E ? x[e0 + i + j] : -INFINITY;
+                for (int j = 0; j < (NPL % 4 == 0 ? 4 : 1); ++j) l[(i + j) % NPL] = e0 + i + j < E ? x[e0 + i + j] : -INFINITY;
+            }
         }
-    }
-    float mx = -INFINITY, unit = 1.f;  // unit: no score is above it
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-        if (!(fabsf(l[i]) < INFINITY)) l[i] = -INFINITY;
-        mx = fmaxf(mx, l[i]);
-    }
-    if (!a.sigmoid) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, o));
-        if (!(mx > -INFINITY)) mx = 0.f;
-        float total = 0.f;
-#pragma unroll
-        for (int i = 0; i < NPL; ++i) {
-            s[i] = expf(l[i] - mx);
-            total += s[i];
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
-        const float inv = total > 0.f ? __fdiv_rn(1.f, total) : 0.f;
-#pragma unroll
-        for (int i = 0; i < NPL; ++i) s[i] *= inv;
-        unit = inv;
-    } else {
-#pragma unroll
-        for (int i = 0; i < NPL; ++i) {
-            const float z = expf(-fabsf(l[i]));  // in (0, 1]: no overflow on either side
-            s[i] = __fdividef(l[i] < 0.f ? z : 1.f, 1.f + z);
-        }
-    }
-    bool near = false;  // two scores too near for fp32
-    uint32_t key[NPL];
-    if (a.bias != nullptr) {
-#pragma unroll
-        for (int i = 0; i < NPL; ++i) key[i] = e0 + i < E && l[i] > -INFINITY ? order(s[i] + a.bias[e0 + i]) : 0u;
-    } else {
-#pragma unroll
-        for (int i = 0; i < NPL; ++i) key[i] = order(l[i]);
-    }
-    double *sw = smem + (size_t)warp * 2 * E;
-    if (a.n_groups > 1) {
-        const int per = E / a.n_groups;
-        float *c = reinterpret_cast<float *>(sw);
 #pragma unroll
         for (int i = 0; i < NPL; ++i)
-            if (e0 + i < E) c[e0 + i] = key[i] == 0u ? -INFINITY : a.bias != nullptr ? value(key[i]) : s[i];
+            if (!(fabsf(l[i]) < INFINITY)) l[i] = -INFINITY;
+        const bool all = a.bias != nullptr || a.n_groups > 1;  // every expert's score is needed, not the chosen ones' alone
+        if (!a.sigmoid) {
+            mx = l[0];
+#pragma unroll
+            for (int i = 1; i < NPL; ++i) mx = fmaxf(mx, l[i]);
+            const uint32_t k = warp_max(order(mx));
+            mx = k != 0 ? value(k) : 0.f;
+            if (all || !a.renorm) {
+                T total = 0;
+#pragma unroll
+                for (int i = 0; i < NPL; ++i) total += exp_of((T)l[i] - (T)mx);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
+                inv = total > 0 ? (T)1 / total : (T)0;
+                unit = inv;
+            }
+        }
+        if (all) {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) {
+                const bool there = e0 + i < E && l[i] > -INFINITY;
+                const T s = score_of(a.sigmoid, l[i], mx, inv);
+                const T v = a.bias != nullptr && there ? s + (T)a.bias[e0 + i] : s;
+                key[i] = there ? a.bias != nullptr ? order(v) : order((T)l[i]) : (K)0;
+                if (a.n_groups > 1 && e0 + i < E) c[e0 + i] = key[i] != 0 ? v : (T)-INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) key[i] = order((T)l[i]);
+        }
+    }
+    // How far an fp32 score is from its value, in parts of unit: the exponential 2 units of 2^-24, its rounded argument
+    // 0.4, 1 + z or the product 1, the quotient 2, and in a softmax the sum's NPL + 5 additions and inverse.  Sums of scores
+    // are rounded once more, 2^-24 of themselves.
+    const T score_err = (T)((a.sigmoid ? 8 : NPL + 14) * 5.9604645e-8), sum_err = (T)1.2e-7;
+    if (a.n_groups > 1) {
+        const int per = E / a.n_groups;
         __syncwarp();
         // 32 / n_groups lanes (a power of two) look through each group
         const int share = 1 << (31 - __clz(32 / a.n_groups));
         const int g = lane / share, j = lane % share;
-        float b0 = -INFINITY, b1 = -INFINITY;
+        T b0 = -INFINITY, b1 = -INFINITY;
         if (g < a.n_groups)
+#pragma unroll 4
             for (int e = j; e < per; e += share) {
-                const float v = c[g * per + e];
-                b1 = fmaxf(b1, fminf(b0, v));
-                b0 = fmaxf(b0, v);
+                const T v = c[g * per + e];
+                b1 = fmax(b1, fmin(b0, v));
+                b0 = fmax(b0, v);
             }
         for (int o = share / 2; o > 0; o /= 2) {
-            const float v0 = __shfl_xor_sync(kAll, b0, o), v1 = __shfl_xor_sync(kAll, b1, o);
-            b1 = fmaxf(fmaxf(b1, v1), fminf(b0, v0));
-            b0 = fmaxf(b0, v0);
+            const T v0 = __shfl_xor_sync(kAll, b0, o), v1 = __shfl_xor_sync(kAll, b1, o);
+            b1 = fmax(fmax(b1, v1), fmin(b0, v0));
+            b0 = fmax(b0, v0);
         }
         const bool two = a.group_best > 1 && b1 > -INFINITY;
-        const float score = two ? b0 + b1 : b0;  // (the same in every lane of a group)
-        const float size = fabsf(b0) + (two ? fabsf(b1) : 0.f) + unit;
+        const T score = two ? b0 + b1 : b0;  // (the same in every lane of a group)
+        const T size = sum_err * (fabs(b0) + (two ? fabs(b1) : (T)0)) + 2 * score_err * unit;
         int better = 0;
         unsigned close = 0;  // groups whose scores are too near to this one's, bit o * share
+#pragma unroll 1
         for (int o = 0; o < a.n_groups; ++o) {
-            const float v = __shfl_sync(kAll, score, o * share), z = __shfl_sync(kAll, size, o * share);
+            const T v = __shfl_sync(kAll, score, o * share);
             better += v > score || (v == score && o < g);
-            if (fabsf(v - score) <= kNear * (size + z)) close |= 1u << (o * share);
+            if (fast && fabs(v - score) <= size + __shfl_sync(kAll, size, o * share)) close |= 1u << (o * share);
         }
         const bool stays = g < a.n_groups && j == 0 && score > -INFINITY && better < a.top_groups;
         const unsigned open = __ballot_sync(kAll, stays);  // bit g * share
-        near = __any_sync(kAll, j == 0 && g < a.n_groups && score > -INFINITY && ((stays ? ~open : open) & close) != 0);
+        if (fast && __any_sync(kAll, j == 0 && g < a.n_groups && score > -INFINITY && ((stays ? ~open : open) & close) != 0)) return false;
         int gi = e0 / per, rest = e0 - gi * per;
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
-            if (e0 + i < E && !(open >> (gi * share) & 1u)) key[i] = 0u;
+            if (e0 + i < E && !(open >> (gi * share) & 1u)) key[i] = 0;
             if (++rest == per) rest = 0, ++gi;
         }
-        __syncwarp();
     }
     // k rounds (one more where the border could be near): the warp's largest key, its lowest lane, that lane's first
-    uint32_t top = 0;
+    K top = 0;
     int where = 0;
     auto lane_best = [&] {
         top = key[0], where = 0;
@@ -221,56 +175,68 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(const __grid_constan
             if (key[i] > top) top = key[i], where = i;
     };
     lane_best();
-    const int rounds = a.bias != nullptr ? a.k + 1 : a.k;
-    float mine = 0.f, sum = 0.f, last = 0.f;
+    const bool check = fast && a.bias != nullptr;
+    const int rounds = check ? a.k + 1 : a.k;
+    T last = 0;
     int mine_e = -1;
+#pragma unroll 1
     for (int r = 0; r < rounds; ++r) {
-        const uint32_t best = __reduce_max_sync(kAll, top);
-        if (best == 0u) break;
-        const int owner = __ffs(__ballot_sync(kAll, top == best)) - 1;
-        const float c = value(best);
-        if (a.bias != nullptr) {
-            if (r > 0 && last - c <= kNear * (fabsf(c) + fabsf(last) + unit)) near = true;
-            last = c;
+        const K best = warp_max(top);
+        if (best == 0) break;
+        if (check) {
+            const T v = value(best);
+            if (r > 0 && last - v <= sum_err * (fabs(v) + fabs(last)) + 2 * score_err * unit) return false;
+            last = v;
             if (r == a.k) break;
         }
-        float p = 0.f;
+        const int owner = __ffs(__ballot_sync(kAll, top == best)) - 1;
+        const int e = __shfl_sync(kAll, e0 + where, owner);
+        if (lane == r) mine_e = e;
         if (lane == owner) {
 #pragma unroll
             for (int i = 0; i < NPL; ++i)
-                if (i == where) {
-                    p = s[i];
-                    key[i] = 0u;
-                }
+                if (i == where) key[i] = 0;
+            lane_best();
         }
-        const int e = __shfl_sync(kAll, e0 + where, owner);
-        p = __shfl_sync(kAll, p, owner);
-        sum += p;
-        if (lane == r) mine = p, mine_e = e;
-        if (lane == owner) lane_best();
     }
-    near = near || (a.renorm && !(sum >= kTiny));
-    if (near) {
-        route_exact(a, token, sw, sw + E);
-        return;
+    // lane r has the r-th
+    const T mine = mine_e >= 0 ? score_of(a.sigmoid, x[mine_e], mx, inv) : (T)0;
+    T w = mine;
+    if (a.renorm) {
+        T sum = mine;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+        if (fast && !(sum >= (T)kTiny)) return false;
+        w = sum > 0 ? mine / sum : (T)0;
     }
     if (lane < a.k) {
-        const float w = a.renorm ? __fdiv_rn(mine, sum) : mine;
         a.top_idx[(int64_t)token * a.k + lane] = mine_e;
-        a.top_w[(int64_t)token * a.k + lane] = w * a.scale;
+        a.top_w[(int64_t)token * a.k + lane] = (float)(w * (T)a.scale);
     }
+    return true;
+}
+
+template <int NPL>
+__device__ __noinline__ void choose_exactly(const RouteArgs &a, int token, double *c) {
+    choose<double, NPL>(a, token, c);
+}
+
+template <int NPL>
+__global__ void __launch_bounds__(32 * kWarps) route_kernel(const __grid_constant__ RouteArgs a) {
+    extern __shared__ double smem[];  // n_experts per warp where there are groups
+    const int warp = threadIdx.x / 32, token = blockIdx.x * kWarps + warp;
+    if (token >= a.tokens) return;
+    double *c = smem + (size_t)warp * a.n_experts;
+    if (!choose<float, NPL>(a, token, reinterpret_cast<float *>(c))) choose_exactly<NPL>(a, token, c);
 }
 
 template <int NPL>
 cudaError_t launch(const RouteArgs &a, cudaStream_t s) {
-    const size_t smem = sizeof(double) * 2 * kWarps * (size_t)a.n_experts;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(route_kernel<NPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
+    const size_t smem = a.n_groups > 1 ? sizeof(double) * kWarps * (size_t)a.n_experts : 0;
     route_kernel<NPL><<<(a.tokens + kWarps - 1) / kWarps, 32 * kWarps, smem, s>>>(a);
     return cudaGetLastError();
 }
+static_assert(sizeof(double) * kWarps * kRouteMaxExperts <= 48 * 1024, "shared memory without asking for more");
 }  // namespace
 
 cudaError_t route_launch(const RouteArgs &a, int sms, cudaStream_t s) {
