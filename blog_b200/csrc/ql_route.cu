@@ -38,7 +38,9 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
     const uint32_t hi = __reduce_max_sync(kAll, (uint32_t)(k >> 32));
     return (uint64_t)hi << 32 | __reduce_max_sync(kAll, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
 }
-// In (0, 1]: no overflow on either side of the sigmoid.
+// For x <= 0.  The fast one, for the order: 2 + 1.2 |x| units in the last place, at most 4 of exp(0)'s.
+__device__ __forceinline__ float exp_fast(float x) { return __expf(x); }
+__device__ __forceinline__ double exp_fast(double x) { return exp(x); }
 __device__ __forceinline__ float exp_of(float x) { return expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 __device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }
@@ -56,16 +58,19 @@ struct Key<double> {
 };
 
 // The score of a logit that may be chosen; mx and inv: the softmax's largest logit and the inverse of its sum.
-template <typename T>
-__device__ __forceinline__ T score_of(bool sigmoid, float l, float mx, T inv) {
-    if (!sigmoid) return exp_of((T)l - (T)mx) * inv;
-    const T z = exp_of(-fabs((T)l));
+template <bool SIGMOID, bool FAST, typename T>
+__device__ __forceinline__ T score_of(float l, float mx, T inv) {
+    if (!SIGMOID) {
+        const T d = (T)l - (T)mx;
+        return (FAST ? exp_fast(d) : exp_of(d)) * inv;
+    }
+    const T d = -fabs((T)l), z = FAST ? exp_fast(d) : exp_of(d);  // (in (0, 1]: no overflow on either side)
     return quotient(l < 0.f ? z : (T)1, (T)1 + z);
 }
 
 // One token by one warp, in fp32 or in 64 bits.  c: n_experts values in shared memory where there are groups.  false: two
 // scores are too near for fp32, nothing is written.
-template <typename T, int NPL>
+template <typename T, int NPL, bool SIGMOID>
 __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
     using K = typename Key<T>::type;
     constexpr bool fast = sizeof(T) == 4;
@@ -75,7 +80,11 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
     float mx = 0.f;
     T inv = 1, unit = 1;  // unit: no score is above it
     {
-        float l[NPL];
+        float l[NPL], bias[NPL];
+        if (a.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < NPL; ++i) bias[i] = e0 + i < E ? a.bias[e0 + i] : 0.f;
+        }
         const bool vec = NPL % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
 #pragma unroll
         for (int i = 0; i < NPL; i += NPL % 4 == 0 ? 4 : 1) {
@@ -91,7 +100,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
         for (int i = 0; i < NPL; ++i)
             if (!(fabsf(l[i]) < INFINITY)) l[i] = -INFINITY;
         const bool all = a.bias != nullptr || a.n_groups > 1;  // every expert's score is needed, not the chosen ones' alone
-        if (!a.sigmoid) {
+        if (!SIGMOID) {
             mx = l[0];
 #pragma unroll
             for (int i = 1; i < NPL; ++i) mx = fmaxf(mx, l[i]);
@@ -100,7 +109,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
             if (all || !a.renorm) {
                 T total = 0;
 #pragma unroll
-                for (int i = 0; i < NPL; ++i) total += exp_of((T)l[i] - (T)mx);
+                for (int i = 0; i < NPL; ++i) total += exp_fast((T)l[i] - (T)mx);
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
                 inv = total > 0 ? (T)1 / total : (T)0;
@@ -111,8 +120,8 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
 #pragma unroll
             for (int i = 0; i < NPL; ++i) {
                 const bool there = e0 + i < E && l[i] > -INFINITY;
-                const T s = score_of(a.sigmoid, l[i], mx, inv);
-                const T v = a.bias != nullptr && there ? s + (T)a.bias[e0 + i] : s;
+                const T s = score_of<SIGMOID, true>(l[i], mx, inv);
+                const T v = a.bias != nullptr && there ? s + (T)bias[i] : s;
                 key[i] = there ? a.bias != nullptr ? order(v) : order((T)l[i]) : (K)0;
                 if (a.n_groups > 1 && e0 + i < E) c[e0 + i] = key[i] != 0 ? v : (T)-INFINITY;
             }
@@ -121,10 +130,10 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
             for (int i = 0; i < NPL; ++i) key[i] = order((T)l[i]);
         }
     }
-    // How far an fp32 score is from its value, in parts of unit: the exponential 2 units of 2^-24, its rounded argument
-    // 0.4, 1 + z or the product 1, the quotient 2, and in a softmax the sum's NPL + 5 additions and inverse.  Sums of scores
-    // are rounded once more, 2^-24 of themselves.
-    const T score_err = (T)((a.sigmoid ? 8 : NPL + 14) * 5.9604645e-8), sum_err = (T)1.2e-7;
+    // How far an fp32 score is from its value, in units of 2^-24 of "unit": the exponential 4, its rounded argument 0.4,
+    // 1 + z or the product 1, the quotient 4, and in a softmax the sum's NPL + 5 additions, its terms and inverse.  Sums of
+    // scores are rounded once more, 2^-24 of themselves.
+    const T score_err = (T)((SIGMOID ? 12 : NPL + 16) * 5.9604645e-8), sum_err = (T)1.2e-7;
     if (a.n_groups > 1) {
         const int per = E / a.n_groups;
         __syncwarp();
@@ -149,11 +158,18 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
         const T size = sum_err * (fabs(b0) + (two ? fabs(b1) : (T)0)) + 2 * score_err * unit;
         int better = 0;
         unsigned close = 0;  // groups whose scores are too near to this one's, bit o * share
+        const int turns = (a.n_groups + share - 1) / share;  // a group's lanes look at the others in turn
 #pragma unroll 1
-        for (int o = 0; o < a.n_groups; ++o) {
-            const T v = __shfl_sync(kAll, score, o * share);
+        for (int n = 0; n < turns; ++n) {
+            const int o = n * share + j, from = min(o, a.n_groups - 1) * share;
+            const T v = __shfl_sync(kAll, score, from), z = fast ? __shfl_sync(kAll, size, from) : (T)0;
+            if (o >= a.n_groups) continue;
             better += v > score || (v == score && o < g);
-            if (fast && fabs(v - score) <= size + __shfl_sync(kAll, size, o * share)) close |= 1u << (o * share);
+            if (fast && fabs(v - score) <= size + z) close |= 1u << (o * share);
+        }
+        for (int o = share / 2; o > 0; o /= 2) {
+            better += __shfl_xor_sync(kAll, better, o);
+            if (fast) close |= __shfl_xor_sync(kAll, close, o);
         }
         const bool stays = g < a.n_groups && j == 0 && score > -INFINITY && better < a.top_groups;
         const unsigned open = __ballot_sync(kAll, stays);  // bit g * share
@@ -200,7 +216,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
         }
     }
     // lane r has the r-th
-    const T mine = mine_e >= 0 ? score_of(a.sigmoid, x[mine_e], mx, inv) : (T)0;
+    const T mine = mine_e >= 0 ? score_of<SIGMOID, false>(x[mine_e], mx, inv) : (T)0;
     T w = mine;
     if (a.renorm) {
         T sum = mine;
@@ -216,24 +232,29 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
     return true;
 }
 
-template <int NPL>
+template <int NPL, bool SIGMOID>
 __device__ __noinline__ void choose_exactly(const RouteArgs &a, int token, double *c) {
-    choose<double, NPL>(a, token, c);
+    choose<double, NPL, SIGMOID>(a, token, c);
 }
 
-template <int NPL>
-__global__ void __launch_bounds__(32 * kWarps) route_kernel(const __grid_constant__ RouteArgs a) {
+// (the registers of eight CTAs an SM: 55 warps have to be there for 8192 tokens at once; the seldom 64-bit form may spill)
+template <int NPL, bool SIGMOID>
+__global__ void __launch_bounds__(32 * kWarps, NPL <= 8 ? 12 : NPL <= 16 ? 8 : 4) route_kernel(const __grid_constant__ RouteArgs a) {
     extern __shared__ double smem[];  // n_experts per warp where there are groups
     const int warp = threadIdx.x / 32, token = blockIdx.x * kWarps + warp;
     if (token >= a.tokens) return;
     double *c = smem + (size_t)warp * a.n_experts;
-    if (!choose<float, NPL>(a, token, reinterpret_cast<float *>(c))) choose_exactly<NPL>(a, token, c);
+    if (!choose<float, NPL, SIGMOID>(a, token, reinterpret_cast<float *>(c))) choose_exactly<NPL, SIGMOID>(a, token, c);
 }
 
 template <int NPL>
 cudaError_t launch(const RouteArgs &a, cudaStream_t s) {
     const size_t smem = a.n_groups > 1 ? sizeof(double) * kWarps * (size_t)a.n_experts : 0;
-    route_kernel<NPL><<<(a.tokens + kWarps - 1) / kWarps, 32 * kWarps, smem, s>>>(a);
+    const unsigned grid = (unsigned)((a.tokens + kWarps - 1) / kWarps);
+    if (a.sigmoid)
+        route_kernel<NPL, true><<<grid, 32 * kWarps, smem, s>>>(a);
+    else
+        route_kernel<NPL, false><<<grid, 32 * kWarps, smem, s>>>(a);
     return cudaGetLastError();
 }
 static_assert(sizeof(double) * kWarps * kRouteMaxExperts <= 48 * 1024, "shared memory without asking for more");
