@@ -4,10 +4,11 @@
 //   the k experts of largest c in them, the lowest id among equals, by descending c
 //   w_e = s_e [/ sum of the chosen s] * scale
 // Without a bias experts stand by their logits, which no rounding touches.  Otherwise the order is that of 64-bit scores:
-// the kernel first goes by scores in fp32, whose errors have a bound, and where two that stand next to each other in the
-// order, or at the border of the groups, are nearer than that, the token is done again in 64 bits.  So neighbours 1e-7
-// apart come out as the definition says at the cost of fp32 (64-bit exponentials for every score would take 2 us per
-// million of them on their own).
+// the kernel goes by scores in fp32, whose errors have a bound, and picks on past the k-th until the next one is clearly
+// less.  Where two that stand next to each other in that order are nearer than the bound, the picked ones, one per lane, are
+// ranked by their scores in 64 bits; where the border of the groups is in doubt, the groups are counted again in 64 bits.
+// So neighbours 1e-7 apart come out as the definition says.  (Everything in 64 bits for such a token: one in 200 held
+// 8192 tokens up to 23 us.)
 //
 // Bound: the launch and a warp's chain of loads, scores and k rounds of a maximum; a round is one warp reduction of an
 // order-preserving key and one ballot.  Lane l has the NPL consecutive experts from l * NPL.
@@ -68,8 +69,100 @@ __device__ __forceinline__ T score_of(float l, float mx, T inv) {
     return quotient(l < 0.f ? z : (T)1, (T)1 + z);
 }
 
-// One token by one warp, in fp32 or in 64 bits.  c: n_experts values in shared memory where there are groups.  false: two
-// scores are too near for fp32, nothing is written.
+// Lanes that look through a group (a power of two).
+__device__ __forceinline__ int group_share(const RouteArgs &a) { return 1 << (31 - __clz(32 / a.n_groups)); }
+
+// The groups that stay, bit g * group_share, by the values in c (-inf: not to be chosen); near: in fp32 the border is in doubt.
+template <typename T>
+__device__ __forceinline__ unsigned groups_open(const RouteArgs &a, const T *c, T score_err, T sum_err, T unit, bool &near) {
+    constexpr bool fast = sizeof(T) == 4;
+    const int lane = threadIdx.x % 32, per = a.n_experts / a.n_groups, share = group_share(a);
+    const int g = lane / share, j = lane % share;
+    T b0 = -INFINITY, b1 = -INFINITY;
+    if (g < a.n_groups)
+#pragma unroll 4
+        for (int e = j; e < per; e += share) {
+            const T v = c[g * per + e];
+            b1 = fmax(b1, fmin(b0, v));
+            b0 = fmax(b0, v);
+        }
+#pragma unroll 1
+    for (int o = share / 2; o > 0; o /= 2) {
+        const T v0 = __shfl_xor_sync(kAll, b0, o), v1 = __shfl_xor_sync(kAll, b1, o);
+        b1 = fmax(fmax(b1, v1), fmin(b0, v0));
+        b0 = fmax(b0, v0);
+    }
+    const bool two = a.group_best > 1 && b1 > -INFINITY;
+    const T score = two ? b0 + b1 : b0;  // (the same in every lane of a group)
+    const T size = sum_err * (fabs(b0) + (two ? fabs(b1) : (T)0)) + 2 * score_err * unit;
+    int better = 0;
+    unsigned close = 0;  // groups whose scores are too near to this one's, bit o * share
+    const int turns = (a.n_groups + share - 1) / share;  // a group's lanes look at the others in turn
+#pragma unroll 1
+    for (int n = 0; n < turns; ++n) {
+        const int o = n * share + j, from = min(o, a.n_groups - 1) * share;
+        const T v = __shfl_sync(kAll, score, from), z = fast ? __shfl_sync(kAll, size, from) : (T)0;
+        if (o >= a.n_groups) continue;
+        better += v > score || (v == score && o < g);
+        if (fast && fabs(v - score) <= size + z) close |= 1u << (o * share);
+    }
+#pragma unroll 1
+    for (int o = share / 2; o > 0; o /= 2) {
+        better += __shfl_xor_sync(kAll, better, o);
+        if (fast) close |= __shfl_xor_sync(kAll, close, o);
+    }
+    const bool stays = g < a.n_groups && j == 0 && score > -INFINITY && better < a.top_groups;
+    const unsigned open = __ballot_sync(kAll, stays);
+    if (fast) near = __any_sync(kAll, j == 0 && g < a.n_groups && score > -INFINITY && ((stays ? ~open : open) & close) != 0);
+    return open;
+}
+
+// 64 bits: the inverse of the softmax's sum, and the groups that stay.
+template <bool SIGMOID>
+__device__ __noinline__ double exact_inverse(const RouteArgs &a, int token, float mx) {
+    if (SIGMOID) return 1.0;
+    const float *x = a.logits + (int64_t)token * a.logits_stride;
+    double total = 0.0;
+#pragma unroll 2
+    for (int e = threadIdx.x % 32; e < a.n_experts; e += 32)
+        if (fabsf(x[e]) < INFINITY) total += exp((double)x[e] - (double)mx);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
+    return total > 0.0 ? 1.0 / total : 0.0;
+}
+template <bool SIGMOID>
+__device__ __noinline__ unsigned groups_exactly(const RouteArgs &a, int token, float mx, double *c) {
+    const float *x = a.logits + (int64_t)token * a.logits_stride;
+    const double inv = exact_inverse<SIGMOID>(a, token, mx);
+    __syncwarp();
+#pragma unroll 2
+    for (int e = threadIdx.x % 32; e < a.n_experts; e += 32) {
+        double v = -INFINITY;
+        if (fabsf(x[e]) < INFINITY) v = score_of<SIGMOID, false>(x[e], mx, inv) + (a.bias != nullptr ? (double)a.bias[e] : 0.0);
+        c[e] = v > -INFINITY ? v : -INFINITY;
+    }
+    __syncwarp();
+    bool near;
+    return groups_open(a, c, 0.0, 0.0, 0.0, near);
+}
+// Of m candidates, lane i's expert e, the rank of each by its score in 64 bits (equal ones by id).
+template <bool SIGMOID>
+__device__ __noinline__ int rank_exactly(const RouteArgs &a, int token, float mx, int e, int m) {
+    const double inv = exact_inverse<SIGMOID>(a, token, mx);
+    double v = -INFINITY;
+    if (e >= 0) v = score_of<SIGMOID, false>(a.logits[(int64_t)token * a.logits_stride + e], mx, inv) + (double)a.bias[e];
+    int rank = 0;
+#pragma unroll 1
+    for (int i = 0; i < m; ++i) {
+        const double w = __shfl_sync(kAll, v, i);
+        const int f = __shfl_sync(kAll, e, i);
+        rank += w > v || (w == v && f < e);
+    }
+    return rank;
+}
+
+// One token by one warp, in fp32 or in 64 bits.  c: n_experts values in shared memory where there are groups.  false: not
+// to be decided in fp32, nothing is written.
 template <typename T, int NPL, bool SIGMOID>
 __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
     using K = typename Key<T>::type;
@@ -135,45 +228,11 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
     // scores are rounded once more, 2^-24 of themselves.
     const T score_err = (T)((SIGMOID ? 12 : NPL + 16) * 5.9604645e-8), sum_err = (T)1.2e-7;
     if (a.n_groups > 1) {
-        const int per = E / a.n_groups;
+        const int per = E / a.n_groups, share = group_share(a);
         __syncwarp();
-        // 32 / n_groups lanes (a power of two) look through each group
-        const int share = 1 << (31 - __clz(32 / a.n_groups));
-        const int g = lane / share, j = lane % share;
-        T b0 = -INFINITY, b1 = -INFINITY;
-        if (g < a.n_groups)
-#pragma unroll 4
-            for (int e = j; e < per; e += share) {
-                const T v = c[g * per + e];
-                b1 = fmax(b1, fmin(b0, v));
-                b0 = fmax(b0, v);
-            }
-        for (int o = share / 2; o > 0; o /= 2) {
-            const T v0 = __shfl_xor_sync(kAll, b0, o), v1 = __shfl_xor_sync(kAll, b1, o);
-            b1 = fmax(fmax(b1, v1), fmin(b0, v0));
-            b0 = fmax(b0, v0);
-        }
-        const bool two = a.group_best > 1 && b1 > -INFINITY;
-        const T score = two ? b0 + b1 : b0;  // (the same in every lane of a group)
-        const T size = sum_err * (fabs(b0) + (two ? fabs(b1) : (T)0)) + 2 * score_err * unit;
-        int better = 0;
-        unsigned close = 0;  // groups whose scores are too near to this one's, bit o * share
-        const int turns = (a.n_groups + share - 1) / share;  // a group's lanes look at the others in turn
-#pragma unroll 1
-        for (int n = 0; n < turns; ++n) {
-            const int o = n * share + j, from = min(o, a.n_groups - 1) * share;
-            const T v = __shfl_sync(kAll, score, from), z = fast ? __shfl_sync(kAll, size, from) : (T)0;
-            if (o >= a.n_groups) continue;
-            better += v > score || (v == score && o < g);
-            if (fast && fabs(v - score) <= size + z) close |= 1u << (o * share);
-        }
-        for (int o = share / 2; o > 0; o /= 2) {
-            better += __shfl_xor_sync(kAll, better, o);
-            if (fast) close |= __shfl_xor_sync(kAll, close, o);
-        }
-        const bool stays = g < a.n_groups && j == 0 && score > -INFINITY && better < a.top_groups;
-        const unsigned open = __ballot_sync(kAll, stays);  // bit g * share
-        if (fast && __any_sync(kAll, j == 0 && g < a.n_groups && score > -INFINITY && ((stays ? ~open : open) & close) != 0)) return false;
+        bool near = false;
+        unsigned open = groups_open(a, c, score_err, sum_err, unit, near);  // bit g * share
+        if (fast && near) open = groups_exactly<SIGMOID>(a, token, mx, reinterpret_cast<double *>(c));
         int gi = e0 / per, rest = e0 - gi * per;
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
@@ -181,7 +240,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
             if (++rest == per) rest = 0, ++gi;
         }
     }
-    // k rounds (one more where the border could be near): the warp's largest key, its lowest lane, that lane's first
+    // k rounds (more where the border is in doubt): the warp's largest key, its lowest lane, that lane's first
     K top = 0;
     int where = 0;
     auto lane_best = [&] {
@@ -192,22 +251,25 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
     };
     lane_best();
     const bool check = fast && a.bias != nullptr;
-    const int rounds = check ? a.k + 1 : a.k;
     T last = 0;
-    int mine_e = -1;
+    int mine_e = -1, n = 0;
+    bool near = false;
 #pragma unroll 1
-    for (int r = 0; r < rounds; ++r) {
+    for (;; ++n) {
+        if (!check && n == a.k) break;
         const K best = warp_max(top);
         if (best == 0) break;
         if (check) {
             const T v = value(best);
-            if (r > 0 && last - v <= sum_err * (fabs(v) + fabs(last)) + 2 * score_err * unit) return false;
+            const bool close = n > 0 && last - v <= sum_err * (fabs(v) + fabs(last)) + 2 * score_err * unit;
+            if (n >= a.k && !close) break;
+            if (n == 32) return false;  // (more than a lane each)
+            near |= close;
             last = v;
-            if (r == a.k) break;
         }
         const int owner = __ffs(__ballot_sync(kAll, top == best)) - 1;
         const int e = __shfl_sync(kAll, e0 + where, owner);
-        if (lane == r) mine_e = e;
+        if (lane == n) mine_e = e;
         if (lane == owner) {
 #pragma unroll
             for (int i = 0; i < NPL; ++i)
@@ -215,6 +277,17 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
             lane_best();
         }
     }
+    if (check && near) {  // lane i's candidate to the lane of its rank
+        const int rank = rank_exactly<SIGMOID>(a, token, mx, mine_e, n);
+        int e = -1;
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            const int to = __shfl_sync(kAll, rank, i), f = __shfl_sync(kAll, mine_e, i);
+            if (to == lane) e = f;
+        }
+        mine_e = e;
+    }
+    if (lane >= a.k) mine_e = -1;
     // lane r has the r-th
     const T mine = mine_e >= 0 ? score_of<SIGMOID, false>(x[mine_e], mx, inv) : (T)0;
     T w = mine;
