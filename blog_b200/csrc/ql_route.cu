@@ -21,20 +21,33 @@ constexpr int kWarps = 4;
 constexpr float kTiny = 1e-30f;  // chosen scores whose sum is below this are taken in 64 bits, too
 constexpr unsigned kAll = 0xffffffffu;
 
-// Order-preserving keys: larger key, larger value; 0 for what cannot be chosen (-inf, NaN).
-__device__ __forceinline__ uint32_t order(float v) {
-    if (!(v > -INFINITY)) return 0u;
-    const uint32_t u = __float_as_uint(v == 0.f ? 0.f : v);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
+// What is compared: fp32 values as they are, 64-bit ones as order-preserving words (a warp's maximum takes 32 bits at a time);
+// the lowest of each for what cannot be chosen (-inf, NaN).
+template <typename T>
+struct Key;
+template <>
+struct Key<float> {
+    using type = float;
+    static constexpr float none = -INFINITY;
+};
+template <>
+struct Key<double> {
+    using type = uint64_t;
+    static constexpr uint64_t none = 0;
+};
+__device__ __forceinline__ float order(float v) { return v > -INFINITY ? v : -INFINITY; }
 __device__ __forceinline__ uint64_t order(double v) {
     if (!(v > -INFINITY)) return 0ull;
     const uint64_t u = (uint64_t)__double_as_longlong(v == 0.0 ? 0.0 : v);
     return (u >> 63) ? ~u : (u | 1ull << 63);
 }
-__device__ __forceinline__ float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+__device__ __forceinline__ float value(float k) { return k; }
 __device__ __forceinline__ double value(uint64_t k) { return __longlong_as_double((long long)(k >> 63 ? k ^ (1ull << 63) : ~k)); }
-__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(kAll, k); }
+__device__ __forceinline__ float warp_max(float k) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(k));
+    return r;
+}
 __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
     const uint32_t hi = __reduce_max_sync(kAll, (uint32_t)(k >> 32));
     return (uint64_t)hi << 32 | __reduce_max_sync(kAll, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
@@ -46,17 +59,6 @@ __device__ __forceinline__ float exp_of(float x) { return expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 __device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }
 __device__ __forceinline__ double quotient(double a, double b) { return a / b; }
-
-template <typename T>
-struct Key;
-template <>
-struct Key<float> {
-    using type = uint32_t;
-};
-template <>
-struct Key<double> {
-    using type = uint64_t;
-};
 
 // The score of a logit that may be chosen; mx and inv: the softmax's largest logit and the inverse of its sum.
 template <bool SIGMOID, bool FAST, typename T>
@@ -167,6 +169,7 @@ template <typename T, int NPL, bool SIGMOID>
 __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
     using K = typename Key<T>::type;
     constexpr bool fast = sizeof(T) == 4;
+    constexpr K none = Key<T>::none;
     const int lane = threadIdx.x % 32, E = a.n_experts, e0 = lane * NPL;
     const float *x = a.logits + (int64_t)token * a.logits_stride;
     K key[NPL];
@@ -197,8 +200,8 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
             mx = l[0];
 #pragma unroll
             for (int i = 1; i < NPL; ++i) mx = fmaxf(mx, l[i]);
-            const uint32_t k = warp_max(order(mx));
-            mx = k != 0 ? value(k) : 0.f;
+            mx = warp_max(mx);
+            if (!(mx > -INFINITY)) mx = 0.f;
             if (all || !a.renorm) {
                 T total = 0;
 #pragma unroll
@@ -215,8 +218,8 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
                 const bool there = e0 + i < E && l[i] > -INFINITY;
                 const T s = score_of<SIGMOID, true>(l[i], mx, inv);
                 const T v = a.bias != nullptr && there ? s + (T)bias[i] : s;
-                key[i] = there ? a.bias != nullptr ? order(v) : order((T)l[i]) : (K)0;
-                if (a.n_groups > 1 && e0 + i < E) c[e0 + i] = key[i] != 0 ? v : (T)-INFINITY;
+                key[i] = there ? a.bias != nullptr ? order(v) : order((T)l[i]) : none;
+                if (a.n_groups > 1 && e0 + i < E) c[e0 + i] = key[i] != none ? v : (T)-INFINITY;
             }
         } else {
 #pragma unroll
@@ -236,12 +239,12 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
         int gi = e0 / per, rest = e0 - gi * per;
 #pragma unroll
         for (int i = 0; i < NPL; ++i) {
-            if (e0 + i < E && !(open >> (gi * share) & 1u)) key[i] = 0;
+            if (e0 + i < E && !(open >> (gi * share) & 1u)) key[i] = none;
             if (++rest == per) rest = 0, ++gi;
         }
     }
     // k rounds (more where the border is in doubt): the warp's largest key, its lowest lane, that lane's first
-    K top = 0;
+    K top = none;
     int where = 0;
     auto lane_best = [&] {
         top = key[0], where = 0;
@@ -258,7 +261,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
     for (;; ++n) {
         if (!check && n == a.k) break;
         const K best = warp_max(top);
-        if (best == 0) break;
+        if (best == none) break;
         if (check) {
             const T v = value(best);
             const bool close = n > 0 && last - v <= sum_err * (fabs(v) + fabs(last)) + 2 * score_err * unit;
@@ -273,7 +276,7 @@ __device__ __forceinline__ bool choose(const RouteArgs &a, int token, T *c) {
         if (lane == owner) {
 #pragma unroll
             for (int i = 0; i < NPL; ++i)
-                if (i == where) key[i] = 0;
+                if (i == where) key[i] = none;
             lane_best();
         }
     }
