@@ -1578,7 +1578,7 @@ int ql_moe_route(const float *logits, int64_t logits_stride, int32_t *top_idx, f
         a.sigmoid = rule->score == QL_ROUTE_SIGMOID, a.renorm = rule->renormalise != 0;
         a.n_groups = rule->n_groups, a.top_groups = rule->top_groups, a.group_best = rule->group_best;
         a.scale = rule->scale;
-        const cudaError_t e = route_launch(a, ws->sms, g_stream);
+        const cudaError_t e = route_launch(a, g_stream);
         ++t_launches;
         return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
     });
@@ -1671,7 +1671,7 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
             lora_tiles_plan(a, type, distinct, ws->sms) && lora_maps(maps, a, width, type == 2)) {
             e = lora_tiles_launch(a, maps, type, g_stream);
         } else {
-            const int tm = lora_plan(a, type, distinct, ws->sms);
+            const int tm = lora_plan(a, distinct, ws->sms);
             if (((int64_t)rows + kLoraChunk - 1) / kLoraChunk * a.chunk_tiles * a.cluster > INT32_MAX)
                 return fail(QL_EINVAL, what + ": too many rows for one call");
             e = lora_launch(a, type, tm, g_stream);

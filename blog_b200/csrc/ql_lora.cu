@@ -232,8 +232,8 @@ __device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, 
     }
 }
 
-__device__ __forceinline__ void prefetch_l2_bulk(const void *p, uint32_t bytes) {  // both multiples of 16
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+__device__ __forceinline__ void prefetch_l2_bulk(const void *p, int64_t bytes) {  // both multiples of 16; 4 MB at most
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((uint32_t)min(bytes, (int64_t)4 << 20)) : "memory");
 }
 __device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
         constexpr int el = Weight<WT>::bytes;
         const char *w = static_cast<const char *>(a.b[proj]) + ((int64_t)tile.id * a.out[proj] + o_begin * 32) * a.max_rank * el;
         if (2 * rank > a.max_rank) {
-            if (tid == 0) prefetch_l2_bulk(w, (uint32_t)n_mine * a.max_rank * el);
+            if (tid == 0) prefetch_l2_bulk(w, (int64_t)n_mine * a.max_rank * el);
         } else {  // (rows with long gaps)
 #pragma unroll 1
             for (int r = tid; r < n_mine; r += kThreads)
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
         }
     }
     if (a.base != nullptr && a.y_vec && n_mine > 0 && warp == 1 && lane < tile.n)
-        prefetch_l2_bulk(a.base + (int64_t)list[lane] * a.base_stride + a.col[proj] + o_begin * 32, (uint32_t)n_mine / 4 * 16);
+        prefetch_l2_bulk(a.base + (int64_t)list[lane] * a.base_stride + a.col[proj] + o_begin * 32, (int64_t)n_mine * 4);
     const int padded = (a.max_rank + 31) / 32 * 32, pitch = padded + (WT == kW32 ? 4 : 8);
     float *h = smem;                    // [padded][TM], this CTA's share; read by its cluster
     float *limb = smem + padded * TM;   // [limbs][TM][pitch] of h, 16 bits each or 32; before that the warps' sums
@@ -493,13 +493,19 @@ size_t smem_bytes(int max_rank, int TM) {
     return sizeof(float) * (padded * TM + std::max(2 * TM * (padded + 8), kWarps * kPass * TM));
 }
 
+// The kernel may have what the largest rank takes: the same for every call, so that calls of several threads do not undo it.
+template <int WT, int NT>
+cudaError_t allow_smem() {
+    return cudaFuncSetAttribute(lora_kernel<WT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(kLoraMaxRank, 8 * NT));
+}
+
 template <int WT, int NT>
 cudaError_t launch(const LoraArgs &a, cudaStream_t s) {
     const size_t smem = smem_bytes(a.max_rank, 8 * NT);
-    cudaError_t e = cudaFuncSetAttribute(lora_kernel<WT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_smem<WT, NT>();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    const int chunks = (a.rows + kLoraChunk - 1) / kLoraChunk;
+    const int chunks = (a.rows - 1) / kLoraChunk + 1;
     cfg.gridDim = dim3((unsigned)(chunks * a.chunk_tiles * a.cluster), (unsigned)a.n_proj, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = smem;
@@ -526,16 +532,17 @@ int clusters_at_once(int nt, int c, int sms) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return std::max(1, sms / c);
     int n = known[dev][k][c].load();
     if (n == 0) {
-        const void *f = k == 0 ? (const void *)lora_kernel<kWB16, 1> : k == 1 ? (const void *)lora_kernel<kWB16, 2> : (const void *)lora_kernel<kWB16, 4>;
-        const int smem = (int)smem_bytes(64, 8 * nt);
+        const void *f = k == 0   ? (const void *)lora_kernel<kWB16, 1>
+                        : k == 1 ? (const void *)lora_kernel<kWB16, 2>
+                                 : (const void *)lora_kernel<kWB16, 4>;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem;
+        cfg.gridDim = dim3(c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem_bytes(64, 8 * nt);
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim = {(unsigned)c, 1, 1};
         cfg.attrs = at, cfg.numAttrs = 1;
-        if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&n, f, &cfg) != cudaSuccess || n <= 0) {
+        const cudaError_t e = k == 0 ? allow_smem<kWB16, 1>() : k == 1 ? allow_smem<kWB16, 2>() : allow_smem<kWB16, 4>();
+        if (e != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, f, &cfg) != cudaSuccess || n <= 0) {
             (void)cudaGetLastError();
             n = std::max(1, sms / c);
         }
@@ -545,16 +552,16 @@ int clusters_at_once(int nt, int c, int sms) {
 }
 }  // namespace
 
-int lora_plan(LoraArgs &a, int type, int distinct, int sms) {
-    (void)type;
+int lora_plan(LoraArgs &a, int distinct, int sms) {
     const int each = a.rows / distinct, tm = each <= 8 ? 8 : each <= 16 ? 16 : 32;
     const int chunk = std::min(a.rows, kLoraChunk);
     // n rows of d adapters make at most (n + d (tm - 1)) / tm tiles, and about half of those that are not full
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (tm - 1)) / tm);
     const int kinds = std::max(1, std::min(a.n_seqs, a.n_adapters));
     const double tiles = std::max<double>(std::min(kinds, a.rows), (double)a.rows / tm + kinds / 2) * a.n_proj;
-    // CTAs per tile: what the rounds of the GPU take in all (parts of rounds count, tiles of low rank end early); beside its share a CTA takes as long as 2400 columns (one
-    // 64-row call of 7B q/k/v, rank 16: 41, 25, 17, 12 us with 1, 2, 4, 8)
+    // CTAs per tile: what the rounds of the GPU take in all (parts of rounds count, tiles of low rank end early); beside its
+    // share a CTA takes as long as 2400 columns (64 rows of one adapter of rank 16, 4096 -> 4096 x 3: 41, 25, 17, 12 us with
+    // 1, 2, 4, 8)
     int widest = 0;
     for (int p = 0; p < a.n_proj; ++p) widest = std::max(widest, a.out[p]);
     double best = 0;

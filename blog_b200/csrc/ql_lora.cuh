@@ -239,7 +239,7 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
 }
 
 // Fills in what the launch needs; returns the rows of a tile.
-int lora_plan(LoraArgs &a, int type, int distinct, int sms);
+int lora_plan(LoraArgs &a, int distinct, int sms);
 cudaError_t lora_launch(const LoraArgs &a, int type, int tile_rows, cudaStream_t s);
 // Tiles of 128 rows: fills in what the launch needs; false: not for these sizes or this alignment.
 bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms);

@@ -1,5 +1,5 @@
 // Low-rank adapters beside a shared projection for prompts: h = scale x A^T, y = base + h B^T over tiles of 128 rows of
-// one adapter on tcgen05 (kind::tf32), one launch.
+// one adapter on tcgen05, one launch.
 //
 // A cluster of CTAs has a tile: each CTA takes its share of x's columns, all projections' ranks side by side (N of one
 // product), adds the shares through distributed shared memory and takes its share of the outputs, 64 at a time.  x, the
@@ -989,10 +989,18 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
     }
 }
 
+constexpr int kSmem = 224 * 1024;  // of the rings together, at most
+
+// The same for every call, so that calls of several threads do not undo it.
+template <int WT>
+cudaError_t allow_smem() {
+    return cudaFuncSetAttribute(lora_tiles_kernel<WT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + kSmem);
+}
+
 template <int WT>
 cudaError_t launch(const LoraArgs &a, const LoraMaps &maps, cudaStream_t s) {
     const int smem = 1024 + kRowWarps * kDepth * kSlot + a.ring * a.ring_bytes + a.raw_total;
-    cudaError_t e = cudaFuncSetAttribute(lora_tiles_kernel<WT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = allow_smem<WT>();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     const int chunks = (a.rows + kLoraChunk - 1) / kLoraChunk;
@@ -1017,14 +1025,13 @@ int clusters_at_once(int c, int sms) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return std::max(1, sms / c);
     int n = known[dev][c].load();
     if (n == 0) {
-        constexpr int smem = 224 * 1024;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = smem;
+        cfg.gridDim = dim3(c), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = kSmem;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeClusterDimension;
         at[0].val.clusterDim = {(unsigned)c, 1, 1};
         cfg.attrs = at, cfg.numAttrs = 1;
-        if (cudaFuncSetAttribute(lora_tiles_kernel<kWB16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        if (allow_smem<kWB16>() != cudaSuccess ||
             cudaOccupancyMaxActiveClusters(&n, lora_tiles_kernel<kWB16>, &cfg) != cudaSuccess || n <= 0) {
             (void)cudaGetLastError();
             n = std::max(1, sms / c);
@@ -1044,7 +1051,7 @@ bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
     a.raw_bytes = (ranks * 4 + 127) / 128 * 128 * 16 * limbs;
     // (bf16: none on the way; others: four stages of A, five of B)
     a.raw_total = type == 2 ? 0 : std::max(kRaw * a.raw_bytes, (kAhead + 1) * 2 * 128 * 16 * limbs);
-    a.ring = std::min(kMaxRing, (224 * 1024 - kRowWarps * kDepth * kSlot - a.raw_total) / a.ring_bytes);
+    a.ring = std::min(kMaxRing, (kSmem - kRowWarps * kDepth * kSlot - a.raw_total) / a.ring_bytes);
     if (a.ring < 2) return false;
     const int chunk = std::min(a.rows, kLoraChunk);
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (kTile - 1)) / kTile);

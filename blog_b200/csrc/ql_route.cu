@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(32 * kWarps, NPL <= 8 ? 12 : NPL <= 16 ? 8 : 4
 template <int NPL>
 cudaError_t launch(const RouteArgs &a, cudaStream_t s) {
     const size_t smem = a.n_groups > 1 ? sizeof(double) * kWarps * (size_t)a.n_experts : 0;
-    const unsigned grid = (unsigned)((a.tokens + kWarps - 1) / kWarps);
+    const unsigned grid = (unsigned)((a.tokens - 1) / kWarps + 1);
     if (a.sigmoid)
         route_kernel<NPL, true><<<grid, 32 * kWarps, smem, s>>>(a);
     else
@@ -336,8 +336,7 @@ cudaError_t launch(const RouteArgs &a, cudaStream_t s) {
 static_assert(sizeof(double) * kWarps * kRouteMaxExperts <= 48 * 1024, "shared memory without asking for more");
 }  // namespace
 
-cudaError_t route_launch(const RouteArgs &a, int sms, cudaStream_t s) {
-    (void)sms;
+cudaError_t route_launch(const RouteArgs &a, cudaStream_t s) {
     const int need = (a.n_experts + 31) / 32;
     return need <= 2    ? launch<2>(a, s)
            : need <= 4  ? launch<4>(a, s)

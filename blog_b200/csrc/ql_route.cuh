@@ -18,6 +18,6 @@ struct RouteArgs {
     float scale;
 };
 
-cudaError_t route_launch(const RouteArgs &a, int sms, cudaStream_t s);
+cudaError_t route_launch(const RouteArgs &a, cudaStream_t s);
 
 }  // namespace ql
