@@ -406,10 +406,10 @@ QL_API int ql_add_rms_norm(int32_t type, const void *x, int64_t x_stride, const 
  *   counted by the sum of its group_best (1 or 2) largest c;
  *   the k experts of largest c in them, by descending c; equal ones by the lower id (groups likewise);
  *   w_e = s_e [renormalise: / sum of the chosen s, 0 where that is 0] * scale   (the bias is not in the weights)
- * c is compared as 64-bit scores (without a bias, logits); weights are f32 within 2^-18 of the token's largest score (with renormalise of
- * 1) times scale.  A logit that is not finite counts as -inf; such an expert, or one with a bias of -inf or NaN, is never chosen, nor is a
- * group of none but them.  Where fewer than k are left the rest of top_idx is -1 with weight 0 (the grouped experts
- * skip those).  n_experts <= 1024, k <= 32, n_groups <= 32; tokens' rows of logits are logits_stride floats apart. */
+ * c is compared as 64-bit scores (without a bias, logits); weights are f32 within 2^-18 of the token's largest score (with
+ * renormalise of 1) times scale.  A logit that is not finite counts as -inf; such an expert, or one with a bias of -inf or
+ * NaN, is never chosen, nor is a group of none but them.  Where fewer than k are left the rest of top_idx is -1 with weight
+ * 0 (the grouped experts skip those).  n_experts <= 1024, k <= 32, n_groups <= 32; tokens' rows of logits are logits_stride floats apart. */
 #define QL_ROUTE_SOFTMAX 0
 #define QL_ROUTE_SIGMOID 1
 typedef struct ql_moe_route_rule {
@@ -426,13 +426,15 @@ QL_API int ql_moe_route(const float *logits, int64_t logits_stride, int32_t *top
  * For rows x of many requests, each with its own adapter i of a pool, beside one to three projections of the same x
  * whose outputs stand side by side in a row of y (q, k and v; gate and up):
  *   h = scale[i] x A_i^T,   y = base + h B_i^T
- * base is what the shared (quantised) projection gave; it may be y (same stride), or NULL for 0.  A row without an
- * adapter gets y = base.  x and y must not overlap.
+ * base is what the shared (quantised) projection gave; it may be y (same stride), else it must not overlap y, or NULL for
+ * 0.  A row without an adapter gets y = base.  x and y must not overlap.
  * The pool keeps n_adapters slots for each projection, of max_rank ranks; adapter i uses the first rank[i] of them
  * (0: as none), what stands in the rest is not used.  type: QL_F16, QL_BF16 or QL_F32, of A and B.  in_dim: a
  * multiple of 32; max_rank: a multiple of 8 up to 256; out_dim: any.  a and b start on 16 bytes; a pair that is NULL is
- * a projection without adapters.  fp32 results: x, h and f32 weights enter the tensor cores as two tf32 limbs (22 bits),
- * f16 and bf16 weights exactly, and sums are fp32. */
+ * a projection without adapters.  fp32 results: f16 and bf16 weights enter the tensor cores exactly, f32 ones as two
+ * tf32 limbs (22 bits); x and h as three bf16 limbs beside bf16 weights (every bit), else as two limbs (22 bits; h beside
+ * f16 weights 22 bits of its row's largest in calls of few rows); sums are fp32.  A row of x that is not finite, or an h
+ * that passes fp32's range, gives NaN, in that row alone. */
 typedef struct ql_lora_pool {
     int32_t type, n_proj;
     const void *a[3];    /* [n_adapters][max_rank][in_dim] */
@@ -445,8 +447,9 @@ typedef struct ql_lora_pool {
 /* adapter: device, [n_seqs], the adapter of each sequence, < 0: none.  q_start == NULL: row s is the one row of sequence s
  * (rows == n_seqs); otherwise sequence s has rows q_start[s] .. q_start[s + 1] - 1 (device, [n_seqs + 1], not falling; none is
  * allowed), and rows before the first and behind the last sequence are left as they are.  Both are read on the device, so a
- * captured CUDA graph follows them.  Rows of different sequences with one adapter share its weights.  An adapter outside the pool, or
- * a rank outside 0 .. max_rank, counts as none and is reported by the next ql_check_device (QL_EDEVICE).  One launch. */
+ * captured CUDA graph follows them.  Rows of different sequences with one adapter share its weights.  An adapter outside the
+ * pool, or a rank outside 0 .. max_rank, counts as none and is reported by the next ql_check_device (QL_EDEVICE).  One
+ * launch; the same call gives the same bits. */
 QL_API int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, const float *base, int64_t base_stride,
                        float *y, int64_t y_stride, const int32_t *adapter, int n_seqs, const int32_t *q_start, int rows);
 
