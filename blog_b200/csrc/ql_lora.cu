@@ -232,11 +232,6 @@ __device__ __forceinline__ void expand(const LoraArgs &a, const LoraTile &tile, 
     }
 }
 
-__device__ __forceinline__ void prefetch_l2_bulk(const void *p, int64_t bytes) {  // both multiples of 16; 4 MB at most
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((uint32_t)min(bytes, (int64_t)4 << 20)) : "memory");
-}
-__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
 template <int WT, int NT>
 __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const __grid_constant__ LoraArgs a) {
     constexpr int TM = 8 * NT;
@@ -257,24 +252,8 @@ __global__ void __launch_bounds__(kThreads, NT <= 2 ? 2 : 1) lora_kernel(const _
         }
     }
     if (rank == 0 && a.y == a.base) return;
-    // this CTA's outputs, and what they need asked for while h is computed
-    const int n32 = (a.out[proj] + 31) / 32;
+    const int n32 = (a.out[proj] + 31) / 32;  // this CTA's outputs
     const int o_begin = (int)((uint32_t)n32 * part / parts), o_end = (int)((uint32_t)n32 * (part + 1) / parts);
-    const int n_mine = min(o_end * 32, a.out[proj]) - o_begin * 32;
-    if (rank > 0 && n_mine > 0) {
-        constexpr int el = Weight<WT>::bytes;
-        const char *w = static_cast<const char *>(a.b[proj]) + ((int64_t)tile.id * a.out[proj] + o_begin * 32) * a.max_rank * el;
-        if (2 * rank > a.max_rank) {
-            if (tid == 0) prefetch_l2_bulk(w, (int64_t)n_mine * a.max_rank * el);
-        } else {  // (rows with long gaps)
-#pragma unroll 1
-            for (int r = tid; r < n_mine; r += kThreads)
-#pragma unroll 1
-                for (int at = 0; at < rank * el; at += 128) prefetch_l2(w + (int64_t)r * a.max_rank * el + at);
-        }
-    }
-    if (a.base != nullptr && a.y_vec && n_mine > 0 && warp == 1 && lane < tile.n)
-        prefetch_l2_bulk(a.base + (int64_t)list[lane] * a.base_stride + a.col[proj] + o_begin * 32, (int64_t)n_mine * 4);
     const int padded = (a.max_rank + 31) / 32 * 32, pitch = padded + (WT == kW32 ? 4 : 8);
     float *h = smem;                    // [padded][TM], this CTA's share; read by its cluster
     float *limb = smem + padded * TM;   // [limbs][TM][pitch] of h, 16 bits each or 32; before that the warps' sums

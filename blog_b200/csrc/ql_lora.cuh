@@ -8,6 +8,7 @@ namespace ql {
 
 constexpr int kLoraMaxRank = 256, kLoraMaxProj = 3;
 constexpr int kLoraChunk = 512;  // rows among which those of one adapter are brought together
+constexpr int kPairs = 128;      // rows of a chunk that are compared with one another
 constexpr int kLoraTile = 128;   // rows of a tile on tcgen05, for calls of at least so many rows, and so many of each
 constexpr int kLoraTileRows = 400, kLoraTileFrom = 48;  // adapter on average
 
@@ -96,7 +97,7 @@ struct LoraTile {
 // What find_tile needs of shared memory.
 struct LoraFind {
     int starts[kLoraChunk + 1], adapters[kLoraChunk];  // of the sequences, where there are no more
-    int2 kinds[24 * 32];                               // per warp (24 at most): adapters and how many of its rows have them
+    alignas(16) int2 kinds[24 * 32];                               // per warp (24 at most): adapters and how many of its rows have them
     int n_kinds[24], leaders[24];
     int found[3];
 };
@@ -146,7 +147,7 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
     unsigned same[kPer];
 #pragma unroll
     for (int h = 0; h < kPer; ++h) {
-        const int i = h * THREADS + tid, w = h * kWarps + tid / 32;
+        const int i = h * THREADS + tid;
         id[h] = kOutside;
         if (i < n) {
             int s = r0 + i;
@@ -171,6 +172,43 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
                 id[h] = max(id[h], kNone);
             }
         }
+    }
+    if (n <= kPairs) {  // few rows: a thread looks at all of them
+        int *ids = reinterpret_cast<int *>(f.kinds);
+        if (tid < kPairs) ids[tid] = id[0];  // (from n on: outside)
+        __syncthreads();
+        int before = 0, all = 0;
+        bool lead = false;
+        if (tid < kPairs) {
+#pragma unroll 4
+            for (int j = 0; j < n; j += 4) {
+                const int4 v = *reinterpret_cast<const int4 *>(ids + j);
+                const int e0 = v.x == id[0], e1 = v.y == id[0], e2 = v.z == id[0], e3 = v.w == id[0];
+                all += e0 + e1 + e2 + e3;
+                before += (e0 && j < tid) + (e1 && j + 1 < tid) + (e2 && j + 2 < tid) + (e3 && j + 3 < tid);
+            }
+            lead = id[0] != kOutside && before % tm == 0;
+            const unsigned m = __ballot_sync(0xffffffffu, lead);
+            if (lane == 0) f.leaders[tid / 32] = __popc(m);
+            same[0] = __popc(m & ((1u << lane) - 1));
+        }
+        __syncthreads();
+        if (lead) {
+            int k = (int)same[0];
+#pragma unroll
+            for (int w = 0; w < kPairs / 32 - 1; ++w) k += w < tid / 32 ? f.leaders[w] : 0;
+            if (k == t) f.found[0] = min(tm, all - before), f.found[1] = id[0], f.found[2] = before;
+        }
+        __syncthreads();
+        const LoraTile found{f.found[1], f.found[2], f.found[0]};
+        if (tid < kPairs && id[0] == found.id && before >= found.first && before < found.first + found.n)
+            list[before - found.first] = r0 + tid;
+        __syncthreads();
+        return found;
+    }
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+        const int w = h * kWarps + tid / 32;
         // the warp's adapters, each with its rows: their lowest lanes write them down
         same[h] = __match_any_sync(0xffffffffu, id[h]);
         const unsigned firsts = __ballot_sync(0xffffffffu, __ffs(same[h]) - 1 == lane);
