@@ -1667,11 +1667,17 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
         for (int p = 0; p < a.n_proj; ++p) a.y_vec = a.y_vec && a.out[p] % 4 == 0;
         cudaError_t e;
         LoraMaps maps;
-        if (rows >= kLoraTileRows && rows / distinct >= kLoraTileFrom && rows <= INT32_MAX / 8 && (int64_t)a.n_adapters * a.max_rank <= INT32_MAX &&
-            lora_tiles_plan(a, type, distinct, ws->sms) && lora_maps(maps, a, width, type == 2)) {
-            e = lora_tiles_launch(a, maps, type, g_stream);
+        // Two kernels: tiles of at most 32 rows on mma.sync, whose many CTAs serve few rows and low ranks, and tiles of 128 on
+        // tcgen05.  The one that is to be the faster by both plans' estimates (512 rows on 7B down, rank 16: 49 and 59 us;
+        // 2048 rows on 72B q/k/v, rank 64: 226 and 89 us).
+        LoraArgs tiles = a;
+        double us = 0, tiles_us = 0;
+        const int tm = lora_plan(a, type, distinct, ws->sms, us);
+        if (rows >= kLoraTile && rows / distinct >= kLoraTileFrom && rows <= INT32_MAX / 8 &&
+            (int64_t)a.n_adapters * a.max_rank <= INT32_MAX && lora_tiles_plan(tiles, type, distinct, ws->sms, tiles_us) &&
+            tiles_us < us && lora_maps(maps, tiles, width, type == 2)) {
+            e = lora_tiles_launch(tiles, maps, type, g_stream);
         } else {
-            const int tm = lora_plan(a, distinct, ws->sms);
             if (((int64_t)rows + kLoraChunk - 1) / kLoraChunk * a.chunk_tiles * a.cluster > INT32_MAX)
                 return fail(QL_EINVAL, what + ": too many rows for one call");
             e = lora_launch(a, type, tm, g_stream);

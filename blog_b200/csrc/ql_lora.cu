@@ -15,11 +15,19 @@
 //   f32 weights   m16n8k8 tf32, two limbs on both sides
 // A warp has columns of its own, so nothing is shared before the warps' sums.  The tensor cores cut what they add up off
 // towards zero, so their sums are added to others with rounding every 64 columns or 32 ranks.
+//
+// Bound: latency.  One token over 3584 -> 3584 + 512 + 512 at rank 16 takes 6.5 us: the launch, finding the tile, loads of A,
+// the cluster's sum, loads of B, each after the other.  64 tokens of 16 adapters of ranks up to 64 over 3584 -> 2 x 18944
+// take 32 us where the bytes take 8: every group of outputs waits once for its weights, and the CTAs of the highest ranks
+// end last.  Slower there: weights of all outputs asked into L2 before h (38 us: A waits behind them), a ring of weights
+// filled ahead in shared memory by cp.async (38 us: more instructions per output), two tiles of outputs at a time (37 us),
+// three CTAs an SM (40 us).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "ql_lora.cuh"
@@ -531,23 +539,32 @@ int clusters_at_once(int nt, int c, int sms) {
 }
 }  // namespace
 
-int lora_plan(LoraArgs &a, int distinct, int sms) {
+int lora_plan(LoraArgs &a, int type, int distinct, int sms, double &us) {
     const int each = a.rows / distinct, tm = each <= 8 ? 8 : each <= 16 ? 16 : 32;
     const int chunk = std::min(a.rows, kLoraChunk);
     // n rows of d adapters make at most (n + d (tm - 1)) / tm tiles, and about half of those that are not full
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (tm - 1)) / tm);
     const int kinds = std::max(1, std::min(a.n_seqs, a.n_adapters));
     const double tiles = std::max<double>(std::min(kinds, a.rows), (double)a.rows / tm + kinds / 2) * a.n_proj;
-    // CTAs per tile: what the rounds of the GPU take in all (parts of rounds count, tiles of low rank end early); beside its
-    // share a CTA takes as long as 2400 columns (64 rows of one adapter of rank 16, 4096 -> 4096 x 3: 41, 25, 17, 12 us with
-    // 1, 2, 4, 8)
-    int widest = 0;
-    for (int p = 0; p < a.n_proj; ++p) widest = std::max(widest, a.out[p]);
-    double best = 0;
-    for (int c = 1; c <= 8; c *= 2) {
-        const int at_once = clusters_at_once(tm / 8, c, sms);
-        const double time = std::max(1.0, tiles / at_once) * ((a.in_dim + 2.0 * widest) / c + 2400.0);
-        if (best == 0 || time < best) best = time, a.cluster = c;
+    double widest = 0, mean = 0;
+    for (int p = 0; p < a.n_proj; ++p) widest = std::max<double>(widest, a.out[p]), mean += (double)a.out[p] / a.n_proj;
+    // CTAs per tile: what the rounds of the GPU take in all.
+    us = 0;
+    for (int c = 1; c <= 8; c += tm < 32 ? c : 1) {
+        const double rounds = tiles / clusters_at_once(tm / 8, c, sms);
+        double time;
+        if (tm < 32) {
+            // parts of rounds count, tiles of low rank end early; beside its share a CTA takes as long as 2400 columns (64
+            // rows of one adapter of rank 16, 4096 -> 4096 x 3: 41, 25, 17, 12 us with 1, 2, 4, 8)
+            time = std::max(1.0, rounds) * ((a.in_dim + 2.0 * widest) / c + 2400.0) * 0.0035;
+        } else {
+            // us of a CTA, from measured times of 128 rows: a column costs as much up to 16 ranks, and again up to 64
+            const double per_in = a.max_rank <= 16 ? 0.0033 : (type == 0 ? 0.0134 : 0.0105) * ((a.max_rank + kPass - 1) / kPass);
+            const double per_out = 0.008 + (type == 0 ? 0.0002 : 0.00011) * a.max_rank;
+            time = rounds <= 1 ? 1 : kinds == 1 ? std::ceil(rounds) : (rounds + std::ceil(rounds)) / 2;
+            time *= 7.5 + 0.05 * a.max_rank + (per_in * a.in_dim + per_out * (rounds <= 1 ? widest : mean)) / c;
+        }
+        if (us == 0 || time < us) us = time, a.cluster = c;
     }
     return tm;
 }

