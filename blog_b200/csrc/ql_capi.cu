@@ -1668,8 +1668,8 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
         cudaError_t e;
         LoraMaps maps;
         // Two kernels: tiles of at most 32 rows on mma.sync, whose many CTAs serve few rows and low ranks, and tiles of 128 on
-        // tcgen05.  The one that is to be the faster by both plans' estimates (512 rows on 7B down, rank 16: 49 and 59 us;
-        // 2048 rows on 72B q/k/v, rank 64: 226 and 89 us).
+        // tcgen05.  The one that is to be the faster by both plans' estimates (512 rows, 18944 -> 3584 at rank 16: 33 and 59 us;
+        // 2048 rows, 8192 -> 8192 + 1024 + 1024 at rank 64: 226 and 89 us).
         LoraArgs tiles = a;
         double us = 0, tiles_us = 0;
         const int tm = lora_plan(a, type, distinct, ws->sms, us);
