@@ -9,8 +9,8 @@
 // thread has groups of 4 consecutive values (16 bytes in f32), so the 8 threads of an 8-bit block are neighbours and
 // its maximum and sums take three shuffles.  Squares are summed in fp32, a tree over the threads.
 //
-// Measured, residual and Q8_1 rows: 4096 rows of 8192 f32 with sum and y 93.5 us (6.14 TB/s, 0.94 of a plain copy); 777 rows
-// of 2048, no y, 8.1 us; 64 rows of 8192 bf16 4.2 us and one row of 3584 2.8 us: a launch, a load and two reductions.
+// Measured, residual and Q8_1 rows: 4096 rows of 8192 f32 with sum and y 91.7 us (6.26 TB/s, 0.96 of a plain copy); 777 rows
+// of 2048, no y, 7.8 us; 64 rows of 8192 bf16 4.2 us and one row of 3584 2.8 us: a launch, a load and two reductions.
 #include <cuda_bf16.h>
 
 #include "ql_norm.cuh"
@@ -214,12 +214,13 @@ template <bool BF16>
 cudaError_t pick(const AddNormArgs &a, int sms, cudaStream_t s) {
     const int groups = (a.hidden + 31) / 32 * 8;  // of 4 values, whole 8-bit blocks
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
-    // few rows: one group per thread (latency); many: four, so that loads in flight do not need many threads
-    const bool few = a.rows <= 2 * sms;
+    // One group per thread where rows are few (latency) or narrow; else two, so that loads in flight do not need many threads
+    // (one, two, four of them: 5000 rows of 3584 f32 59, 49, 51 us, 300 rows of 896 2.6, 3.0, 4.0 us; eight are slower
+    // everywhere), and more for rows that need them.
+    const bool few = a.rows <= 2 * sms || (a.rows <= 8 * sms && threads(1) <= 256);
     if (few && threads(1) <= 1024) return launch<BF16, 1, 1024>(a, threads(1), s);
-    if (few && threads(2) <= 1024) return launch<BF16, 2, 1024>(a, threads(2), s);
-    if (threads(4) <= 512) return launch<BF16, 4, 512>(a, threads(4), s);
-    if (threads(8) <= 512) return launch<BF16, 8, 512>(a, threads(8), s);
+    if (threads(2) <= 1024) return launch<BF16, 2, 1024>(a, threads(2), s);
+    if (threads(4) <= 1024) return launch<BF16, 4, 1024>(a, threads(4), s);
     return launch<BF16, 8, 1024>(a, threads(8), s);
 }
 }  // namespace
