@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const __grid_constant__ 
         ss = squares();
     }
     const float inv = rsqrtf(__fadd_rn(__fdiv_rn(ss, (float)H), eps));
-    const int nb = (H + 31) / 32;
+    const int nb = (H + 31) / 32, written = a.mmq ? (nb + 3) / 4 * 4 : nb;  // (the packed layout has whole groups of four)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if (NV > 4) scales(i);
@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(MAXT) add_norm_kernel(const __grid_constant__ 
             for (int o = 4; o > 0; o >>= 1) qs += __shfl_xor_sync(0xffffffffu, qs, o);
             total = __fmul_rn(d, (float)qs);
         }
-        if (b < nb) {
+        if (b >= nb) total = 0.f;  // (behind the row: zeros beside a row of NaN too)
+        if (b < written) {
             uint8_t *ds, *qd;
             if (a.mmq) {
                 uint8_t *grp = a.xq + ((int64_t)(b / 4) * a.rows + row) * 144;
@@ -212,7 +213,7 @@ cudaError_t launch(const AddNormArgs &a, int threads, cudaStream_t s) {
 }
 template <bool BF16>
 cudaError_t pick(const AddNormArgs &a, int sms, cudaStream_t s) {
-    const int groups = (a.hidden + 31) / 32 * 8;  // of 4 values, whole 8-bit blocks
+    const int groups = a.mmq ? (a.hidden + 127) / 128 * 32 : (a.hidden + 31) / 32 * 8;  // of 4 values, whole 8-bit blocks, or four
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
     // One group per thread where rows are few (latency) or narrow; else two, so that loads in flight do not need many threads
     // (one, two, four of them: 5000 rows of 3584 f32 59, 49, 51 us, 300 rows of 896 2.6, 3.0, 4.0 us; eight are slower
