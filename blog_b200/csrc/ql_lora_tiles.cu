@@ -824,197 +824,199 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
             __syncwarp();
             cluster_wait();
         }
-    } else if (warp == 13) {
-        // ------------------------------------ rows that lie together, to and from memory ------------------------------------
-        reg_dec<kOtherRegs>();
-        int issued[2] = {0, 0};
-        bool ok = true;
-        auto load = [&](int half, const CUtensorMap *map, int col) {  // null: the slot only
-            const int m = issued[half], st = m % kDepth;
-            if (m >= kDepth && !wait(&b.free[half][st], m / kDepth - 1)) return false;
-            if (map != nullptr) {
-                mbar_arrive_expect_tx(&b.land[half][st], 4 * kSlot);
-                tma_box2d(ring + (st * kRowWarps + 4 * half) * kSlot, map, col, row0, &b.land[half][st]);
-            } else {
-                mbar_arrive(&b.land[half][st]);
-            }
-            ++issued[half];
-            return true;
-        };
-        Slice next[2] = {from, from};
-        int asked[2] = {j0, j0};
-        // the next base of a half, unless its slot is one of those below `from_slot`
-        auto load_base = [&](int half, int from_slot) {
-#pragma unroll 1
-            while (asked[half] < j1 && width_of(next[half], half) <= 0) next[half].step(a), ++asked[half];
-            if (asked[half] >= j1 || issued[half] % kDepth < from_slot) return false;
-            ok = ok && load(half, a.base != nullptr ? &maps.base : nullptr, col_of(next[half], half));
-            next[half].step(a), ++asked[half];
-            return ok;
-        };
-        int ahead[2] = {0, 0};
-        if (joint && lane == 0) {
-#pragma unroll 1
-            for (int i = 0; i < n_blocks && ok; ++i) {
-                if (i & 1)
-                    ok = load(1, &maps.x, (i0 + i) * 32);
-                else
-                    ok = load(0, &maps.x, (i0 + i) * 32);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-                while (ok && ahead[h] < kDepth && load_base(h, taken)) ++ahead[h];
-        }
-        __syncwarp();
-        if (R > 0) {
-            cluster_arrive();
-            cluster_wait();
-            cluster_arrive();
-            cluster_wait();
-            ok = __all_sync(0xffffffffu, wait(&b.h_full, 0)) && ok;  // (the sums are read: their slots are free)
-            fence_proxy_async_smem();
-        }
-        if (joint && lane == 0) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-                while (ok && ahead[h] < kDepth && load_base(h, 0)) ++ahead[h];
-            // A slot is filled again when its store has read it, three stores later.
-            int used[2] = {(n_blocks + 1) / 2, n_blocks / 2}, stored = 0;
-            unsigned order = 0;  // the halves of the last stores, the latest in bit 0
-            Slice s = from;
-#pragma unroll 1
-            for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int width = width_of(s, h);
-                    if (width <= 0 || !ok) continue;
-                    const int st = used[h] % kDepth;
-                    ok = wait(&b.free[h][st], used[h] / kDepth);
-                    if (!ok) break;
-                    ++used[h], ++stored, order = order << 1 | h;
-                    if (tile.n == kTile && width == 32)
-                        tma_store_2d(&maps.y, col_of(s, h), row0, smem_u32(ring + (st * kRowWarps + 4 * h) * kSlot));
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                    if (stored > 3) {
-                        stores_read<3>();
-                        if (order >> 3 & 1)
-                            load_base(1, 0);
-                        else
-                            load_base(0, 0);
-                    }
-                }
-            }
-            // never leave with copies in flight
-            stores_read<0>();
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll 1
-                for (int m = max(0, issued[h] - kDepth); m < issued[h]; ++m)
-                    mbar_wait(&b.land[h][m % kDepth], (uint32_t)(m / kDepth) & 1u, nullptr, 0);
-        }
-        __syncwarp();
     } else {
-        // ------------------------------------ products ------------------------------------
+        // (all four warps of a group change their registers at one place)
         reg_dec<kOtherRegs>();
-        if (R > 0) {
+        if (warp == 13) {
+            // ------------------------------------ rows that lie together, to and from memory ------------------------------------
+            int issued[2] = {0, 0};
             bool ok = true;
-            if (warp == 12) {
-                const uint32_t idesc = idesc_of<B16>(R);
-                Turn w_at;
+            auto load = [&](int half, const CUtensorMap *map, int col) {  // null: the slot only
+                const int m = issued[half], st = m % kDepth;
+                if (m >= kDepth && !wait(&b.free[half][st], m / kDepth - 1)) return false;
+                if (map != nullptr) {
+                    mbar_arrive_expect_tx(&b.land[half][st], 4 * kSlot);
+                    tma_box2d(ring + (st * kRowWarps + 4 * half) * kSlot, map, col, row0, &b.land[half][st]);
+                } else {
+                    mbar_arrive(&b.land[half][st]);
+                }
+                ++issued[half];
+                return true;
+            };
+            Slice next[2] = {from, from};
+            int asked[2] = {j0, j0};
+            // the next base of a half, unless its slot is one of those below `from_slot`
+            auto load_base = [&](int half, int from_slot) {
+#pragma unroll 1
+                while (asked[half] < j1 && width_of(next[half], half) <= 0) next[half].step(a), ++asked[half];
+                if (asked[half] >= j1 || issued[half] % kDepth < from_slot) return false;
+                ok = ok && load(half, a.base != nullptr ? &maps.base : nullptr, col_of(next[half], half));
+                next[half].step(a), ++asked[half];
+                return ok;
+            };
+            int ahead[2] = {0, 0};
+            if (joint && lane == 0) {
 #pragma unroll 1
                 for (int i = 0; i < n_blocks && ok; ++i) {
-                    const int wg = i & 1, g = i / kGroup, buf = g & 1, st = w_at.at;
-                    if (i % kGroup == 0 && g >= 2) ok = wait(&b.sum_empty[buf], g / 2 - 1);
-                    ok = ok && wait(&b.x_full[wg], i >> 1) && wait(&b.w_full[st], w_at.round);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t d = tmem + buf * (kLimbs / 2), x = tmem + kLimbs + wg * 64;
-                        const uint32_t w = desc_lo(smem_u32(weights + st * a.ring_bytes));
-                        if constexpr (B16) {
-#pragma unroll
-                            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                                for (int l = 2; l >= 0; --l)
-                                    mma<true>(d, x + 16 * l + 8 * k, w + 4 * wg + 2 * k, idesc, i % kGroup != 0 || k != 0 || l != 2);
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                mma<false>(d, x + 32 + 8 * k, w + 2 * k, idesc, i % kGroup != 0 || k != 0);
-                                if (WT == kW32) mma<false>(d, x + 8 * k, w + a.ring_bytes / 32 + 2 * k, idesc, 1);
-                                mma<false>(d, x + 8 * k, w + 2 * k, idesc, 1);
-                            }
-                        }
-                        mma_commit(&b.x_empty[wg]);
-                        if (!B16 || wg == 1 || i == n_blocks - 1) mma_commit(&b.w_empty[st]);
-                        if (i % kGroup == kGroup - 1 || i == n_blocks - 1) mma_commit(&b.sum_full[buf]);
-                        if (i == n_blocks - 1) mma_commit(&b.v_free);
-                    }
-                    __syncwarp();
-                    if (!B16 || wg == 1) w_at.next(a.ring);
+                    if (i & 1)
+                        ok = load(1, &maps.x, (i0 + i) * 32);
+                    else
+                        ok = load(0, &maps.x, (i0 + i) * 32);
                 }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+                    while (ok && ahead[h] < kDepth && load_base(h, taken)) ++ahead[h];
             }
             __syncwarp();
-            cluster_arrive();
-            cluster_wait();
-            cluster_arrive();
-            if (warp == 12 && ok) {
-                constexpr int kBytes = kSlice * 128 * LW;
-                const uint32_t idesc = idesc_of<B16>(kSlice);
-                const int n_out = min(kMaxOut, a.ring * a.ring_bytes / kBytes), steps = (rank + kPer - 1) / kPer;
-                const uint32_t second = apart ? kSlice : 0;  // the lower limbs' accumulators
-                Turn in, out;  // the stages of B, and the accumulators
+            if (R > 0) {
+                cluster_arrive();
+                cluster_wait();
+                cluster_arrive();
+                cluster_wait();
+                ok = __all_sync(0xffffffffu, wait(&b.h_full, 0)) && ok;  // (the sums are read: their slots are free)
+                fence_proxy_async_smem();
+            }
+            if (joint && lane == 0) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll 1
+                    while (ok && ahead[h] < kDepth && load_base(h, 0)) ++ahead[h];
+                // A slot is filled again when its store has read it, three stores later.
+                int used[2] = {(n_blocks + 1) / 2, n_blocks / 2}, stored = 0;
+                unsigned order = 0;  // the halves of the last stores, the latest in bit 0
                 Slice s = from;
-                ok = __all_sync(0xffffffffu, wait(&b.h_full, 0));
 #pragma unroll 1
                 for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
-                    const int h0 = pick(need, s.p);
-                    if (h0 < 0) continue;
-                    const int buf = out.at;
-                    if (out.round > 0) ok = __all_sync(0xffffffffu, wait(&b.y_empty[buf], out.round - 1));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int width = width_of(s, h);
+                        if (width <= 0 || !ok) continue;
+                        const int st = used[h] % kDepth;
+                        ok = wait(&b.free[h][st], used[h] / kDepth);
+                        if (!ok) break;
+                        ++used[h], ++stored, order = order << 1 | h;
+                        if (tile.n == kTile && width == 32)
+                            tma_store_2d(&maps.y, col_of(s, h), row0, smem_u32(ring + (st * kRowWarps + 4 * h) * kSlot));
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        if (stored > 3) {
+                            stores_read<3>();
+                            if (order >> 3 & 1)
+                                load_base(1, 0);
+                            else
+                                load_base(0, 0);
+                        }
+                    }
+                }
+                // never leave with copies in flight
+                stores_read<0>();
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
 #pragma unroll 1
-                    for (int k = 0; k < steps && ok; ++k) {
-                        const int st = in.at;
-                        ok = __all_sync(0xffffffffu, wait(&b.v_full[st], in.round));
+                    for (int m = max(0, issued[h] - kDepth); m < issued[h]; ++m)
+                        mbar_wait(&b.land[h][m % kDepth], (uint32_t)(m / kDepth) & 1u, nullptr, 0);
+            }
+            __syncwarp();
+        } else {
+            // ------------------------------------ products ------------------------------------
+            if (R > 0) {
+                bool ok = true;
+                if (warp == 12) {
+                    const uint32_t idesc = idesc_of<B16>(R);
+                    Turn w_at;
+#pragma unroll 1
+                    for (int i = 0; i < n_blocks && ok; ++i) {
+                        const int wg = i & 1, g = i / kGroup, buf = g & 1, st = w_at.at;
+                        if (i % kGroup == 0 && g >= 2) ok = wait(&b.sum_empty[buf], g / 2 - 1);
+                        ok = ok && wait(&b.x_full[wg], i >> 1) && wait(&b.w_full[st], w_at.round);
+                        ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         tc_fence_after();
                         if (elect_one()) {
-                            const uint32_t d = tmem + out_at(buf);
-                            const uint32_t w = desc_lo(smem_u32(weights + st * kBytes));
+                            const uint32_t d = tmem + buf * (kLimbs / 2), x = tmem + kLimbs + wg * 64;
+                            const uint32_t w = desc_lo(smem_u32(weights + st * a.ring_bytes));
                             if constexpr (B16) {
-                                const uint32_t h = tmem + (h0 + 64 * k) / 2;
 #pragma unroll
-                                for (int m = 0; m < 4; ++m) {
-                                    if (64 * k + 16 * m >= r16) break;
+                                for (int k = 0; k < 2; ++k)
 #pragma unroll
                                     for (int l = 2; l >= 0; --l)
-                                        mma<true>(d + (l > 0 ? second : 0), h + l * limb_cols + 8 * m, w + 2 * m, idesc,
-                                                  k != 0 || m != 0 || (l != 2 && (l != 0 || !apart)));
-                                }
+                                        mma<true>(d, x + 16 * l + 8 * k, w + 4 * wg + 2 * k, idesc, i % kGroup != 0 || k != 0 || l != 2);
                             } else {
-                                const uint32_t h = tmem + h0 + 32 * k;
 #pragma unroll
-                                for (int m = 0; m < 4; ++m) {
-                                    if (32 * k + 8 * m >= r16) break;
-                                    mma<false>(d + second, h + limb_cols + 8 * m, w + 2 * m, idesc, k + m != 0);
-                                    if (WT == kW32) mma<false>(d + second, h + 8 * m, w + kBytes / 32 + 2 * m, idesc, 1);
-                                    mma<false>(d, h + 8 * m, w + 2 * m, idesc, k + m != 0 || !apart);
+                                for (int k = 0; k < 4; ++k) {
+                                    mma<false>(d, x + 32 + 8 * k, w + 2 * k, idesc, i % kGroup != 0 || k != 0);
+                                    if (WT == kW32) mma<false>(d, x + 8 * k, w + a.ring_bytes / 32 + 2 * k, idesc, 1);
+                                    mma<false>(d, x + 8 * k, w + 2 * k, idesc, 1);
                                 }
                             }
-                            mma_commit(&b.v_empty[st]);
-                            if (k == steps - 1) mma_commit(&b.y_full[buf]);
+                            mma_commit(&b.x_empty[wg]);
+                            if (!B16 || wg == 1 || i == n_blocks - 1) mma_commit(&b.w_empty[st]);
+                            if (i % kGroup == kGroup - 1 || i == n_blocks - 1) mma_commit(&b.sum_full[buf]);
+                            if (i == n_blocks - 1) mma_commit(&b.v_free);
                         }
                         __syncwarp();
-                        in.next(n_out);
+                        if (!B16 || wg == 1) w_at.next(a.ring);
                     }
-                    out.next(bufs);
                 }
+                __syncwarp();
+                cluster_arrive();
+                cluster_wait();
+                cluster_arrive();
+                if (warp == 12 && ok) {
+                    constexpr int kBytes = kSlice * 128 * LW;
+                    const uint32_t idesc = idesc_of<B16>(kSlice);
+                    const int n_out = min(kMaxOut, a.ring * a.ring_bytes / kBytes), steps = (rank + kPer - 1) / kPer;
+                    const uint32_t second = apart ? kSlice : 0;  // the lower limbs' accumulators
+                    Turn in, out;  // the stages of B, and the accumulators
+                    Slice s = from;
+                    ok = __all_sync(0xffffffffu, wait(&b.h_full, 0));
+#pragma unroll 1
+                    for (int j = j0; j < j1 && ok; ++j, s.step(a)) {
+                        const int h0 = pick(need, s.p);
+                        if (h0 < 0) continue;
+                        const int buf = out.at;
+                        if (out.round > 0) ok = __all_sync(0xffffffffu, wait(&b.y_empty[buf], out.round - 1));
+#pragma unroll 1
+                        for (int k = 0; k < steps && ok; ++k) {
+                            const int st = in.at;
+                            ok = __all_sync(0xffffffffu, wait(&b.v_full[st], in.round));
+                            if (!ok) break;
+                            tc_fence_after();
+                            if (elect_one()) {
+                                const uint32_t d = tmem + out_at(buf);
+                                const uint32_t w = desc_lo(smem_u32(weights + st * kBytes));
+                                if constexpr (B16) {
+                                    const uint32_t h = tmem + (h0 + 64 * k) / 2;
+#pragma unroll
+                                    for (int m = 0; m < 4; ++m) {
+                                        if (64 * k + 16 * m >= r16) break;
+#pragma unroll
+                                        for (int l = 2; l >= 0; --l)
+                                            mma<true>(d + (l > 0 ? second : 0), h + l * limb_cols + 8 * m, w + 2 * m, idesc,
+                                                      k != 0 || m != 0 || (l != 2 && (l != 0 || !apart)));
+                                    }
+                                } else {
+                                    const uint32_t h = tmem + h0 + 32 * k;
+#pragma unroll
+                                    for (int m = 0; m < 4; ++m) {
+                                        if (32 * k + 8 * m >= r16) break;
+                                        mma<false>(d + second, h + limb_cols + 8 * m, w + 2 * m, idesc, k + m != 0);
+                                        if (WT == kW32) mma<false>(d + second, h + 8 * m, w + kBytes / 32 + 2 * m, idesc, 1);
+                                        mma<false>(d, h + 8 * m, w + 2 * m, idesc, k + m != 0 || !apart);
+                                    }
+                                }
+                                mma_commit(&b.v_empty[st]);
+                                if (k == steps - 1) mma_commit(&b.y_full[buf]);
+                            }
+                            __syncwarp();
+                            in.next(n_out);
+                        }
+                        out.next(bufs);
+                    }
+                }
+                __syncwarp();
+                cluster_wait();
             }
-            __syncwarp();
-            cluster_wait();
         }
     }
     tc_fence_before();
