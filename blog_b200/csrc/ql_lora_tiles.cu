@@ -285,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) tmem_alloc(&b.tmem, 512);
+    fence_proxy_async_smem();  // (the search's tables stand where copies will)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -608,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_tiles_kernel(const __grid_co
                             *reinterpret_cast<float4 *>(a.y + list[32 * q + r] * a.y_stride + col + c) =
                                 *reinterpret_cast<const float4 *>(slot + place(r, lane & 7));
                     }
+                    if (joint) fence_proxy_async_smem();  // (the slot's next content is a copy's)
                 }
                 give_back();
                 fetch_base();
