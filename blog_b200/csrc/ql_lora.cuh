@@ -42,10 +42,13 @@ struct LoraMaps {
 
 enum { kW32, kW16, kWB16 };  // types of the weights
 
-// v = hi + lo + less than 2^-22 |v|, both tf32.  (hi is cut off, so that it cannot overflow; the rest is exact.)
+// v = hi + lo + less than 2^-22 |v|, both tf32.  (hi is cut off, so that it cannot overflow; the rest is exact.)  Of a v that
+// is not finite lo is NaN: the rest is 0x7FFFFFFF then, and the half added to round it would carry into the sign; as signed
+// numbers that is the one sum which is not the larger.
 __device__ __forceinline__ void limbs(float v, uint32_t &hi, uint32_t &lo) {
     hi = __float_as_uint(v) & 0xFFFFE000u;
-    lo = (__float_as_uint(v - __uint_as_float(hi)) + 0x1000u) & 0xFFFFE000u;
+    const uint32_t rest = __float_as_uint(v - __uint_as_float(hi));
+    lo = (uint32_t)max((int)(rest + 0x1000u), (int)rest) & 0xFFFFE000u;
 }
 
 // Two values in three bf16 limbs, cut off one after another (8 bits each: nothing is left), packed.
