@@ -100,25 +100,27 @@ __device__ __forceinline__ unsigned groups_open(const RouteArgs &a, const T *c, 
     const bool two = a.group_best > 1 && b1 > -INFINITY;
     const T score = two ? b0 + b1 : b0;  // (the same in every lane of a group)
     const T size = sum_err * (fabs(b0) + (two ? fabs(b1) : (T)0)) + 2 * score_err * unit;
+    // Groups with an expert to choose.  (Not by the sum of two, which passes fp32's range where biases are of its lowest value.)
+    const unsigned some = __ballot_sync(kAll, g < a.n_groups && j == 0 && b0 > -INFINITY);
     int better = 0;
-    unsigned close = 0;  // groups whose scores are too near to this one's, bit o * share
+    unsigned close = 0;  // groups whose scores are too near to this one's, or both beyond the range, bit o * share
     const int turns = (a.n_groups + share - 1) / share;  // a group's lanes look at the others in turn
 #pragma unroll 1
     for (int n = 0; n < turns; ++n) {
         const int o = n * share + j, from = min(o, a.n_groups - 1) * share;
         const T v = __shfl_sync(kAll, score, from), z = fast ? __shfl_sync(kAll, size, from) : (T)0;
-        if (o >= a.n_groups) continue;
+        if (o >= a.n_groups || !(some >> (o * share) & 1u)) continue;
         better += v > score || (v == score && o < g);
-        if (fast && fabs(v - score) <= size + z) close |= 1u << (o * share);
+        if (fast && !(fabs(v - score) > size + z)) close |= 1u << (o * share);
     }
 #pragma unroll 1
     for (int o = share / 2; o > 0; o /= 2) {
         better += __shfl_xor_sync(kAll, better, o);
         if (fast) close |= __shfl_xor_sync(kAll, close, o);
     }
-    const bool stays = g < a.n_groups && j == 0 && score > -INFINITY && better < a.top_groups;
+    const bool stays = (some >> lane & 1u) && better < a.top_groups;
     const unsigned open = __ballot_sync(kAll, stays);
-    if (fast) near = __any_sync(kAll, j == 0 && g < a.n_groups && score > -INFINITY && ((stays ? ~open : open) & close) != 0);
+    if (fast) near = __any_sync(kAll, (some >> lane & 1u) && ((stays ? ~open : open) & close) != 0);
     return open;
 }
 
