@@ -72,6 +72,7 @@ SIGNATURES = {
     "ql_add_rms_norm": (I, [I32, P, I64, P, I64, P, I64, P, F, P, I64, P, I, I, I, I]),
     "ql_moe_route": (I, [P, I64, P, P, I, I, I, P]),
     "ql_lora_add": (I, [P, P, I64, P, I64, P, I64, P, I, P, I]),
+    "ql_lora_add_form": (I, [P]),
     "ql_moe_swiglu_grouped": (I, [I32, P, P, SZ, SZ, SZ, SZ, P, I64, P, I, I, P, I, I, I, I]),
     "ql_moe_down_grouped_accum_ordered": (I, [I32, P, SZ, SZ, P, P, I, I, P, P, I64, I, I, I, I]),
     "ql_quant_embedding": (I, [I32, P, P, P, SZ, I, I]),
@@ -481,6 +482,15 @@ def lora_pool(t, a, b, out_dims, in_dim, n_adapters, max_rank, rank=None, scale=
 def lora_add(pool, x, x_stride, base, base_stride, y, y_stride, adapter, n_seqs, q_start, rows):
     """y = base + the rows' adapters applied to x (see include/qlinear_b200.h)."""
     _call("ql_lora_add", C.byref(pool), x, x_stride, base, base_stride, y, y_stride, adapter, n_seqs, q_start, rows)
+
+
+LORA_FORM_ROWS, LORA_FORM_TILES = 1, 2
+
+
+def lora_add_form():
+    """(form, CTAs that shared a tile of rows) of this thread's last lora_add (see include/qlinear_b200.h)."""
+    ctas = C.c_int(0)
+    return int(lib().ql_lora_add_form(C.byref(ctas))), ctas.value
 
 
 def moe_swiglu_grouped(t, gw, uw, geb, ueb, grb, urb, x, x_stride, ids, expert_begin, n_experts, act, tokens, k,

@@ -91,6 +91,7 @@ cudaStream_t g_stream = nullptr;
 thread_local std::string t_err;
 thread_local int t_launches = 0;
 thread_local int t_kv8_form = 0, t_kv8_ctas = 0;  // of this thread's last ql_kv8_attend
+thread_local int t_lora_form = 0, t_lora_ctas = 0;  // of this thread's last ql_lora_add
 
 int fail(int code, const std::string &msg) {
     t_err = msg;
@@ -1617,6 +1618,7 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
     return guarded([&] {
         const std::string what = "ql_lora_add";
         t_launches = 0;
+        t_lora_form = t_lora_ctas = 0;
         if (!pool) return fail(QL_EINVAL, what + ": null pool");
         if (pool->type != QL_F32 && pool->type != QL_F16 && pool->type != QL_BF16)
             return fail(QL_EINVAL, what + ": type must be QL_F32, QL_F16 or QL_BF16");
@@ -1673,18 +1675,29 @@ int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, cons
         LoraArgs tiles = a;
         double us = 0, tiles_us = 0;
         const int tm = lora_plan(a, type, distinct, ws->sms, us);
+        bool tiled = false;
         if (rows >= kLoraTile && rows / distinct >= kLoraTileFrom && rows <= INT32_MAX / 8 &&
             (int64_t)a.n_adapters * a.max_rank <= INT32_MAX && lora_tiles_plan(tiles, type, distinct, ws->sms, tiles_us) &&
             tiles_us < us && lora_maps(maps, tiles, width, type == 2)) {
             e = lora_tiles_launch(tiles, maps, type, g_stream);
+            tiled = true;
         } else {
             if (((int64_t)rows + kLoraChunk - 1) / kLoraChunk * a.chunk_tiles * a.cluster > INT32_MAX)
                 return fail(QL_EINVAL, what + ": too many rows for one call");
             e = lora_launch(a, type, tm, g_stream);
         }
         ++t_launches;
+        if (e == cudaSuccess) {
+            t_lora_form = tiled ? QL_LORA_FORM_TILES : QL_LORA_FORM_ROWS;
+            t_lora_ctas = tiled ? tiles.cluster : a.cluster;
+        }
         return e == cudaSuccess ? (int)QL_OK : cuda_fail(e, what.c_str());
     });
+}
+
+int ql_lora_add_form(int *ctas) {
+    if (ctas) *ctas = t_lora_ctas;
+    return t_lora_form;
 }
 
 // ---- opt-in Q8_1 activation path ----------------------------------------------------

@@ -452,6 +452,11 @@ typedef struct ql_lora_pool {
  * launch; the same call gives the same bits. */
 QL_API int ql_lora_add(const ql_lora_pool *pool, const float *x, int64_t x_stride, const float *base, int64_t base_stride,
                        float *y, int64_t y_stride, const int32_t *adapter, int n_seqs, const int32_t *q_start, int rows);
+/* Which kernel this thread's last ql_lora_add launched: QL_LORA_FORM_ROWS (tiles of up to 32 rows of an adapter),
+ * QL_LORA_FORM_TILES (tiles of 128 rows on tcgen05), 0 none.  ctas (nullable): the CTAs that shared a tile. */
+#define QL_LORA_FORM_ROWS 1
+#define QL_LORA_FORM_TILES 2
+QL_API int ql_lora_add_form(int *ctas);
 
 /* ---- opt-in int8 activation path, Q8_1 (reference kernel.cuh:47-52) -------------------
  * Changes numerics (activations rounded to int8 per 32), as in the reference, which keeps it off
