@@ -135,9 +135,26 @@ int init_device(int dev) {
     return QL_OK;
 }
 
+// A thread has no current context before its first runtime call that needs one, and without one no tensor map is encoded: its
+// device's primary context, then.  (A context that is there stays, and nothing that a capture forbids is called.)
+cudaError_t bind_context(int dev) {
+    static PFN_cuCtxGetCurrent_v4000 get = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            get = reinterpret_cast<PFN_cuCtxGetCurrent_v4000>(p);
+    });
+    CUcontext ctx = nullptr;
+    if (get == nullptr || get(&ctx) != CUDA_SUCCESS || ctx != nullptr) return cudaSuccess;
+    return cudaSetDevice(dev);
+}
+
 Workspace *workspace(int *status) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = bind_context(dev);
     if (e != cudaSuccess) {
         *status = cuda_fail(e, "cudaGetDevice");
         return nullptr;

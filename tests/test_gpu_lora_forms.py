@@ -1,11 +1,14 @@
 """The kernel that a call of adapters takes (ql_lora_add_form), and the tiles of 128 rows over all that can differ between two of
-their calls: CTAs per tile, rows that lie together or do not, bases, strides, row starts, replays."""
+their calls: CTAs per tile, rows that lie together or do not, bases, strides, row starts, threads, replays."""
+import threading
+
 import numpy as np
 import pytest
 
 import blog_b200 as Q
 from test_gpu_layer import QKV, H, Layer
 from test_gpu_lora import TYPES, Case
+from test_gpu_lora_slots import FAR
 
 pytestmark = pytest.mark.gpu
 
@@ -21,7 +24,7 @@ def _runs(rows, n=37):
 def _checked(c, form=TILES):
     far = c.check()
     assert Q.lora_add_form()[0] == form
-    assert far < 1e-6, far
+    assert far < FAR, far
     return Q.lora_add_form()[1]
 
 
@@ -96,6 +99,35 @@ def test_outside_the_pool(type_):
     c.rank[1] = 0
     c.adapter = [0, -1, 1, 2]
     _checked(c)
+
+
+def test_calls_of_several_threads():
+    """Pools of unlike types and ranks, which take unlike amounts of shared memory, in both kernels; every thread is told of its
+    own calls."""
+    import torch
+    Q.set_stream(None)
+    cases = [(TILES, Case(t, *WIDE, [0, 1], lens=[1500, 800], max_rank=m, seed=m)) for t, m in
+             ((Q.BF16, 16), (Q.BF16, 64), (Q.F16, 48), (Q.F32, 32), (Q.F32, 64))]
+    cases += [(ROWS, Case(Q.BF16, 1024, (64,), [0, 1, 2], max_rank=m, seed=m)) for m in (8, 256)]
+    failed = []
+
+    def many(form, c):
+        try:
+            for _ in range(100):
+                c.call()
+                assert Q.lora_add_form()[0] == form
+        except BaseException as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=many, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for form, c in cases:
+        _checked(c, form)
 
 
 @pytest.mark.parametrize("type_", TYPES)
