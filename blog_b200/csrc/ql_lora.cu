@@ -545,13 +545,16 @@ int lora_plan(LoraArgs &a, int type, int distinct, int sms, double &us) {
     // n rows of d adapters make at most (n + d (tm - 1)) / tm tiles, and about half of those that are not full
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (tm - 1)) / tm);
     const int kinds = std::max(1, std::min(a.n_seqs, a.n_adapters));
-    const double tiles = std::max<double>(std::min(kinds, a.rows), (double)a.rows / tm + kinds / 2) * a.n_proj;
+    const double tiles = (a.rows > kLoraChunk ? lora_filled(a, tm)
+                                              : std::max<double>(std::min(kinds, a.rows), (double)a.rows / tm + kinds / 2)) * a.n_proj;
+    const double launched = (double)((a.rows - 1) / kLoraChunk + 1) * a.chunk_tiles * a.n_proj;
     double widest = 0, mean = 0;
     for (int p = 0; p < a.n_proj; ++p) widest = std::max<double>(widest, a.out[p]), mean += (double)a.out[p] / a.n_proj;
     // CTAs per tile: what the rounds of the GPU take in all.
     us = 0;
     for (int c = 1; c <= 8; c += tm < 32 ? c : 1) {
-        const double rounds = tiles / clusters_at_once(tm / 8, c, sms);
+        const int at_once = clusters_at_once(tm / 8, c, sms);
+        const double rounds = tiles / at_once;
         double time;
         if (tm < 32) {
             // parts of rounds count, tiles of low rank end early; beside its share a CTA takes as long as 2400 columns (64
@@ -562,8 +565,9 @@ int lora_plan(LoraArgs &a, int type, int distinct, int sms, double &us) {
             const double per_in = a.max_rank <= 16 ? 0.0033 : (type == 0 ? 0.0134 : 0.0105) * ((a.max_rank + kPass - 1) / kPass);
             const double per_out = 0.008 + (type == 0 ? 0.0002 : 0.00011) * a.max_rank;
             time = rounds <= 1 ? 1 : kinds == 1 ? std::ceil(rounds) : (rounds + std::ceil(rounds)) / 2;
-            time *= 7.5 + 0.05 * a.max_rank + (per_in * a.in_dim + per_out * (rounds <= 1 ? widest : mean)) / c;
+            time *= 7.5 + lora_search_us(a) + 0.05 * a.max_rank + (per_in * a.in_dim + per_out * (rounds <= 1 ? widest : mean)) / c;
         }
+        time += lora_empty_us(a, launched, tiles, at_once);
         if (us == 0 || time < us) us = time, a.cluster = c;
     }
     return tm;

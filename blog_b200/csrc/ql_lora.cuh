@@ -2,6 +2,9 @@
 #pragma once
 #include <cuda.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "ql_common.cuh"
 
 namespace ql {
@@ -277,6 +280,31 @@ __device__ LoraTile find_tile(const LoraArgs &a, int t, int r0, int n, int tm, L
     }
     __syncthreads();
     return LoraTile{found.id, found.first, f.found[0]};
+}
+
+// Adapters among n neighbouring rows, about: those of the sequences that touch them.
+inline double lora_kinds(const LoraArgs &a, int n) {
+    return std::min<double>(std::max(1, std::min(a.n_adapters, a.n_seqs)), (double)n * a.n_seqs / a.rows + (a.q_start != nullptr ? 1 : 0));
+}
+// About how many tiles of tm rows of a call of several chunks have rows: at least one for each adapter of a chunk, and half a tile
+// more for each but one.
+inline double lora_filled(const LoraArgs &a, int tm) {
+    const int chunks = (a.rows - 1) / kLoraChunk + 1;
+    const double kinds = lora_kinds(a, kLoraChunk);
+    return std::max(chunks * kinds, (double)a.rows / tm + 0.5 * chunks * (kinds - 1));
+}
+// What a search takes beyond 2 us where a chunk's warps have more than four adapters each: a lane looks through those of all.
+inline double lora_search_us(const LoraArgs &a) {
+    const double kinds = lora_kinds(a, 32);
+    return a.rows > kLoraChunk && kinds > 4 ? 0.0156 * (kLoraChunk / 32) * kinds : 0;
+}
+// A launch has tiles for every adapter of the call in every chunk of rows (which chunk has which is known on the device alone).
+// What those without rows take in all: each occupies its CTAs until its search ends, 2 us where the sequences' starts stand in
+// shared memory, 2.6 us beyond (65536 rows of 1024 prompts, 896 -> 896 + 128 + 128 at rank 16, with 1 and 1024 adapters: tiles of
+// 128 rows 213 and 1340 us, of 32 rows 634 and 3940 us).  at_once: tiles that run at once; where all of them do, empty ones pass
+// beside the others.
+inline double lora_empty_us(const LoraArgs &a, double launched, double filled, int at_once) {
+    return launched <= at_once ? 0 : std::max(0.0, launched - filled) / at_once * (a.n_seqs <= kLoraChunk ? 2.0 : 2.6);
 }
 
 // Fills in what the launch needs and about how long it takes; returns the rows of a tile.

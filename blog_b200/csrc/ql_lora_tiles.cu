@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "ql_lora.cuh"
 
@@ -1045,7 +1046,7 @@ cudaError_t launch(const LoraArgs &a, const LoraMaps &maps, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     const int chunks = (a.rows + kLoraChunk - 1) / kLoraChunk;
-    cfg.gridDim = dim3((unsigned)(chunks * a.chunk_tiles * a.cluster), (unsigned)(a.split ? a.n_proj : 1), 1);
+    cfg.gridDim = dim3((unsigned)chunks * a.chunk_tiles * a.cluster, (unsigned)(a.split ? a.n_proj : 1), 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -1098,19 +1099,23 @@ bool lora_tiles_plan(LoraArgs &a, int type, int distinct, int sms, double &us) {
     a.chunk_tiles = (int)std::min<int64_t>(chunk, (chunk + (int64_t)distinct * (kTile - 1)) / kTile);
     // CTAs per tile: what the rounds of the GPU take in all.  us of a CTA, from measured times of 512 rows: what passes before,
     // between and after the products (more with the ranks, whose sums go from CTA to CTA), its columns and its outputs.
-    const int64_t tiles = (((int64_t)a.rows + kTile - 1) / kTile + distinct - 1) * (a.split ? a.n_proj : 1);
+    const int grid_y = a.split ? a.n_proj : 1;
+    const double tiles = (a.rows > kLoraChunk ? lora_filled(a, kTile) : (a.rows + kTile - 1) / kTile + distinct - 1) * grid_y;
+    const int64_t launched = ((int64_t)a.rows + kLoraChunk - 1) / kLoraChunk * a.chunk_tiles;
     double out = 0;
-    for (int p = 0; p < a.n_proj; ++p) out += (double)a.out[p] / (a.split ? a.n_proj : 1);
+    for (int p = 0; p < a.n_proj; ++p) out += (double)a.out[p] / grid_y;
     const double per_in = type == 0 ? 0.0165 : type == 1 ? 0.022 : 0.0145, per_out = type == 0 ? 0.026 : type == 1 ? 0.027 : 0.024;
     us = 0;
     a.cluster = 1;
     for (int c = 1; c <= std::min(8, a.in_dim / 32); ++c) {
         const int at_once = clusters_at_once(c, sms);
-        const double time = (double)((tiles + at_once - 1) / at_once) *
-                            (9.5 + (type == 0 ? 0.11 : 0.065) * ranks + (per_in * a.in_dim + per_out * out) / c);
+        if (launched * c > INT32_MAX) break;
+        const double time = std::ceil(tiles / at_once) *
+                                (9.5 + lora_search_us(a) + (type == 0 ? 0.11 : 0.065) * ranks + (per_in * a.in_dim + per_out * out) / c) +
+                            lora_empty_us(a, (double)launched * grid_y, tiles, at_once);
         if (us == 0 || time < us) us = time, a.cluster = c;
     }
-    return true;
+    return us > 0;
 }
 
 cudaError_t lora_tiles_launch(const LoraArgs &a, const LoraMaps &maps, int type, cudaStream_t s) {

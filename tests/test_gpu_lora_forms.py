@@ -212,6 +212,21 @@ def test_sizes_meant_for_tiles_take_them(type_, n_in, outs, max_rank, lens, n_ad
     assert Q.lora_add_form()[0] == (TILES if fits else ROWS)
 
 
+@pytest.mark.parametrize("n,lens,form", [(256, [40] * 300, TILES), (64, [1] * 4096, ROWS), (4, [1000] * 4, TILES)])
+def test_many_adapters(n, lens, form):
+    """Which kernel, where many tiles of a launch have no rows.  (12000 rows of 256 adapters on 3584 -> 3584 + 512 + 512 at rank 16:
+    tiles of 128 rows 518 us, of 32 rows 771; 4096 tokens of 64 on 18944 -> 3584 at rank 64: 2512 and 1089.)"""
+    n_in, outs, rank = (3584, (3584, 512, 512), 16) if n in (4, 256) else (18944, (3584,), 64)
+    r = np.random.default_rng(n)
+    c = Case(Q.BF16, n_in, outs, [int(v) for v in r.integers(0, n, len(lens))], lens=lens, n_adapters=n, max_rank=rank)
+    Q.set_stream(None)
+    c.call()
+    Q.check_device()
+    assert Q.lora_add_form()[0] == form
+    if len(lens) <= 300:
+        _checked(c, form)
+
+
 def test_calls_that_launch_nothing():
     c = Case(Q.BF16, 64, (32,), [0, 1])
     Q.set_stream(None)
