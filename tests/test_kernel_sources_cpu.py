@@ -6,7 +6,7 @@ import re
 import pytest
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "blog_b200", "csrc")
-SOURCES = sorted(p for p in glob.glob(os.path.join(CSRC, "*.cu")) if "setmaxnreg" in open(p).read())
+SOURCES = sorted(p for p in glob.glob(os.path.join(CSRC, "*.cu")) if "reg_dec<" in open(p).read())
 
 
 def _conditions(text, at):
