@@ -5,12 +5,13 @@
 //   of the Q8_1 quantiser (ql_q81.cu) for that y, in either of its layouts, with the same arithmetic and the same
 //   order of the raw sum.
 //
-// Bound: HBM, every value read once and written once; a CTA holds its row in registers between the two uses.  A
+// Bound: HBM in f32, every value read once and written once; a CTA holds its row in registers between the two uses.  A
 // thread has groups of 4 consecutive values (16 bytes in f32), so the 8 threads of an 8-bit block are neighbours and
 // its maximum and sums take three shuffles.  Squares are summed in fp32, a tree over the threads.
 //
 // Measured, residual and Q8_1 rows: 4096 rows of 8192 f32 with sum and y 91.7 us (6.26 TB/s, 0.96 of a plain copy); 777 rows
-// of 2048, no y, 7.8 us; 64 rows of 8192 bf16 4.2 us and one row of 3584 2.8 us: a launch, a load and two reductions.
+// of 2048, no y, 7.8 us; 64 rows of 8192 bf16 4.2 us and one row of 3584 2.8 us: a launch, a load and two reductions.  5000
+// rows of 8192 bf16 93 us (0.61 of a copy): 81 % of the issue slots, since a value takes as many instructions as in f32.
 #include <cuda_bf16.h>
 
 #include "ql_norm.cuh"

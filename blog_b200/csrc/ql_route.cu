@@ -12,7 +12,7 @@
 //
 // Bound: one token or few, the launch and a warp's chain of loads, scores and k rounds of a maximum (2.3 us for one token of
 // 64 experts, 5.3 us for 64 of 256 in groups); thousands, issue slots: 8191 tokens of 384 experts by softmax 11.7 us at some
-// 900 instructions a warp, 8192 of 256 by sigmoid in 8 groups 18.6 us at 1500 (58 and 65 % of the slots; HBM 10 and 4 %).
+// 900 instructions a warp, 8192 of 256 by sigmoid in 8 groups 18.7 us at 1500 (58 and 65 % of the slots; HBM 10 and 4 %).
 // So: a warp per token, everything in registers; a round is one warp reduction of the values as they are and one ballot.
 // Lane l has the NPL consecutive experts from l * NPL.
 #include "ql_route.cuh"
@@ -318,7 +318,8 @@ __device__ __noinline__ void choose_exactly(const RouteArgs &a, int token, doubl
     choose<double, NPL, SIGMOID>(a, token, c);
 }
 
-// (the registers of eight CTAs an SM: 55 warps have to be there for 8192 tokens at once; the seldom 64-bit form may spill)
+// The registers of 12, 8 or 4 CTAs: 48, 32 or 16 warps an SM.  (8192 tokens are 55 warps an SM: 1.15 rounds of them with 8
+// experts a lane, 1.7 with 12.  The seldom 64-bit form may spill.)
 template <int NPL, bool SIGMOID>
 __global__ void __launch_bounds__(32 * kWarps, NPL <= 8 ? 12 : NPL <= 16 ? 8 : 4) route_kernel(const __grid_constant__ RouteArgs a) {
     extern __shared__ double smem[];  // n_experts per warp where there are groups

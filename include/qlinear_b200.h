@@ -392,7 +392,8 @@ QL_API int ql_logits_apply(const float *logits, int64_t logits_stride, float *ou
  * x or residual (same stride); y (NULL: not stored) x or residual.  Strides in elements, at least hidden.
  * xq receives y (before its rounding to type) as Q8_1 rows: layout QL_Q8_ROWS, the bytes that ql_quantize_q8_1 gives
  * for y, rows ql_q8_1_row_bytes(hidden) apart, or QL_Q8_MMQ, those of ql_quantize_q8_1_mmq; QL_Q8_NONE: xq unused.
- * hidden: any up to 32768 (a last block of fewer than 32 is filled with zeros).  fp32 sums; one launch. */
+ * hidden: any up to 32768 (a last block of fewer than 32 is filled with zeros, and the last group of QL_Q8_MMQ with blocks
+ * of zeros).  fp32 sums; one launch. */
 #define QL_Q8_NONE 0
 #define QL_Q8_ROWS 1
 #define QL_Q8_MMQ 2
