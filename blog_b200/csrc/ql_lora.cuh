@@ -301,10 +301,10 @@ inline double lora_search_us(const LoraArgs &a) {
 // A launch has tiles for every adapter of the call in every chunk of rows (which chunk has which is known on the device alone).
 // What those without rows take in all: each occupies its CTAs until its search ends, 2 us where the sequences' starts stand in
 // shared memory, 2.6 us beyond (65536 rows of 1024 prompts, 896 -> 896 + 128 + 128 at rank 16, with 1 and 1024 adapters: tiles of
-// 128 rows 213 and 1340 us, of 32 rows 634 and 3940 us).  at_once: tiles that run at once; where all of them do, empty ones pass
-// beside the others.
+// 128 rows 213 and 1340 us, of 32 rows 634 and 3940 us).  at_once: tiles that run at once; what does not fill a round of its own
+// passes beside the others.
 inline double lora_empty_us(const LoraArgs &a, double launched, double filled, int at_once) {
-    return launched <= at_once ? 0 : std::max(0.0, launched - filled) / at_once * (a.n_seqs <= kLoraChunk ? 2.0 : 2.6);
+    return std::max(0.0, std::floor(launched / at_once) - std::ceil(filled / at_once)) * (a.n_seqs <= kLoraChunk ? 2.0 : 2.6);
 }
 
 // Fills in what the launch needs and about how long it takes; returns the rows of a tile.
